@@ -15,7 +15,7 @@ LIB_PATH = os.environ.get("VQ2_B200_LIB", os.path.join(_HERE, "lib", "libvq2_b20
 HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "vq2_b200.h")
 
 VQ2_OK, VQ2_ERR_SHAPE, VQ2_ERR_DTYPE, VQ2_ERR_ALIGN, VQ2_ERR_LAUNCH, VQ2_ERR_TIMEOUT, VQ2_ERR_ARG = range(7)
-VQ2_F16, VQ2_BF16, VQ2_F32 = 0, 1, 2
+VQ2_F16, VQ2_BF16, VQ2_F32, VQ2_I8 = 0, 1, 2, 3
 VQ2_ACT_ROTATED, VQ2_ACT_RHT, VQ2_ACT_SWIGLU_RHT = 0, 1, 2
 
 _DTYPE_CODE = {torch.float16: VQ2_F16, torch.bfloat16: VQ2_BF16, torch.float32: VQ2_F32}
@@ -73,6 +73,14 @@ SIGNATURES = {
     "vq2_moe_layer_ep": [_p, _i32, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _p, _i32,
                          _p, _p, _i64, _f32, _p, _p, _i64, _f32, _p, _i64, _p, _i32, _i32, _i64, _p, _p, _i64, _p, _i32,
                          _p],
+    "vq2_rotary": [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i32, _i64, _i64, _p, _i32, _p, _i64, _i32, _f32, _i32,
+                   _p, _p, _p],
+    "vq2_cache_write": [_p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _i32, _i64, _p, _i64, _i32, _f32,
+                        _p, _p, _i32, _p, _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _p],
+    "vq2_cache_read": [_p, _p, _i32, _p, _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _i64, _p, _p, _i32, _i64, _p],
+    "vq2_paged_attention_workspace": [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i64],
+    "vq2_paged_attention": [_p, _i64, _i64, _i32, _i64, _i64, _p, _p, _i32, _p, _p, _i64, _i64, _i64, _i64, _p, _i64,
+                            _i64, _p, _p, _i64, _i64, _i64, _f32, _i32, _i64, _p, _p, _p, _i64, _p],
     "vq2_lru_state_ints": [_i64, _i64],
     "vq2_lru_step": [_p, _p, _i64, _p, _p, _p],
     "vq2_fetch_records": [_p, _p, _i64, _p, _i64, _p, _i64, _i64, _p],

@@ -44,6 +44,7 @@ extern "C" {
 #define VQ2_F16 0
 #define VQ2_BF16 1
 #define VQ2_F32 2
+#define VQ2_I8 3  /* quantised key/value pages only */
 
 /* ABI version of this header (bumped on any signature change). */
 VQ2_API int vq2_abi_version(void);
@@ -596,6 +597,83 @@ VQ2_API int vq2_paged_moe_t1(const void* h, int h_dtype, int64_t top_k, const in
                              const int8_t* sign_mid, int64_t hb_mid, float scale_mid, const void* image_dev,
                              const int64_t* rec_off, int64_t num_experts, void* workspace,
                              int64_t workspace_bytes, void* out, int out_dtype, void* stream);
+
+/*
+ * Rotary positions, the paged key/value cache and attention over it: what stands between a decoder
+ * layer's q/k/v projections and its output projection (no reference counterpart: the reference
+ * leaves its attention blocks to the transformers modules, vq2/load_and_test_full_35b.py:124-223).
+ *
+ * Shared arguments. Tokens: q [tokens, q_heads, head_size], k and v [tokens, kv_heads, head_size],
+ * fp16 or bf16 (dtype), strides in elements, last dimension contiguous; head_size a multiple of 16,
+ * 16..256. Cache: k_pages, v_pages [pages, kv_heads, page_size, head_size] contiguous, page_size a
+ * power of two 16..256; kv_dtype = dtype, or VQ2_I8 with fp32 k_scale, v_scale [pages, kv_heads,
+ * page_size] (value = int8 * scale). table: int32 [seqs, table_cols] page ids (row stride
+ * table_stride): position p of sequence b is row p % page_size of page table[b][p / page_size].
+ * lens: int32 [seqs] tokens of each sequence in the cache, the new ones included. starts: int32
+ * [seqs + 1], ascending: sequence b's new tokens are starts[b] .. starts[b + 1] - 1 and sit at
+ * positions lens[b] - count .. lens[b] - 1; NULL: one new token per sequence (tokens = seqs).
+ * Page ids outside the pool and lengths past the table are never followed.
+ */
+
+/*
+ * Rotary positions of q and k (either may have 0 heads) into contiguous q_out, k_out: pair i of the
+ * first `rot` values of every head -- (x[i], x[i + rot/2]), or (x[2i], x[2i+1]) when interleaved --
+ * is turned by positions[t] * inv_freq[i] and multiplied by factor; the other values are copied.
+ * inverse: turned back (the gradient of the forward pass). positions: int32 or (positions64) int64.
+ */
+VQ2_API int vq2_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t q_heads,
+                       const void* k, int64_t k_token_stride, int64_t k_head_stride, int64_t k_heads,
+                       int dtype, int64_t tokens, int64_t head_size, const void* positions,
+                       int positions64, const float* inv_freq, int64_t rot, int interleaved,
+                       float factor, int inverse, void* q_out, void* k_out, void* stream);
+
+/*
+ * Write the new tokens' k and v into their cache rows; with inv_freq (rot values) k, and q when
+ * q_heads > 0, are turned first (q into q_out, contiguous). 8-bit cache: per (token, head)
+ * scale = amax / 127 and int8 = round-to-even(x * (127 / amax)) of the turned values in 32 bits;
+ * amax < 1e-30 stores zeros with scale 0, a row with an infinity or a NaN stores scale NaN. Tokens
+ * without a page (a position outside the table, a page id outside the pool) are not stored.
+ */
+VQ2_API int vq2_cache_write(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t q_heads,
+                            void* q_out, const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                            const void* v, int64_t v_token_stride, int64_t v_head_stride, int dtype,
+                            int64_t tokens, const float* inv_freq, int64_t rot, int interleaved,
+                            float factor, void* k_pages, void* v_pages, int kv_dtype, float* k_scale,
+                            float* v_scale, int64_t pages, int64_t kv_heads, int64_t page_size,
+                            int64_t head_size, const int32_t* table, int64_t table_stride,
+                            int64_t table_cols, const int32_t* lens, const int32_t* starts, int64_t seqs,
+                            void* stream);
+
+/*
+ * Read whole sequences back: positions 0 .. starts[b+1] - starts[b] - 1 of sequence b into rows
+ * starts[b].. of k_out, v_out [total, kv_heads, head_size] (out_dtype, contiguous). Rows past
+ * starts[seqs] and rows without a page are zero.
+ */
+VQ2_API int vq2_cache_read(const void* k_pages, const void* v_pages, int kv_dtype, const float* k_scale,
+                           const float* v_scale, int64_t pages, int64_t kv_heads, int64_t page_size,
+                           int64_t head_size, const int32_t* table, int64_t table_stride,
+                           int64_t table_cols, const int32_t* starts, int64_t seqs, void* k_out,
+                           void* v_out, int out_dtype, int64_t total, void* stream);
+
+/*
+ * out[t, h] = sum_l softmax_l(scale * q[t, h] . k[l, h / (q_heads / kv_heads)]) v[l, ..] over the
+ * keys l that token t sees: l < its sequence's length, l <= its position when causal, l > its
+ * position - window when window > 0. A token that sees none gives zeros (lse -inf). out: contiguous,
+ * dtype; lse (may be NULL): fp32 [tokens, q_heads], the natural logarithm of the sum. max_new and
+ * max_len bound every sequence's new tokens and length (larger is only slower). q: 16-byte aligned,
+ * strides multiples of 8. workspace: vq2_paged_attention_workspace(...) bytes, 16-byte aligned.
+ */
+VQ2_API int64_t vq2_paged_attention_workspace(int64_t tokens, int64_t q_heads, int64_t kv_heads,
+                                              int64_t head_size, int64_t seqs, int64_t max_new,
+                                              int64_t max_len, int causal, int64_t window);
+VQ2_API int vq2_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype,
+                                int64_t tokens, int64_t q_heads, const void* k_pages, const void* v_pages,
+                                int kv_dtype, const float* k_scale, const float* v_scale, int64_t pages,
+                                int64_t kv_heads, int64_t page_size, int64_t head_size,
+                                const int32_t* table, int64_t table_stride, int64_t table_cols,
+                                const int32_t* lens, const int32_t* starts, int64_t seqs, int64_t max_new,
+                                int64_t max_len, float scale, int causal, int64_t window, void* out,
+                                float* lse, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
