@@ -1,0 +1,73 @@
+// What the attention kernels share: arguments, the keys that query rows see, and how rows are split
+// along the keys and joined.
+#pragma once
+#include "kv_dev.cuh"
+
+namespace vq2 {
+
+struct AttnArgs {
+  PagedKV kv;
+  const void* q;
+  int64_t q_ts, q_hs;   // strides of q, elements
+  int T, hq, D, G;      // G: query heads per key/value head
+  int q_bf16;           // type of q and out
+  float scale_log2;     // scale * log2(e): scores in powers of two
+  int causal, window;
+  void* out;            // [T, hq, D]
+  float* lse;           // [T, hq] or null
+  // Split s of a block of rows takes the keys lo + s * chunk .. lo + (s + 1) * chunk - 1 of the keys
+  // [lo, hi) that the block sees, lo rounded down to 16. rows_per_block: query rows a block takes.
+  int chunk, splits, rows_per_block, row_blocks;
+  float* part_o;        // [T * hq, splits, D]: weighted sums of V relative to the maximum
+  float2* part_ml;      // [T * hq, splits]: (maximum score in powers of two, sum of weights)
+};
+
+constexpr float kLn2 = 0.69314718055994530942f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A sequence's new tokens, and the block of query rows [r0, r0 + rows) among its count * G: row r is
+// new token r / G, head r % G of the key/value head.
+struct AttnRows {
+  int first, count, len;  // first new token, new tokens, length of the sequence
+  int r0, rows;
+};
+
+__device__ __forceinline__ AttnRows attn_rows(const AttnArgs& a, int b, int rb) {
+  AttnRows w;
+  sequence_rows(a.kv, b, w.first, w.count);
+  w.first = max(0, min(w.first, a.T));
+  w.count = max(0, min(w.count, a.T - w.first));
+  w.len = length_of(a.kv, b);
+  w.r0 = rb * a.rows_per_block;
+  w.rows = (int)max((int64_t)0, min((int64_t)a.rows_per_block, (int64_t)w.count * a.G - w.r0));
+  return w;
+}
+
+// Keys that new token i sees: [row_lo, row_hi).
+__device__ __forceinline__ int row_lo(const AttnArgs& a, const AttnRows& w, int i) {
+  return a.window ? max(0, w.len - w.count + i - a.window + 1) : 0;
+}
+__device__ __forceinline__ int row_hi(const AttnArgs& a, const AttnRows& w, int i) {
+  return a.causal ? max(0, min(w.len, w.len - w.count + i + 1)) : w.len;
+}
+
+// Keys that any row of the block sees, the start rounded down to 16; no more than the splits cover.
+__device__ __forceinline__ void block_keys(const AttnArgs& a, const AttnRows& w, int& lo, int& hi) {
+  lo = row_lo(a, w, w.r0 / a.G) & ~15;
+  hi = w.rows > 0 ? row_hi(a, w, (w.r0 + w.rows - 1) / a.G) : 0;
+  hi = (int)min((int64_t)hi, lo + (int64_t)a.splits * a.chunk);
+}
+
+// Joins the splits of every row (launched after a kernel that left more than one).
+int launch_attn_join(const AttnArgs& a, cudaStream_t st);
+// One token to a few rows per key/value head: see attn_decode.cu.
+int launch_attn_decode(const AttnArgs& a, bool i8, cudaStream_t st);
+// Sets chunk, splits, rows_per_block and row_blocks.
+void plan_attn_decode(AttnArgs& a, int64_t max_new, int64_t max_len);
+
+}  // namespace vq2
