@@ -78,7 +78,8 @@ SIGNATURES = {
     "vq2_cache_write": [_p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _i32, _i64, _p, _i64, _i32, _f32,
                         _p, _p, _i32, _p, _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _p],
     "vq2_cache_read": [_p, _p, _i32, _p, _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _i64, _p, _p, _i32, _i64, _p],
-    "vq2_paged_attention_workspace": [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i64],
+    "vq2_paged_attention_workspace": [_i64, _i64, _i64, _i64, _i32, _i64, _i64, _i64, _i64],
+    "vq2_attention_status": [_i32],
     "vq2_paged_attention": [_p, _i64, _i64, _i32, _i64, _i64, _p, _p, _i32, _p, _p, _i64, _i64, _i64, _i64, _p, _i64,
                             _i64, _p, _p, _i64, _i64, _i64, _f32, _i32, _i64, _p, _p, _p, _i64, _p],
     "vq2_lru_state_ints": [_i64, _i64],

@@ -245,7 +245,7 @@ def paged_attention(q, k_pages, v_pages, table, lens, starts=None, *, k_scale=No
     if not T:
         return (out, lse) if return_lse else out
     lib = _lib._lib or _lib.load()
-    nbytes = lib.vq2_paged_attention_workspace(T, hq, h, d, seqs, max_new, max_len, causal, window)
+    nbytes = lib.vq2_paged_attention_workspace(T, hq, h, d, pools[2], seqs, max_new, max_len, window)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _call("vq2_paged_attention", dev, q.data_ptr(), q.stride(0), q.stride(1), _Q_CODE[q.dtype], T, hq, *pools, *shape,
           lens_p, starts_p, seqs, max_new, max_len, d ** -0.5 if scale is None else scale, causal, window,

@@ -9,9 +9,14 @@
 namespace vq2 {
 namespace {
 
-// Splits of the keys and the bytes that joining them takes: a function of shapes and bounds alone.
-int64_t plan(AttnArgs& a, int64_t max_new, int64_t max_len) {
-  plan_attn_decode(a, max_new, max_len);
+// Which kernel, and the splits of the keys: a function of shapes and bounds alone. Returns the bytes
+// that joining the splits takes.
+int64_t plan(AttnArgs& a, bool i8, int64_t max_new, int64_t max_len, bool& chunked) {
+  // Rows that share a key: the decode kernel holds 16 (head size above 128) or 32 of them; from there
+  // on it would read the keys again for every 16 or 32, and the tensor-core kernel takes over.
+  chunked = !i8 && max_new * a.G > (a.D > 128 ? 16 : 32);
+  if (chunked) plan_attn_chunk(a, max_new, max_len);
+  else plan_attn_decode(a, max_new, max_len);
   if (a.splits == 1) return 0;
   return (int64_t)a.T * a.hq * a.splits * (a.D * 4 + 8);
 }
@@ -29,7 +34,7 @@ bool bad_attn(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t seqs, i
 using namespace vq2;
 
 extern "C" int64_t vq2_paged_attention_workspace(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_size,
-                                                 int64_t seqs, int64_t max_new, int64_t max_len, int causal,
+                                                 int kv_dtype, int64_t seqs, int64_t max_new, int64_t max_len,
                                                  int64_t window) {
   if (bad_attn(tokens, q_heads, kv_heads, seqs, max_new, max_len, window) || bad_head_size(head_size)) return 0;
   AttnArgs a = {};
@@ -39,9 +44,9 @@ extern "C" int64_t vq2_paged_attention_workspace(int64_t tokens, int64_t q_heads
   a.kv.seqs = (int)seqs;
   a.D = (int)head_size;
   a.G = a.hq / a.kv.heads;
-  a.causal = causal;
   a.window = (int)window;
-  return tokens && seqs ? plan(a, max_new, max_len) : 0;
+  bool chunked;
+  return tokens && seqs ? plan(a, kv_dtype == VQ2_I8, max_new, max_len, chunked) : 0;
 }
 
 extern "C" int vq2_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype,
@@ -75,7 +80,8 @@ extern "C" int vq2_paged_attention(const void* q, int64_t q_token_stride, int64_
   a.window = (int)window;
   a.out = out;
   a.lse = lse;
-  const int64_t bytes = plan(a, starts ? max_new : 1, max_len);
+  bool chunked;
+  const int64_t bytes = plan(a, kv_dtype == VQ2_I8, starts ? max_new : 1, max_len, chunked);
   if (bytes) {
     if (!workspace || workspace_bytes < bytes) return VQ2_ERR_ARG;
     a.part_o = static_cast<float*>(workspace);
@@ -83,7 +89,7 @@ extern "C" int vq2_paged_attention(const void* q, int64_t q_token_stride, int64_
   }
   if ((int64_t)a.kv.seqs * a.row_blocks > 0x7fffffff) return VQ2_ERR_SHAPE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  s = launch_attn_decode(a, kv_dtype == VQ2_I8, st);
+  s = chunked ? launch_attn_chunk(a, st) : launch_attn_decode(a, kv_dtype == VQ2_I8, st);
   if (s != VQ2_OK || a.splits == 1) return s;
   return launch_attn_join(a, st);
 }

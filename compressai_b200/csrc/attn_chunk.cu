@@ -1,0 +1,593 @@
+// Attention of many query rows per key/value head over a paged cache: chunks and whole prompts, on
+// the tensor cores (tcgen05) with scores and output in tensor memory.
+//
+//   S = Q K^T,   P = 2^(S * scale - m),   O += P V      (128 rows x 128 keys a step)
+//
+// Rows are (new token, head of the group) pairs, so one tile of keys serves every head that shares
+// it. A block owns ROWS = 256 rows (head size up to 128) or 128 (up to 256), O staying in tensor
+// memory, and walks the keys once. Roles:
+//   * one warp brings keys and values by TMA, straight from their pages: 16 KB blocks in a ring, a
+//     K block being 128 keys x 64 values, a V block 8192 / DP keys x all values, 128-byte swizzle;
+//   * one thread issues the MMAs: S from shared memory, O with P as the operand in tensor memory
+//     (P overwrites its S) and V with its values contiguous (the descriptor's transposed form);
+//   * a warpgroup per 128 rows does the softmax, a row per thread: no shuffles. Maxima, sums and O
+//     are 32 bits; P is rounded to the cache's 16 bits for the second product.
+// With two row tiles the tensor core works on one while the softmax works on the other; with one
+// (head size 256, O takes half of tensor memory) S is double-buffered and QK of the next tile runs
+// under the softmax.
+//
+// The running maximum moves only when a score passes it by 8 powers of two (P is then at most 256),
+// which is rare after the first tiles: O is rescaled in tensor memory by the softmax threads
+// themselves, and no separate correction stage stands in the loop.
+//
+// Bound: at 2 * 128 * 128 * DP flops for 128 * 128 exponentials per product pair, the tensor core
+// and (head size 128) the 16 exponentials a clock an SM are about equally busy.
+//
+// Rows of a page past the keys that the block sees may hold anything, NaN too: their scores are
+// replaced, and their V rows zeroed in shared memory by the loading warp before the MMA may read
+// them (at most one block per launch block holds such rows; blocks and pages wholly outside are not
+// read: the copy's coordinate is put past the pool, which fills zeros).
+//
+// Every wait is bounded by the SM clock (about 2 s): one that gives up raises the abort flag and
+// vq2_attention_status, every role leaves its loop, copies and MMAs in flight are drained.
+#include <atomic>
+#include <type_traits>
+
+#include "attn_dev.cuh"
+#include "tcgen05.cuh"
+
+// Sticky status of the chunk kernel: VQ2_ERR_TIMEOUT once any bounded wait gave up.
+__device__ int32_t g_attention_status;
+
+namespace vq2 {
+namespace {
+
+constexpr long long kWaitCycles = 4000000000LL;  // ~2 s at 1.965 GHz
+constexpr int kBlock = 16384;                    // bytes of a ring block
+
+template <int DP>
+struct ChunkShape {
+  static constexpr int NQ = DP > 128 ? 1 : 2;        // row tiles of 128
+  static constexpr int B = DP / 64;                  // ring blocks of a 128-key tile, K or V
+  static constexpr int KB = 8192 / DP;               // keys of a V block
+  static constexpr int Q = NQ * 128 * DP * 2;
+  static constexpr int NB = (232448 - 2048 - Q) / kBlock;   // ring blocks: 10, or 12 at head size 64
+  static constexpr int Smem = 1024 + Q + NB * kBlock + 512;
+  static constexpr int Threads = (4 * NQ + 2) * 32;
+  static constexpr uint32_t O0 = 256;                // first TMEM column of O; S buffers at 0 and 128
+};
+
+struct ChunkCtl {
+  uint64_t full[12], empty[12];   // ring
+  uint64_t s_full[2], p_full[2];  // score buffers: scores ready, weights ready
+  uint64_t o_full[2];             // the last product of a row tile is in O
+  uint64_t pv;                    // one row tile: each product into O (before a rescale)
+  uint64_t tail;                  // V rows past the last key are zeroed
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort;
+};
+static_assert(sizeof(ChunkCtl) <= 512, "control block");
+
+__device__ __forceinline__ void chunk_fail(ChunkCtl* c) {
+  *reinterpret_cast<volatile int*>(&c->abort) = 1;
+  atomicMax(&g_attention_status, VQ2_ERR_TIMEOUT);
+}
+__device__ __forceinline__ bool chunk_wait(uint32_t bar, uint32_t parity, ChunkCtl* c) {
+  if (mbar_try(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try(bar, parity)) {
+    if (*reinterpret_cast<volatile int*>(&c->abort)) return false;
+    if (clock64() - t0 > kWaitCycles) {
+      chunk_fail(c);
+      return false;
+    }
+  }
+  return true;
+}
+__device__ __forceinline__ void chunk_drain(uint32_t bar, uint32_t parity) {
+  const long long t0 = clock64();
+  while (!mbar_try(bar, parity))
+    if (clock64() - t0 > kWaitCycles) {
+      atomicMax(&g_attention_status, VQ2_ERR_TIMEOUT);
+      return;
+    }
+}
+
+// Descriptor of a V block: values contiguous (64 in a 128-byte swizzled row, the next 64 KB keys * 128
+// bytes on: the leading byte offset), keys 128 bytes apart, 8-key groups 1024 (stride byte offset).
+template <int KB>
+__device__ __forceinline__ uint64_t v_desc(uint32_t saddr) {
+  return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(KB * 128 >> 4) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
+}
+
+// 32 columns of this thread's lane, not yet waited for; tmem_wait passes the registers through the
+// wait so that no use of them can be moved ahead of it.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld(float* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+               :
+               : "memory");
+  asm volatile("" : "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]),
+                    "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+        "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]),
+        "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]),
+        "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int DP, typename T>
+__global__ void __launch_bounds__(ChunkShape<DP>::Threads, 1)
+    attn_chunk_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+  using S = ChunkShape<DP>;
+  constexpr int NQ = S::NQ, B = S::B, KB = S::KB, NB = S::NB;
+  constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ unsigned char chunk_raw[];
+  unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(chunk_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* ring = sm + S::Q;
+  ChunkCtl* ctl = reinterpret_cast<ChunkCtl*>(ring + NB * kBlock);
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kMma = 4 * NQ, kTma = 4 * NQ + 1;
+  // the last rows see the most keys: they go first
+  const int b = blockIdx.x / a.row_blocks, rb = a.row_blocks - 1 - (blockIdx.x - b * a.row_blocks);
+  const int split = blockIdx.y, h = blockIdx.z;
+  const AttnRows w = attn_rows(a, b, rb);
+  if (w.rows <= 0) return;
+  int lo, hi;
+  block_keys(a, w, lo, hi);
+  const int s0 = lo + split * a.chunk, s1 = min(hi, s0 + a.chunk);
+  if (split > 0 && s0 >= hi) return;  // split 0 stays: it writes the rows that see nothing
+  const bool alone = hi - lo <= a.chunk;
+  const int tiles = s1 > s0 ? (s1 - s0 + 127) >> 7 : 0;
+  const int nq = NQ == 2 && w.rows > 128 ? 2 : 1;  // row tiles in use
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NB; ++i) {
+      mbar_init(su32(&ctl->full[i]), 1);
+      mbar_init(su32(&ctl->empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(su32(&ctl->s_full[i]), 1);
+      mbar_init(su32(&ctl->p_full[i]), 4);
+      mbar_init(su32(&ctl->o_full[i]), 1);
+    }
+    mbar_init(su32(&ctl->pv), 1);
+    mbar_init(su32(&ctl->tail), 1);
+    mbar_init(su32(&ctl->drain), 1);
+    ctl->abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kMma) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&ctl->tmem_base)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  // ---- queries into 128-byte swizzled blocks [row tile][64 values][128 rows]; rows past the last are zeros
+  for (int e = threadIdx.x; e < nq * 128 * (DP / 8); e += blockDim.x) {
+    const int r = e / (DP / 8), v = e - r * (DP / 8);  // row, 8-value piece
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (r < w.rows && 8 * v < a.D) {
+      const int row = w.r0 + r;
+      x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (w.first + row / a.G) * a.q_ts +
+                                          (h * a.G + row % a.G) * a.q_hs + 8 * v);
+      if (a.scale_log2 < 0.f) x = make_uint4(x.x ^ 0x80008000u, x.y ^ 0x80008000u, x.z ^ 0x80008000u, x.w ^ 0x80008000u);
+    }
+    const int rr = r & 127;
+    *reinterpret_cast<uint4*>(sm + ((r >> 7) * B + (v >> 3)) * kBlock + rr * 128 + (((v & 7) ^ (rr & 7)) << 4)) = x;
+  }
+  fence_proxy_async();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl->tmem_base;
+  // Ring order of the 128-key tiles' operands, in blocks: K0 V0 K1 V1 .. with two row tiles, K0 K1 V0
+  // K2 V1 .. with one, as the MMAs take them.
+  auto k_block = [&](int j) { return NQ == 2 ? 2 * j * B : j == 0 ? 0 : (2 * j - 1) * B; };
+  auto v_block = [&](int j) { return NQ == 2 || j == tiles - 1 ? (2 * j + 1) * B : (2 * j + 2) * B; };
+  const int gran = min(1 << a.kv.page_log2, KB);   // keys of one V copy
+  const int tail = (s1 & (gran - 1)) ? s1 : -1;    // rows from here on, up to the copy's end, hold anything
+
+  if (warp == kTma) {
+    // ---------------------------------------------------------------------------- loads
+    const int32_t* table = a.kv.table + b * a.kv.table_stride;
+    const int seen = row_lo(a, w, w.r0 / a.G);   // pages that end before the first key seen may be gone
+    const int page_mask = (1 << a.kv.page_log2) - 1, pool_rows = (a.kv.pages * a.kv.heads) << a.kv.page_log2;
+    // pool row of key k, or past the pool (zeros) where there is none
+    auto row_of = [&](int k) {
+      if (k >= s1 || (k | page_mask) < seen) return pool_rows;
+      const int page = table[k >> a.kv.page_log2];
+      return page < 0 || page >= a.kv.pages ? pool_rows : ((page * a.kv.heads + h) << a.kv.page_log2) + (k & page_mask);
+    };
+    int q = 0;
+    bool ok = true;
+    const int rk = min(1 << a.kv.page_log2, 128);   // keys of one K copy
+    // lane i's copy of a K block: keys i * rk ..; of a V block: values 64 * (i % B), keys (i / B) * gran ..
+    auto load = [&](bool is_v, int j) {
+      const int k0 = s0 + 128 * j;
+      int row[B];   // this lane's pool row for each block, looked up ahead of the waits
+#pragma unroll
+      for (int c = 0; c < B; ++c) row[c] = pool_rows;
+      if (!is_v) {
+        if (lane * rk < 128) row[0] = row_of(k0 + lane * rk);
+      } else {
+#pragma unroll
+        for (int c = 0; c < B; ++c)
+          if ((lane / B) * gran < KB) row[c] = row_of(k0 + c * KB + (lane / B) * gran);
+      }
+#pragma unroll 1
+      for (int c = 0; c < B && ok; ++c, ++q) {
+        const int slot = q % NB;
+        ok = chunk_wait(su32(&ctl->empty[slot]), ((q / NB) & 1) ^ 1, ctl);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint32_t bar = su32(&ctl->full[slot]), dst = su32(ring + slot * kBlock);
+        if (lane == 0) mbar_arrive_tx(bar, kBlock);
+        __syncwarp();
+        if (!is_v) {
+          if (lane * rk < 128) tma_load_2d(dst + lane * rk * 128, &kmap, 64 * c, row[0], bar);
+        } else {
+          int r = row[0];
+#pragma unroll
+          for (int i = 1; i < B; ++i)
+            if (i == c) r = row[i];
+          if ((lane / B) * gran < KB)
+            tma_load_2d(dst + (lane % B) * KB * 128 + (lane / B) * gran * 128, &vmap, 64 * (lane % B), r, bar);
+          const int kb = k0 + c * KB;
+          if (tail > kb && tail < kb + KB) {  // zero what follows the last key in its copy
+            ok = __all_sync(0xffffffffu, chunk_wait(bar, (q / NB) & 1, ctl));
+            if (!ok) { ++q; break; }
+            const int from = tail - kb, to = (from + gran - 1) / gran * gran;
+            for (int e = lane; e < (to - from) * B * 8; e += 32) {
+              const int rr = from + e / (B * 8), p = e % (B * 8);
+              *reinterpret_cast<uint4*>(ring + slot * kBlock + (p >> 3) * KB * 128 + rr * 128 + ((p & 7) << 4)) =
+                  make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(su32(&ctl->tail));
+          }
+        }
+      }
+    };
+    if (tiles > 0) load(false, 0);
+    if (NQ == 2) {
+      for (int j = 0; j < tiles && ok; ++j) {
+        load(true, j);
+        if (j + 1 < tiles && ok) load(false, j + 1);
+      }
+    } else {
+      for (int j = 0; j < tiles && ok; ++j) {
+        if (j + 1 < tiles) load(false, j + 1);
+        if (ok) load(true, j);
+      }
+    }
+    // copies this warp started have landed before the block's shared memory goes away
+    if (!ok)
+      for (int i = max(0, q - NB); i < q; ++i) chunk_drain(su32(&ctl->full[i % NB]), (i / NB) & 1);
+  } else if (warp == kMma) {
+    // ---------------------------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t QK = umma_idesc<128, BF>(), PV = umma_idesc<DP, BF>(true);
+      bool ok = true;
+      // scores of row tile i with key tile j into buffer s
+      auto qk = [&](int i, int j, int s) {
+        const int q0 = k_block(j);
+#pragma unroll 1
+        for (int c = 0; c < B && ok; ++c) {
+          const int slot = (q0 + c) % NB;
+          if (i == 0) {
+            ok = chunk_wait(su32(&ctl->full[slot]), ((q0 + c) / NB) & 1, ctl);
+            if (!ok) return;
+            tc_fence_after();
+          }
+          const uint64_t ad = sw128_desc(su32(sm + (i * B + c) * kBlock)), bd = sw128_desc(su32(ring + slot * kBlock));
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) umma_f16(tmem + 128 * s, ad + 2 * kk, bd + 2 * kk, QK, (c | kk) != 0);
+          if (i == nq - 1) umma_commit(su32(&ctl->empty[slot]));
+        }
+        umma_commit(su32(&ctl->s_full[s]));
+      };
+      // O of row tile i += weights in buffer s times V tile j
+      auto pv = [&](int i, int j, int s) {
+        const int q0 = v_block(j);
+#pragma unroll 1
+        for (int c = 0; c < B && ok; ++c) {
+          const int slot = (q0 + c) % NB;
+          if (i == 0) {
+            ok = chunk_wait(su32(&ctl->full[slot]), ((q0 + c) / NB) & 1, ctl);
+            const int kb = s0 + 128 * j + c * KB;
+            if (ok && tail > kb && tail < kb + KB) ok = chunk_wait(su32(&ctl->tail), 0, ctl);
+            if (!ok) return;
+            tc_fence_after();
+          }
+          const uint64_t bd = v_desc<KB>(su32(ring + slot * kBlock));
+          const uint32_t p = tmem + 128 * s + c * (KB / 2);
+#pragma unroll
+          for (int kk = 0; kk < KB / 16; ++kk)
+            umma_f16_ts(tmem + S::O0 + i * DP, p + 8 * kk, bd + 128 * kk, PV, (j | c | kk) != 0);
+          if (i == nq - 1) umma_commit(su32(&ctl->empty[slot]));
+        }
+        if (NQ == 1) umma_commit(su32(&ctl->pv));
+        if (j == tiles - 1) umma_commit(su32(&ctl->o_full[i]));
+      };
+      if (NQ == 2) {
+        if (tiles > 0)
+          for (int i = 0; i < nq && ok; ++i) qk(i, 0, i);
+        for (int j = 0; j < tiles && ok; ++j)
+          for (int i = 0; i < nq && ok; ++i) {
+            ok = chunk_wait(su32(&ctl->p_full[i]), j & 1, ctl);
+            if (!ok) break;
+            tc_fence_after();
+            pv(i, j, i);
+            if (j + 1 < tiles && ok) qk(i, j + 1, i);
+          }
+      } else {
+        if (tiles > 0) qk(0, 0, 0);
+        for (int j = 0; j < tiles && ok; ++j) {
+          if (j + 1 < tiles) qk(0, j + 1, (j + 1) & 1);
+          if (ok) ok = chunk_wait(su32(&ctl->p_full[j & 1]), (j >> 1) & 1, ctl);
+          if (!ok) break;
+          tc_fence_after();
+          pv(0, j, j & 1);
+        }
+      }
+      umma_commit(su32(&ctl->drain));   // every MMA issued has completed before TMEM is freed
+      chunk_drain(su32(&ctl->drain), 0);
+    }
+    __syncwarp();
+  } else if ((warp >> 2) < nq) {
+    // ---------------------------------------------------------------------------- softmax
+    const int i = warp >> 2;
+    const int r = 128 * i + (threadIdx.x & 127);   // row of the block
+    const bool mine = r < w.rows;
+    const int row = w.r0 + (mine ? r : 0), tok = row / a.G;
+    const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+    const uint32_t o_col = tmem + lanes + S::O0 + i * DP;
+    const int klo = mine ? row_lo(a, w, tok) : 0, khi = mine ? min(row_hi(a, w, tok), s1) : s1;
+    const int all_lo = __reduce_max_sync(0xffffffffu, klo), all_hi = __reduce_min_sync(0xffffffffu, khi);
+    const float scale = fabsf(a.scale_log2);
+    const int32_t* table = a.kv.table + b * a.kv.table_stride;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < tiles; ++j) {
+      const int k0 = s0 + 128 * j, buf = NQ == 2 ? i : j & 1;
+      // 16-key groups whose page exists (or that lie past the keys, where khi masks)
+      bool there = true;
+      if (lane < 8 && k0 + 16 * lane < s1) {
+        const int page = table[(k0 + 16 * lane) >> a.kv.page_log2];
+        there = page >= 0 && page < a.kv.pages;
+      }
+      const uint32_t missing = __ballot_sync(0xffffffffu, !there);
+      ok = __all_sync(0xffffffffu, chunk_wait(su32(&ctl->s_full[buf]), (NQ == 2 ? j : j >> 1) & 1, ctl));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t s_col = tmem + lanes + 128 * buf;
+      float s[128];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(s_col + 32 * c, s + 32 * c);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_wait_ld(s + 32 * c);
+      if (k0 < all_lo || k0 + 128 > all_hi || missing) {
+#pragma unroll
+        for (int k = 0; k < 128; ++k)
+          if (k0 + k < klo || k0 + k >= khi || ((missing >> (k >> 4)) & 1)) s[k] = -INFINITY;
+      }
+      float top[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) top[c] = s[c];
+#pragma unroll
+      for (int k = 4; k < 128; ++k) top[k & 3] = fmaxf(top[k & 3], s[k]);
+      const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+      if (__any_sync(0xffffffffu, mx > m + 8.f)) {
+        const float mn = fmaxf(m, mx), by = mn == -INFINITY ? 1.f : ex2(m - mn);
+        m = mn;
+        l *= by;
+        if (j > 0) {
+          // scores of tile j follow the product of tile j - 1 (two row tiles) or j - 2 (one)
+          if (NQ == 1) {
+            ok = __all_sync(0xffffffffu, chunk_wait(su32(&ctl->pv), (j - 1) & 1, ctl));
+            if (!ok) break;
+            tc_fence_after();
+          }
+#pragma unroll 1
+          for (int c = 0; c < DP; c += 32) {
+            float o[32];
+            tmem_ld32(o_col + c, o);
+            tmem_wait_ld(o);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] *= by;
+            tmem_st32(o_col + c, reinterpret_cast<const uint32_t*>(o));
+          }
+        }
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t p[32];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          const float x = ex2(fmaf(s[64 * c + 2 * k], scale, -base)), y = ex2(fmaf(s[64 * c + 2 * k + 1], scale, -base));
+          sum[(2 * k) & 3] += x;
+          sum[(2 * k + 1) & 3] += y;
+          p[k] = pack2<T>(x, y);
+        }
+        tmem_st32(s_col + 32 * c, p);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(su32(&ctl->p_full[buf]));
+    }
+    // ---- the rows' output, or their share of it
+    if (ok && tiles > 0) ok = __all_sync(0xffffffffu, chunk_wait(su32(&ctl->o_full[i]), 0, ctl));
+    if (ok) {
+      tc_fence_after();
+      const int64_t at = (int64_t)(w.first + tok) * a.hq + h * a.G + row % a.G;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+      for (int c = 0; c < DP; c += 32) {
+        float o[32];
+        if (tiles > 0) {
+          __syncwarp();
+          tmem_ld32(o_col + c, o);
+          tmem_wait_ld(o);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] = 0.f;
+        }
+        if (!mine) continue;
+        if (alone) {
+#pragma unroll
+          for (int k = 0; k < 32; k += 8) {
+            if (c + k >= a.D) break;
+            const uint4 y = make_uint4(pack2<T>(o[k] * inv, o[k + 1] * inv), pack2<T>(o[k + 2] * inv, o[k + 3] * inv),
+                                       pack2<T>(o[k + 4] * inv, o[k + 5] * inv), pack2<T>(o[k + 6] * inv, o[k + 7] * inv));
+            *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at * a.D + c + k) = y;
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; k += 4) {
+            if (c + k >= a.D) break;
+            *reinterpret_cast<float4*>(a.part_o + (at * a.splits + split) * a.D + c + k) =
+                make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+          }
+        }
+      }
+      if (mine) {
+        if (!alone) a.part_ml[at * a.splits + split] = make_float2(m, l);
+        else if (a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMma) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+// A pool [rows, D] (every page's every head) as copies of `box` rows x 64 values, 128-byte swizzle;
+// values past D and rows past the pool read as zeros.
+bool make_pool_map(CUtensorMap* map, const void* base, int64_t rows, int D, int box, bool bf16) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(D) * 2};
+  const cuuint32_t boxes[2] = {64, static_cast<cuuint32_t>(box)};
+  const cuuint32_t es[2] = {1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims,
+            strides, boxes, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DP, typename T>
+int launch(const AttnArgs& a, cudaStream_t st) {
+  using S = ChunkShape<DP>;
+  auto kern = attn_chunk_kernel<DP, T>;
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (!(done.load() & bit)) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::Smem);
+    if (e != cudaSuccess) {
+      set_last_cuda_error(e);
+      return VQ2_ERR_LAUNCH;
+    }
+    done.fetch_or(bit);
+  }
+  const int page = 1 << a.kv.page_log2;
+  const int64_t rows = ((int64_t)a.kv.pages * a.kv.heads) << a.kv.page_log2;
+  CUtensorMap kmap, vmap;
+  if (!make_pool_map(&kmap, a.kv.k, rows, a.D, page < 128 ? page : 128, a.q_bf16) ||
+      !make_pool_map(&vmap, a.kv.v, rows, a.D, page < S::KB ? page : S::KB, a.q_bf16))
+    return VQ2_ERR_LAUNCH;
+  const dim3 grid((unsigned)(a.kv.seqs * a.row_blocks), (unsigned)a.splits, (unsigned)a.kv.heads);
+  return launch_kernel(kern, grid, dim3(S::Threads), S::Smem, st, a, kmap, vmap);
+}
+
+template <typename T>
+int launch_shape(const AttnArgs& a, cudaStream_t st) {
+  return a.D > 128 ? launch<256, T>(a, st) : a.D > 64 ? launch<128, T>(a, st) : launch<64, T>(a, st);
+}
+
+}  // namespace
+
+void plan_attn_chunk(AttnArgs& a, int64_t max_new, int64_t max_len) {
+  const int64_t rows = max_new * a.G;
+  a.rows_per_block = a.D > 128 ? 128 : 256;
+  a.row_blocks = (int)((rows + a.rows_per_block - 1) / a.rows_per_block);
+  if (a.row_blocks < 1) a.row_blocks = 1;
+  a.lo_mask = ~127;
+  // One block an SM. Where the blocks are fewer than two an SM, split the keys so that there are
+  // about two: a split is at least 512 keys (its start, output and joining cost about as much as 256).
+  int64_t keys = max_len;
+  if (a.window && a.window + max_new + 128 < keys) keys = a.window + max_new + 128;
+  const int64_t blocks = (int64_t)a.kv.seqs * a.kv.heads * a.row_blocks;
+  const int64_t want = blocks >= 2 * sm_count() ? 1 : 2 * sm_count() / blocks;
+  int64_t chunk = (keys + 127 + want - 1) / want;
+  if (chunk < (keys + 127 + 63) / 64) chunk = (keys + 127 + 63) / 64;
+  if (chunk < 512) chunk = 512;
+  chunk = (chunk + 127) & ~int64_t(127);
+  a.chunk = (int)chunk;
+  a.splits = (int)((keys + 127 + chunk - 1) / chunk);   // the first key is rounded down by up to 127
+  if (a.splits < 1) a.splits = 1;
+}
+
+int launch_attn_chunk(const AttnArgs& a, cudaStream_t st) {
+  if (!encode_fn()) return VQ2_ERR_LAUNCH;
+  return a.q_bf16 ? launch_shape<__nv_bfloat16>(a, st) : launch_shape<__half>(a, st);
+}
+
+}  // namespace vq2
+
+extern "C" int vq2_attention_status(int reset) {
+  int32_t v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, g_attention_status, sizeof(v));
+  if (e == cudaSuccess && reset) {
+    const int32_t z = 0;
+    e = cudaMemcpyToSymbol(g_attention_status, &z, sizeof(z));
+  }
+  if (e != cudaSuccess) {
+    vq2::set_last_cuda_error(e);
+    return VQ2_ERR_LAUNCH;
+  }
+  return v;
+}

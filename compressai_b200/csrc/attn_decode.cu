@@ -576,6 +576,7 @@ void plan_attn_decode(AttnArgs& a, int64_t max_new, int64_t max_len) {
   a.rows_per_block = 8 * nt;
   a.row_blocks = (int)((rows + 8 * nt - 1) / (8 * nt));
   if (a.row_blocks < 1) a.row_blocks = 1;
+  a.lo_mask = ~15;
   // Split the keys until there are four rounds of blocks (two an SM): ragged lengths then even out.
   // A split is at least 64 keys (a warp's latency to start is about what 64 keys take) and there
   // are at most 64 of them.

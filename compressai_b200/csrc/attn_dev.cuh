@@ -16,8 +16,8 @@ struct AttnArgs {
   void* out;            // [T, hq, D]
   float* lse;           // [T, hq] or null
   // Split s of a block of rows takes the keys lo + s * chunk .. lo + (s + 1) * chunk - 1 of the keys
-  // [lo, hi) that the block sees, lo rounded down to 16. rows_per_block: query rows a block takes.
-  int chunk, splits, rows_per_block, row_blocks;
+  // [lo, hi) that the block sees, lo rounded down by lo_mask. rows_per_block: query rows a block takes.
+  int chunk, splits, rows_per_block, row_blocks, lo_mask;
   float* part_o;        // [T * hq, splits, D]: weighted sums of V relative to the maximum
   float2* part_ml;      // [T * hq, splits]: (maximum score in powers of two, sum of weights)
 };
@@ -56,18 +56,20 @@ __device__ __forceinline__ int row_hi(const AttnArgs& a, const AttnRows& w, int 
   return a.causal ? max(0, min(w.len, w.len - w.count + i + 1)) : w.len;
 }
 
-// Keys that any row of the block sees, the start rounded down to 16; no more than the splits cover.
+// Keys that any row of the block sees, the start rounded down; no more than the splits cover.
 __device__ __forceinline__ void block_keys(const AttnArgs& a, const AttnRows& w, int& lo, int& hi) {
-  lo = row_lo(a, w, w.r0 / a.G) & ~15;
+  lo = row_lo(a, w, w.r0 / a.G) & a.lo_mask;
   hi = w.rows > 0 ? row_hi(a, w, (w.r0 + w.rows - 1) / a.G) : 0;
   hi = (int)min((int64_t)hi, lo + (int64_t)a.splits * a.chunk);
 }
 
 // Joins the splits of every row (launched after a kernel that left more than one).
 int launch_attn_join(const AttnArgs& a, cudaStream_t st);
-// One token to a few rows per key/value head: see attn_decode.cu.
+// Few rows per key/value head (attn_decode.cu), and many (attn_chunk.cu, 16-bit caches). The plans set
+// chunk, splits, rows_per_block, row_blocks and lo_mask.
 int launch_attn_decode(const AttnArgs& a, bool i8, cudaStream_t st);
-// Sets chunk, splits, rows_per_block and row_blocks.
 void plan_attn_decode(AttnArgs& a, int64_t max_new, int64_t max_len);
+int launch_attn_chunk(const AttnArgs& a, cudaStream_t st);
+void plan_attn_chunk(AttnArgs& a, int64_t max_new, int64_t max_len);
 
 }  // namespace vq2

@@ -38,15 +38,13 @@
 //
 // Semantics: the batched form of reference vq2/kernels.py:32-78 (whose Triton path serves
 // M = 1 only; vq2/runtime.py:105-110 dequantizes and calls F.linear for M > 1).
-#include <cuda.h>  // CUtensorMap and its enums (the encoder is fetched from the driver at run time)
-
 #include <atomic>
 #include <cstdlib>
 #include <cstring>
-#include <mutex>
 #include <type_traits>
 
 #include "gemv_dev.cuh"
+#include "tcgen05.cuh"
 
 // Sticky status of the tcgen05 GEMV: VQ2_ERR_TIMEOUT once any bounded wait gave up.
 __device__ int32_t g_umma_status;
@@ -61,120 +59,6 @@ constexpr int kUmEpiWarp0 = 9;             // warps 9..12: epilogue
 constexpr int kUmThreads = 13 * 32;
 static_assert(kUmEpiWarp0 == kUmMmaWarp + 1 && kUmThreads == (kUmEpiWarp0 + 4) * 32, "warp roles");
 constexpr long long kUmWaitCycles = 4000000000LL;  // ~2 s at 1.965 GHz
-
-// ---- PTX wrappers ------------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t su32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// Generic-proxy writes to shared memory become visible to the async proxy (tensor core, TMA).
-__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
-      : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// Shared-memory matrix descriptor of a K-major operand tile in the 128-byte swizzle layout: rows
-// of 128 bytes, 8-row groups 1024 bytes apart (SBO), tile base 1024-byte aligned. Bits: start
-// address >> 4 [0,14), leading byte offset >> 4 [16,30) (unused by this layout: 1), stride byte
-// offset >> 4 [32,46), descriptor version 1 [46,48), layout 2 = 128-byte swizzle [61,64).
-// Advancing K by 16 elements (32 bytes) inside the swizzle row adds 2 to the address field.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
-  return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(1) << 16) |
-         (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) |
-         (static_cast<uint64_t>(2) << 61);
-}
-
-// Instruction descriptor of kind::f16: D fp32 [4,6) = 1, A / B type [7,10) / [10,13) (0 fp16,
-// 1 bf16), both K-major (bits 15, 16 = 0), N >> 3 at [17,23), M >> 4 at [24,29).
-template <int N, bool BF16>
-constexpr uint32_t umma_idesc() {
-  return (1u << 4) | ((BF16 ? 1u : 0u) << 7) | ((BF16 ? 1u : 0u) << 10) | (static_cast<uint32_t>(N >> 3) << 17) |
-         (static_cast<uint32_t>(kUmRows >> 4) << 24);
-}
-
-__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                         uint32_t accumulate) {
-  const uint32_t z = 0;  // no output lanes disabled
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
-      ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(z)
-      : "memory");
-}
-// The same MMA with the A operand read from tensor memory (lane = row, 16-bit K values packed two
-// per 32-bit column, K = 16 per instruction = 8 columns).
-__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
-                                            uint32_t accumulate) {
-  const uint32_t z = 0;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}"
-      ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(z)
-      : "memory");
-}
-
-// This thread's 32 consecutive 32-bit TMEM columns of its lane (32x32b shape; warp-collective),
-// waited for before returning.
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint4 (&v)[8]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n\t"
-      "tcgen05.wait::st.sync.aligned;"
-      ::"r"(taddr), "r"(v[0].x), "r"(v[0].y), "r"(v[0].z), "r"(v[0].w), "r"(v[1].x), "r"(v[1].y), "r"(v[1].z),
-        "r"(v[1].w), "r"(v[2].x), "r"(v[2].y), "r"(v[2].z), "r"(v[2].w), "r"(v[3].x), "r"(v[3].y), "r"(v[3].z),
-        "r"(v[3].w), "r"(v[4].x), "r"(v[4].y), "r"(v[4].z), "r"(v[4].w), "r"(v[5].x), "r"(v[5].y), "r"(v[5].z),
-        "r"(v[5].w), "r"(v[6].x), "r"(v[6].y), "r"(v[6].z), "r"(v[6].w), "r"(v[7].x), "r"(v[7].y), "r"(v[7].z),
-        "r"(v[7].w)
-      : "memory");
-}
-
-// Arrive on `bar` once every MMA this thread issued so far has completed.
-__device__ __forceinline__ void umma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-
-// 16 consecutive fp32 columns of this thread's TMEM lane (32x32b shape), waited for in the same
-// statement so no use of the registers can move ahead of the wait.
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
-  uint32_t r[16];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15}, [%16];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-}
 
 // Shared control block: per stage, the producers' arrivals (4 warps), the TMA copy (one arrival
 // + transaction bytes) and the MMA's release; per accumulator, "MMAs done" and "epilogue done".
@@ -501,24 +385,6 @@ __global__ void __launch_bounds__(kUmThreads, 1) vq_umma_kernel(const GemvArgs a
 }
 
 // ---- host side ---------------------------------------------------------------------------------
-// cuTensorMapEncodeTiled, fetched once from the driver (the library links only the CUDA runtime).
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  });
-  return fn;
-}
-
 // [rows, n] 16-bit row-major operand at `base`, boxes of NT rows x 64 elements, 128-byte swizzle
 // (the UMMA K-major layout); rows past `rows` read as zeros.
 bool make_operand_map(CUtensorMap* map, const void* base, int64_t rows, int64_t n, int NT, bool bf16) {

@@ -664,8 +664,8 @@ VQ2_API int vq2_cache_read(const void* k_pages, const void* v_pages, int kv_dtyp
  * strides multiples of 8. workspace: vq2_paged_attention_workspace(...) bytes, 16-byte aligned.
  */
 VQ2_API int64_t vq2_paged_attention_workspace(int64_t tokens, int64_t q_heads, int64_t kv_heads,
-                                              int64_t head_size, int64_t seqs, int64_t max_new,
-                                              int64_t max_len, int causal, int64_t window);
+                                              int64_t head_size, int kv_dtype, int64_t seqs,
+                                              int64_t max_new, int64_t max_len, int64_t window);
 VQ2_API int vq2_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype,
                                 int64_t tokens, int64_t q_heads, const void* k_pages, const void* v_pages,
                                 int kv_dtype, const float* k_scale, const float* v_scale, int64_t pages,
@@ -674,6 +674,9 @@ VQ2_API int vq2_paged_attention(const void* q, int64_t q_token_stride, int64_t q
                                 const int32_t* lens, const int32_t* starts, int64_t seqs, int64_t max_new,
                                 int64_t max_len, float scale, int causal, int64_t window, void* out,
                                 float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+/* Sticky status word of vq2_paged_attention's tensor-core kernel: VQ2_ERR_TIMEOUT once a bounded
+ * on-chip wait gave up (its output is then not valid); cleared when reset is non-zero. Synchronises. */
+VQ2_API int vq2_attention_status(int reset);
 
 #ifdef __cplusplus
 }
