@@ -576,9 +576,7 @@ int launch_attn_chunk(const AttnArgs& a, cudaStream_t st) {
   return a.q_bf16 ? launch_shape<__nv_bfloat16>(a, st) : launch_shape<__half>(a, st);
 }
 
-}  // namespace vq2
-
-extern "C" int vq2_attention_status(int reset) {
+int attn_chunk_status(int reset) {
   int32_t v = 0;
   cudaError_t e = cudaMemcpyFromSymbol(&v, g_attention_status, sizeof(v));
   if (e == cudaSuccess && reset) {
@@ -586,8 +584,10 @@ extern "C" int vq2_attention_status(int reset) {
     e = cudaMemcpyToSymbol(g_attention_status, &z, sizeof(z));
   }
   if (e != cudaSuccess) {
-    vq2::set_last_cuda_error(e);
+    set_last_cuda_error(e);
     return VQ2_ERR_LAUNCH;
   }
   return v;
 }
+
+}  // namespace vq2

@@ -71,5 +71,6 @@ int launch_attn_decode(const AttnArgs& a, bool i8, cudaStream_t st);
 void plan_attn_decode(AttnArgs& a, int64_t max_new, int64_t max_len);
 int launch_attn_chunk(const AttnArgs& a, cudaStream_t st);
 void plan_attn_chunk(AttnArgs& a, int64_t max_new, int64_t max_len);
+int attn_chunk_status(int reset);   // its part of vq2_attention_status
 
 }  // namespace vq2

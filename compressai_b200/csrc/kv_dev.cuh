@@ -32,7 +32,7 @@ inline int paged_kv(PagedKV& kv, const void* k, const void* v, int kv_dtype, con
     return VQ2_ERR_SHAPE;
   if (pages > 0x7fffffff / page_size || pages * page_size > 0x7fffffff / heads || cols > 0x7fffffff / page_size)
     return VQ2_ERR_SHAPE;  // a pool's rows and a sequence's positions are counted in 32 bits
-  if (!aligned(k, 16) || !aligned(v, 16)) return VQ2_ERR_ALIGN;
+  if (!aligned(k, 16) || !aligned(v, 16) || !aligned(k_scale, 16) || !aligned(v_scale, 16)) return VQ2_ERR_ALIGN;
   int l = 4;
   while ((1 << l) < page_size) ++l;
   kv = {k, v, k_scale, v_scale, table, lens, starts, table_stride, (int32_t)pages, (int32_t)heads, l, (int32_t)cols,
