@@ -9,9 +9,11 @@
 //   * one warp brings keys and values by TMA, straight from their pages: 16 KB blocks in a ring, a
 //     K block being 128 keys x 64 values, a V block 8192 / DP keys x all values, 128-byte swizzle;
 //   * one thread issues the MMAs: S from shared memory, O with P as the operand in tensor memory
-//     (P overwrites its S) and V with its values contiguous (the descriptor's transposed form);
-//   * a warpgroup per 128 rows does the softmax, a row per thread: no shuffles. Maxima, sums and O
-//     are 32 bits; P is rounded to the cache's 16 bits for the second product.
+//     (P overwrites its S, each softmax thread's within its own columns) and V with its values contiguous (the descriptor's transposed form);
+//   * 16 warps do the softmax, 2 or 4 threads a row: with one thread a row (a warp a scheduler and
+//     row tile) the chain of its 128 maxima and exponentials set the pace: 3 us a step where the
+//     MMAs take 1.1. The threads of a row agree through one named barrier whether any score asks
+//     for a new maximum. Maxima, sums and O are 32 bits; P is rounded to the cache's 16 bits.
 // With two row tiles the tensor core works on one while the softmax works on the other; with one
 // (head size 256, O takes half of tensor memory) S is double-buffered and QK of the next tile runs
 // under the softmax.
@@ -51,9 +53,12 @@ struct ChunkShape {
   static constexpr int B = DP / 64;                  // ring blocks of a 128-key tile, K or V
   static constexpr int KB = 8192 / DP;               // keys of a V block
   static constexpr int Q = NQ * 128 * DP * 2;
-  static constexpr int NB = (232448 - 2048 - Q) / kBlock;   // ring blocks: 10, or 12 at head size 64
-  static constexpr int Smem = 1024 + Q + NB * kBlock + 512;
-  static constexpr int Threads = (4 * NQ + 2) * 32;
+  static constexpr int NB = DP == 64 ? 12 : 10;      // ring blocks
+  static constexpr int Smem = Q + NB * kBlock + 512 + 2048;
+  static_assert(Smem <= 232448, "shared memory");
+  static constexpr int TPR = 4 / NQ;                 // threads of a row in the softmax
+  static constexpr int W = 128 / TPR;                // keys of a tile that one of them takes
+  static constexpr int Threads = 18 * 32;
   static constexpr uint32_t O0 = 256;                // first TMEM column of O; S buffers at 0 and 128
 };
 
@@ -102,6 +107,42 @@ __device__ __forceinline__ uint64_t v_desc(uint32_t saddr) {
          (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
 }
 
+// Barrier `id` of n threads (whole warps): whether any of them says p.
+__device__ __forceinline__ bool any_of(int id, int n, bool p) {
+  int r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %3, 0;\n\t"
+      "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
+      "selp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(n), "r"(static_cast<int>(p))
+      : "memory");
+  return r != 0;
+}
+
+// Two sums or products at once.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // 32 columns of this thread's lane, not yet waited for; tmem_wait passes the registers through the
 // wait so that no use of them can be moved ahead of it.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
@@ -136,6 +177,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
         "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+        "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 template <typename T>
@@ -154,14 +202,18 @@ __global__ void __launch_bounds__(ChunkShape<DP>::Threads, 1)
   using S = ChunkShape<DP>;
   constexpr int NQ = S::NQ, B = S::B, KB = S::KB, NB = S::NB;
   constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
-  extern __shared__ unsigned char chunk_raw[];
-  unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(chunk_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) unsigned char sm[];
   unsigned char* ring = sm + S::Q;
   ChunkCtl* ctl = reinterpret_cast<ChunkCtl*>(ring + NB * kBlock);
+  float* part_s = reinterpret_cast<float*>(ring + NB * kBlock + 512);   // a word of each softmax thread
   pdl_wait();
   pdl_trigger();
+  if (su32(sm) & 1023) {   // the swizzle needs it; the only shared memory here, so it starts a 1024-byte line
+    if (threadIdx.x == 0) atomicMax(&g_attention_status, VQ2_ERR_ALIGN);
+    return;
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kMma = 4 * NQ, kTma = 4 * NQ + 1;
+  constexpr int kMma = 16, kTma = 17, TPR = S::TPR, W = S::W;
   // the last rows see the most keys: they go first
   const int b = blockIdx.x / a.row_blocks, rb = a.row_blocks - 1 - (blockIdx.x - b * a.row_blocks);
   const int split = blockIdx.y, h = blockIdx.z;
@@ -182,7 +234,7 @@ __global__ void __launch_bounds__(ChunkShape<DP>::Threads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(su32(&ctl->s_full[i]), 1);
-      mbar_init(su32(&ctl->p_full[i]), 4);
+      mbar_init(su32(&ctl->p_full[i]), 4 * S::TPR);
       mbar_init(su32(&ctl->o_full[i]), 1);
     }
     mbar_init(su32(&ctl->pv), 1);
@@ -213,10 +265,6 @@ __global__ void __launch_bounds__(ChunkShape<DP>::Threads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = ctl->tmem_base;
-  // Ring order of the 128-key tiles' operands, in blocks: K0 V0 K1 V1 .. with two row tiles, K0 K1 V0
-  // K2 V1 .. with one, as the MMAs take them.
-  auto k_block = [&](int j) { return NQ == 2 ? 2 * j * B : j == 0 ? 0 : (2 * j - 1) * B; };
-  auto v_block = [&](int j) { return NQ == 2 || j == tiles - 1 ? (2 * j + 1) * B : (2 * j + 2) * B; };
   const int gran = min(1 << a.kv.page_log2, KB);   // keys of one V copy
   const int tail = (s1 & (gran - 1)) ? s1 : -1;    // rows from here on, up to the copy's end, hold anything
 
@@ -299,131 +347,173 @@ __global__ void __launch_bounds__(ChunkShape<DP>::Threads, 1)
       for (int i = max(0, q - NB); i < q; ++i) chunk_drain(su32(&ctl->full[i % NB]), (i / NB) & 1);
   } else if (warp == kMma) {
     // ---------------------------------------------------------------------------- MMA issuer
-    if (lane == 0) {
+    // One elected thread. elect.sync rather than a lane number: the compiler then knows a single thread
+    // runs and keeps descriptors in uniform registers; behind `lane == 0` each MMA was issued in about
+    // 140 cycles, twice what it takes to execute.
+    if (elect_one()) {
       constexpr uint32_t QK = umma_idesc<128, BF>(), PV = umma_idesc<DP, BF>(true);
+      const uint64_t qd = sw128_desc(su32(sm)), kd = sw128_desc(su32(ring)), vd = v_desc<KB>(su32(ring));
+      const uint32_t full0 = su32(&ctl->full[0]), empty0 = su32(&ctl->empty[0]);
       bool ok = true;
-      // scores of row tile i with key tile j into buffer s
-      auto qk = [&](int i, int j, int s) {
-        const int q0 = k_block(j);
-#pragma unroll 1
-        for (int c = 0; c < B && ok; ++c) {
-          const int slot = (q0 + c) % NB;
+      int ks = 0, vs = 0, kp = 0, vp = 0;   // slot and parity of the next K and V tile's first block
+      auto skip = [&](int& slot, int& parity, int n) {
+        slot += n;
+        if (slot >= NB) {
+          slot -= NB;
+          parity ^= 1;
+        }
+      };
+      // scores of row tile i with the next key tile into buffer s
+      auto qk = [&](int i, int s) {
+        int slot = ks, parity = kp;
+#pragma unroll
+        for (int c = 0; c < B; ++c) {
           if (i == 0) {
-            ok = chunk_wait(su32(&ctl->full[slot]), ((q0 + c) / NB) & 1, ctl);
-            if (!ok) return;
+            if (!chunk_wait(full0 + 8 * slot, parity, ctl)) return false;
             tc_fence_after();
           }
-          const uint64_t ad = sw128_desc(su32(sm + (i * B + c) * kBlock)), bd = sw128_desc(su32(ring + slot * kBlock));
+          const uint64_t ad = qd + (i * B + c) * (kBlock >> 4), bd = kd + slot * (kBlock >> 4);
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) umma_f16(tmem + 128 * s, ad + 2 * kk, bd + 2 * kk, QK, (c | kk) != 0);
-          if (i == nq - 1) umma_commit(su32(&ctl->empty[slot]));
+          if (i == nq - 1) umma_commit(empty0 + 8 * slot);
+          skip(slot, parity, 1);
         }
         umma_commit(su32(&ctl->s_full[s]));
+        return true;
       };
       // O of row tile i += weights in buffer s times V tile j
       auto pv = [&](int i, int j, int s) {
-        const int q0 = v_block(j);
-#pragma unroll 1
-        for (int c = 0; c < B && ok; ++c) {
-          const int slot = (q0 + c) % NB;
+        int slot = vs, parity = vp;
+#pragma unroll
+        for (int c = 0; c < B; ++c) {
           if (i == 0) {
-            ok = chunk_wait(su32(&ctl->full[slot]), ((q0 + c) / NB) & 1, ctl);
             const int kb = s0 + 128 * j + c * KB;
-            if (ok && tail > kb && tail < kb + KB) ok = chunk_wait(su32(&ctl->tail), 0, ctl);
-            if (!ok) return;
+            if (!chunk_wait(full0 + 8 * slot, parity, ctl)) return false;
+            if (tail > kb && tail < kb + KB && !chunk_wait(su32(&ctl->tail), 0, ctl)) return false;
             tc_fence_after();
           }
-          const uint64_t bd = v_desc<KB>(su32(ring + slot * kBlock));
-          const uint32_t p = tmem + 128 * s + c * (KB / 2);
+          const uint64_t bd = vd + slot * (kBlock >> 4);
 #pragma unroll
-          for (int kk = 0; kk < KB / 16; ++kk)
-            umma_f16_ts(tmem + S::O0 + i * DP, p + 8 * kk, bd + 128 * kk, PV, (j | c | kk) != 0);
-          if (i == nq - 1) umma_commit(su32(&ctl->empty[slot]));
+          for (int kk = 0; kk < KB / 16; ++kk) {
+            const int key = c * KB + 16 * kk;   // of the tile: its weights stand in the columns of its part's scores
+            umma_f16_ts(tmem + S::O0 + i * DP, tmem + 128 * s + key / S::W * S::W + key % S::W / 2, bd + 128 * kk, PV,
+                        (c | kk) != 0 || j > 0);
+          }
+          if (i == nq - 1) umma_commit(empty0 + 8 * slot);
+          skip(slot, parity, 1);
         }
         if (NQ == 1) umma_commit(su32(&ctl->pv));
         if (j == tiles - 1) umma_commit(su32(&ctl->o_full[i]));
+        return true;
       };
+      // ring order K0 V0 K1 V1 .. with two row tiles, K0 K1 V0 K2 V1 .. with one
       if (NQ == 2) {
         if (tiles > 0)
-          for (int i = 0; i < nq && ok; ++i) qk(i, 0, i);
-        for (int j = 0; j < tiles && ok; ++j)
+          for (int i = 0; i < nq && ok; ++i) ok = qk(i, i);
+        skip(vs, vp, B);
+        skip(ks, kp, 2 * B);
+        for (int j = 0; j < tiles && ok; ++j) {
           for (int i = 0; i < nq && ok; ++i) {
             ok = chunk_wait(su32(&ctl->p_full[i]), j & 1, ctl);
             if (!ok) break;
             tc_fence_after();
-            pv(i, j, i);
-            if (j + 1 < tiles && ok) qk(i, j + 1, i);
+            ok = pv(i, j, i) && (j + 1 == tiles || qk(i, i));
           }
+          skip(vs, vp, 2 * B);
+          skip(ks, kp, 2 * B);
+        }
       } else {
-        if (tiles > 0) qk(0, 0, 0);
+        if (tiles > 0) ok = qk(0, 0);
+        skip(ks, kp, B);
+        skip(vs, vp, tiles > 1 ? 2 * B : B);
         for (int j = 0; j < tiles && ok; ++j) {
-          if (j + 1 < tiles) qk(0, j + 1, (j + 1) & 1);
-          if (ok) ok = chunk_wait(su32(&ctl->p_full[j & 1]), (j >> 1) & 1, ctl);
+          if (j + 1 < tiles) ok = qk(0, (j + 1) & 1);
+          skip(ks, kp, 2 * B);
+          ok = ok && chunk_wait(su32(&ctl->p_full[j & 1]), (j >> 1) & 1, ctl);
           if (!ok) break;
           tc_fence_after();
-          pv(0, j, j & 1);
+          ok = pv(0, j, j & 1);
+          skip(vs, vp, j + 2 == tiles ? B : 2 * B);   // the last V follows the one before it
         }
       }
       umma_commit(su32(&ctl->drain));   // every MMA issued has completed before TMEM is freed
       chunk_drain(su32(&ctl->drain), 0);
     }
     __syncwarp();
-  } else if ((warp >> 2) < nq) {
+  } else if (warp / (4 * TPR) < nq) {
     // ---------------------------------------------------------------------------- softmax
-    const int i = warp >> 2;
-    const int r = 128 * i + (threadIdx.x & 127);   // row of the block
+    const int i = warp / (4 * TPR), part = (warp >> 2) % TPR, quarter = warp & 3;
+    const int r = 128 * i + 32 * quarter + lane;   // row of the block
     const bool mine = r < w.rows;
     const int row = w.r0 + (mine ? r : 0), tok = row / a.G;
-    const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+    const uint32_t lanes = static_cast<uint32_t>(32 * quarter) << 16;
     const uint32_t o_col = tmem + lanes + S::O0 + i * DP;
+    const int bar = 1 + 4 * i + quarter;           // of the warps that share these rows
     const int klo = mine ? row_lo(a, w, tok) : 0, khi = mine ? min(row_hi(a, w, tok), s1) : s1;
     const int all_lo = __reduce_max_sync(0xffffffffu, klo), all_hi = __reduce_min_sync(0xffffffffu, khi);
     const float scale = fabsf(a.scale_log2);
     const int32_t* table = a.kv.table + b * a.kv.table_stride;
-    float m = -INFINITY, l = 0.f;
+    // what the threads of this row leave for one another
+    float* said = part_s + (warp - 4 * part) * 32 + lane;   // part p: said[128 * p]
+    float m = -INFINITY;
+    uint64_t l2 = pair(0.f, 0.f), l3 = l2;
+    float l = 0.f;
     bool ok = true;
     for (int j = 0; j < tiles; ++j) {
-      const int k0 = s0 + 128 * j, buf = NQ == 2 ? i : j & 1;
-      // 16-key groups whose page exists (or that lie past the keys, where khi masks)
+      const int k0 = s0 + 128 * j + W * part, buf = NQ == 2 ? i : j & 1;   // this thread's first key
+      // 16-key groups whose page does not exist (past the keys khi masks)
       bool there = true;
-      if (lane < 8 && k0 + 16 * lane < s1) {
+      if (lane < W / 16 && k0 + 16 * lane < s1) {
         const int page = table[(k0 + 16 * lane) >> a.kv.page_log2];
         there = page >= 0 && page < a.kv.pages;
       }
       const uint32_t missing = __ballot_sync(0xffffffffu, !there);
       ok = __all_sync(0xffffffffu, chunk_wait(su32(&ctl->s_full[buf]), (NQ == 2 ? j : j >> 1) & 1, ctl));
-      if (!ok) break;
       tc_fence_after();
       const uint32_t s_col = tmem + lanes + 128 * buf;
-      float s[128];
+      // The scores are read twice, 32 at a time, rather than held: 64 of them do not fit beside the
+      // weights in 96 registers, and the spills set the pace (D 128: 591 us where one thread a row
+      // took 410 on the three chunks).
+      const uint32_t own = s_col + W * part;
+      const bool masked = k0 < all_lo || k0 + W > all_hi || missing;
+      auto mask = [&](float* s, int c) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(s_col + 32 * c, s + 32 * c);
+        for (int k = 0; k < 32; ++k)
+          if (k0 + c + k < klo || k0 + c + k >= khi || ((missing >> ((c + k) >> 4)) & 1)) s[k] = -INFINITY;
+      };
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_wait_ld(s + 32 * c);
-      if (k0 < all_lo || k0 + 128 > all_hi || missing) {
+      for (int c = 0; c < W; c += 32) {
+        float s[32];
+        tmem_ld32(own + c, s);
+        tmem_wait_ld(s);
+        if (masked) mask(s, c);
 #pragma unroll
-        for (int k = 0; k < 128; ++k)
-          if (k0 + k < klo || k0 + k >= khi || ((missing >> (k >> 4)) & 1)) s[k] = -INFINITY;
+        for (int k = 0; k < 32; k += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], fmaxf(s[k + e], s[k + e + 4]));
       }
-      float top[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) top[c] = s[c];
-#pragma unroll
-      for (int k = 4; k < 128; ++k) top[k & 3] = fmaxf(top[k & 3], s[k]);
       const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
-      if (__any_sync(0xffffffffu, mx > m + 8.f)) {
-        const float mn = fmaxf(m, mx), by = mn == -INFINITY ? 1.f : ex2(m - mn);
+      // One that gave up waiting says so here, so that all leave together.
+      if (any_of(bar, 32 * TPR, mx > m + 8.f || !ok)) {
+        said[128 * part] = ok ? mx : NAN;
+        ok = !any_of(bar, 32 * TPR, !ok);
+        if (!ok) break;
+        float all = mx;
+#pragma unroll
+        for (int p = 0; p < TPR; ++p) all = fmaxf(all, said[128 * p]);
+        const float mn = fmaxf(m, all), by = mn == -INFINITY ? 1.f : ex2(m - mn);
         m = mn;
-        l *= by;
+        l2 = fma2(l2, pair(by, by), pair(0.f, 0.f));
+        l3 = fma2(l3, pair(by, by), pair(0.f, 0.f));
         if (j > 0) {
           // scores of tile j follow the product of tile j - 1 (two row tiles) or j - 2 (one)
           if (NQ == 1) {
             ok = __all_sync(0xffffffffu, chunk_wait(su32(&ctl->pv), (j - 1) & 1, ctl));
-            if (!ok) break;
             tc_fence_after();
           }
 #pragma unroll 1
-          for (int c = 0; c < DP; c += 32) {
+          for (int c = part * (DP / TPR); c < (part + 1) * (DP / TPR); c += 32) {
             float o[32];
             tmem_ld32(o_col + c, o);
             tmem_wait_ld(o);
@@ -432,35 +522,49 @@ __global__ void __launch_bounds__(ChunkShape<DP>::Threads, 1)
             tmem_st32(o_col + c, reinterpret_cast<const uint32_t*>(o));
           }
         }
+        any_of(bar, 32 * TPR, false);   // `said` has been read by all
       }
       const float base = m == -INFINITY ? 0.f : m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t scale2 = pair(scale, scale), base2 = pair(-base, -base);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t p[32];
+      for (int c = 0; c < W; c += 32) {
+        float s[32];
+        uint32_t p[16];
+        tmem_ld32(own + c, s);
+        tmem_wait_ld(s);
+        if (masked) mask(s, c);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) {
-          const float x = ex2(fmaf(s[64 * c + 2 * k], scale, -base)), y = ex2(fmaf(s[64 * c + 2 * k + 1], scale, -base));
-          sum[(2 * k) & 3] += x;
-          sum[(2 * k + 1) & 3] += y;
-          p[k] = pack2<T>(x, y);
+        for (int k = 0; k < 16; ++k) {
+          const float2 x = unpair(fma2(pair(s[2 * k], s[2 * k + 1]), scale2, base2));
+          const float y0 = ex2(x.x), y1 = ex2(x.y);
+          if (k & 1) l3 = add2(l3, pair(y0, y1));
+          else l2 = add2(l2, pair(y0, y1));
+          p[k] = pack2<T>(y0, y1);
         }
-        tmem_st32(s_col + 32 * c, p);
+        tmem_st16(own + c / 2, p);   // over scores that this thread has read
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(su32(&ctl->p_full[buf]));
     }
+    {
+      const float2 x = unpair(l2), y = unpair(l3);
+      l = (x.x + x.y) + (y.x + y.y);
+    }
     // ---- the rows' output, or their share of it
     if (ok && tiles > 0) ok = __all_sync(0xffffffffu, chunk_wait(su32(&ctl->o_full[i]), 0, ctl));
+    said[128 * part] = l;
+    ok = !any_of(bar, 32 * TPR, !ok);
     if (ok) {
       tc_fence_after();
+      l = 0.f;
+#pragma unroll
+      for (int p = 0; p < TPR; ++p) l += said[128 * p];
       const int64_t at = (int64_t)(w.first + tok) * a.hq + h * a.G + row % a.G;
       const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
-      for (int c = 0; c < DP; c += 32) {
+      for (int c = part * (DP / TPR); c < (part + 1) * (DP / TPR); c += 32) {
         float o[32];
         if (tiles > 0) {
           __syncwarp();
@@ -488,7 +592,7 @@ __global__ void __launch_bounds__(ChunkShape<DP>::Threads, 1)
           }
         }
       }
-      if (mine) {
+      if (mine && part == 0) {
         if (!alone) a.part_ml[at * a.splits + split] = make_float2(m, l);
         else if (a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
       }
