@@ -14,8 +14,8 @@ namespace {
 int64_t plan(AttnArgs& a, bool i8, int64_t max_new, int64_t max_len, bool& chunked) {
   // Rows that share a key: the decode kernel holds 16 (head size above 128) or 32 of them; from there
   // on it would read the keys again for every 16 or 32, and the tensor-core kernel takes over.
-  chunked = !i8 && max_new * a.G > (a.D > 128 ? 16 : 32);
-  if (chunked) plan_attn_chunk(a, max_new, max_len);
+  chunked = max_new * a.G > (a.D > 128 ? 16 : 32);
+  if (chunked) plan_attn_chunk(a, i8, max_new, max_len);
   else plan_attn_decode(a, max_new, max_len);
   if (a.splits == 1) return 0;
   return (int64_t)a.T * a.hq * a.splits * (a.D * 4 + 8);
@@ -89,7 +89,8 @@ extern "C" int vq2_paged_attention(const void* q, int64_t q_token_stride, int64_
   }
   if ((int64_t)a.kv.seqs * a.row_blocks > 0x7fffffff) return VQ2_ERR_SHAPE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  s = chunked ? launch_attn_chunk(a, st) : launch_attn_decode(a, kv_dtype == VQ2_I8, st);
+  const bool i8 = kv_dtype == VQ2_I8;
+  s = chunked ? launch_attn_chunk(a, i8, st) : launch_attn_decode(a, i8, st);
   if (s != VQ2_OK || a.splits == 1) return s;
   return launch_attn_join(a, st);
 }

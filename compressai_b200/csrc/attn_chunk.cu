@@ -9,7 +9,8 @@
 //   * one warp brings keys and values by TMA, straight from their pages: 16 KB blocks in a ring, a
 //     K block being 128 keys x 64 values, a V block 8192 / DP keys x all values, 128-byte swizzle;
 //   * one thread issues the MMAs: S from shared memory, O with P as the operand in tensor memory
-//     (P overwrites its S, each softmax thread's within its own columns) and V with its values contiguous (the descriptor's transposed form);
+//     (P overwrites its S, each softmax thread's within its own columns) and V with its values
+//     contiguous (the descriptor's transposed form);
 //   * 16 warps do the softmax, 2 or 4 threads a row: with one thread a row (a warp a scheduler and
 //     row tile) the chain of its 128 maxima and exponentials set the pace: 3 us a step where the
 //     MMAs take 1.1. The threads of a row agree through one named barrier whether any score asks
@@ -24,6 +25,11 @@
 //
 // Bound: at 2 * 128 * 128 * DP flops for 128 * 128 exponentials per product pair, the tensor core
 // and (head size 128) the 16 exponentials a clock an SM are about equally busy.
+//
+// 8-bit caches: seven warps take TMA's place. They load 16 values a piece, the next operand tile under
+// way in registers, and store exact fp16 (an int8 is; see attn_decode.cu, also for the scales: the key's
+// multiplies the score, the value's the weight, relative to a power of two) into the same ring. One row
+// tile and 8 softmax warps, for the conversion's warps need the registers.
 //
 // Rows of a page past the keys that the block sees may hold anything, NaN too: their scores are
 // replaced, and their V rows zeroed in shared memory by the loading warp before the MMA may read
@@ -47,18 +53,21 @@ namespace {
 constexpr long long kWaitCycles = 4000000000LL;  // ~2 s at 1.965 GHz
 constexpr int kBlock = 16384;                    // bytes of a ring block
 
-template <int DP>
+template <int DP, bool I8>
 struct ChunkShape {
-  static constexpr int NQ = DP > 128 ? 1 : 2;        // row tiles of 128
+  static constexpr int NQ = DP > 128 || I8 ? 1 : 2;  // row tiles of 128
   static constexpr int B = DP / 64;                  // ring blocks of a 128-key tile, K or V
   static constexpr int KB = 8192 / DP;               // keys of a V block
   static constexpr int Q = NQ * 128 * DP * 2;
-  static constexpr int NB = DP == 64 ? 12 : 10;      // ring blocks
-  static constexpr int Smem = Q + NB * kBlock + 512 + 2048;
-  static_assert(Smem <= 232448, "shared memory");
-  static constexpr int TPR = 4 / NQ;                 // threads of a row in the softmax
+  static constexpr int NB = I8 && DP == 256 ? 9 : DP == 64 && !I8 ? 12 : 10;   // ring blocks
+  static constexpr int TPR = I8 ? 2 : 4 / NQ;        // threads of a row in the softmax
   static constexpr int W = 128 / TPR;                // keys of a tile that one of them takes
-  static constexpr int Threads = 18 * 32;
+  static constexpr int Mma = 4 * NQ * TPR;           // warp that issues the MMAs; the softmax is before it
+  static constexpr int Load = I8 ? 7 : 1;            // warps after it: conversion, or TMA
+  static constexpr int Threads = (Mma + 1 + Load) * 32;
+  static constexpr int Scales = I8 ? 8 * 1024 + 512 : 0;   // K's and V's of 8 tiles; the rows' powers of two
+  static constexpr int Smem = Q + NB * kBlock + 512 + 2048 + Scales;
+  static_assert(Smem <= 232448, "shared memory");
   static constexpr uint32_t O0 = 256;                // first TMEM column of O; S buffers at 0 and 128
 };
 
@@ -69,6 +78,7 @@ struct ChunkCtl {
   uint64_t pv;                    // one row tile: each product into O (before a rescale)
   uint64_t tail;                  // V rows past the last key are zeroed
   uint64_t drain;
+  uint64_t scales[8];             // 8-bit cache: the scales of tile j (mod 8) are there
   uint32_t tmem_base;
   int abort;
 };
@@ -186,26 +196,20 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if (std::is_same<T, __half>::value) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-template <int DP, typename T>
-__global__ void __launch_bounds__(ChunkShape<DP>::Threads, 1)
+// T: of queries and output. The products run in T, over an 8-bit cache in fp16.
+template <int DP, typename T, bool I8>
+__global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
     attn_chunk_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
-  using S = ChunkShape<DP>;
+  using S = ChunkShape<DP, I8>;
+  using M = typename std::conditional<I8, __half, T>::type;
   constexpr int NQ = S::NQ, B = S::B, KB = S::KB, NB = S::NB;
-  constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+  constexpr bool BF = std::is_same<M, __nv_bfloat16>::value;
   extern __shared__ __align__(1024) unsigned char sm[];
   unsigned char* ring = sm + S::Q;
   ChunkCtl* ctl = reinterpret_cast<ChunkCtl*>(ring + NB * kBlock);
   float* part_s = reinterpret_cast<float*>(ring + NB * kBlock + 512);   // a word of each softmax thread
+  float* scale_s = part_s + 512;      // 8-bit: [8 tiles][K 128, V 128], then what undoes each row's power of two
+  float* undo_s = scale_s + 8 * 256;
   pdl_wait();
   pdl_trigger();
   if (su32(sm) & 1023) {   // the swizzle needs it; the only shared memory here, so it starts a 1024-byte line
@@ -213,7 +217,7 @@ __global__ void __launch_bounds__(ChunkShape<DP>::Threads, 1)
     return;
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kMma = 16, kTma = 17, TPR = S::TPR, W = S::W;
+  constexpr int kMma = S::Mma, kLoad = kMma + 1, TPR = S::TPR, W = S::W;
   // the last rows see the most keys: they go first
   const int b = blockIdx.x / a.row_blocks, rb = a.row_blocks - 1 - (blockIdx.x - b * a.row_blocks);
   const int split = blockIdx.y, h = blockIdx.z;
@@ -229,7 +233,7 @@ __global__ void __launch_bounds__(ChunkShape<DP>::Threads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < NB; ++i) {
-      mbar_init(su32(&ctl->full[i]), 1);
+      mbar_init(su32(&ctl->full[i]), S::Load);
       mbar_init(su32(&ctl->empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -240,6 +244,7 @@ __global__ void __launch_bounds__(ChunkShape<DP>::Threads, 1)
     mbar_init(su32(&ctl->pv), 1);
     mbar_init(su32(&ctl->tail), 1);
     mbar_init(su32(&ctl->drain), 1);
+    for (int i = 0; i < 8; ++i) mbar_init(su32(&ctl->scales[i]), 4);
     ctl->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -257,6 +262,28 @@ __global__ void __launch_bounds__(ChunkShape<DP>::Threads, 1)
                                           (h * a.G + row % a.G) * a.q_hs + 8 * v);
       if (a.scale_log2 < 0.f) x = make_uint4(x.x ^ 0x80008000u, x.y ^ 0x80008000u, x.z ^ 0x80008000u, x.w ^ 0x80008000u);
     }
+    if (I8) {   // fp16, from bf16 by a power of two that brings the row's largest value to 2^13 .. 2^14
+      float back = 1.f;
+      if (a.q_bf16) {
+        float f[8], top = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 y = unpack2<__nv_bfloat16>((&x.x)[j]);
+          f[2 * j] = y.x;
+          f[2 * j + 1] = y.y;
+          top = fmaxf(top, fmaxf(fabsf(y.x), fabsf(y.y)));
+        }
+#pragma unroll
+        for (int o = 1; o < DP / 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        int up = 0;
+        if (top > 1e-30f && top < 1e30f) up = 13 - ilogbf(top);
+        const float by = __int_as_float((127 + up) << 23);
+        back = __int_as_float((127 - up) << 23);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) (&x.x)[j] = pack2<__half>(f[2 * j] * by, f[2 * j + 1] * by);
+      }
+      if (v == 0) undo_s[r] = back;
+    }
     const int rr = r & 127;
     *reinterpret_cast<uint4*>(sm + ((r >> 7) * B + (v >> 3)) * kBlock + rr * 128 + (((v & 7) ^ (rr & 7)) << 4)) = x;
   }
@@ -268,11 +295,113 @@ __global__ void __launch_bounds__(ChunkShape<DP>::Threads, 1)
   const int gran = min(1 << a.kv.page_log2, KB);   // keys of one V copy
   const int tail = (s1 & (gran - 1)) ? s1 : -1;    // rows from here on, up to the copy's end, hold anything
 
-  if (warp == kTma) {
+  const int32_t* table = a.kv.table + b * a.kv.table_stride;
+  const int page_mask = (1 << a.kv.page_log2) - 1;
+  const int seen = row_lo(a, w, w.r0 / a.G);   // pages that end before the first key seen may be gone
+
+  if (I8 && warp >= kLoad) {
+    // ---------------------------------------------------------------------------- loads and conversion
+    // Operand tiles in the MMAs' order (K0 K1 V0 K2 V1 ..), 16 values a piece. Each thread has the next
+    // tile's pieces under way in registers while it converts this one's.
+    constexpr int kThreads = 32 * S::Load, NV = (B * 512 + kThreads - 1) / kThreads;
+    const int tid = threadIdx.x - 32 * kLoad;
+    auto is_v = [&](int n) { return n == 2 * tiles - 1 || (n > 0 && !(n & 1)); };
+    auto tile_of = [&](int n) { return n == 2 * tiles - 1 ? tiles - 1 : is_v(n) ? n / 2 - 1 : (n + 1) / 2; };
+    // pool row of the first key of this lane's 16-key group of operand tile n, or -1
+    auto group_of = [&](int n) {
+      const int k = n < 2 * tiles ? s0 + 128 * tile_of(n) + 16 * (lane & 7) : s1;
+      if (k >= s1 || (k | page_mask) < seen) return -1;
+      const int page = table[k >> a.kv.page_log2];
+      return page < 0 || page >= a.kv.pages ? -1 : ((page * a.kv.heads + h) << a.kv.page_log2) + (k & page_mask);
+    };
+    // piece v of a tile: block, key of the tile, 16-value group of the head
+    auto place = [&](bool isv, int v, int& c, int& key, int& d16) {
+      c = v >> 9;
+      const int u = v & 511, sub = isv ? u / (KB * 4) : 0;
+      key = isv ? c * KB + u % (KB * 4) / 4 : u >> 2;
+      d16 = (isv ? sub : c) * 4 + (u & 3);
+    };
+    auto load = [&](int n, int group, uint4 (&x)[NV], float2& sc) {
+      const bool isv = is_v(n);
+      const int k0 = s0 + 128 * tile_of(n);
+      const char* pool = static_cast<const char*>(isv ? a.kv.v : a.kv.k);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int v = tid + kThreads * i;
+        int c, key, d16;
+        place(isv, v < B * 512 ? v : 0, c, key, d16);
+        const int row = __shfl_sync(0xffffffffu, group, key >> 4);
+        x[i] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);   // zeros in offset binary
+        if (v < B * 512 && row >= 0 && k0 + key < s1 && 16 * d16 < a.D) {
+          x[i] = *reinterpret_cast<const uint4*>(pool + (int64_t)(row + (key & 15)) * a.D + 16 * d16);
+          x[i] = make_uint4(x[i].x ^ 0x80808080u, x[i].y ^ 0x80808080u, x[i].z ^ 0x80808080u, x[i].w ^ 0x80808080u);
+        }
+      }
+      const int row = __shfl_sync(0xffffffffu, group, (tid >> 4) & 7);
+      sc = make_float2(0.f, 0.f);
+      if (!isv && tid < 128 && row >= 0 && k0 + tid < s1)
+        sc = make_float2(a.kv.k_scale[row + (tid & 15)], a.kv.v_scale[row + (tid & 15)]);
+    };
+    bool ok = true;
+    uint4 next[NV];
+    float2 next_sc;
+    load(0, group_of(0), next, next_sc);
+    int group = group_of(1), slot0 = 0, parity0 = 0;
+    for (int n = 0; n < 2 * tiles; ++n) {
+      uint4 x[NV];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) x[i] = next[i];
+      const float2 sc = next_sc;
+      if (n + 1 < 2 * tiles) load(n + 1, group, next, next_sc);
+      group = group_of(n + 2);
+      int slot = slot0, parity = parity0;
+#pragma unroll
+      for (int c = 0; c < B; ++c) {
+        ok = ok && chunk_wait(su32(&ctl->empty[slot]), parity ^ 1, ctl);
+        if (++slot == NB) {
+          slot = 0;
+          parity ^= 1;
+        }
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const bool isv = is_v(n);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int v = tid + kThreads * i;
+        if (v >= B * 512) break;
+        int c, key, d16;
+        place(isv, v, c, key, d16);
+        const int at = slot0 + c < NB ? slot0 + c : slot0 + c - NB;
+        const int rr = isv ? key - c * KB : key, piece = (d16 & 3) * 2;
+        unsigned char* dst = ring + at * kBlock + (isv ? (d16 >> 2) * KB * 128 : 0) + rr * 128;
+        uint4 y[2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          (&y[j >> 1].x)[2 * (j & 1)] = bytes_f16((&x[i].x)[j], 0x4140);
+          (&y[j >> 1].x)[2 * (j & 1) + 1] = bytes_f16((&x[i].x)[j], 0x4342);
+        }
+        *reinterpret_cast<uint4*>(dst + ((piece ^ (rr & 7)) << 4)) = y[0];
+        *reinterpret_cast<uint4*>(dst + (((piece + 1) ^ (rr & 7)) << 4)) = y[1];
+      }
+      fence_proxy_async();
+      const int j = tile_of(n);
+      if (!isv && tid < 128) {
+        scale_s[(j & 7) * 256 + tid] = sc.x;
+        scale_s[(j & 7) * 256 + 128 + tid] = sc.y;
+      }
+      __syncwarp();
+      if (lane < B) {
+        const int at = slot0 + lane < NB ? slot0 + lane : slot0 + lane - NB;
+        mbar_arrive(su32(&ctl->full[at]));
+      }
+      if (!isv && tid < 128 && lane == 0) mbar_arrive(su32(&ctl->scales[j & 7]));
+      slot0 = slot;
+      parity0 = parity;
+    }
+  } else if (!I8 && warp == kLoad) {
     // ---------------------------------------------------------------------------- loads
-    const int32_t* table = a.kv.table + b * a.kv.table_stride;
-    const int seen = row_lo(a, w, w.r0 / a.G);   // pages that end before the first key seen may be gone
-    const int page_mask = (1 << a.kv.page_log2) - 1, pool_rows = (a.kv.pages * a.kv.heads) << a.kv.page_log2;
+    const int pool_rows = (a.kv.pages * a.kv.heads) << a.kv.page_log2;
     // pool row of key k, or past the pool (zeros) where there is none
     auto row_of = [&](int k) {
       if (k >= s1 || (k | page_mask) < seen) return pool_rows;
@@ -389,7 +518,7 @@ __global__ void __launch_bounds__(ChunkShape<DP>::Threads, 1)
           if (i == 0) {
             const int kb = s0 + 128 * j + c * KB;
             if (!chunk_wait(full0 + 8 * slot, parity, ctl)) return false;
-            if (tail > kb && tail < kb + KB && !chunk_wait(su32(&ctl->tail), 0, ctl)) return false;
+            if (!I8 && tail > kb && tail < kb + KB && !chunk_wait(su32(&ctl->tail), 0, ctl)) return false;
             tc_fence_after();
           }
           const uint64_t bd = vd + slot * (kBlock >> 4);
@@ -451,15 +580,13 @@ __global__ void __launch_bounds__(ChunkShape<DP>::Threads, 1)
     const int bar = 1 + 4 * i + quarter;           // of the warps that share these rows
     const int klo = mine ? row_lo(a, w, tok) : 0, khi = mine ? min(row_hi(a, w, tok), s1) : s1;
     const int all_lo = __reduce_max_sync(0xffffffffu, klo), all_hi = __reduce_min_sync(0xffffffffu, khi);
-    const float scale = fabsf(a.scale_log2);
-    const int32_t* table = a.kv.table + b * a.kv.table_stride;
+    const float scale = fabsf(a.scale_log2) * (I8 ? undo_s[r] : 1.f);
     // what the threads of this row leave for one another
     float* said = part_s + (warp - 4 * part) * 32 + lane;   // part p: said[128 * p]
-    float m = -INFINITY;
+    float m = -INFINITY, l = 0.f, vref = 0.f, vinv = 0.f;   // vref: a power of two above the V scales so far
     uint64_t l2 = pair(0.f, 0.f), l3 = l2;
-    float l = 0.f;
-    bool ok = true;
-    for (int j = 0; j < tiles; ++j) {
+    bool ok = true, leave = false;   // a wait that gives up; all threads of the rows know of one
+    for (int j = 0; j < tiles && !leave; ++j) {
       const int k0 = s0 + 128 * j + W * part, buf = NQ == 2 ? i : j & 1;   // this thread's first key
       // 16-key groups whose page does not exist (past the keys khi masks)
       bool there = true;
@@ -468,26 +595,53 @@ __global__ void __launch_bounds__(ChunkShape<DP>::Threads, 1)
         there = page >= 0 && page < a.kv.pages;
       }
       const uint32_t missing = __ballot_sync(0xffffffffu, !there);
-      ok = __all_sync(0xffffffffu, chunk_wait(su32(&ctl->s_full[buf]), (NQ == 2 ? j : j >> 1) & 1, ctl));
-      tc_fence_after();
-      const uint32_t s_col = tmem + lanes + 128 * buf;
-      // The scores are read twice, 32 at a time, rather than held: 64 of them do not fit beside the
-      // weights in 96 registers, and the spills set the pace (D 128: 591 us where one thread a row
-      // took 410 on the three chunks).
-      const uint32_t own = s_col + W * part;
-      const bool masked = k0 < all_lo || k0 + W > all_hi || missing;
-      auto mask = [&](float* s, int c) {
+      float vmax = 0.f;
+      const float *ks = nullptr, *vs = nullptr;
+      if (I8) {
+        ok = ok && chunk_wait(su32(&ctl->scales[j & 7]), (j >> 3) & 1, ctl);
+        ks = scale_s + (j & 7) * 256 + W * part;
+        vs = ks + 128;
+        const float4 f = *reinterpret_cast<const float4*>(scale_s + (j & 7) * 256 + 128 + 4 * lane);
+        // the largest of the tile; a NaN or an infinity (a value that was stored as such) sets no reference
+        uint32_t x = 0;
 #pragma unroll
-        for (int k = 0; k < 32; ++k)
-          if (k0 + c + k < klo || k0 + c + k >= khi || ((missing >> ((c + k) >> 4)) & 1)) s[k] = -INFINITY;
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t y = __float_as_uint((&f.x)[e]);
+          if (y < 0x7f800000u) x = max(x, y);
+        }
+        vmax = __uint_as_float(__reduce_max_sync(0xffffffffu, x));
+      }
+      ok = __all_sync(0xffffffffu, ok && chunk_wait(su32(&ctl->s_full[buf]), (NQ == 2 ? j : j >> 1) & 1, ctl));
+      tc_fence_after();
+      const uint32_t own = tmem + lanes + 128 * buf + W * part;
+      const bool masked = k0 < all_lo || k0 + W > all_hi || missing;
+      // The scores are read twice, 32 at a time, rather than held: 64 of them do not fit beside the
+      // weights in 96 registers (spilled: 591 us where this takes 247 on the three chunks; weighed
+      // before the maximum is agreed on, and again where it moves: 474 us).
+      auto scores = [&](int c, float* s) {
+        tmem_ld32(own + c, s);
+        tmem_wait_ld(s);
+        if (I8) {
+#pragma unroll
+          for (int k = 0; k < 32; k += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(ks + c + k);
+            s[k] *= f.x;
+            s[k + 1] *= f.y;
+            s[k + 2] *= f.z;
+            s[k + 3] *= f.w;
+          }
+        }
+        if (masked) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            if (k0 + c + k < klo || k0 + c + k >= khi || ((missing >> ((c + k) >> 4)) & 1)) s[k] = -INFINITY;
+        }
       };
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int c = 0; c < W; c += 32) {
         float s[32];
-        tmem_ld32(own + c, s);
-        tmem_wait_ld(s);
-        if (masked) mask(s, c);
+        scores(c, s);
 #pragma unroll
         for (int k = 0; k < 32; k += 8)
 #pragma unroll
@@ -495,14 +649,21 @@ __global__ void __launch_bounds__(ChunkShape<DP>::Threads, 1)
       }
       const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
       // One that gave up waiting says so here, so that all leave together.
-      if (any_of(bar, 32 * TPR, mx > m + 8.f || !ok)) {
-        said[128 * part] = ok ? mx : NAN;
-        ok = !any_of(bar, 32 * TPR, !ok);
-        if (!ok) break;
+      if (any_of(bar, 32 * TPR, mx > m + 8.f || vmax > vref || !ok)) {
+        said[128 * part] = mx;
+        leave = any_of(bar, 32 * TPR, !ok);
+        if (leave) break;
         float all = mx;
 #pragma unroll
-        for (int p = 0; p < TPR; ++p) all = fmaxf(all, said[128 * p]);
+        for (int q = 0; q < TPR; ++q) all = fmaxf(all, said[128 * q]);
         const float mn = fmaxf(m, all), by = mn == -INFINITY ? 1.f : ex2(m - mn);
+        float undo = 1.f;
+        if (I8 && vmax > vref) {   // at most 2^120 or so: its inverse is a normal number too
+          const float ref = fminf(__uint_as_float((__float_as_uint(vmax) & 0x7f800000u) + 0x00800000u), 1.3e36f);
+          undo = vref / ref;
+          vref = ref;
+          vinv = 1.f / ref;
+        }
         m = mn;
         l2 = fma2(l2, pair(by, by), pair(0.f, 0.f));
         l3 = fma2(l3, pair(by, by), pair(0.f, 0.f));
@@ -518,7 +679,7 @@ __global__ void __launch_bounds__(ChunkShape<DP>::Threads, 1)
             tmem_ld32(o_col + c, o);
             tmem_wait_ld(o);
 #pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] *= by;
+            for (int k = 0; k < 32; ++k) o[k] *= by * undo;
             tmem_st32(o_col + c, reinterpret_cast<const uint32_t*>(o));
           }
         }
@@ -530,16 +691,23 @@ __global__ void __launch_bounds__(ChunkShape<DP>::Threads, 1)
       for (int c = 0; c < W; c += 32) {
         float s[32];
         uint32_t p[16];
-        tmem_ld32(own + c, s);
-        tmem_wait_ld(s);
-        if (masked) mask(s, c);
+        scores(c, s);
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const float2 x = unpair(fma2(pair(s[2 * k], s[2 * k + 1]), scale2, base2));
-          const float y0 = ex2(x.x), y1 = ex2(x.y);
-          if (k & 1) l3 = add2(l3, pair(y0, y1));
-          else l2 = add2(l2, pair(y0, y1));
-          p[k] = pack2<T>(y0, y1);
+        for (int k = 0; k < 32; k += 4) {
+          const float2 x = unpair(fma2(pair(s[k], s[k + 1]), scale2, base2));
+          const float2 z = unpair(fma2(pair(s[k + 2], s[k + 3]), scale2, base2));
+          float y0 = ex2(x.x), y1 = ex2(x.y), y2 = ex2(z.x), y3 = ex2(z.y);
+          l2 = add2(l2, pair(y0, y1));
+          l3 = add2(l3, pair(y2, y3));
+          if (I8) {   // a masked key's scale may be anything
+            const float4 f = *reinterpret_cast<const float4*>(vs + c + k);
+            y0 = masked && y0 == 0.f ? 0.f : y0 * (f.x * vinv);
+            y1 = masked && y1 == 0.f ? 0.f : y1 * (f.y * vinv);
+            y2 = masked && y2 == 0.f ? 0.f : y2 * (f.z * vinv);
+            y3 = masked && y3 == 0.f ? 0.f : y3 * (f.w * vinv);
+          }
+          p[k / 2] = pack2<M>(y0, y1);
+          p[k / 2 + 1] = pack2<M>(y2, y3);
         }
         tmem_st16(own + c / 2, p);   // over scores that this thread has read
       }
@@ -553,9 +721,9 @@ __global__ void __launch_bounds__(ChunkShape<DP>::Threads, 1)
       l = (x.x + x.y) + (y.x + y.y);
     }
     // ---- the rows' output, or their share of it
-    if (ok && tiles > 0) ok = __all_sync(0xffffffffu, chunk_wait(su32(&ctl->o_full[i]), 0, ctl));
+    if (ok && !leave && tiles > 0) ok = __all_sync(0xffffffffu, chunk_wait(su32(&ctl->o_full[i]), 0, ctl));
     said[128 * part] = l;
-    ok = !any_of(bar, 32 * TPR, !ok);
+    ok = !any_of(bar, 32 * TPR, !ok || leave);
     if (ok) {
       tc_fence_after();
       l = 0.f;
@@ -573,6 +741,10 @@ __global__ void __launch_bounds__(ChunkShape<DP>::Threads, 1)
         } else {
 #pragma unroll
           for (int k = 0; k < 32; ++k) o[k] = 0.f;
+        }
+        if (I8) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] *= vref;
         }
         if (!mine) continue;
         if (alone) {
@@ -621,10 +793,10 @@ bool make_pool_map(CUtensorMap* map, const void* base, int64_t rows, int D, int 
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DP, typename T>
+template <int DP, typename T, bool I8>
 int launch(const AttnArgs& a, cudaStream_t st) {
-  using S = ChunkShape<DP>;
-  auto kern = attn_chunk_kernel<DP, T>;
+  using S = ChunkShape<DP, I8>;
+  auto kern = attn_chunk_kernel<DP, T, I8>;
   static std::atomic<uint64_t> done{0};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -637,26 +809,28 @@ int launch(const AttnArgs& a, cudaStream_t st) {
     }
     done.fetch_or(bit);
   }
-  const int page = 1 << a.kv.page_log2;
-  const int64_t rows = ((int64_t)a.kv.pages * a.kv.heads) << a.kv.page_log2;
-  CUtensorMap kmap, vmap;
-  if (!make_pool_map(&kmap, a.kv.k, rows, a.D, page < 128 ? page : 128, a.q_bf16) ||
-      !make_pool_map(&vmap, a.kv.v, rows, a.D, page < S::KB ? page : S::KB, a.q_bf16))
-    return VQ2_ERR_LAUNCH;
+  CUtensorMap kmap = {}, vmap = {};
+  if (!I8) {
+    const int page = 1 << a.kv.page_log2;
+    const int64_t rows = ((int64_t)a.kv.pages * a.kv.heads) << a.kv.page_log2;
+    if (!encode_fn() || !make_pool_map(&kmap, a.kv.k, rows, a.D, page < 128 ? page : 128, a.q_bf16) ||
+        !make_pool_map(&vmap, a.kv.v, rows, a.D, page < S::KB ? page : S::KB, a.q_bf16))
+      return VQ2_ERR_LAUNCH;
+  }
   const dim3 grid((unsigned)(a.kv.seqs * a.row_blocks), (unsigned)a.splits, (unsigned)a.kv.heads);
   return launch_kernel(kern, grid, dim3(S::Threads), S::Smem, st, a, kmap, vmap);
 }
 
-template <typename T>
+template <typename T, bool I8>
 int launch_shape(const AttnArgs& a, cudaStream_t st) {
-  return a.D > 128 ? launch<256, T>(a, st) : a.D > 64 ? launch<128, T>(a, st) : launch<64, T>(a, st);
+  return a.D > 128 ? launch<256, T, I8>(a, st) : a.D > 64 ? launch<128, T, I8>(a, st) : launch<64, T, I8>(a, st);
 }
 
 }  // namespace
 
-void plan_attn_chunk(AttnArgs& a, int64_t max_new, int64_t max_len) {
+void plan_attn_chunk(AttnArgs& a, bool i8, int64_t max_new, int64_t max_len) {
   const int64_t rows = max_new * a.G;
-  a.rows_per_block = a.D > 128 ? 128 : 256;
+  a.rows_per_block = a.D > 128 || i8 ? 128 : 256;
   a.row_blocks = (int)((rows + a.rows_per_block - 1) / a.rows_per_block);
   if (a.row_blocks < 1) a.row_blocks = 1;
   a.lo_mask = ~127;
@@ -675,9 +849,9 @@ void plan_attn_chunk(AttnArgs& a, int64_t max_new, int64_t max_len) {
   if (a.splits < 1) a.splits = 1;
 }
 
-int launch_attn_chunk(const AttnArgs& a, cudaStream_t st) {
-  if (!encode_fn()) return VQ2_ERR_LAUNCH;
-  return a.q_bf16 ? launch_shape<__nv_bfloat16>(a, st) : launch_shape<__half>(a, st);
+int launch_attn_chunk(const AttnArgs& a, bool i8, cudaStream_t st) {
+  if (i8) return a.q_bf16 ? launch_shape<__nv_bfloat16, true>(a, st) : launch_shape<__half, true>(a, st);
+  return a.q_bf16 ? launch_shape<__nv_bfloat16, false>(a, st) : launch_shape<__half, false>(a, st);
 }
 
 int attn_chunk_status(int reset) {

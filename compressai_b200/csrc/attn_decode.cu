@@ -66,24 +66,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   return r;
 }
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if (std::is_same<T, __half>::value) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-// Two bytes of w (offset binary, v + 128), chosen by sel's nibbles 0 and 2, as two exact fp16 values.
-__device__ __forceinline__ uint32_t bytes_f16(uint32_t w, uint32_t sel) {
-  const uint32_t p = __byte_perm(w, 0x64646464u, sel);  // 0x6400 | u = 1024 + u
-  const uint32_t bias = 0x64806480u;                    // 1152
-  const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&p), *reinterpret_cast<const __half2*>(&bias));
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 // Shapes of one variant. DP: head size rounded up (values past D are zeros); NT: 8-row tiles.
 template <int DP, int NT, bool I8>
 struct DecodeShape {

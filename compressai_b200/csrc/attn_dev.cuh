@@ -1,6 +1,8 @@
 // What the attention kernels share: arguments, the keys that query rows see, and how rows are split
 // along the keys and joined.
 #pragma once
+#include <type_traits>
+
 #include "kv_dev.cuh"
 
 namespace vq2 {
@@ -28,6 +30,24 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Two bytes of w (offset binary, v + 128), chosen by sel's nibbles 0 and 2, as two exact fp16 values.
+__device__ __forceinline__ uint32_t bytes_f16(uint32_t w, uint32_t sel) {
+  const uint32_t p = __byte_perm(w, 0x64646464u, sel);  // 0x6400 | u = 1024 + u
+  const uint32_t bias = 0x64806480u;                    // 1152
+  const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&p), *reinterpret_cast<const __half2*>(&bias));
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // A sequence's new tokens, and the block of query rows [r0, r0 + rows) among its count * G: row r is
@@ -65,12 +85,12 @@ __device__ __forceinline__ void block_keys(const AttnArgs& a, const AttnRows& w,
 
 // Joins the splits of every row (launched after a kernel that left more than one).
 int launch_attn_join(const AttnArgs& a, cudaStream_t st);
-// Few rows per key/value head (attn_decode.cu), and many (attn_chunk.cu, 16-bit caches). The plans set
+// Few rows per key/value head (attn_decode.cu), and many (attn_chunk.cu). The plans set
 // chunk, splits, rows_per_block, row_blocks and lo_mask.
 int launch_attn_decode(const AttnArgs& a, bool i8, cudaStream_t st);
 void plan_attn_decode(AttnArgs& a, int64_t max_new, int64_t max_len);
-int launch_attn_chunk(const AttnArgs& a, cudaStream_t st);
-void plan_attn_chunk(AttnArgs& a, int64_t max_new, int64_t max_len);
+int launch_attn_chunk(const AttnArgs& a, bool i8, cudaStream_t st);
+void plan_attn_chunk(AttnArgs& a, bool i8, int64_t max_new, int64_t max_len);
 int attn_chunk_status(int reset);   // its part of vq2_attention_status
 
 }  // namespace vq2
