@@ -9,16 +9,35 @@
 namespace vq2 {
 namespace {
 
-// Which kernel, and the splits of the keys: a function of shapes and bounds alone. Returns the bytes
-// that joining the splits takes.
-int64_t plan(AttnArgs& a, bool i8, int64_t max_new, int64_t max_len, bool& chunked) {
+// Which kernel, the splits of the keys and the workspace they and a widened 8-bit cache take: a function
+// of shapes and bounds alone. Points into `ws` where it is given; returns its bytes.
+int64_t plan(AttnArgs& a, bool i8, int64_t max_new, int64_t max_len, bool& chunked, char* ws) {
   // Rows that share a key: the decode kernel holds 16 (head size above 128) or 32 of them; from there
-  // on it would read the keys again for every 16 or 32, and the tensor-core kernel takes over.
-  chunked = max_new * a.G > (a.D > 128 ? 16 : 32);
-  if (chunked) plan_attn_chunk(a, i8, max_new, max_len);
+  // on it would read the keys again for every 16 or 32, and the tensor-core kernel takes over. Its fp16
+  // copy of an 8-bit cache is kept to 4 GB; past that (a batch of very long sequences) the decode kernel
+  // reads the 8 bits again after all.
+  const int64_t wide_len = (max_len + 127) & ~int64_t(127), wide_rows = a.kv.seqs * (int64_t)a.kv.heads * wide_len;
+  chunked = max_new * a.G > (a.D > 128 ? 16 : 32) && (!i8 || wide_rows * a.D <= int64_t(1) << 30);
+  if (chunked) plan_attn_chunk(a, max_new, max_len);
   else plan_attn_decode(a, max_new, max_len);
-  if (a.splits == 1) return 0;
-  return (int64_t)a.T * a.hq * a.splits * (a.D * 4 + 8);
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    char* p = ws ? ws + at : nullptr;
+    at += (bytes + 255) & ~int64_t(255);
+    return p;
+  };
+  if (a.splits > 1) {
+    a.part_o = reinterpret_cast<float*>(take((int64_t)a.T * a.hq * a.splits * a.D * 4));
+    a.part_ml = reinterpret_cast<float2*>(take((int64_t)a.T * a.hq * a.splits * 8));
+  }
+  if (chunked && i8) {
+    a.wide_len = (int)wide_len;
+    a.wide_k = take(wide_rows * a.D * 2);
+    a.wide_v = take(wide_rows * a.D * 2);
+    a.wide_ks = reinterpret_cast<float*>(take(wide_rows * 4));
+    a.wide_vs = reinterpret_cast<float*>(take(wide_rows * 4));
+  }
+  return at;
 }
 
 bool bad_attn(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t seqs, int64_t max_new, int64_t max_len,
@@ -46,7 +65,7 @@ extern "C" int64_t vq2_paged_attention_workspace(int64_t tokens, int64_t q_heads
   a.G = a.hq / a.kv.heads;
   a.window = (int)window;
   bool chunked;
-  return tokens && seqs ? plan(a, kv_dtype == VQ2_I8, max_new, max_len, chunked) : 0;
+  return tokens && seqs ? plan(a, kv_dtype == VQ2_I8, max_new, max_len, chunked, nullptr) : 0;
 }
 
 extern "C" int vq2_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype,
@@ -81,15 +100,11 @@ extern "C" int vq2_paged_attention(const void* q, int64_t q_token_stride, int64_
   a.out = out;
   a.lse = lse;
   bool chunked;
-  const int64_t bytes = plan(a, kv_dtype == VQ2_I8, starts ? max_new : 1, max_len, chunked);
-  if (bytes) {
-    if (!workspace || workspace_bytes < bytes) return VQ2_ERR_ARG;
-    a.part_o = static_cast<float*>(workspace);
-    a.part_ml = reinterpret_cast<float2*>(a.part_o + (int64_t)a.T * a.hq * a.splits * a.D);
-  }
+  const bool i8 = kv_dtype == VQ2_I8;
+  const int64_t bytes = plan(a, i8, starts ? max_new : 1, max_len, chunked, static_cast<char*>(workspace));
+  if (bytes && (!workspace || workspace_bytes < bytes)) return VQ2_ERR_ARG;
   if ((int64_t)a.kv.seqs * a.row_blocks > 0x7fffffff) return VQ2_ERR_SHAPE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool i8 = kv_dtype == VQ2_I8;
   s = chunked ? launch_attn_chunk(a, i8, st) : launch_attn_decode(a, i8, st);
   if (s != VQ2_OK || a.splits == 1) return s;
   return launch_attn_join(a, st);

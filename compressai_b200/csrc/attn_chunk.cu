@@ -26,10 +26,12 @@
 // Bound: at 2 * 128 * 128 * DP flops for 128 * 128 exponentials per product pair, the tensor core
 // and (head size 128) the 16 exponentials a clock an SM are about equally busy.
 //
-// 8-bit caches: seven warps take TMA's place. They load 16 values a piece, the next operand tile under
-// way in registers, and store exact fp16 (an int8 is; see attn_decode.cu, also for the scales: the key's
-// multiplies the score, the value's the weight, relative to a power of two) into the same ring. One row
-// tile and 8 softmax warps, for the conversion's warps need the registers.
+// 8-bit caches: a launch before this one writes the visible keys and values out once as exact fp16 (an
+// int8 is; see attn_decode.cu, also for the scales: the key's multiplies the score, the value's the
+// weight, relative to a power of two), in order and without pages, and this kernel reads those. Every
+// block of rows would convert the same keys again: warps that did so inside this kernel, beside the
+// softmax, took 4700 cycles an operand tile (two chunks of 257 tokens over 16385, 34 blocks a
+// sequence: 359 us).
 //
 // Rows of a page past the keys that the block sees may hold anything, NaN too: their scores are
 // replaced, and their V rows zeroed in shared memory by the loading warp before the MMA may read
@@ -55,17 +57,16 @@ constexpr int kBlock = 16384;                    // bytes of a ring block
 
 template <int DP, bool I8>
 struct ChunkShape {
-  static constexpr int NQ = DP > 128 || I8 ? 1 : 2;  // row tiles of 128
+  static constexpr int NQ = DP > 128 ? 1 : 2;        // row tiles of 128
   static constexpr int B = DP / 64;                  // ring blocks of a 128-key tile, K or V
   static constexpr int KB = 8192 / DP;               // keys of a V block
   static constexpr int Q = NQ * 128 * DP * 2;
-  static constexpr int NB = I8 && DP == 256 ? 9 : DP == 64 && !I8 ? 12 : 10;   // ring blocks
-  static constexpr int TPR = I8 ? 2 : 4 / NQ;        // threads of a row in the softmax
+  static constexpr int NB = I8 ? (DP == 64 ? 10 : 9) : DP == 64 ? 12 : 10;   // ring blocks
+  static constexpr int TPR = 4 / NQ;                 // threads of a row in the softmax
   static constexpr int W = 128 / TPR;                // keys of a tile that one of them takes
-  static constexpr int Mma = 4 * NQ * TPR;           // warp that issues the MMAs; the softmax is before it
-  static constexpr int Load = I8 ? 7 : 1;            // warps after it: conversion, or TMA
-  static constexpr int Threads = (Mma + 1 + Load) * 32;
-  static constexpr int Scales = I8 ? 8 * 1024 + 512 : 0;   // K's and V's of 8 tiles; the rows' powers of two
+  static constexpr int Mma = 16, Load = 17;          // warps: softmax before, MMA issuer, TMA
+  static constexpr int Threads = 18 * 32;
+  static constexpr int Scales = I8 ? 8 * 1024 + 1024 : 0;   // K's and V's of 8 tiles; the rows' powers of two
   static constexpr int Smem = Q + NB * kBlock + 512 + 2048 + Scales;
   static_assert(Smem <= 232448, "shared memory");
   static constexpr uint32_t O0 = 256;                // first TMEM column of O; S buffers at 0 and 128
@@ -78,6 +79,7 @@ struct ChunkCtl {
   uint64_t pv;                    // one row tile: each product into O (before a rescale)
   uint64_t tail;                  // V rows past the last key are zeroed
   uint64_t drain;
+  uint64_t q_full;                // the queries are in shared memory
   uint64_t scales[8];             // 8-bit cache: the scales of tile j (mod 8) are there
   uint32_t tmem_base;
   int abort;
@@ -217,7 +219,7 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
     return;
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kMma = S::Mma, kLoad = kMma + 1, TPR = S::TPR, W = S::W;
+  constexpr int kMma = S::Mma, TPR = S::TPR, W = S::W;
   // the last rows see the most keys: they go first
   const int b = blockIdx.x / a.row_blocks, rb = a.row_blocks - 1 - (blockIdx.x - b * a.row_blocks);
   const int split = blockIdx.y, h = blockIdx.z;
@@ -233,7 +235,7 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < NB; ++i) {
-      mbar_init(su32(&ctl->full[i]), S::Load);
+      mbar_init(su32(&ctl->full[i]), 1);
       mbar_init(su32(&ctl->empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -244,7 +246,8 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
     mbar_init(su32(&ctl->pv), 1);
     mbar_init(su32(&ctl->tail), 1);
     mbar_init(su32(&ctl->drain), 1);
-    for (int i = 0; i < 8; ++i) mbar_init(su32(&ctl->scales[i]), 4);
+    mbar_init(su32(&ctl->q_full), 4 * TPR * nq);
+    for (int i = 0; i < 8; ++i) mbar_init(su32(&ctl->scales[i]), 1);
     ctl->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -252,165 +255,31 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&ctl->tmem_base)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  // ---- queries into 128-byte swizzled blocks [row tile][64 values][128 rows]; rows past the last are zeros
-  for (int e = threadIdx.x; e < nq * 128 * (DP / 8); e += blockDim.x) {
-    const int r = e / (DP / 8), v = e - r * (DP / 8);  // row, 8-value piece
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (r < w.rows && 8 * v < a.D) {
-      const int row = w.r0 + r;
-      x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (w.first + row / a.G) * a.q_ts +
-                                          (h * a.G + row % a.G) * a.q_hs + 8 * v);
-      if (a.scale_log2 < 0.f) x = make_uint4(x.x ^ 0x80008000u, x.y ^ 0x80008000u, x.z ^ 0x80008000u, x.w ^ 0x80008000u);
-    }
-    if (I8) {   // fp16, from bf16 by a power of two that brings the row's largest value to 2^13 .. 2^14
-      float back = 1.f;
-      if (a.q_bf16) {
-        float f[8], top = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 y = unpack2<__nv_bfloat16>((&x.x)[j]);
-          f[2 * j] = y.x;
-          f[2 * j + 1] = y.y;
-          top = fmaxf(top, fmaxf(fabsf(y.x), fabsf(y.y)));
-        }
-#pragma unroll
-        for (int o = 1; o < DP / 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        int up = 0;
-        if (top > 1e-30f && top < 1e30f) up = 13 - ilogbf(top);
-        const float by = __int_as_float((127 + up) << 23);
-        back = __int_as_float((127 - up) << 23);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) (&x.x)[j] = pack2<__half>(f[2 * j] * by, f[2 * j + 1] * by);
-      }
-      if (v == 0) undo_s[r] = back;
-    }
-    const int rr = r & 127;
-    *reinterpret_cast<uint4*>(sm + ((r >> 7) * B + (v >> 3)) * kBlock + rr * 128 + (((v & 7) ^ (rr & 7)) << 4)) = x;
-  }
-  fence_proxy_async();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = ctl->tmem_base;
-  const int gran = min(1 << a.kv.page_log2, KB);   // keys of one V copy
-  const int tail = (s1 & (gran - 1)) ? s1 : -1;    // rows from here on, up to the copy's end, hold anything
+  const int gran = I8 ? KB : min(1 << a.kv.page_log2, KB);   // keys of one V copy
+  const int tail = !I8 && (s1 & (gran - 1)) ? s1 : -1;    // rows from here on, up to the copy's end, hold anything
 
   const int32_t* table = a.kv.table + b * a.kv.table_stride;
   const int page_mask = (1 << a.kv.page_log2) - 1;
   const int seen = row_lo(a, w, w.r0 / a.G);   // pages that end before the first key seen may be gone
 
-  if (I8 && warp >= kLoad) {
-    // ---------------------------------------------------------------------------- loads and conversion
-    // Operand tiles in the MMAs' order (K0 K1 V0 K2 V1 ..), 16 values a piece. Each thread has the next
-    // tile's pieces under way in registers while it converts this one's.
-    constexpr int kThreads = 32 * S::Load, NV = (B * 512 + kThreads - 1) / kThreads;
-    const int tid = threadIdx.x - 32 * kLoad;
-    auto is_v = [&](int n) { return n == 2 * tiles - 1 || (n > 0 && !(n & 1)); };
-    auto tile_of = [&](int n) { return n == 2 * tiles - 1 ? tiles - 1 : is_v(n) ? n / 2 - 1 : (n + 1) / 2; };
-    // pool row of the first key of this lane's 16-key group of operand tile n, or -1
-    auto group_of = [&](int n) {
-      const int k = n < 2 * tiles ? s0 + 128 * tile_of(n) + 16 * (lane & 7) : s1;
-      if (k >= s1 || (k | page_mask) < seen) return -1;
-      const int page = table[k >> a.kv.page_log2];
-      return page < 0 || page >= a.kv.pages ? -1 : ((page * a.kv.heads + h) << a.kv.page_log2) + (k & page_mask);
-    };
-    // piece v of a tile: block, key of the tile, 16-value group of the head
-    auto place = [&](bool isv, int v, int& c, int& key, int& d16) {
-      c = v >> 9;
-      const int u = v & 511, sub = isv ? u / (KB * 4) : 0;
-      key = isv ? c * KB + u % (KB * 4) / 4 : u >> 2;
-      d16 = (isv ? sub : c) * 4 + (u & 3);
-    };
-    auto load = [&](int n, int group, uint4 (&x)[NV], float2& sc) {
-      const bool isv = is_v(n);
-      const int k0 = s0 + 128 * tile_of(n);
-      const char* pool = static_cast<const char*>(isv ? a.kv.v : a.kv.k);
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int v = tid + kThreads * i;
-        int c, key, d16;
-        place(isv, v < B * 512 ? v : 0, c, key, d16);
-        const int row = __shfl_sync(0xffffffffu, group, key >> 4);
-        x[i] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);   // zeros in offset binary
-        if (v < B * 512 && row >= 0 && k0 + key < s1 && 16 * d16 < a.D) {
-          x[i] = *reinterpret_cast<const uint4*>(pool + (int64_t)(row + (key & 15)) * a.D + 16 * d16);
-          x[i] = make_uint4(x[i].x ^ 0x80808080u, x[i].y ^ 0x80808080u, x[i].z ^ 0x80808080u, x[i].w ^ 0x80808080u);
-        }
-      }
-      const int row = __shfl_sync(0xffffffffu, group, (tid >> 4) & 7);
-      sc = make_float2(0.f, 0.f);
-      if (!isv && tid < 128 && row >= 0 && k0 + tid < s1)
-        sc = make_float2(a.kv.k_scale[row + (tid & 15)], a.kv.v_scale[row + (tid & 15)]);
-    };
-    bool ok = true;
-    uint4 next[NV];
-    float2 next_sc;
-    load(0, group_of(0), next, next_sc);
-    int group = group_of(1), slot0 = 0, parity0 = 0;
-    for (int n = 0; n < 2 * tiles; ++n) {
-      uint4 x[NV];
-#pragma unroll
-      for (int i = 0; i < NV; ++i) x[i] = next[i];
-      const float2 sc = next_sc;
-      if (n + 1 < 2 * tiles) load(n + 1, group, next, next_sc);
-      group = group_of(n + 2);
-      int slot = slot0, parity = parity0;
-#pragma unroll
-      for (int c = 0; c < B; ++c) {
-        ok = ok && chunk_wait(su32(&ctl->empty[slot]), parity ^ 1, ctl);
-        if (++slot == NB) {
-          slot = 0;
-          parity ^= 1;
-        }
-      }
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      const bool isv = is_v(n);
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int v = tid + kThreads * i;
-        if (v >= B * 512) break;
-        int c, key, d16;
-        place(isv, v, c, key, d16);
-        const int at = slot0 + c < NB ? slot0 + c : slot0 + c - NB;
-        const int rr = isv ? key - c * KB : key, piece = (d16 & 3) * 2;
-        unsigned char* dst = ring + at * kBlock + (isv ? (d16 >> 2) * KB * 128 : 0) + rr * 128;
-        uint4 y[2];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          (&y[j >> 1].x)[2 * (j & 1)] = bytes_f16((&x[i].x)[j], 0x4140);
-          (&y[j >> 1].x)[2 * (j & 1) + 1] = bytes_f16((&x[i].x)[j], 0x4342);
-        }
-        *reinterpret_cast<uint4*>(dst + ((piece ^ (rr & 7)) << 4)) = y[0];
-        *reinterpret_cast<uint4*>(dst + (((piece + 1) ^ (rr & 7)) << 4)) = y[1];
-      }
-      fence_proxy_async();
-      const int j = tile_of(n);
-      if (!isv && tid < 128) {
-        scale_s[(j & 7) * 256 + tid] = sc.x;
-        scale_s[(j & 7) * 256 + 128 + tid] = sc.y;
-      }
-      __syncwarp();
-      if (lane < B) {
-        const int at = slot0 + lane < NB ? slot0 + lane : slot0 + lane - NB;
-        mbar_arrive(su32(&ctl->full[at]));
-      }
-      if (!isv && tid < 128 && lane == 0) mbar_arrive(su32(&ctl->scales[j & 7]));
-      slot0 = slot;
-      parity0 = parity;
-    }
-  } else if (!I8 && warp == kLoad) {
+  if (warp == S::Load) {
     // ---------------------------------------------------------------------------- loads
     const int pool_rows = (a.kv.pages * a.kv.heads) << a.kv.page_log2;
+    const int wide_row0 = I8 ? (b * a.kv.heads + h) * a.wide_len : 0;
     // pool row of key k, or past the pool (zeros) where there is none
     auto row_of = [&](int k) {
+      if (I8) return wide_row0 + k;
       if (k >= s1 || (k | page_mask) < seen) return pool_rows;
       const int page = table[k >> a.kv.page_log2];
       return page < 0 || page >= a.kv.pages ? pool_rows : ((page * a.kv.heads + h) << a.kv.page_log2) + (k & page_mask);
     };
-    int q = 0;
+    int q = 0, said = 0;
     bool ok = true;
-    const int rk = min(1 << a.kv.page_log2, 128);   // keys of one K copy
+    const int rk = I8 ? 128 : min(1 << a.kv.page_log2, 128);   // keys of one K copy
     // lane i's copy of a K block: keys i * rk ..; of a V block: values 64 * (i % B), keys (i / B) * gran ..
     auto load = [&](bool is_v, int j) {
       const int k0 = s0 + 128 * j;
@@ -423,6 +292,13 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
 #pragma unroll
         for (int c = 0; c < B; ++c)
           if ((lane / B) * gran < KB) row[c] = row_of(k0 + c * KB + (lane / B) * gran);
+      }
+      if (I8 && !is_v) said = j + 1;
+      if (I8 && !is_v && lane == 0) {   // the tile's scales, with K; their place is free long before the ring's is
+        const uint32_t bar = su32(&ctl->scales[j & 7]), dst = su32(scale_s + (j & 7) * 256);
+        mbar_arrive_tx(bar, 1024);
+        bulk_load(dst, a.wide_ks + wide_row0 + k0, 512, bar);
+        bulk_load(dst + 512, a.wide_vs + wide_row0 + k0, 512, bar);
       }
 #pragma unroll 1
       for (int c = 0; c < B && ok; ++c, ++q) {
@@ -472,8 +348,11 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
       }
     }
     // copies this warp started have landed before the block's shared memory goes away
-    if (!ok)
+    if (!ok) {
       for (int i = max(0, q - NB); i < q; ++i) chunk_drain(su32(&ctl->full[i % NB]), (i / NB) & 1);
+      if (I8)   // scales: at most 8 tiles' are under way; those waited for already answer at once
+        for (int i = max(0, said - 8); i < said; ++i) chunk_drain(su32(&ctl->scales[i & 7]), (i >> 3) & 1);
+    }
   } else if (warp == kMma) {
     // ---------------------------------------------------------------------------- MMA issuer
     // One elected thread. elect.sync rather than a lane number: the compiler then knows a single thread
@@ -483,7 +362,7 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
       constexpr uint32_t QK = umma_idesc<128, BF>(), PV = umma_idesc<DP, BF>(true);
       const uint64_t qd = sw128_desc(su32(sm)), kd = sw128_desc(su32(ring)), vd = v_desc<KB>(su32(ring));
       const uint32_t full0 = su32(&ctl->full[0]), empty0 = su32(&ctl->empty[0]);
-      bool ok = true;
+      bool ok = tiles == 0 || chunk_wait(su32(&ctl->q_full), 0, ctl);
       int ks = 0, vs = 0, kp = 0, vp = 0;   // slot and parity of the next K and V tile's first block
       auto skip = [&](int& slot, int& parity, int n) {
         slot += n;
@@ -552,7 +431,7 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
           skip(ks, kp, 2 * B);
         }
       } else {
-        if (tiles > 0) ok = qk(0, 0);
+        if (tiles > 0 && ok) ok = qk(0, 0);
         skip(ks, kp, B);
         skip(vs, vp, tiles > 1 ? 2 * B : B);
         for (int j = 0; j < tiles && ok; ++j) {
@@ -574,27 +453,92 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
     const int i = warp / (4 * TPR), part = (warp >> 2) % TPR, quarter = warp & 3;
     const int r = 128 * i + 32 * quarter + lane;   // row of the block
     const bool mine = r < w.rows;
-    const int row = w.r0 + (mine ? r : 0), tok = row / a.G;
+    // Row rr of the block is new token t0 + (g0 + rr) / G, head (g0 + rr) % G: small numbers, divided by
+    // a multiplication.
+    const int t0 = w.r0 / a.G, g0 = w.r0 - t0 * a.G;
+    const uint32_t by_g = 0xffffffffu / a.G + 1;
+    auto token_of = [&](int rr, int& head) {
+      const int n = g0 + rr, q = a.G == 1 ? n : (int)__umulhi(n, by_g);
+      head = n - q * a.G;
+      return t0 + q;
+    };
+    // ---- the tile's queries into 128-byte swizzled blocks of 64 values; rows past the last are zeros.
+    // The loads of a round go out together.
+    if (tiles > 0) {
+      constexpr int kThreads = 128 * TPR, N = 128 * (DP / 8) / kThreads, R = N < 8 ? N : 8;
+      const int tid = (warp - 4 * TPR * i) * 32 + lane;
+#pragma unroll 1
+      for (int n0 = 0; n0 < N; n0 += R) {
+        uint4 x[R];
+#pragma unroll
+        for (int n = 0; n < R; ++n) {
+          const int e = tid + (n0 + n) * kThreads, rr = e / (DP / 8), v = e % (DP / 8);  // row of the tile, 8-value piece
+          x[n] = make_uint4(0, 0, 0, 0);
+          if (128 * i + rr < w.rows && 8 * v < a.D) {
+            int head;
+            const int t = token_of(128 * i + rr, head);
+            x[n] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(w.first + t) * a.q_ts +
+                                                   (int64_t)(h * a.G + head) * a.q_hs + 8 * v);
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < R; ++n) {
+          const int e = tid + (n0 + n) * kThreads, rr = e / (DP / 8), v = e % (DP / 8);
+          if (a.scale_log2 < 0.f)
+            x[n] = make_uint4(x[n].x ^ 0x80008000u, x[n].y ^ 0x80008000u, x[n].z ^ 0x80008000u, x[n].w ^ 0x80008000u);
+          if (I8) {   // fp16, from bf16 by a power of two that brings the row's largest value to 2^13 .. 2^14
+            float back = 1.f;
+            if (a.q_bf16) {
+              float f[8], big = 0.f;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float2 y = unpack2<__nv_bfloat16>((&x[n].x)[j]);
+                f[2 * j] = y.x;
+                f[2 * j + 1] = y.y;
+                big = fmaxf(big, fmaxf(fabsf(y.x), fabsf(y.y)));
+              }
+#pragma unroll
+              for (int o = 1; o < DP / 8; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+              int up = 0;
+              if (big > 1e-30f && big < 1e30f) up = 13 - ilogbf(big);
+              const float by = __int_as_float((127 + up) << 23);
+              back = __int_as_float((127 - up) << 23);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) (&x[n].x)[j] = pack2<__half>(f[2 * j] * by, f[2 * j + 1] * by);
+            }
+            if (v == 0) undo_s[128 * i + rr] = back;
+          }
+          *reinterpret_cast<uint4*>(sm + (i * B + (v >> 3)) * kBlock + rr * 128 + (((v & 7) ^ (rr & 7)) << 4)) = x[n];
+        }
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(su32(&ctl->q_full));
+    }
+    int head = 0;
+    const int tok = token_of(mine ? r : 0, head);
     const uint32_t lanes = static_cast<uint32_t>(32 * quarter) << 16;
     const uint32_t o_col = tmem + lanes + S::O0 + i * DP;
     const int bar = 1 + 4 * i + quarter;           // of the warps that share these rows
     const int klo = mine ? row_lo(a, w, tok) : 0, khi = mine ? min(row_hi(a, w, tok), s1) : s1;
     const int all_lo = __reduce_max_sync(0xffffffffu, klo), all_hi = __reduce_min_sync(0xffffffffu, khi);
-    const float scale = fabsf(a.scale_log2) * (I8 ? undo_s[r] : 1.f);
+    bool ok = true, leave = false;   // a wait that gives up; all threads of the rows know of one
+    float scale = fabsf(a.scale_log2);
+    if (I8 && tiles > 0) {
+      ok = chunk_wait(su32(&ctl->q_full), 0, ctl);
+      scale *= undo_s[r];
+    }
     // what the threads of this row leave for one another
     float* said = part_s + (warp - 4 * part) * 32 + lane;   // part p: said[128 * p]
     float m = -INFINITY, l = 0.f, vref = 0.f, vinv = 0.f;   // vref: a power of two above the V scales so far
     uint64_t l2 = pair(0.f, 0.f), l3 = l2;
-    bool ok = true, leave = false;   // a wait that gives up; all threads of the rows know of one
+    auto page_at = [&](int k) { return lane < W / 16 && k + 16 * lane < s1 ? table[(k + 16 * lane) >> a.kv.page_log2] : 0; };
+    int page = page_at(s0 + W * part);   // a tile ahead
     for (int j = 0; j < tiles && !leave; ++j) {
       const int k0 = s0 + 128 * j + W * part, buf = NQ == 2 ? i : j & 1;   // this thread's first key
       // 16-key groups whose page does not exist (past the keys khi masks)
-      bool there = true;
-      if (lane < W / 16 && k0 + 16 * lane < s1) {
-        const int page = table[(k0 + 16 * lane) >> a.kv.page_log2];
-        there = page >= 0 && page < a.kv.pages;
-      }
-      const uint32_t missing = __ballot_sync(0xffffffffu, !there);
+      const uint32_t missing = __ballot_sync(0xffffffffu, page < 0 || page >= a.kv.pages);
+      page = page_at(k0 + 128);
       float vmax = 0.f;
       const float *ks = nullptr, *vs = nullptr;
       if (I8) {
@@ -729,41 +673,56 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
       l = 0.f;
 #pragma unroll
       for (int p = 0; p < TPR; ++p) l += said[128 * p];
-      const int64_t at = (int64_t)(w.first + tok) * a.hq + h * a.G + row % a.G;
       const float inv = l == 0.f ? 0.f : 1.f / l;
+      // 16 values of 32 rows at a time through 2 KB of the tile's queries, which nobody reads any more:
+      // a row's 16 values then go out as whole sectors.
+      unsigned char* mine_s = sm + i * B * kBlock + (warp - 4 * TPR * i) * 2048;
 #pragma unroll 1
-      for (int c = part * (DP / TPR); c < (part + 1) * (DP / TPR); c += 32) {
-        float o[32];
-        if (tiles > 0) {
-          __syncwarp();
-          tmem_ld32(o_col + c, o);
-          tmem_wait_ld(o);
-        } else {
+      for (int c = part * (DP / TPR); c < (part + 1) * (DP / TPR); c += 16) {
+        float o[16];
+        __syncwarp();
+        if (tiles > 0) tmem_ld16(o_col + c, o);
+        else
 #pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = 0.f;
-        }
-        if (I8) {
+          for (int k = 0; k < 16; ++k) o[k] = 0.f;
+        const float by = (alone ? inv : 1.f) * (I8 ? vref : 1.f);
 #pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] *= vref;
-        }
-        if (!mine) continue;
+        for (int k = 0; k < 16; ++k) o[k] *= by;
         if (alone) {
 #pragma unroll
-          for (int k = 0; k < 32; k += 8) {
-            if (c + k >= a.D) break;
-            const uint4 y = make_uint4(pack2<T>(o[k] * inv, o[k + 1] * inv), pack2<T>(o[k + 2] * inv, o[k + 3] * inv),
-                                       pack2<T>(o[k + 4] * inv, o[k + 5] * inv), pack2<T>(o[k + 6] * inv, o[k + 7] * inv));
-            *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at * a.D + c + k) = y;
+          for (int k = 0; k < 2; ++k)
+            *reinterpret_cast<uint4*>(mine_s + lane * 32 + ((k ^ (lane >> 2 & 1)) << 4)) =
+                make_uint4(pack2<T>(o[8 * k], o[8 * k + 1]), pack2<T>(o[8 * k + 2], o[8 * k + 3]),
+                           pack2<T>(o[8 * k + 4], o[8 * k + 5]), pack2<T>(o[8 * k + 6], o[8 * k + 7]));
+          __syncwarp();
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const int rl = 16 * n + (lane >> 1), k = lane & 1, rr = 128 * i + 32 * quarter + rl;
+            int hd;
+            const int t = token_of(rr, hd);
+            if (rr < w.rows && c + 8 * k < a.D)
+              *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + ((int64_t)(w.first + t) * a.hq + h * a.G + hd) * a.D + c + 8 * k) =
+                  *reinterpret_cast<const uint4*>(mine_s + rl * 32 + ((k ^ (rl >> 2 & 1)) << 4));
           }
         } else {
 #pragma unroll
-          for (int k = 0; k < 32; k += 4) {
-            if (c + k >= a.D) break;
-            *reinterpret_cast<float4*>(a.part_o + (at * a.splits + split) * a.D + c + k) =
-                make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+          for (int k = 0; k < 4; ++k)
+            *reinterpret_cast<float4*>(mine_s + lane * 64 + ((k ^ (lane >> 1 & 3)) << 4)) =
+                make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          __syncwarp();
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const int rl = 8 * n + (lane >> 2), k = lane & 3, rr = 128 * i + 32 * quarter + rl;
+            int hd;
+            const int t = token_of(rr, hd);
+            if (rr < w.rows && c + 4 * k < a.D)
+              *reinterpret_cast<float4*>(
+                  a.part_o + (((int64_t)(w.first + t) * a.hq + h * a.G + hd) * a.splits + split) * a.D + c + 4 * k) =
+                  *reinterpret_cast<const float4*>(mine_s + rl * 64 + ((k ^ (rl >> 1 & 3)) << 4));
           }
         }
       }
+      const int64_t at = (int64_t)(w.first + tok) * a.hq + h * a.G + head;
       if (mine && part == 0) {
         if (!alone) a.part_ml[at * a.splits + split] = make_float2(m, l);
         else if (a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
@@ -793,6 +752,65 @@ bool make_pool_map(CUtensorMap* map, const void* base, int64_t rows, int D, int 
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+constexpr int kWidenKeys = 64;
+
+// The visible keys and values of an 8-bit cache as fp16 integers [seqs, heads, wide_len, D], their scales
+// [seqs, heads, wide_len] beside them; zeros past a sequence's end (to the next 128 keys) and where a
+// page does not exist. 64 keys a block; bound by memory (a key of 256 values: 516 bytes read, 1032
+// written).
+__global__ void __launch_bounds__(256) widen_kernel(const AttnArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  const int per = a.wide_len / kWidenKeys;
+  const int bh = blockIdx.x / per, k0 = (blockIdx.x - bh * per) * kWidenKeys;
+  const int b = bh / a.kv.heads, h = bh - b * a.kv.heads;
+  AttnArgs all = a;
+  all.rows_per_block = 0x7fffffff;
+  const AttnRows w = attn_rows(all, b, 0);
+  if (w.rows <= 0) return;
+  const int first = row_lo(a, w, 0) & a.lo_mask, end = min((w.len + 127) & ~127, a.wide_len);
+  if (k0 + kWidenKeys <= first || k0 >= end) return;
+  const int32_t* table = a.kv.table + b * a.kv.table_stride;
+  const int page_mask = (1 << a.kv.page_log2) - 1, seen = row_lo(a, w, 0);
+  __shared__ int row_s[kWidenKeys];
+  if (threadIdx.x < kWidenKeys) {
+    const int k = k0 + threadIdx.x;
+    int row = -1;
+    if (k < w.len && (k | page_mask) >= seen) {
+      const int page = table[k >> a.kv.page_log2];
+      if (page >= 0 && page < a.kv.pages) row = ((page * a.kv.heads + h) << a.kv.page_log2) + (k & page_mask);
+    }
+    row_s[threadIdx.x] = row;
+    const int64_t at = (int64_t)bh * a.wide_len + k;
+    a.wide_ks[at] = row < 0 ? 0.f : a.kv.k_scale[row];
+    a.wide_vs[at] = row < 0 ? 0.f : a.kv.v_scale[row];
+  }
+  __syncthreads();
+  const int pieces = a.D >> 4, n = kWidenKeys * pieces;
+  const int64_t out0 = ((int64_t)bh * a.wide_len + k0) * a.D;
+#pragma unroll
+  for (int v = 0; v < 2; ++v) {
+    const char* src = static_cast<const char*>(v ? a.kv.v : a.kv.k);
+    unsigned char* dst = static_cast<unsigned char*>(v ? a.wide_v : a.wide_k);
+#pragma unroll 4
+    for (int e = threadIdx.x; e < n; e += 256) {
+      const int key = e / pieces, p = e - key * pieces, row = row_s[key];
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (row >= 0) x = *reinterpret_cast<const uint4*>(src + (int64_t)row * a.D + 16 * p);
+      uint4 y[2];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t u = (&x.x)[j] ^ 0x80808080u;   // offset binary
+        (&y[j >> 1].x)[2 * (j & 1)] = bytes_f16(u, 0x4140);
+        (&y[j >> 1].x)[2 * (j & 1) + 1] = bytes_f16(u, 0x4342);
+      }
+      uint4* to = reinterpret_cast<uint4*>(dst + (out0 + 16 * e) * 2);
+      to[0] = y[0];
+      to[1] = y[1];
+    }
+  }
+}
+
 template <int DP, typename T, bool I8>
 int launch(const AttnArgs& a, cudaStream_t st) {
   using S = ChunkShape<DP, I8>;
@@ -809,14 +827,12 @@ int launch(const AttnArgs& a, cudaStream_t st) {
     }
     done.fetch_or(bit);
   }
-  CUtensorMap kmap = {}, vmap = {};
-  if (!I8) {
-    const int page = 1 << a.kv.page_log2;
-    const int64_t rows = ((int64_t)a.kv.pages * a.kv.heads) << a.kv.page_log2;
-    if (!encode_fn() || !make_pool_map(&kmap, a.kv.k, rows, a.D, page < 128 ? page : 128, a.q_bf16) ||
-        !make_pool_map(&vmap, a.kv.v, rows, a.D, page < S::KB ? page : S::KB, a.q_bf16))
-      return VQ2_ERR_LAUNCH;
-  }
+  CUtensorMap kmap, vmap;
+  const int page = I8 ? 128 : 1 << a.kv.page_log2;
+  const int64_t rows = I8 ? (int64_t)a.kv.seqs * a.kv.heads * a.wide_len : ((int64_t)a.kv.pages * a.kv.heads) << a.kv.page_log2;
+  if (!encode_fn() || !make_pool_map(&kmap, I8 ? a.wide_k : a.kv.k, rows, a.D, page < 128 ? page : 128, !I8 && a.q_bf16) ||
+      !make_pool_map(&vmap, I8 ? a.wide_v : a.kv.v, rows, a.D, page < S::KB ? page : S::KB, !I8 && a.q_bf16))
+    return VQ2_ERR_LAUNCH;
   const dim3 grid((unsigned)(a.kv.seqs * a.row_blocks), (unsigned)a.splits, (unsigned)a.kv.heads);
   return launch_kernel(kern, grid, dim3(S::Threads), S::Smem, st, a, kmap, vmap);
 }
@@ -828,21 +844,25 @@ int launch_shape(const AttnArgs& a, cudaStream_t st) {
 
 }  // namespace
 
-void plan_attn_chunk(AttnArgs& a, bool i8, int64_t max_new, int64_t max_len) {
+void plan_attn_chunk(AttnArgs& a, int64_t max_new, int64_t max_len) {
   const int64_t rows = max_new * a.G;
-  a.rows_per_block = a.D > 128 || i8 ? 128 : 256;
+  a.rows_per_block = a.D > 128 ? 128 : 256;
   a.row_blocks = (int)((rows + a.rows_per_block - 1) / a.rows_per_block);
   if (a.row_blocks < 1) a.row_blocks = 1;
   a.lo_mask = ~127;
-  // One block an SM. Where the blocks are fewer than two an SM, split the keys so that there are
-  // about two: a split is at least 512 keys (its start, output and joining cost about as much as 256).
+  // One block an SM. Where the blocks do not fill the card, the keys are split for one round of blocks,
+  // 256 keys at least: a split costs its start and, per row, its share of O written and read again
+  // (9 sequences of 5 drafts over 1024 keys, 18 blocks: 128 keys 20.5 us, 256 15.9, 512 18.3, whole 26;
+  // 64 tokens over 8000, 8 blocks: 256 33, 512 25.6, 1024 37). From a quarter of the card on rows are so
+  // many that a split has to take 2048 keys to pay (2048 tokens, 64 blocks: 1024 99 us, whole 69).
   int64_t keys = max_len;
   if (a.window && a.window + max_new + 128 < keys) keys = a.window + max_new + 128;
   const int64_t blocks = (int64_t)a.kv.seqs * a.kv.heads * a.row_blocks;
-  const int64_t want = blocks >= 2 * sm_count() ? 1 : 2 * sm_count() / blocks;
+  const int64_t want = blocks >= sm_count() ? 1 : sm_count() / blocks;
   int64_t chunk = (keys + 127 + want - 1) / want;
   if (chunk < (keys + 127 + 63) / 64) chunk = (keys + 127 + 63) / 64;
-  if (chunk < 512) chunk = 512;
+  const int64_t least = 4 * blocks > sm_count() ? 2048 : 256;
+  if (chunk < least) chunk = least;
   chunk = (chunk + 127) & ~int64_t(127);
   a.chunk = (int)chunk;
   a.splits = (int)((keys + 127 + chunk - 1) / chunk);   // the first key is rounded down by up to 127
@@ -850,7 +870,12 @@ void plan_attn_chunk(AttnArgs& a, bool i8, int64_t max_new, int64_t max_len) {
 }
 
 int launch_attn_chunk(const AttnArgs& a, bool i8, cudaStream_t st) {
-  if (i8) return a.q_bf16 ? launch_shape<__nv_bfloat16, true>(a, st) : launch_shape<__half, true>(a, st);
+  if (i8) {
+    const int64_t blocks = (int64_t)a.kv.seqs * a.kv.heads * (a.wide_len / kWidenKeys);
+    const int s = launch_kernel(widen_kernel, dim3((unsigned)blocks), dim3(256), 0, st, a);
+    if (s != VQ2_OK) return s;
+    return a.q_bf16 ? launch_shape<__nv_bfloat16, true>(a, st) : launch_shape<__half, true>(a, st);
+  }
   return a.q_bf16 ? launch_shape<__nv_bfloat16, false>(a, st) : launch_shape<__half, false>(a, st);
 }
 

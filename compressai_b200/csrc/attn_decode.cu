@@ -103,13 +103,6 @@ __device__ __forceinline__ bool copy_wait(uint32_t bar, uint32_t parity) {
   return true;
 }
 
-// `bytes` consecutive bytes (a multiple of 16) to shared memory, counted on `bar`.
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
-}
-
 template <int DP, int NT, bool I8, typename T>
 __global__ void __launch_bounds__(DecodeShape<DP, NT, I8>::kWarps * 32, DecodeShape<DP, NT, I8>::kPerSm)
     attn_decode_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
@@ -597,6 +590,50 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
   }
 }
 
+// The same for many rows and at most 32 splits: a warp a row, 8 heads of a token a block.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_join_rows_kernel(const AttnArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  const int t = blockIdx.x, hq = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int b = sequence_of(a.kv, t);
+  if (b < 0 || hq >= a.hq) return;
+  int first, count, lo, hi;
+  sequence_rows(a.kv, b, first, count);
+  block_keys(a, attn_rows(a, b, ((t - first) * a.G + hq % a.G) / a.rows_per_block), lo, hi);
+  if (hi - lo <= a.chunk) return;   // written already
+  const int n = min(32, (hi - lo + a.chunk - 1) / a.chunk);
+  const int64_t at = (int64_t)t * a.hq + hq;
+  const float2 x = lane < n ? a.part_ml[at * a.splits + lane] : make_float2(-INFINITY, 0.f);
+  float top = x.x;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float base = top == -INFINITY ? 0.f : top, by = ex2(x.x - base);
+  float sum = x.y * by;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  for (int d0 = 0; d0 < a.D; d0 += 128) {
+    const int d = d0 + 4 * lane;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) {
+      const float w = __shfl_sync(0xffffffffu, by, k);
+      if (d < a.D) {
+        const float4 z = *reinterpret_cast<const float4*>(a.part_o + (at * a.splits + k) * a.D + d);
+        y.x += z.x * w;
+        y.y += z.y * w;
+        y.z += z.z * w;
+        y.w += z.w * w;
+      }
+    }
+    if (d < a.D)
+      *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at * a.D + d) =
+          make_uint2(pack2<T>(y.x * inv, y.y * inv), pack2<T>(y.z * inv, y.w * inv));
+  }
+  if (a.lse && lane == 0) a.lse[at] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * kLn2;
+}
+
 // A pool [rows, D] as boxes of `keys` rows x 128 bytes, 128-byte swizzle; values past D read as zeros.
 bool make_pool_map(CUtensorMap* map, const void* base, const AttnArgs& a, bool i8, int keys) {
   const cuuint64_t e = i8 ? 1 : 2;
@@ -684,6 +721,12 @@ int launch_attn_decode(const AttnArgs& a, bool i8, cudaStream_t st) {
 }
 
 int launch_attn_join(const AttnArgs& a, cudaStream_t st) {
+  // Rows enough to fill the card with a warp a row (7000 rows over 2 splits: 25 us with a block a row).
+  if (a.splits <= 32 && (int64_t)a.T * a.hq >= 12 * sm_count()) {
+    const dim3 grid((unsigned)a.T, (unsigned)((a.hq + 7) / 8));
+    return a.q_bf16 ? launch_kernel(attn_join_rows_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, a)
+                    : launch_kernel(attn_join_rows_kernel<__half>, grid, dim3(256), 0, st, a);
+  }
   // Few splits: a whole row a block. Many: 64 values a block, 16 splits read at once (one sequence of
   // 701 tokens over 12 splits, whole step: 9.1 us with whole rows, 8.2 with 64 values; 64 sequences of
   // up to 8000 over 11: 103.5 and 108.6 us).

@@ -22,6 +22,10 @@ struct AttnArgs {
   int chunk, splits, rows_per_block, row_blocks, lo_mask;
   float* part_o;        // [T * hq, splits, D]: weighted sums of V relative to the maximum
   float2* part_ml;      // [T * hq, splits]: (maximum score in powers of two, sum of weights)
+  // 8-bit cache, many rows: the visible keys and values as fp16 [seqs, heads, wide_len, D], their scales
+  void *wide_k, *wide_v;
+  float *wide_ks, *wide_vs;
+  int wide_len;
 };
 
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -90,7 +94,7 @@ int launch_attn_join(const AttnArgs& a, cudaStream_t st);
 int launch_attn_decode(const AttnArgs& a, bool i8, cudaStream_t st);
 void plan_attn_decode(AttnArgs& a, int64_t max_new, int64_t max_len);
 int launch_attn_chunk(const AttnArgs& a, bool i8, cudaStream_t st);
-void plan_attn_chunk(AttnArgs& a, bool i8, int64_t max_new, int64_t max_len);
+void plan_attn_chunk(AttnArgs& a, int64_t max_new, int64_t max_len);
 int attn_chunk_status(int reset);   // its part of vq2_attention_status
 
 }  // namespace vq2
