@@ -84,36 +84,49 @@ __device__ __forceinline__ uint4 narrow8(const float (&f)[8]) {
   return r;
 }
 
-// Turn the 8 values at i0 in 32 bits; cs holds (cos, sin) * factor of each pair.
-__device__ __forceinline__ void rotate8(float (&x)[8], const float (&w)[8], int i0, int rot, int interleaved,
-                                        const float2* cs) {
-  if (interleaved) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int e = i0 + 2 * j;
-      if (e < rot) {
-        const float2 c = cs[e >> 1];
-        const float a = x[2 * j], b = x[2 * j + 1];
-        x[2 * j] = a * c.x - b * c.y;
-        x[2 * j + 1] = b * c.x + a * c.y;
-      }
-    }
-    return;
-  }
-  const int h = rot >> 1;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int e = i0 + j;
-    if (e < rot) {
-      const float2 c = cs[e < h ? e : e - h];
-      x[j] = x[j] * c.x + (e < h ? -w[j] : w[j]) * c.y;
-    }
-  }
+// Maximum that a NaN passes through.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
+// (cos, sin) of the 8 values at i0 -- of their 4 pairs where neighbours are paired, else of each, the
+// sine's sign the value's side -- and the turn in 32 bits. Values past the rotary width: (1, 0).
+template <bool INTER>
+struct Turn {
+  float2 c[INTER ? 4 : 8];
+  __device__ __forceinline__ void load(int i0, int rot, const float2* cs) {
+    const int h = rot >> 1;
+#pragma unroll
+    for (int j = 0; j < (INTER ? 4 : 8); ++j) {
+      const int e = INTER ? i0 + 2 * j : i0 + j;
+      c[j] = make_float2(1.f, 0.f);
+      if (e < rot) {
+        c[j] = cs[INTER ? e >> 1 : e < h ? e : e - h];
+        if (!INTER && e < h) c[j].y = -c[j].y;
+      }
+    }
+  }
+  __device__ __forceinline__ void apply(float (&x)[8], const float (&w)[8]) const {
+    if (INTER) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float a = x[2 * j], b = x[2 * j + 1];
+        x[2 * j] = a * c[j].x - b * c[j].y;
+        x[2 * j + 1] = b * c[j].x + a * c[j].y;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = x[j] * c[j].x + w[j] * c[j].y;
+    }
+  }
+};
+
 // MODE 0: rotary of q and k into contiguous outputs. MODE 1: rotary of q, k (rotated) and v into a
-// 16-bit cache. MODE 2: the same into an 8-bit cache. NIT rows per lane group.
-template <typename T, int MODE, int NIT>
+// 16-bit cache. MODE 2: the same into an 8-bit cache. NIT rows per lane group. INTER: neighbours are
+// paired, and no partners are loaded (also where nothing is turned).
+template <typename T, int MODE, int NIT, bool INTER>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
   __shared__ float2 cs[128];
   pdl_wait();
@@ -125,18 +138,19 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
   const int i0 = lane * 8;
   const bool turning = a.inv_freq != nullptr;
 
-  uint4 x[NIT], w[NIT];
+  uint4 x[NIT], w[INTER ? 1 : NIT];
 #pragma unroll
   for (int n = 0; n < NIT; ++n) {
     const int r = (blockIdx.y * NIT + n) * groups + g;
-    x[n] = w[n] = make_uint4(0, 0, 0, 0);
+    x[n] = make_uint4(0, 0, 0, 0);
+    if (!INTER) w[n] = make_uint4(0, 0, 0, 0);
     if (r < rows && i0 < a.D) {
       const int kind = r < rows_q ? 0 : r < rows_q + rows_k ? 1 : 2;
       const RopeRows& in = a.in[kind];
       const int h = kind == 0 ? r : kind == 1 ? r - rows_q : r - rows_q - rows_k;
       const T* row = static_cast<const T*>(in.x) + t * in.ts + h * in.hs;
       x[n] = load8(row + i0, in.vec);
-      if (turning && !a.interleaved && kind < 2 && i0 < a.rot) w[n] = load_partner(row, i0, a.rot, in.vec);
+      if (!INTER && turning && kind < 2 && i0 < a.rot) w[n] = load_partner(row, i0, a.rot, in.vec);
     }
   }
 
@@ -154,16 +168,18 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
   }
   if (turning) {
     for (int i = threadIdx.x; i < (a.rot >> 1); i += blockDim.x) {
-      // The angle in 64 bits, brought to one turn before it is rounded: at position 10^5 the
+      // The angle in turns in 64 bits, whole turns dropped before it is rounded: at position 10^5 the
       // product rounded to 32 bits is off by up to 0.004 rad.
-      const double full = (double)pos * (double)a.inv_freq[i];
-      const double turns = rint(full * 0.15915494309189533577);
+      const double turns = (double)pos * (double)a.inv_freq[i] * 0.15915494309189533577;
       float s, c;
-      sincosf((float)(full - turns * 6.28318530717958647692), &s, &c);
+      sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
       cs[i] = make_float2(c * a.factor, s * a.factor * a.sign);
     }
     __syncthreads();
   }
+  // a lane has the same values of every row: one set of (cos, sin) in registers
+  Turn<INTER> turn;
+  if (turning) turn.load(i0, a.rot, cs);
 
 #pragma unroll
   for (int n = 0; n < NIT; ++n) {
@@ -175,8 +191,8 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
     widen8<T>(x[n], f);
     const bool turned = turning && kind < 2 && i0 < a.rot;
     if (turned) {
-      widen8<T>(w[n], p);
-      rotate8(f, p, i0, a.rot, a.interleaved, cs);
+      if (!INTER) widen8<T>(w[n], p);
+      turn.apply(f, p);
     }
     if (MODE != 2 || kind == 0) {
       if (mine && (MODE != 1 || kind == 0 || slot >= 0)) {
@@ -187,30 +203,30 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
         *reinterpret_cast<uint4*>(dst + i0) = turned ? narrow8<T>(f) : x[n];
       }
     }
-    if (MODE == 2) {
-      // amax over the row's lanes as bit patterns: an infinity or a NaN is above every number. Rows
-      // of different kinds can share a warp, so every lane takes part.
-      uint32_t top = 0;
+    if (MODE == 2 && __any_sync(0xffffffffu, kind != 0)) {
+      // amax over the row's lanes, a NaN above all numbers. Rows of different kinds can share a warp, so
+      // every lane takes part.
+      float amax = 0.f;
       if (mine) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(fabsf(f[j])));
+        for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(f[j]));
       }
-      for (int o = 1; o < (1 << a.lanes_log2); o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      for (int o = 1; o < (1 << a.lanes_log2); o <<= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
       if (kind == 0 || !mine || slot < 0) continue;
-      const float amax = __uint_as_float(top);
-      float scale = 0.f, inv = 0.f;
-      if (top >= 0x7f800000u) scale = __uint_as_float(0x7fc00000u);
+      float scale = 0.f;
+      uint32_t o[2] = {0, 0};
+      if (!(amax < INFINITY)) scale = __uint_as_float(0x7fc00000u);
       else if (amax >= 1e-30f) {
         scale = __fdiv_rn(amax, 127.f);
-        inv = __fdiv_rn(127.f, amax);
-      }
-      uint32_t o[2] = {0, 0};
-      if (inv != 0.f) {
+        const float inv = __fdiv_rn(127.f, amax);
+        // |x * inv| <= 127 (1 + 2^-23): no clamp. Adding 1.5 * 2^23 rounds to the nearest even integer
+        // and leaves it in the low byte.
+        uint32_t u[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int v = max(-127, min(127, __float2int_rn(__fmul_rn(f[j], inv))));
-          o[j >> 2] |= (uint32_t)(v & 255) << (8 * (j & 3));
-        }
+        for (int j = 0; j < 8; ++j) u[j] = __float_as_uint(__fadd_rn(__fmul_rn(f[j], inv), 12582912.f));
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          o[j] = __byte_perm(__byte_perm(u[4 * j], u[4 * j + 1], 0x0040), __byte_perm(u[4 * j + 2], u[4 * j + 3], 0x0040), 0x5410);
       }
       const int64_t row = pool_row(a.kv, slot, h);
       int8_t* dst = static_cast<int8_t*>(const_cast<void*>(kind == 1 ? a.kv.k : a.kv.v)) + row * a.D;
@@ -293,17 +309,23 @@ int launch_rope(const RopeArgs& a, int64_t T_, cudaStream_t st) {
   const int rows = a.in[0].heads + a.in[1].heads * (MODE ? 2 : 1);
   const int per = kRopeThreads >> a.lanes_log2;
   // One row per lane group while the blocks are fewer than the card holds at once (2048 threads an
-  // SM): a lone token is spread over blocks. Then four, so that a block's table of cos and sin and
-  // its sequence lookup serve more rows.
+  // SM): a lone token is spread over blocks. Then four, so that a block's
+  // table of cos and sin and its sequence lookup serve more rows; six in the 8-bit write, which
+  // instructions bound (11,731 tokens of 32 + 16 heads of 128: four rows 78 us, six 70, eight 75).
   const int64_t blocks1 = T_ * ((rows + per - 1) / per);
   const bool wide = blocks1 > (int64_t)sm_count() * 8;
-  const int nit = wide ? 4 : 1;
+  const bool inter = a.interleaved || !a.inv_freq;
+  constexpr int kRows = MODE == 2 ? 6 : 4;
+  const int nit = !wide ? 1 : inter ? kRows : 4;
   const int y = (rows + per * nit - 1) / (per * nit);
   const int groups = (rows + y * nit - 1) / (y * nit);        // groups a block needs
   const int threads = (((groups << a.lanes_log2) + 31) / 32) * 32;
   const dim3 grid((unsigned)T_, (unsigned)y);
-  return wide ? launch_kernel(rope_kernel<T, MODE, 4>, grid, dim3(threads), 0, st, a)
-              : launch_kernel(rope_kernel<T, MODE, 1>, grid, dim3(threads), 0, st, a);
+  if (inter)
+    return wide ? launch_kernel(rope_kernel<T, MODE, kRows, true>, grid, dim3(threads), 0, st, a)
+                : launch_kernel(rope_kernel<T, MODE, 1, true>, grid, dim3(threads), 0, st, a);
+  return wide ? launch_kernel(rope_kernel<T, MODE, 4, false>, grid, dim3(threads), 0, st, a)
+              : launch_kernel(rope_kernel<T, MODE, 1, false>, grid, dim3(threads), 0, st, a);
 }
 
 RopeRows rows_of(const void* x, int64_t ts, int64_t hs, int64_t heads) {
