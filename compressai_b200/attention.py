@@ -12,15 +12,13 @@ they hold then. ``PagedKVCache`` keeps them for a program that has no allocator 
 The reference leaves these blocks to the transformers modules (vq2/load_and_test_full_35b.py:124-223),
 whose cache is concatenated anew every step.
 """
+import ctypes
 import math
+import os
 
 import torch
 
 from . import _lib
-
-_KV_CODE = {torch.float16: _lib.VQ2_F16, torch.bfloat16: _lib.VQ2_BF16, torch.int8: _lib.VQ2_I8}
-_Q_CODE = {torch.float16: _lib.VQ2_F16, torch.bfloat16: _lib.VQ2_BF16}
-
 
 def rope_frequencies(rot, theta=10000.0, scaling=None):
     """(inv_freq fp32 [rot / 2] on the CPU, factor): the angle per position of each pair, theta^(-2i/rot),
@@ -63,74 +61,27 @@ def rope_frequencies(rot, theta=10000.0, scaling=None):
     return f.float(), float(factor)
 
 
-def _call(name, device, *args):
-    """The entry point on the current stream of ``device`` (its last argument)."""
-    index = device.index
-    if index == torch._C._cuda_getDevice():
-        status = getattr(_lib._lib or _lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(device):
-            status = getattr(_lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
-    if status:
-        _lib.check(status, name)
+_host = None
 
 
-def _rows(x, name, like=None):
-    """[T, H, D] fp16 / bf16 CUDA tensor with a contiguous last dimension."""
-    if not x.is_cuda:
-        _lib.require_cuda(x)
-    if x.dim() != 3 or x.dtype not in _Q_CODE:
-        raise ValueError(f"{name} must be [tokens, heads, head_size] in fp16 or bf16; got {tuple(x.shape)} {x.dtype}")
-    if like is not None and (x.dtype != like.dtype or x.shape[0] != like.shape[0] or x.shape[2] != like.shape[2]
-                             or x.device != like.device):
-        raise ValueError(f"{name} {tuple(x.shape)} {x.dtype} does not go with {tuple(like.shape)} {like.dtype}")
-    return x if x.stride(2) == 1 or x.shape[2] == 1 else x.contiguous()
-
-
-def _int32(x, name, shape, device):
-    if x.dtype != torch.int32 or x.shape != shape or x.device != device or not x.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)} on {device}; got "
-                         f"{x.dtype} {tuple(x.shape)} on {x.device}")
-    return x.data_ptr()
-
-
-def _pools(k_pages, v_pages, k_scale, v_scale, table, dtype, heads, head_size, device):
-    """The cache's arguments as the entry points take them: (pools and scales, pages .. table cols)."""
-    code = _KV_CODE.get(k_pages.dtype)
-    if code is None or v_pages.dtype != k_pages.dtype:
-        raise ValueError(f"pools hold fp16, bf16 or int8, both the same; got {k_pages.dtype} and {v_pages.dtype}")
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or not (k_pages.is_contiguous() and v_pages.is_contiguous()):
-        raise ValueError("pools must be contiguous [pages, kv_heads, page_size, head_size], k and v alike")
-    if k_pages.device != device or v_pages.device != device:
-        raise ValueError(f"pools on {k_pages.device} and {v_pages.device}, tokens on {device}")
-    pages, h, page, d = k_pages.shape
-    ks = vs = None
-    if code == _lib.VQ2_I8:
-        for s in (k_scale, v_scale):
-            if (s is None or s.dtype != torch.float32 or s.shape != (pages, h, page) or not s.is_contiguous()
-                    or s.device != device):
-                raise ValueError("int8 pools need contiguous fp32 k_scale and v_scale [pages, kv_heads, page_size]")
-        ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
-    elif k_scale is not None or v_scale is not None:
-        raise ValueError("scales go with int8 pools only")
-    elif dtype is not None and k_pages.dtype != dtype:
-        raise ValueError(f"pools hold {k_pages.dtype}, the tokens are {dtype}")
-    if (heads is not None and h != heads) or (head_size is not None and d != head_size):
-        raise ValueError(f"pools have {h} heads of {d}; the tokens {heads} of {head_size}")
-    if table.dtype != torch.int32 or table.dim() != 2 or table.device != device or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError("table must be int32 [seqs, cols] with contiguous rows, on the tokens' device")
-    cols = table.shape[1]
-    return ((k_pages.data_ptr(), v_pages.data_ptr(), code, ks, vs),
-            (pages, h, page, d, table.data_ptr(), max(table.stride(0), cols), cols))
-
-
-def _freq(inv_freq, head_size, device):
-    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or inv_freq.device != device:
-        raise ValueError("inv_freq must be a contiguous fp32 vector on the tokens' device")
-    rot = 2 * inv_freq.shape[0]
-    if not 2 <= rot <= head_size:
-        raise ValueError(f"inv_freq turns {rot} values of a head of {head_size}")
-    return inv_freq.data_ptr(), rot
+def _load():
+    """The host module (built beside the library), with the library's entry points bound."""
+    global _host
+    if _host is None:
+        import importlib.util
+        lib = _lib.load()
+        path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "_attention_host.so")
+        if not os.path.exists(path):
+            raise _lib.VQ2Error(f"compressai_b200 attention host module not built: {path} is missing "
+                                "(run `python -m compressai_b200.build`); there is no fallback")
+        spec = importlib.util.spec_from_file_location("_attention_host", path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        names = ("vq2_rotary", "vq2_cache_write", "vq2_cache_read", "vq2_paged_attention", "vq2_paged_attention_workspace")
+        mod.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names}, _lib.check,
+                 torch.OutOfMemoryError)
+        _host = mod
+    return _host
 
 
 def rotary(q, k, positions, inv_freq, *, interleaved=False, factor=1.0, inverse=False):
@@ -138,25 +89,7 @@ def rotary(q, k, positions, inv_freq, *, interleaved=False, factor=1.0, inverse=
     (q', k'). Pair i of the first 2 * len(inv_freq) values of a head -- (x[i], x[i + len]), or (x[2i], x[2i+1]) when
     ``interleaved`` -- turns by positions * inv_freq[i] and is multiplied by ``factor``; the rest is copied. The angle
     is exact to 32 bits at any position below 2^31. ``inverse`` turns back: the gradient of the forward pass."""
-    q = _rows(q, "q")
-    T, hq, d = q.shape
-    dev = q.device
-    if positions.shape != (T,) or positions.dtype not in (torch.int32, torch.int64) or positions.device != dev:
-        raise ValueError(f"positions must be int32 or int64 [{T}] on {dev}")
-    f, rot = _freq(inv_freq, d, dev)
-    q_out = torch.empty(T, hq, d, dtype=q.dtype, device=dev)
-    k_out, k_args = None, (None, 0, 0, 0)
-    if k is not None:
-        k = _rows(k, "k", q)
-        k_out = torch.empty(T, k.shape[1], d, dtype=q.dtype, device=dev)
-        k_args = (k.data_ptr(), k.stride(0), k.stride(1), k.shape[1])
-    if not T:
-        return q_out, k_out
-    positions = positions.contiguous()
-    _call("vq2_rotary", dev, q.data_ptr(), q.stride(0), q.stride(1), hq, *k_args, _Q_CODE[q.dtype], T, d,
-          positions.data_ptr(), positions.dtype == torch.int64, f, rot, interleaved, factor, inverse, q_out.data_ptr(),
-          None if k is None else k_out.data_ptr())
-    return q_out, k_out
+    return (_host or _load()).rotary(q, k, positions, inv_freq, interleaved, factor, inverse)
 
 
 def cache_write(k, v, k_pages, v_pages, table, lens, starts=None, *, k_scale=None, v_scale=None, q=None, inv_freq=None,
@@ -165,49 +98,14 @@ def cache_write(k, v, k_pages, v_pages, table, lens, starts=None, *, k_scale=Non
     its position first, and ``q`` [T, Hq, D] with it: the turned q is returned (None without q). int8 pools: every
     (token, head) row is quantised with its own scale, amax / 127, from the turned values in 32 bits; a row with an
     infinity or a NaN reads back as NaN. Tokens whose position has no page in ``table`` are not stored."""
-    k = _rows(k, "k")
-    v = _rows(v, "v", k)
-    T, h, d = k.shape
-    dev = k.device
-    pools, shape = _pools(k_pages, v_pages, k_scale, v_scale, table, k.dtype, h, d, dev)
-    if v.shape[1] != h:
-        raise ValueError("k and v must have the same heads")
-    seqs = table.shape[0]
-    lens_p = _int32(lens, "lens", (seqs,), dev)
-    if starts is None and T != seqs:
-        raise ValueError(f"without starts every sequence has one new token; got {T} tokens for {seqs} sequences")
-    starts_p = None if starts is None else _int32(starts, "starts", (seqs + 1,), dev)
-    f, rot = (None, 0) if inv_freq is None else _freq(inv_freq, d, dev)
-    q_out, q_args = None, (None, 0, 0, 0, None)
-    if q is not None:
-        q = _rows(q, "q", k)
-        q_out = torch.empty(T, q.shape[1], d, dtype=q.dtype, device=dev)
-        q_args = (q.data_ptr(), q.stride(0), q.stride(1), q.shape[1], q_out.data_ptr())
-    if not T:
-        return q_out
-    _call("vq2_cache_write", dev, *q_args, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-          _Q_CODE[k.dtype], T, f, rot, interleaved, factor, *pools, *shape, lens_p, starts_p, seqs)
-    return q_out
+    return (_host or _load()).cache_write(k, v, k_pages, v_pages, table, k_scale, v_scale, lens, starts, q, inv_freq,
+                                          interleaved, factor)
 
 
 def cache_read(k_pages, v_pages, table, starts, total, *, k_scale=None, v_scale=None, dtype=None):
     """Whole sequences back out of the pools: (k, v) [total, kv_heads, D], sequence b's first starts[b+1] - starts[b]
     positions from row starts[b] on. ``dtype``: of the result for int8 pools (default bf16)."""
-    if not k_pages.is_cuda:
-        _lib.require_cuda(k_pages)
-    dev = k_pages.device
-    if dtype is None:
-        dtype = torch.bfloat16 if k_pages.dtype == torch.int8 else k_pages.dtype
-    if dtype not in _Q_CODE:
-        raise ValueError(f"a cache is read back as fp16 or bf16; got {dtype}")
-    pools, shape = _pools(k_pages, v_pages, k_scale, v_scale, table, dtype, None, None, dev)
-    seqs = table.shape[0]
-    starts_p = _int32(starts, "starts", (seqs + 1,), dev)
-    k, v = (torch.empty(total, shape[1], shape[3], dtype=dtype, device=dev) for _ in range(2))
-    if not total:
-        return k, v
-    _call("vq2_cache_read", dev, *pools, *shape, starts_p, seqs, k.data_ptr(), v.data_ptr(), _Q_CODE[dtype], total)
-    return k, v
+    return (_host or _load()).cache_read(k_pages, v_pages, table, k_scale, v_scale, starts, total, dtype)
 
 
 def paged_attention(q, k_pages, v_pages, table, lens, starts=None, *, k_scale=None, v_scale=None, scale=None, causal=True,
@@ -218,36 +116,5 @@ def paged_attention(q, k_pages, v_pages, table, lens, starts=None, *, k_scale=No
     defaults to D^-0.5. ``max_new`` and ``max_len`` bound every sequence's new tokens and length; the defaults (all of
     T, all that ``table`` has room for) are right and size the launch for more than may be needed. ``return_lse``:
     also fp32 [T, Hq], the natural logarithm of each row's sum of exponentials (-inf where no key is seen)."""
-    q = _rows(q, "q")
-    T, hq, d = q.shape
-    dev = q.device
-    pools, shape = _pools(k_pages, v_pages, k_scale, v_scale, table, q.dtype, None, d, dev)
-    h = shape[1]
-    if hq % h or not hq:
-        raise ValueError(f"{hq} query heads do not share {h} key/value heads")
-    seqs = table.shape[0]
-    lens_p = _int32(lens, "lens", (seqs,), dev)
-    room = shape[6] * shape[2]
-    max_len = room if max_len is None else min(int(max_len), room)
-    if starts is None:
-        if T != seqs:
-            raise ValueError(f"without starts every sequence has one new token; got {T} tokens for {seqs} sequences")
-        max_new, starts_p = 1, None
-    else:
-        starts_p = _int32(starts, "starts", (seqs + 1,), dev)
-        max_new = T if max_new is None else min(int(max_new), T)
-    if window < 0 or max_len < 0 or max_new < 0:
-        raise ValueError("window, max_new and max_len count tokens: none is negative")
-    if q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(1) % 8:  # the kernels read 16 bytes at a time
-        q = q.clone(memory_format=torch.contiguous_format)
-    out = torch.empty(T, hq, d, dtype=q.dtype, device=dev)
-    lse = torch.empty(T, hq, dtype=torch.float32, device=dev) if return_lse else None
-    if not T:
-        return (out, lse) if return_lse else out
-    lib = _lib._lib or _lib.load()
-    nbytes = lib.vq2_paged_attention_workspace(T, hq, h, d, pools[2], seqs, max_new, max_len, window)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _call("vq2_paged_attention", dev, q.data_ptr(), q.stride(0), q.stride(1), _Q_CODE[q.dtype], T, hq, *pools, *shape,
-          lens_p, starts_p, seqs, max_new, max_len, d ** -0.5 if scale is None else scale, causal, window,
-          out.data_ptr(), lse.data_ptr() if return_lse else None, ws.data_ptr() if nbytes else None, nbytes)
-    return (out, lse) if return_lse else out
+    return (_host or _load()).paged_attention(q, k_pages, v_pages, table, k_scale, v_scale, lens, starts, scale, causal, window,
+                                              max_new, max_len, return_lse)

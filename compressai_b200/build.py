@@ -5,6 +5,9 @@ linked into one shared library with a static CUDA runtime; the library exports o
 ``vq2_*`` symbols declared in ``include/vq2_b200.h``. Object files are cached under
 ``compressai_b200/_build`` and rebuilt when a source or header is newer.
 
+``csrc/attention_host.cpp``, the host side of ``compressai_b200.attention``, is compiled by g++
+against the installed torch into ``lib/_attention_host.so`` beside it.
+
 Usage: python -m compressai_b200.build [--force] [--jobs N]
 """
 import argparse
@@ -22,6 +25,7 @@ INCLUDE = os.path.join(REPO, "include")
 BUILD = os.path.join(PKG, "_build")
 LIBDIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIBDIR, "libvq2_b200.so")
+HOST = os.path.join(LIBDIR, "_attention_host.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-fvisibility=hidden",
@@ -60,14 +64,40 @@ def _compile(src, force):
     return obj, log
 
 
+def _build_host(force):
+    """lib/_attention_host.so: a CPython module over torch's C++ headers."""
+    import sysconfig
+
+    import torch
+    src = os.path.join(CSRC, "attention_host.cpp")
+    if not force and not _stale(HOST, src):
+        return HOST
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    tmp = HOST + ".tmp"
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", INCLUDE,
+           "-I", sysconfig.get_paths()["include"], "-isystem", os.path.join(root, "include"),
+           "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           "-isystem", os.path.join(cuda, "include"), src, "-o", tmp, "-L", os.path.join(root, "lib"),
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, HOST)
+    return HOST
+
+
 def build(force=False, jobs=None):
-    """Compile every csrc/*.cu for sm_100a and link lib/libvq2_b200.so. Returns the path."""
+    """Compile every csrc/*.cu for sm_100a and link lib/libvq2_b200.so (returned), and lib/_attention_host.so."""
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(LIBDIR, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
     jobs = jobs or min(len(srcs), os.cpu_count() or 4)
-    with cf.ThreadPoolExecutor(jobs) as ex:
+    with cf.ThreadPoolExecutor(jobs + 1) as ex:
+        host = ex.submit(_build_host, force)
         objs = [o for o, _ in ex.map(lambda s: _compile(s, force), srcs)]
+        host.result()
     if force or not os.path.exists(LIB) or any(os.path.getmtime(o) > os.path.getmtime(LIB) for o in objs):
         tmp = LIB + ".tmp"
         cmd = [nvcc(), *ARCH, "-shared", "-cudart", "static", "-o", tmp, *objs]
