@@ -118,3 +118,76 @@ def paged_attention(q, k_pages, v_pages, table, lens, starts=None, *, k_scale=No
     also fp32 [T, Hq], the natural logarithm of each row's sum of exponentials (-inf where no key is seen)."""
     return (_host or _load()).paged_attention(q, k_pages, v_pages, table, k_scale, v_scale, lens, starts, scale, causal, window,
                                               max_new, max_len, return_lse)
+
+
+class PagedKVCache:
+    """The cache of a model's attention layers: pools for ``layers`` layers that share one page table, and who
+    has which page. A program ``add``s sequences, says with ``begin`` how many tokens each one adds, and then
+    calls ``write`` and ``attend`` once a layer; ``release`` gives a sequence's pages back.
+
+    ``dtype`` is that of q, k and v, or torch.int8, which quantises what is written. The tables are kept on
+    the host and go to the device in one copy a step."""
+
+    def __init__(self, layers, pages, kv_heads, head_size, *, page_size=64, max_len=32768, dtype=torch.bfloat16,
+                 device="cuda"):
+        if pages < 1 or layers < 1 or max_len < 1:
+            raise ValueError("layers, pages and max_len are at least 1")
+        self.page_size, self.max_len, self.device = page_size, max_len, torch.device(device)
+        shape = (pages, kv_heads, page_size, head_size)
+        self.pools = [tuple(torch.empty(shape, dtype=dtype, device=device) for _ in range(2)) for _ in range(layers)]
+        self.scales = [tuple(torch.empty(shape[:3], device=device) for _ in range(2)) if dtype == torch.int8 else (None, None)
+                       for _ in range(layers)]
+        self.free = list(range(pages - 1, -1, -1))
+        self.pages, self.lengths = {}, {}
+        self._next, self.batch = 0, None
+
+    def add(self):
+        """A new, empty sequence's id."""
+        self._next += 1
+        self.pages[self._next], self.lengths[self._next] = [], 0
+        return self._next
+
+    def release(self, seq):
+        self.free += reversed(self.pages.pop(seq))
+        del self.lengths[seq]
+
+    def begin(self, seqs, counts):
+        """The next calls' tokens are ``counts[i]`` new ones of sequence ``seqs[i]``, in this order. Pages are taken
+        for all of them or, with a MemoryError, for none."""
+        if len(seqs) != len(counts) or len(set(seqs)) != len(seqs) or any(c < 0 for c in counts):
+            raise ValueError("seqs are different sequences, counts their numbers of new tokens")
+        P = self.page_size
+        lens = [self.lengths[s] + c for s, c in zip(seqs, counts)]
+        if max(lens, default=0) > self.max_len:
+            raise ValueError(f"a sequence of {max(lens)} tokens: this cache's are at most {self.max_len}")
+        need = [-(-n // P) - len(self.pages[s]) for s, n in zip(seqs, lens)]
+        if sum(need) > len(self.free):
+            raise MemoryError(f"{sum(need)} pages are needed, {len(self.free)} are free")
+        for s, n, k in zip(seqs, lens, need):
+            self.pages[s] += [self.free.pop() for _ in range(k)]
+            self.lengths[s] = n
+        B, cols = len(seqs), max([len(self.pages[s]) for s in seqs] + [1])
+        starts = [0]
+        for c in counts:
+            starts.append(starts[-1] + c)
+        flat = lens + starts + [p for s in seqs for p in self.pages[s] + [-1] * (cols - len(self.pages[s]))]
+        host = torch.tensor(flat, dtype=torch.int32)
+        if self.device.type == "cuda":
+            host = host.pin_memory()
+        t = host.to(self.device, non_blocking=True)
+        one = all(c == 1 for c in counts)
+        self.batch = dict(lens=t[:B], starts=None if one else t[B:2 * B + 1], table=t[2 * B + 1:].view(B, cols),
+                          max_new=max(counts, default=0), max_len=max(lens, default=0))
+
+    def write(self, layer, k, v, *, q=None, inv_freq=None, interleaved=False, factor=1.0):
+        """``cache_write`` of the batch's tokens into a layer."""
+        b = self.batch
+        return cache_write(k, v, *self.pools[layer], b["table"], b["lens"], b["starts"], k_scale=self.scales[layer][0],
+                           v_scale=self.scales[layer][1], q=q, inv_freq=inv_freq, interleaved=interleaved, factor=factor)
+
+    def attend(self, layer, q, *, scale=None, causal=True, window=0):
+        """``paged_attention`` of the batch's tokens over a layer."""
+        b = self.batch
+        return paged_attention(q, *self.pools[layer], b["table"], b["lens"], b["starts"], k_scale=self.scales[layer][0],
+                               v_scale=self.scales[layer][1], scale=scale, causal=causal, window=window,
+                               max_new=b["max_new"], max_len=b["max_len"])

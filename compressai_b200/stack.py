@@ -14,13 +14,16 @@ is built without materialising its dense weights, then
     config has it);
   * norms, the DeltaNet convolution / decay parameters and the rotary tables stay the reference's
     PyTorch modules, initialised here.
+
+``use_paged_attention`` then gives the full-attention layers this library's rotary, paged cache (bf16 or
+int8) and attention in place of the transformers cache, and ``decode(..., cache=...)`` decodes with it.
 """
 import math
 
 import torch
 import torch.nn as nn
 
-from . import ep, moe, runtime, synth, vq
+from . import attention, ep, moe, runtime, synth, vq
 
 
 class VQMoEBlock(nn.Module):
@@ -143,25 +146,78 @@ def build_vq2_moe_model(config=None, device="cuda", seed=0, group=None, max_toke
     return model
 
 
+class PagedAttention(nn.Module):
+    """Drop-in for Qwen3_5MoeAttention: its projections, norms and output gate, around one fused launch
+    that turns q and k and writes k and v into the paged cache, and the attention over it."""
+
+    def __init__(self, attn, cache, layer, inv_freq):
+        super().__init__()
+        self.attn, self.cache, self.layer, self.inv_freq = attn, cache, layer, inv_freq
+
+    def forward(self, hidden_states, position_embeddings=None, attention_mask=None, past_key_values=None, **kwargs):
+        a, lead = self.attn, hidden_states.shape[:-1]
+        q, gate = a.q_proj(hidden_states).reshape(lead.numel(), -1, 2 * a.head_dim).chunk(2, dim=-1)
+        q = a.q_norm(q)
+        k = a.k_norm(a.k_proj(hidden_states).reshape(lead.numel(), -1, a.head_dim))
+        v = a.v_proj(hidden_states).reshape(lead.numel(), -1, a.head_dim)
+        q = self.cache.write(self.layer, k, v, q=q, inv_freq=self.inv_freq)
+        o = self.cache.attend(self.layer, q, scale=a.scaling)
+        return a.o_proj((o * torch.sigmoid(gate)).reshape(*lead, -1)), None
+
+
+def use_paged_attention(model, pages, page_size=64, max_len=32768, dtype=torch.bfloat16):
+    """Replace the model's full-attention layers by PagedAttention over one new PagedKVCache (returned):
+    ``pages`` pages of ``page_size`` tokens, bf16 or int8."""
+    cfg = model.config
+    dev = next(model.parameters()).device
+    layers = [m for m in model.model.layers if hasattr(m, "self_attn")]
+    cache = attention.PagedKVCache(len(layers), pages, cfg.num_key_value_heads, cfg.head_dim, page_size=page_size,
+                                   max_len=max_len, dtype=dtype, device=dev)
+    rope = cfg.rope_parameters
+    if rope.get("rope_type", "default") != "default":
+        raise ValueError(f"rotary type {rope['rope_type']!r}: build inv_freq with attention.rope_frequencies")
+    inv_freq, _ = attention.rope_frequencies(int(cfg.head_dim * rope.get("partial_rotary_factor", 1.0)), rope["rope_theta"])
+    for i, m in enumerate(layers):
+        m.self_attn = PagedAttention(m.self_attn, cache, i, inv_freq.to(dev))
+    return cache
+
+
 @torch.no_grad()
-def decode(model, batch, prompt_len=4, steps=8, warmup=2, seed=0):
+def decode(model, batch, prompt_len=4, steps=8, warmup=2, seed=0, cache=None):
     """Greedy decode of ``batch`` sequences: prefill ``prompt_len`` tokens, then ``warmup`` +
-    ``steps`` one-token steps through the HF cache; returns (seconds per timed step, final ids)."""
+    ``steps`` one-token steps through the HF cache; returns (seconds per timed step, final ids).
+    ``cache``: what use_paged_attention returned, holding the full-attention layers' keys and values
+    (the HF cache then holds the DeltaNet states alone)."""
     dev = next(model.parameters()).device
     g = torch.Generator(device=dev).manual_seed(seed)
     ids = torch.randint(0, model.config.vocab_size, (batch, prompt_len), generator=g, device=dev)
-    out = model(input_ids=ids, use_cache=True)
+    seqs = [cache.add() for _ in range(batch)] if cache is not None else None
+    try:
+        return _decode(model, ids, steps, warmup, cache, seqs)
+    finally:
+        for s in seqs or ():
+            cache.release(s)
+
+
+def _decode(model, ids, steps, warmup, cache, seqs):
+    dev = ids.device
+
+    def forward(ids, past):
+        if cache is not None:
+            cache.begin(seqs, [ids.shape[1]] * len(seqs))
+        return model(input_ids=ids, past_key_values=past, use_cache=True)
+    out = forward(ids, None)
     past = out.past_key_values
     nxt = out.logits[:, -1].argmax(-1, keepdim=True)
     for _ in range(warmup):
-        out = model(input_ids=nxt, past_key_values=past, use_cache=True)
+        out = forward(nxt, past)
         past = out.past_key_values
         nxt = out.logits[:, -1].argmax(-1, keepdim=True)
     torch.cuda.synchronize(dev)
     e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
     e0.record()
     for _ in range(steps):
-        out = model(input_ids=nxt, past_key_values=past, use_cache=True)
+        out = forward(nxt, past)
         past = out.past_key_values
         nxt = out.logits[:, -1].argmax(-1, keepdim=True)
     e1.record()

@@ -1,0 +1,48 @@
+"""PagedKVCache's bookkeeping on the host (no device needed): pages, tables, refusals."""
+import pytest
+import torch
+
+from compressai_b200.attention import PagedKVCache
+
+
+def cache(pages=6, **kw):
+    return PagedKVCache(2, pages, 1, 16, page_size=16, device="cpu", **kw)
+
+
+def test_pages_follow_lengths_and_come_back():
+    c = cache()
+    a, b = c.add(), c.add()
+    c.begin([a, b], [17, 0])
+    assert c.batch["lens"].tolist() == [17, 0] and c.batch["starts"].tolist() == [0, 17, 17]
+    assert c.batch["table"].tolist() == [[0, 1], [-1, -1]] and c.batch["max_new"] == 17 and c.batch["max_len"] == 17
+    c.begin([b, a], [1, 1])
+    assert c.batch["lens"].tolist() == [1, 18] and c.batch["starts"] is None
+    assert c.batch["table"].tolist() == [[2, -1], [0, 1]]
+    c.release(a)
+    c.begin([b], [64])
+    assert c.lengths[b] == 65 and c.pages[b] == [2, 0, 1, 3, 4] and len(c.free) == 1
+    d = c.add()
+    c.begin([d], [16])
+    assert c.pages[d] == [5] and not c.free
+
+
+def test_refusals_change_nothing():
+    c = cache(max_len=90)
+    a, b = c.add(), c.add()
+    c.begin([a], [33])
+    before = (list(c.free), dict(c.lengths), c.batch["lens"].tolist())
+    with pytest.raises(MemoryError):
+        c.begin([a, b], [1, 64])
+    for seqs, counts in (([a], [1, 2]), ([a, a], [1, 1]), ([a], [-1]), ([a], [58])):
+        with pytest.raises(ValueError):
+            c.begin(seqs, counts)
+    assert before == (list(c.free), dict(c.lengths), c.batch["lens"].tolist())
+    for args in ((0, 4, 1, 16), (1, 0, 1, 16)):
+        with pytest.raises(ValueError):
+            PagedKVCache(*args, device="cpu")
+
+
+def test_int8_pools_have_scales():
+    c = cache(dtype=torch.int8)
+    assert c.pools[1][0].dtype == torch.int8 and c.scales[1][1].shape == (6, 1, 16)
+    assert cache(dtype=torch.float16).scales[0] == (None, None)
