@@ -103,7 +103,7 @@ extern "C" int vq2_paged_attention(const void* q, int64_t q_token_stride, int64_
   const bool i8 = kv_dtype == VQ2_I8;
   const int64_t bytes = plan(a, i8, starts ? max_new : 1, max_len, chunked, static_cast<char*>(workspace));
   if (bytes && (!workspace || workspace_bytes < bytes)) return VQ2_ERR_ARG;
-  if ((int64_t)a.kv.seqs * a.row_blocks > 0x7fffffff) return VQ2_ERR_SHAPE;
+  if ((int64_t)a.kv.seqs * a.row_blocks > 0x3fffffff) return VQ2_ERR_SHAPE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   s = chunked ? launch_attn_chunk(a, i8, st) : launch_attn_decode(a, i8, st);
   if (s != VQ2_OK || a.splits == 1) return s;

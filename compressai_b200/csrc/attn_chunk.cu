@@ -15,6 +15,11 @@
 //     row tile) the chain of its 128 maxima and exponentials set the pace: 3 us a step where the
 //     MMAs take 1.1. The threads of a row agree through one named barrier whether any score asks
 //     for a new maximum. Maxima, sums and O are 32 bits; P is rounded to the cache's 16 bits.
+// Head sizes above 128 run as pairs of blocks (cluster of 2, cta_group::2): an MMA then spans both, each
+// holding 128 of 256 rows in its tensor memory and half of K's keys and V's values in its shared memory.
+// One block alone has to bring 128 KB a step for 128 rows, and waited for it 3500 of 4900 cycles (7 TB/s
+// out of L2 over all SMs; prefill of 8192 tokens 684 us); a pair's block brings half of that.
+//
 // With two row tiles the tensor core works on one while the softmax works on the other; with one
 // (head size 256, O takes half of tensor memory) S is double-buffered and QK of the next tile runs
 // under the softmax.
@@ -57,9 +62,11 @@ constexpr int kBlock = 16384;                    // bytes of a ring block
 
 template <int DP, bool I8>
 struct ChunkShape {
-  static constexpr int NQ = DP > 128 ? 1 : 2;        // row tiles of 128
-  static constexpr int B = DP / 64;                  // ring blocks of a 128-key tile, K or V
-  static constexpr int KB = 8192 / DP;               // keys of a V block
+  static constexpr bool Pair = DP > 128;             // two blocks work as one, each with half of K and V
+  static constexpr int NQ = Pair ? 1 : 2;            // row tiles of 128 in a block
+  static constexpr int QC = DP / 64;                 // 16 KB blocks of a row tile's queries
+  static constexpr int B = Pair ? 2 : DP / 64;       // ring blocks of a 128-key tile, K or V
+  static constexpr int KB = Pair ? 64 : 8192 / DP;   // keys of a V block
   static constexpr int Q = NQ * 128 * DP * 2;
   static constexpr int NB = I8 ? (DP == 64 ? 10 : 9) : DP == 64 ? 12 : 10;   // ring blocks
   static constexpr int TPR = 4 / NQ;                 // threads of a row in the softmax
@@ -79,7 +86,8 @@ struct ChunkCtl {
   uint64_t pv;                    // one row tile: each product into O (before a rescale)
   uint64_t tail;                  // V rows past the last key are zeroed
   uint64_t drain;
-  uint64_t q_full;                // the queries are in shared memory
+  uint64_t q_full;                // the queries are in shared memory (a pair: both blocks')
+  uint64_t q_here, tail_here;     // a pair: this block's queries; its copy of the V block with the last key
   uint64_t scales[8];             // 8-bit cache: the scales of tile j (mod 8) are there
   uint32_t tmem_base;
   int abort;
@@ -90,10 +98,12 @@ __device__ __forceinline__ void chunk_fail(ChunkCtl* c) {
   *reinterpret_cast<volatile int*>(&c->abort) = 1;
   atomicMax(&g_attention_status, VQ2_ERR_TIMEOUT);
 }
+template <bool CLUSTER = false>   // CLUSTER: arrivals come from the pair's other block too
 __device__ __forceinline__ bool chunk_wait(uint32_t bar, uint32_t parity, ChunkCtl* c) {
-  if (mbar_try(bar, parity)) return true;
+  auto ready = [&] { return CLUSTER ? mbar_try_cluster(bar, parity) : mbar_try(bar, parity); };
+  if (ready()) return true;
   const long long t0 = clock64();
-  while (!mbar_try(bar, parity)) {
+  while (!ready()) {
     if (*reinterpret_cast<volatile int*>(&c->abort)) return false;
     if (clock64() - t0 > kWaitCycles) {
       chunk_fail(c);
@@ -117,6 +127,27 @@ template <int KB>
 __device__ __forceinline__ uint64_t v_desc(uint32_t saddr) {
   return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(KB * 128 >> 4) << 16) |
          (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
+}
+
+template <bool PAIR>
+__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  if (PAIR) tma_load_2d_pair(dst, map, x, y, bar);
+  else tma_load_2d(dst, map, x, y, bar);
+}
+template <bool PAIR>
+__device__ __forceinline__ void umma(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t accumulate) {
+  if (PAIR) umma2_f16(d, ad, bd, idesc, accumulate);
+  else umma_f16(d, ad, bd, idesc, accumulate);
+}
+template <bool PAIR>
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t at, uint64_t bd, uint32_t idesc, uint32_t accumulate) {
+  if (PAIR) umma2_f16_ts(d, at, bd, idesc, accumulate);
+  else umma_f16_ts(d, at, bd, idesc, accumulate);
+}
+template <bool PAIR>   // of a pair: on the barrier in both blocks
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if (PAIR) umma2_commit(bar);
+  else umma_commit(bar);
 }
 
 // Barrier `id` of n threads (whole warps): whether any of them says p.
@@ -205,6 +236,7 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
   using S = ChunkShape<DP, I8>;
   using M = typename std::conditional<I8, __half, T>::type;
   constexpr int NQ = S::NQ, B = S::B, KB = S::KB, NB = S::NB;
+  constexpr bool PAIR = S::Pair;
   constexpr bool BF = std::is_same<M, __nv_bfloat16>::value;
   extern __shared__ __align__(1024) unsigned char sm[];
   unsigned char* ring = sm + S::Q;
@@ -221,7 +253,9 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kMma = S::Mma, TPR = S::TPR, W = S::W;
   // the last rows see the most keys: they go first
-  const int b = blockIdx.x / a.row_blocks, rb = a.row_blocks - 1 - (blockIdx.x - b * a.row_blocks);
+  const int rank = PAIR ? blockIdx.x & 1 : 0;   // of a pair: which row tile, which half of K's keys and V's values
+  const int bx = PAIR ? blockIdx.x >> 1 : blockIdx.x;
+  const int b = bx / a.row_blocks, rb = a.row_blocks - 1 - (bx - b * a.row_blocks);
   const int split = blockIdx.y, h = blockIdx.z;
   const AttnRows w = attn_rows(a, b, rb);
   if (w.rows <= 0) return;
@@ -240,24 +274,38 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(su32(&ctl->s_full[i]), 1);
-      mbar_init(su32(&ctl->p_full[i]), 4 * S::TPR);
+      mbar_init(su32(&ctl->p_full[i]), 4 * TPR * (PAIR ? 2 : 1));
       mbar_init(su32(&ctl->o_full[i]), 1);
     }
     mbar_init(su32(&ctl->pv), 1);
-    mbar_init(su32(&ctl->tail), 1);
+    mbar_init(su32(&ctl->tail), PAIR ? 2 : 1);
+    mbar_init(su32(&ctl->tail_here), 1);
+    mbar_init(su32(&ctl->q_here), 4 * TPR);
     mbar_init(su32(&ctl->drain), 1);
-    mbar_init(su32(&ctl->q_full), 4 * TPR * nq);
+    mbar_init(su32(&ctl->q_full), 4 * TPR * (PAIR ? 2 : nq));
     for (int i = 0; i < 8; ++i) mbar_init(su32(&ctl->scales[i]), 1);
     ctl->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kMma) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&ctl->tmem_base)) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&ctl->tmem_base)) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&ctl->tmem_base)) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   tc_fence_before();
-  __syncthreads();
+  if (PAIR) cluster_sync();
+  else __syncthreads();
   tc_fence_after();
+  // A pair's MMAs are issued by its first block, which the other's copies, queries and weights report to.
+  auto lead = [&](uint64_t* bar) { return PAIR ? in_block(su32(bar), 0) : su32(bar); };
+  auto arrive = [&](uint64_t* bar) {
+    if (PAIR) mbar_arrive_cluster(in_block(su32(bar), 0));
+    else mbar_arrive(su32(bar));
+  };
   const uint32_t tmem = ctl->tmem_base;
   const int gran = I8 ? KB : min(1 << a.kv.page_log2, KB);   // keys of one V copy
   const int tail = !I8 && (s1 & (gran - 1)) ? s1 : -1;    // rows from here on, up to the copy's end, hold anything
@@ -279,15 +327,18 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
     };
     int q = 0, said = 0;
     bool ok = true;
-    const int rk = I8 ? 128 : min(1 << a.kv.page_log2, 128);   // keys of one K copy
-    // lane i's copy of a K block: keys i * rk ..; of a V block: values 64 * (i % B), keys (i / B) * gran ..
+    constexpr int KK = PAIR ? 64 : 128, KS = PAIR ? 2 : 1;   // keys and 64-value groups of a K block
+    const int rk = I8 ? KK : min(1 << a.kv.page_log2, KK);   // keys of one K copy
+    // lane i's copy of a K block: values 64 * (i % KS), keys (i / KS) * rk ..; of a V block: values
+    // 64 * (i % B), keys (i / B) * gran ..
+    const int ki = lane / KS * rk;
     auto load = [&](bool is_v, int j) {
       const int k0 = s0 + 128 * j;
       int row[B];   // this lane's pool row for each block, looked up ahead of the waits
 #pragma unroll
       for (int c = 0; c < B; ++c) row[c] = pool_rows;
       if (!is_v) {
-        if (lane * rk < 128) row[0] = row_of(k0 + lane * rk);
+        if (ki < KK) row[0] = row_of(k0 + KK * rank + ki);
       } else {
 #pragma unroll
         for (int c = 0; c < B; ++c)
@@ -306,21 +357,29 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
         ok = chunk_wait(su32(&ctl->empty[slot]), ((q / NB) & 1) ^ 1, ctl);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        const uint32_t bar = su32(&ctl->full[slot]), dst = su32(ring + slot * kBlock);
-        if (lane == 0) mbar_arrive_tx(bar, kBlock);
+        const uint32_t dst = su32(ring + slot * kBlock);
+        const int kb = k0 + c * KB;
+        const bool last = is_v && tail > kb && tail < kb + KB;   // the block that holds the last key and what follows it
+        const uint32_t bar = PAIR && last ? su32(&ctl->tail_here) : lead(&ctl->full[slot]);
+        if (lane == 0) {
+          if (!PAIR || last) mbar_arrive_tx(bar, kBlock);
+          if (PAIR && rank == 0) {
+            if (last) mbar_arrive(su32(&ctl->full[slot]));
+            else mbar_arrive_tx(su32(&ctl->full[slot]), 2 * kBlock);   // both blocks' copies
+          }
+        }
         __syncwarp();
         if (!is_v) {
-          if (lane * rk < 128) tma_load_2d(dst + lane * rk * 128, &kmap, 64 * c, row[0], bar);
+          if (ki < KK) load_2d<PAIR>(dst + lane % KS * KK * 128 + ki * 128, &kmap, 64 * (KS * c + lane % KS), row[0], bar);
         } else {
           int r = row[0];
 #pragma unroll
           for (int i = 1; i < B; ++i)
             if (i == c) r = row[i];
           if ((lane / B) * gran < KB)
-            tma_load_2d(dst + (lane % B) * KB * 128 + (lane / B) * gran * 128, &vmap, 64 * (lane % B), r, bar);
-          const int kb = k0 + c * KB;
-          if (tail > kb && tail < kb + KB) {  // zero what follows the last key in its copy
-            ok = __all_sync(0xffffffffu, chunk_wait(bar, (q / NB) & 1, ctl));
+            load_2d<PAIR>(dst + (lane % B) * KB * 128 + (lane / B) * gran * 128, &vmap, 64 * (B * rank + lane % B), r, bar);
+          if (last) {  // zero what follows the last key in its copy
+            ok = __all_sync(0xffffffffu, chunk_wait(bar, PAIR ? 0 : (q / NB) & 1, ctl));
             if (!ok) { ++q; break; }
             const int from = tail - kb, to = (from + gran - 1) / gran * gran;
             for (int e = lane; e < (to - from) * B * 8; e += 32) {
@@ -330,7 +389,7 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
             }
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(su32(&ctl->tail));
+            if (lane == 0) arrive(&ctl->tail);
           }
         }
       }
@@ -349,7 +408,11 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
     }
     // copies this warp started have landed before the block's shared memory goes away
     if (!ok) {
-      for (int i = max(0, q - NB); i < q; ++i) chunk_drain(su32(&ctl->full[i % NB]), (i / NB) & 1);
+      if (PAIR) {   // the other block's copies, and this one's that nobody here can wait for: 100 us is ample
+        const long long t0 = clock64();
+        while (clock64() - t0 < 200000) {}
+      }
+      for (int i = max(0, q - NB); !PAIR && i < q; ++i) chunk_drain(su32(&ctl->full[i % NB]), (i / NB) & 1);
       if (I8)   // scales: at most 8 tiles' are under way; those waited for already answer at once
         for (int i = max(0, said - 8); i < said; ++i) chunk_drain(su32(&ctl->scales[i & 7]), (i >> 3) & 1);
     }
@@ -358,11 +421,11 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
     // One elected thread. elect.sync rather than a lane number: the compiler then knows a single thread
     // runs and keeps descriptors in uniform registers; behind `lane == 0` each MMA was issued in about
     // 140 cycles, twice what it takes to execute.
-    if (elect_one()) {
-      constexpr uint32_t QK = umma_idesc<128, BF>(), PV = umma_idesc<DP, BF>(true);
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t QK = umma_idesc<128, BF>(false, PAIR ? 256 : 128), PV = umma_idesc<DP, BF>(true, PAIR ? 256 : 128);
       const uint64_t qd = sw128_desc(su32(sm)), kd = sw128_desc(su32(ring)), vd = v_desc<KB>(su32(ring));
       const uint32_t full0 = su32(&ctl->full[0]), empty0 = su32(&ctl->empty[0]);
-      bool ok = tiles == 0 || chunk_wait(su32(&ctl->q_full), 0, ctl);
+      bool ok = tiles == 0 || chunk_wait<PAIR>(su32(&ctl->q_full), 0, ctl);
       int ks = 0, vs = 0, kp = 0, vp = 0;   // slot and parity of the next K and V tile's first block
       auto skip = [&](int& slot, int& parity, int n) {
         slot += n;
@@ -377,16 +440,22 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
 #pragma unroll
         for (int c = 0; c < B; ++c) {
           if (i == 0) {
-            if (!chunk_wait(full0 + 8 * slot, parity, ctl)) return false;
+            if (!chunk_wait<PAIR>(full0 + 8 * slot, parity, ctl)) return false;
             tc_fence_after();
           }
-          const uint64_t ad = qd + (i * B + c) * (kBlock >> 4), bd = kd + slot * (kBlock >> 4);
+          constexpr int KS = PAIR ? 2 : 1;   // 64-value groups of the block
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) umma_f16(tmem + 128 * s, ad + 2 * kk, bd + 2 * kk, QK, (c | kk) != 0);
-          if (i == nq - 1) umma_commit(empty0 + 8 * slot);
+          for (int g = 0; g < KS; ++g) {
+            const uint64_t ad = qd + (i * S::QC + KS * c + g) * (kBlock >> 4);
+            const uint64_t bd = kd + slot * (kBlock >> 4) + g * (kBlock / KS >> 4);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma<PAIR>(tmem + 128 * s, ad + 2 * kk, bd + 2 * kk, QK, (c | g | kk) != 0);
+          }
+          if (i == nq - 1) commit<PAIR>(empty0 + 8 * slot);
           skip(slot, parity, 1);
         }
-        umma_commit(su32(&ctl->s_full[s]));
+        commit<PAIR>(su32(&ctl->s_full[s]));
         return true;
       };
       // O of row tile i += weights in buffer s times V tile j
@@ -396,22 +465,22 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
         for (int c = 0; c < B; ++c) {
           if (i == 0) {
             const int kb = s0 + 128 * j + c * KB;
-            if (!chunk_wait(full0 + 8 * slot, parity, ctl)) return false;
-            if (!I8 && tail > kb && tail < kb + KB && !chunk_wait(su32(&ctl->tail), 0, ctl)) return false;
+            if (!chunk_wait<PAIR>(full0 + 8 * slot, parity, ctl)) return false;
+            if (!I8 && tail > kb && tail < kb + KB && !chunk_wait<PAIR>(su32(&ctl->tail), 0, ctl)) return false;
             tc_fence_after();
           }
           const uint64_t bd = vd + slot * (kBlock >> 4);
 #pragma unroll
           for (int kk = 0; kk < KB / 16; ++kk) {
             const int key = c * KB + 16 * kk;   // of the tile: its weights stand in the columns of its part's scores
-            umma_f16_ts(tmem + S::O0 + i * DP, tmem + 128 * s + key / S::W * S::W + key % S::W / 2, bd + 128 * kk, PV,
-                        (c | kk) != 0 || j > 0);
+            umma_ts<PAIR>(tmem + S::O0 + i * DP, tmem + 128 * s + key / S::W * S::W + key % S::W / 2, bd + 128 * kk, PV,
+                          (c | kk) != 0 || j > 0);
           }
-          if (i == nq - 1) umma_commit(empty0 + 8 * slot);
+          if (i == nq - 1) commit<PAIR>(empty0 + 8 * slot);
           skip(slot, parity, 1);
         }
-        if (NQ == 1) umma_commit(su32(&ctl->pv));
-        if (j == tiles - 1) umma_commit(su32(&ctl->o_full[i]));
+        if (NQ == 1) commit<PAIR>(su32(&ctl->pv));
+        if (j == tiles - 1) commit<PAIR>(su32(&ctl->o_full[i]));
         return true;
       };
       // ring order K0 V0 K1 V1 .. with two row tiles, K0 K1 V0 K2 V1 .. with one
@@ -437,21 +506,24 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
         for (int j = 0; j < tiles && ok; ++j) {
           if (j + 1 < tiles) ok = qk(0, (j + 1) & 1);
           skip(ks, kp, 2 * B);
-          ok = ok && chunk_wait(su32(&ctl->p_full[j & 1]), (j >> 1) & 1, ctl);
+          ok = ok && chunk_wait<PAIR>(su32(&ctl->p_full[j & 1]), (j >> 1) & 1, ctl);
           if (!ok) break;
           tc_fence_after();
           ok = pv(0, j, j & 1);
           skip(vs, vp, j + 2 == tiles ? B : 2 * B);   // the last V follows the one before it
         }
       }
-      umma_commit(su32(&ctl->drain));   // every MMA issued has completed before TMEM is freed
+      // every MMA issued has completed before TMEM is freed
+      if (PAIR) umma2_commit_here(su32(&ctl->drain));
+      else umma_commit(su32(&ctl->drain));
       chunk_drain(su32(&ctl->drain), 0);
     }
     __syncwarp();
   } else if (warp / (4 * TPR) < nq) {
     // ---------------------------------------------------------------------------- softmax
     const int i = warp / (4 * TPR), part = (warp >> 2) % TPR, quarter = warp & 3;
-    const int r = 128 * i + 32 * quarter + lane;   // row of the block
+    const int tile = PAIR ? rank : i;              // row tile of the rows
+    const int r = 128 * tile + 32 * quarter + lane;   // row
     const bool mine = r < w.rows;
     // Row rr of the block is new token t0 + (g0 + rr) / G, head (g0 + rr) % G: small numbers, divided by
     // a multiplication.
@@ -474,9 +546,9 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
         for (int n = 0; n < R; ++n) {
           const int e = tid + (n0 + n) * kThreads, rr = e / (DP / 8), v = e % (DP / 8);  // row of the tile, 8-value piece
           x[n] = make_uint4(0, 0, 0, 0);
-          if (128 * i + rr < w.rows && 8 * v < a.D) {
+          if (128 * tile + rr < w.rows && 8 * v < a.D) {
             int head;
-            const int t = token_of(128 * i + rr, head);
+            const int t = token_of(128 * tile + rr, head);
             x[n] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(w.first + t) * a.q_ts +
                                                    (int64_t)(h * a.G + head) * a.q_hs + 8 * v);
           }
@@ -508,12 +580,15 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
             }
             if (v == 0) undo_s[128 * i + rr] = back;
           }
-          *reinterpret_cast<uint4*>(sm + (i * B + (v >> 3)) * kBlock + rr * 128 + (((v & 7) ^ (rr & 7)) << 4)) = x[n];
+          *reinterpret_cast<uint4*>(sm + (i * S::QC + (v >> 3)) * kBlock + rr * 128 + (((v & 7) ^ (rr & 7)) << 4)) = x[n];
         }
       }
       fence_proxy_async();
       __syncwarp();
-      if (lane == 0) mbar_arrive(su32(&ctl->q_full));
+      if (lane == 0) {
+        if (PAIR) mbar_arrive(su32(&ctl->q_here));
+        arrive(&ctl->q_full);
+      }
     }
     int head = 0;
     const int tok = token_of(mine ? r : 0, head);
@@ -525,8 +600,8 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
     bool ok = true, leave = false;   // a wait that gives up; all threads of the rows know of one
     float scale = fabsf(a.scale_log2);
     if (I8 && tiles > 0) {
-      ok = chunk_wait(su32(&ctl->q_full), 0, ctl);
-      scale *= undo_s[r];
+      ok = chunk_wait(su32(PAIR ? &ctl->q_here : &ctl->q_full), 0, ctl);
+      scale *= undo_s[128 * i + 32 * quarter + lane];
     }
     // what the threads of this row leave for one another
     float* said = part_s + (warp - 4 * part) * 32 + lane;   // part p: said[128 * p]
@@ -658,7 +733,7 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(su32(&ctl->p_full[buf]));
+      if (lane == 0) arrive(&ctl->p_full[buf]);
     }
     {
       const float2 x = unpair(l2), y = unpair(l3);
@@ -676,7 +751,7 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
       const float inv = l == 0.f ? 0.f : 1.f / l;
       // 16 values of 32 rows at a time through 2 KB of the tile's queries, which nobody reads any more:
       // a row's 16 values then go out as whole sectors.
-      unsigned char* mine_s = sm + i * B * kBlock + (warp - 4 * TPR * i) * 2048;
+      unsigned char* mine_s = sm + i * S::QC * kBlock + (warp - 4 * TPR * i) * 2048;
 #pragma unroll 1
       for (int c = part * (DP / TPR); c < (part + 1) * (DP / TPR); c += 16) {
         float o[16];
@@ -697,7 +772,7 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
           __syncwarp();
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
-            const int rl = 16 * n + (lane >> 1), k = lane & 1, rr = 128 * i + 32 * quarter + rl;
+            const int rl = 16 * n + (lane >> 1), k = lane & 1, rr = 128 * tile + 32 * quarter + rl;
             int hd;
             const int t = token_of(rr, hd);
             if (rr < w.rows && c + 8 * k < a.D)
@@ -712,7 +787,7 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
           __syncwarp();
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
-            const int rl = 8 * n + (lane >> 2), k = lane & 3, rr = 128 * i + 32 * quarter + rl;
+            const int rl = 8 * n + (lane >> 2), k = lane & 3, rr = 128 * tile + 32 * quarter + rl;
             int hd;
             const int t = token_of(rr, hd);
             if (rr < w.rows && c + 4 * k < a.D)
@@ -731,10 +806,12 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
   }
 
   tc_fence_before();
-  __syncthreads();
+  if (PAIR) cluster_sync();   // neither block's memory goes away while the other may still reach it
+  else __syncthreads();
   if (warp == kMma) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
   }
 }
 
@@ -830,10 +907,12 @@ int launch(const AttnArgs& a, cudaStream_t st) {
   CUtensorMap kmap, vmap;
   const int page = I8 ? 128 : 1 << a.kv.page_log2;
   const int64_t rows = I8 ? (int64_t)a.kv.seqs * a.kv.heads * a.wide_len : ((int64_t)a.kv.pages * a.kv.heads) << a.kv.page_log2;
-  if (!encode_fn() || !make_pool_map(&kmap, I8 ? a.wide_k : a.kv.k, rows, a.D, page < 128 ? page : 128, !I8 && a.q_bf16) ||
+  if (!encode_fn() || !make_pool_map(&kmap, I8 ? a.wide_k : a.kv.k, rows, a.D, page < (S::Pair ? 64 : 128) ? page : S::Pair ? 64 : 128, !I8 && a.q_bf16) ||
       !make_pool_map(&vmap, I8 ? a.wide_v : a.kv.v, rows, a.D, page < S::KB ? page : S::KB, !I8 && a.q_bf16))
     return VQ2_ERR_LAUNCH;
   const dim3 grid((unsigned)(a.kv.seqs * a.row_blocks), (unsigned)a.splits, (unsigned)a.kv.heads);
+  if (S::Pair)
+    return launch_cluster(kern, dim3(2 * grid.x, grid.y, grid.z), dim3(S::Threads), S::Smem, 2, st, a, kmap, vmap);
   return launch_kernel(kern, grid, dim3(S::Threads), S::Smem, st, a, kmap, vmap);
 }
 
@@ -846,7 +925,7 @@ int launch_shape(const AttnArgs& a, cudaStream_t st) {
 
 void plan_attn_chunk(AttnArgs& a, int64_t max_new, int64_t max_len) {
   const int64_t rows = max_new * a.G;
-  a.rows_per_block = a.D > 128 ? 128 : 256;
+  a.rows_per_block = 256;   // head size above 128: of a pair of blocks
   a.row_blocks = (int)((rows + a.rows_per_block - 1) / a.rows_per_block);
   if (a.row_blocks < 1) a.row_blocks = 1;
   a.lo_mask = ~127;
@@ -857,7 +936,7 @@ void plan_attn_chunk(AttnArgs& a, int64_t max_new, int64_t max_len) {
   // many that a split has to take 2048 keys to pay (2048 tokens, 64 blocks: 1024 99 us, whole 69).
   int64_t keys = max_len;
   if (a.window && a.window + max_new + 128 < keys) keys = a.window + max_new + 128;
-  const int64_t blocks = (int64_t)a.kv.seqs * a.kv.heads * a.row_blocks;
+  const int64_t blocks = (int64_t)a.kv.seqs * a.kv.heads * a.row_blocks * (a.D > 128 ? 2 : 1);
   const int64_t want = blocks >= sm_count() ? 1 : sm_count() / blocks;
   int64_t chunk = (keys + 127 + want - 1) / want;
   if (chunk < (keys + 127 + 63) / 64) chunk = (keys + 127 + 63) / 64;
