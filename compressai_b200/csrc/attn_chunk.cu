@@ -733,7 +733,10 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive(&ctl->p_full[buf]);
+      if (lane == 0) {   // the weights are in tensor memory: nothing else to release
+        if (PAIR) mbar_arrive_cluster_relaxed(in_block(su32(&ctl->p_full[buf]), 0));
+        else mbar_arrive(su32(&ctl->p_full[buf]));
+      }
     }
     {
       const float2 x = unpair(l2), y = unpair(l3);
