@@ -91,6 +91,7 @@ struct ChunkCtl {
   uint64_t scales[8];             // 8-bit cache: the scales of tile j (mod 8) are there
   uint32_t tmem_base;
   int abort;
+  int page[4][8];                 // of the key tiles being loaded
 };
 static_assert(sizeof(ChunkCtl) <= 512, "control block");
 
@@ -130,10 +131,17 @@ __device__ __forceinline__ uint64_t v_desc(uint32_t saddr) {
 }
 
 template <bool PAIR>
-__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-  if (PAIR) tma_load_2d_pair(dst, map, x, y, bar);
-  else tma_load_2d(dst, map, x, y, bar);
+__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  if (PAIR) tma_load_3d_pair(dst, map, x, y, z, bar);
+  else tma_load_3d(dst, map, x, y, z, bar);
 }
+
+// 64-value groups that one copy brings: `groups` where the head size is made of whole groups and the
+// copy has all keys of the block (the groups then stand in shared memory as the block wants them).
+__host__ __device__ constexpr int copy_groups(int D, bool all_keys, int groups) {
+  return D % 64 == 0 && all_keys ? groups : 1;
+}
+
 template <bool PAIR>
 __device__ __forceinline__ void umma(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t accumulate) {
   if (PAIR) umma2_f16(d, ad, bd, idesc, accumulate);
@@ -316,94 +324,111 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
 
   if (warp == S::Load) {
     // ---------------------------------------------------------------------------- loads
+    // One elected thread, for the reason given at the MMA issuer: copies issued by several lanes are
+    // serialised through the uniform registers one by one, and the MMAs waited for them.
     const int pool_rows = (a.kv.pages * a.kv.heads) << a.kv.page_log2;
     const int wide_row0 = I8 ? (b * a.kv.heads + h) * a.wide_len : 0;
-    // pool row of key k, or past the pool (zeros) where there is none
-    auto row_of = [&](int k) {
-      if (I8) return wide_row0 + k;
-      if (k >= s1 || (k | page_mask) < seen) return pool_rows;
-      const int page = table[k >> a.kv.page_log2];
-      return page < 0 || page >= a.kv.pages ? pool_rows : ((page * a.kv.heads + h) << a.kv.page_log2) + (k & page_mask);
-    };
-    int q = 0, said = 0;
-    bool ok = true;
     constexpr int KK = PAIR ? 64 : 128, KS = PAIR ? 2 : 1;   // keys and 64-value groups of a K block
     const int rk = I8 ? KK : min(1 << a.kv.page_log2, KK);   // keys of one K copy
-    // lane i's copy of a K block: values 64 * (i % KS), keys (i / KS) * rk ..; of a V block: values
-    // 64 * (i % B), keys (i / B) * gran ..
-    const int ki = lane / KS * rk;
-    auto load = [&](bool is_v, int j) {
-      const int k0 = s0 + 128 * j;
-      int row[B];   // this lane's pool row for each block, looked up ahead of the waits
+    // 64-value groups of one copy: all of the block's where its keys are one copy too
+    const int kg = copy_groups(a.D, rk == KK, KS), vg = copy_groups(a.D, gran == KB, B);
+    int q = 0, said = 0;
+    bool ok = true;
+    if (tiles > 0 && elect_one()) {
+      // The pages of a key tile (128 / page size, at least one) are looked up a tile ahead, and once for K and
+      // V: this thread's instructions, a few cycles each, are what a copy costs.
+      const int shift = a.kv.page_log2, count = max(1, 128 >> shift), first_page = seen >> shift, last_page = (s1 - 1) >> shift;
+      auto look = [&](int j, int i) {
+        const int p = ((s0 + 128 * j) >> shift) + i;
+        return i < count && p >= first_page && p <= last_page ? table[p] : -1;
+      };
+      const uint32_t full0 = PAIR ? in_block(su32(&ctl->full[0]), 0) : su32(&ctl->full[0]), empty0 = su32(&ctl->empty[0]);
+      const int part0 = a.D % 64 == 0 ? 0 : 64, part1 = a.D % 64 == 0;   // where a 64-value group stands in the map
+      int slot = 0, parity = 1;
+      // K or V of key tile j
+      auto load = [&](auto is_v, int j) {
+        constexpr bool V = decltype(is_v)::value;
+        constexpr int keys = V ? KB : KK, groups = V ? B : KS;
+        const int k0 = s0 + 128 * j, step = V ? gran : rk, per = V ? vg : kg;
+        int next[8];
+        if (!I8 && !V && j + 1 < tiles) {
 #pragma unroll
-      for (int c = 0; c < B; ++c) row[c] = pool_rows;
-      if (!is_v) {
-        if (ki < KK) row[0] = row_of(k0 + KK * rank + ki);
-      } else {
+          for (int i = 0; i < 8; ++i)
+            if (i < count) next[i] = look(j + 1, i);
+        }
+        if (I8 && !V) {   // the tile's scales, with K; their place is free long before the ring's is
+          const uint32_t bar = su32(&ctl->scales[j & 7]), dst = su32(scale_s + (j & 7) * 256);
+          mbar_arrive_tx(bar, 1024);
+          bulk_load(dst, a.wide_ks + wide_row0 + k0, 512, bar);
+          bulk_load(dst + 512, a.wide_vs + wide_row0 + k0, 512, bar);
+          said = j + 1;
+        }
 #pragma unroll
-        for (int c = 0; c < B; ++c)
-          if ((lane / B) * gran < KB) row[c] = row_of(k0 + c * KB + (lane / B) * gran);
-      }
-      if (I8 && !is_v) said = j + 1;
-      if (I8 && !is_v && lane == 0) {   // the tile's scales, with K; their place is free long before the ring's is
-        const uint32_t bar = su32(&ctl->scales[j & 7]), dst = su32(scale_s + (j & 7) * 256);
-        mbar_arrive_tx(bar, 1024);
-        bulk_load(dst, a.wide_ks + wide_row0 + k0, 512, bar);
-        bulk_load(dst + 512, a.wide_vs + wide_row0 + k0, 512, bar);
-      }
-#pragma unroll 1
-      for (int c = 0; c < B && ok; ++c, ++q) {
-        const int slot = q % NB;
-        ok = chunk_wait(su32(&ctl->empty[slot]), ((q / NB) & 1) ^ 1, ctl);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const uint32_t dst = su32(ring + slot * kBlock);
-        const int kb = k0 + c * KB;
-        const bool last = is_v && tail > kb && tail < kb + KB;   // the block that holds the last key and what follows it
-        const uint32_t bar = PAIR && last ? su32(&ctl->tail_here) : lead(&ctl->full[slot]);
-        if (lane == 0) {
+        for (int c = 0; c < B; ++c) {
+          if (!chunk_wait(empty0 + 8 * slot, parity, ctl)) return false;
+          const uint32_t dst = su32(ring) + slot * kBlock;
+          const int kb = c * KB;   // of the tile
+          const bool last = V && tail > k0 + kb && tail < k0 + kb + KB;   // the block that holds the last key and what follows it
+          const uint32_t bar = PAIR && last ? su32(&ctl->tail_here) : full0 + 8 * slot;
           if (!PAIR || last) mbar_arrive_tx(bar, kBlock);
           if (PAIR && rank == 0) {
             if (last) mbar_arrive(su32(&ctl->full[slot]));
             else mbar_arrive_tx(su32(&ctl->full[slot]), 2 * kBlock);   // both blocks' copies
           }
-        }
-        __syncwarp();
-        if (!is_v) {
-          if (ki < KK) load_2d<PAIR>(dst + lane % KS * KK * 128 + ki * 128, &kmap, 64 * (KS * c + lane % KS), row[0], bar);
-        } else {
-          int r = row[0];
-#pragma unroll
-          for (int i = 1; i < B; ++i)
-            if (i == c) r = row[i];
-          if ((lane / B) * gran < KB)
-            load_2d<PAIR>(dst + (lane % B) * KB * 128 + (lane / B) * gran * 128, &vmap, 64 * (B * rank + lane % B), r, bar);
-          if (last) {  // zero what follows the last key in its copy
-            ok = __all_sync(0xffffffffu, chunk_wait(bar, PAIR ? 0 : (q / NB) & 1, ctl));
-            if (!ok) { ++q; break; }
-            const int from = tail - kb, to = (from + gran - 1) / gran * gran;
-            for (int e = lane; e < (to - from) * B * 8; e += 32) {
-              const int rr = from + e / (B * 8), p = e % (B * 8);
-              *reinterpret_cast<uint4*>(ring + slot * kBlock + (p >> 3) * KB * 128 + rr * 128 + ((p & 7) << 4)) =
-                  make_uint4(0, 0, 0, 0);
+          const int key0 = V ? kb : KK * rank, g0 = V ? B * rank : KS * c;
+#pragma unroll 1
+          for (int i = 0; i < keys; i += step) {
+            const int k = k0 + key0 + i;
+            int row = wide_row0 + k;
+            if (!I8) {   // past the pool (zeros) where there is no key, or no page
+              const int page = ctl->page[j & 3][(key0 + i) >> shift];
+              row = k >= s1 || page < 0 || page >= a.kv.pages ? pool_rows : ((page * a.kv.heads + h) << shift) + (k & page_mask);
             }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) arrive(&ctl->tail);
+#pragma unroll 1
+            for (int g = 0; g < groups; g += per)
+              load_3d<PAIR>(dst + g * keys * 128 + i * 128, V ? &vmap : &kmap, part0 * (g0 + g), row, part1 * (g0 + g), bar);
+          }
+          ++q;
+          if (++slot == NB) {
+            slot = 0;
+            parity ^= 1;
           }
         }
-      }
-    };
-    if (tiles > 0) load(false, 0);
-    if (NQ == 2) {
+        if (!I8 && !V && j + 1 < tiles) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i < count) ctl->page[(j + 1) & 3][i] = next[i];
+        }
+        return true;
+      };
+      using K_ = std::false_type;
+      using V_ = std::true_type;
+      if (!I8)
+        for (int i = 0; i < count; ++i) ctl->page[0][i] = look(0, i);
+      // the MMAs' order: K0 V0 K1 V1 .. with two row tiles, K0 K1 V0 K2 V1 .. with one
+      ok = load(K_(), 0);
       for (int j = 0; j < tiles && ok; ++j) {
-        load(true, j);
-        if (j + 1 < tiles && ok) load(false, j + 1);
+        if (NQ == 2) ok = load(V_(), j) && (j + 1 == tiles || load(K_(), j + 1));
+        else ok = (j + 1 == tiles || load(K_(), j + 1)) && load(V_(), j);
       }
-    } else {
-      for (int j = 0; j < tiles && ok; ++j) {
-        if (j + 1 < tiles) load(false, j + 1);
-        if (ok) load(true, j);
+    }
+    __syncwarp();
+    ok = __all_sync(0xffffffffu, ok);
+    q = __reduce_max_sync(0xffffffffu, q);
+    said = __reduce_max_sync(0xffffffffu, said);
+    if (ok && tail >= 0 && tiles > 0) {   // the whole warp zeroes what follows the last key in its copy
+      const int kl = s0 + 128 * (tiles - 1), c = (tail - kl) / KB, at = (2 * tiles - 1) * B + c, kb = kl + c * KB;
+      ok = __all_sync(0xffffffffu, chunk_wait(su32(PAIR ? &ctl->tail_here : &ctl->full[at % NB]), PAIR ? 0 : (at / NB) & 1, ctl));
+      if (ok) {
+        const int from = tail - kb, to = (from + gran - 1) / gran * gran;
+        for (int e = lane; e < (to - from) * B * 8; e += 32) {
+          const int rr = from + e / (B * 8), p = e % (B * 8);
+          *reinterpret_cast<uint4*>(ring + at % NB * kBlock + (p >> 3) * KB * 128 + rr * 128 + ((p & 7) << 4)) =
+              make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) arrive(&ctl->tail);
       }
     }
     // copies this warp started have landed before the block's shared memory goes away
@@ -818,16 +843,19 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
   }
 }
 
-// A pool [rows, D] (every page's every head) as copies of `box` rows x 64 values, 128-byte swizzle;
-// values past D and rows past the pool read as zeros.
-bool make_pool_map(CUtensorMap* map, const void* base, int64_t rows, int D, int box, bool bf16) {
+// A pool [rows, D] (every page's every head) as copies of `groups` x `box` rows x 64 values, 128-byte
+// swizzle: three dimensions, 64 values, rows, 64-value groups (head sizes not made of whole groups: D
+// values, rows, 1, a copy a group). Values past D and rows past the pool read as zeros.
+bool make_pool_map(CUtensorMap* map, const void* base, int64_t rows, int D, int box, int groups, bool bf16) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(D) * 2};
-  const cuuint32_t boxes[2] = {64, static_cast<cuuint32_t>(box)};
-  const cuuint32_t es[2] = {1, 1};
-  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims,
+  const bool whole = D % 64 == 0;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(whole ? 64 : D), static_cast<cuuint64_t>(rows),
+                              static_cast<cuuint64_t>(whole ? D / 64 : 1)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(D) * 2, static_cast<cuuint64_t>(whole ? 128 : D * 2)};
+  const cuuint32_t boxes[3] = {64, static_cast<cuuint32_t>(box), static_cast<cuuint32_t>(groups)};
+  const cuuint32_t es[3] = {1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims,
             strides, boxes, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -908,10 +936,11 @@ int launch(const AttnArgs& a, cudaStream_t st) {
     done.fetch_or(bit);
   }
   CUtensorMap kmap, vmap;
-  const int page = I8 ? 128 : 1 << a.kv.page_log2;
+  constexpr int KK = S::Pair ? 64 : 128;   // keys of a K block
+  const int page = I8 ? 128 : 1 << a.kv.page_log2, kbox = page < KK ? page : KK, vbox = page < S::KB ? page : S::KB;
   const int64_t rows = I8 ? (int64_t)a.kv.seqs * a.kv.heads * a.wide_len : ((int64_t)a.kv.pages * a.kv.heads) << a.kv.page_log2;
-  if (!encode_fn() || !make_pool_map(&kmap, I8 ? a.wide_k : a.kv.k, rows, a.D, page < (S::Pair ? 64 : 128) ? page : S::Pair ? 64 : 128, !I8 && a.q_bf16) ||
-      !make_pool_map(&vmap, I8 ? a.wide_v : a.kv.v, rows, a.D, page < S::KB ? page : S::KB, !I8 && a.q_bf16))
+  if (!make_pool_map(&kmap, I8 ? a.wide_k : a.kv.k, rows, a.D, kbox, copy_groups(a.D, kbox == KK, S::Pair ? 2 : 1), !I8 && a.q_bf16) ||
+      !make_pool_map(&vmap, I8 ? a.wide_v : a.kv.v, rows, a.D, vbox, copy_groups(a.D, vbox == S::KB, S::B), !I8 && a.q_bf16))
     return VQ2_ERR_LAUNCH;
   const dim3 grid((unsigned)(a.kv.seqs * a.row_blocks), (unsigned)a.splits, (unsigned)a.kv.heads);
   if (S::Pair)

@@ -303,6 +303,16 @@ def test_attention_page_sizes(page, int8):
     d.check(d.run(starts=None))
 
 
+@pytest.mark.parametrize("page", [16, 64, 128, 256])
+@pytest.mark.parametrize("d", [64, 160, 192, 256])
+def test_attention_pages_end_inside_tiles(page, d):
+    """Sequences that end everywhere in a tile and a page, every unwritten row of it NaN."""
+    lens = [33, 64, 65, 95, 128, 129, 191, 193, 257, 300]
+    s = Setup([min(n, 40) for n in lens], lens, 8, 2, d, torch.float16, False, page, seed=26)
+    s.check(s.run())
+    s.check(s.run(window=70), window=70)
+
+
 @pytest.mark.parametrize("int8", [False, True])
 def test_attention_rows_that_see_nothing(int8):
     """Empty sequences, more new tokens than the cache holds, and tokens of no sequence: zeros, lse -inf."""
