@@ -12,12 +12,14 @@ namespace {
 // Which kernel, the splits of the keys and the workspace they and a widened 8-bit cache take: a function
 // of shapes and bounds alone. Points into `ws` where it is given; returns its bytes.
 int64_t plan(AttnArgs& a, bool i8, int64_t max_new, int64_t max_len, bool& chunked, char* ws) {
-  // Rows that share a key: the decode kernel holds 16 (head size above 128) or 32 of them; from there
-  // on it would read the keys again for every 16 or 32, and the tensor-core kernel takes over. Its fp16
-  // copy of an 8-bit cache is kept to 4 GB; past that (a batch of very long sequences) the decode kernel
-  // reads the 8 bits again after all.
+  // Rows that share a key: the decode kernel holds 16 and would read the keys again for more; from there
+  // on the tensor-core kernel takes over (16 sequences of 4000 tokens, 32/8 heads of 128: 16 rows 60 us
+  // here, 20 to 40 rows 63 us there; 32 rows here took 100). Over an 8-bit cache, which it has to widen
+  // first, from 49 rows on (the same, 32 rows: 96 us here, 156 there; 16/2 heads of 256: 63 and 88). Its
+  // fp16 copy of an 8-bit cache is kept to 4 GB; past that (a batch of very long sequences) the decode
+  // kernel reads the 8 bits again after all.
   const int64_t wide_len = (max_len + 127) & ~int64_t(127), wide_rows = a.kv.seqs * (int64_t)a.kv.heads * wide_len;
-  chunked = max_new * a.G > (a.D > 128 ? 16 : 32) && (!i8 || wide_rows * a.D <= int64_t(1) << 30);
+  chunked = max_new * a.G > (i8 ? 48 : 16) && (!i8 || wide_rows * a.D <= int64_t(1) << 30);
   if (chunked) plan_attn_chunk(a, max_new, max_len);
   else plan_attn_decode(a, max_new, max_len);
   int64_t at = 0;

@@ -70,7 +70,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 template <int DP, int NT, bool I8>
 struct DecodeShape {
   static constexpr int kC = I8 ? DP / 128 : DP / 64;    // 128-byte pieces of a row
-  static constexpr int kU = DP == 256 || NT == 4 ? 1 : 2;   // 16-key tiles a step, as registers allow
+  static constexpr int kU = DP == 256 ? 1 : 2;          // 16-key tiles a step, as registers allow
   static constexpr int kKeys = 16 * kU;
   static constexpr int kBox = kKeys * 128;              // bytes of one piece of a step's keys
   static constexpr int kHalf = kC * kBox;               // K or V of a step
@@ -673,19 +673,17 @@ template <bool I8, typename T>
 int launch_shape(const AttnArgs& a, cudaStream_t st) {
   const int nt = a.rows_per_block / 8;
   if (a.D > 128) return nt == 1 ? launch<256, 1, I8, T>(a, st) : launch<256, 2, I8, T>(a, st);
-  if (I8 || a.D > 64)
-    return nt == 1 ? launch<128, 1, I8, T>(a, st) : nt == 2 ? launch<128, 2, I8, T>(a, st) : launch<128, 4, I8, T>(a, st);
-  return nt == 1 ? launch<64, 1, false, T>(a, st) : nt == 2 ? launch<64, 2, false, T>(a, st) : launch<64, 4, false, T>(a, st);
+  if (I8 || a.D > 64) return nt == 1 ? launch<128, 1, I8, T>(a, st) : launch<128, 2, I8, T>(a, st);
+  return nt == 1 ? launch<64, 1, false, T>(a, st) : launch<64, 2, false, T>(a, st);
 }
 
 }  // namespace
 
 void plan_attn_decode(AttnArgs& a, int64_t max_new, int64_t max_len) {
-  // Rows of a block: all that share a key, up to the accumulators that registers hold.
+  // Rows of a block: 8, or 16 where more share a key (32 spilled and was slower than the tensor-core
+  // kernel: 16 sequences of 4000 tokens, 32 rows, D 128: 100 us).
   const int64_t rows = max_new * a.G;
-  const int cap = a.D > 128 ? 2 : 4;
-  int nt = 1;
-  while (nt < cap && 8 * nt < rows) nt *= 2;
+  const int nt = rows <= 8 ? 1 : 2;
   a.rows_per_block = 8 * nt;
   a.row_blocks = (int)((rows + 8 * nt - 1) / (8 * nt));
   if (a.row_blocks < 1) a.row_blocks = 1;
