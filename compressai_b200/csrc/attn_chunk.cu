@@ -188,6 +188,11 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -668,11 +673,12 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
         if (I8) {
 #pragma unroll
           for (int k = 0; k < 32; k += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(ks + c + k);
-            s[k] *= f.x;
-            s[k + 1] *= f.y;
-            s[k + 2] *= f.z;
-            s[k + 3] *= f.w;
+            const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(ks + c + k);
+            const float2 x = unpair(mul2(pair(s[k], s[k + 1]), f.x)), y = unpair(mul2(pair(s[k + 2], s[k + 3]), f.y));
+            s[k] = x.x;
+            s[k + 1] = x.y;
+            s[k + 2] = y.x;
+            s[k + 3] = y.y;
           }
         }
         if (masked) {
@@ -731,8 +737,8 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
       }
       const float base = m == -INFINITY ? 0.f : m;
       const uint64_t scale2 = pair(scale, scale), base2 = pair(-base, -base);
-#pragma unroll
-      for (int c = 0; c < W; c += 32) {
+      const uint64_t vinv2 = pair(vinv, vinv);
+      auto weigh = [&](auto hides, int c) {   // hides: some keys of the tile are masked
         float s[32];
         uint32_t p[16];
         scores(c, s);
@@ -740,20 +746,30 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
         for (int k = 0; k < 32; k += 4) {
           const float2 x = unpair(fma2(pair(s[k], s[k + 1]), scale2, base2));
           const float2 z = unpair(fma2(pair(s[k + 2], s[k + 3]), scale2, base2));
-          float y0 = ex2(x.x), y1 = ex2(x.y), y2 = ex2(z.x), y3 = ex2(z.y);
-          l2 = add2(l2, pair(y0, y1));
-          l3 = add2(l3, pair(y2, y3));
-          if (I8) {   // a masked key's scale may be anything
-            const float4 f = *reinterpret_cast<const float4*>(vs + c + k);
-            y0 = masked && y0 == 0.f ? 0.f : y0 * (f.x * vinv);
-            y1 = masked && y1 == 0.f ? 0.f : y1 * (f.y * vinv);
-            y2 = masked && y2 == 0.f ? 0.f : y2 * (f.z * vinv);
-            y3 = masked && y3 == 0.f ? 0.f : y3 * (f.w * vinv);
+          uint64_t y = pair(ex2(x.x), ex2(x.y)), w = pair(ex2(z.x), ex2(z.y));
+          l2 = add2(l2, y);
+          l3 = add2(l3, w);
+          if (I8) {
+            const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(vs + c + k);
+            y = mul2(y, mul2(f.x, vinv2));
+            w = mul2(w, mul2(f.y, vinv2));
           }
-          p[k / 2] = pack2<M>(y0, y1);
-          p[k / 2 + 1] = pack2<M>(y2, y3);
+          float2 u = unpair(y), v = unpair(w);
+          if (I8 && decltype(hides)::value) {   // a masked key's scale may be anything, and 0 * NaN is not 0
+            if (s[k] == -INFINITY) u.x = 0.f;
+            if (s[k + 1] == -INFINITY) u.y = 0.f;
+            if (s[k + 2] == -INFINITY) v.x = 0.f;
+            if (s[k + 3] == -INFINITY) v.y = 0.f;
+          }
+          p[k / 2] = pack2<M>(u.x, u.y);
+          p[k / 2 + 1] = pack2<M>(v.x, v.y);
         }
         tmem_st16(own + c / 2, p);   // over scores that this thread has read
+      };
+#pragma unroll
+      for (int c = 0; c < W; c += 32) {
+        if (I8 && masked) weigh(std::true_type(), c);
+        else weigh(std::false_type(), c);
       }
       tmem_wait_st();
       tc_fence_before();
@@ -894,25 +910,31 @@ __global__ void __launch_bounds__(256) widen_kernel(const AttnArgs a) {
     a.wide_vs[at] = row < 0 ? 0.f : a.kv.v_scale[row];
   }
   __syncthreads();
-  const int pieces = a.D >> 4, n = kWidenKeys * pieces;
-  const int64_t out0 = ((int64_t)bh * a.wide_len + k0) * a.D;
+  // 256 / pieces keys a round; the loads of two rounds, K's and V's, go out together
+  const int pieces = a.D >> 4, per_round = 256 / pieces, key0 = threadIdx.x / pieces, p = threadIdx.x - key0 * pieces;
+  if (key0 >= per_round) return;
+  const int64_t out0 = ((int64_t)bh * a.wide_len + k0) * a.D + 16 * p;
+  for (int k = key0; k < kWidenKeys; k += 2 * per_round) {
+    uint4 x[4];
 #pragma unroll
-  for (int v = 0; v < 2; ++v) {
-    const char* src = static_cast<const char*>(v ? a.kv.v : a.kv.k);
-    unsigned char* dst = static_cast<unsigned char*>(v ? a.wide_v : a.wide_k);
-#pragma unroll 4
-    for (int e = threadIdx.x; e < n; e += 256) {
-      const int key = e / pieces, p = e - key * pieces, row = row_s[key];
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (row >= 0) x = *reinterpret_cast<const uint4*>(src + (int64_t)row * a.D + 16 * p);
+    for (int i = 0; i < 4; ++i) {
+      const int key = k + (i >> 1) * per_round, row = key < kWidenKeys ? row_s[key] : -1;
+      const char* src = static_cast<const char*>(i & 1 ? a.kv.v : a.kv.k);
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (row >= 0) x[i] = *reinterpret_cast<const uint4*>(src + (int64_t)row * a.D + 16 * p);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int key = k + (i >> 1) * per_round;
+      if (key >= kWidenKeys) continue;
       uint4 y[2];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t u = (&x.x)[j] ^ 0x80808080u;   // offset binary
+        const uint32_t u = (&x[i].x)[j] ^ 0x80808080u;   // offset binary
         (&y[j >> 1].x)[2 * (j & 1)] = bytes_f16(u, 0x4140);
         (&y[j >> 1].x)[2 * (j & 1) + 1] = bytes_f16(u, 0x4342);
       }
-      uint4* to = reinterpret_cast<uint4*>(dst + (out0 + 16 * e) * 2);
+      uint4* to = reinterpret_cast<uint4*>(static_cast<unsigned char*>(i & 1 ? a.wide_v : a.wide_k) + (out0 + (int64_t)key * a.D) * 2);
       to[0] = y[0];
       to[1] = y[1];
     }
