@@ -4,9 +4,9 @@
 //   S = Q K^T,   P = 2^(S * scale - m),   O += P V      (128 rows x 128 keys a step)
 //
 // Rows are (new token, head of the group) pairs, so one tile of keys serves every head that shares
-// it. A block owns ROWS = 256 rows (head size up to 128) or 128 (up to 256), O staying in tensor
-// memory, and walks the keys once. Roles:
-//   * one warp brings keys and values by TMA, straight from their pages: 16 KB blocks in a ring, a
+// it. A block (head sizes above 128: a pair of blocks) owns 256 rows, O staying in tensor memory, and
+// walks the keys once. Roles:
+//   * one thread brings keys and values by TMA, straight from their pages: 16 KB blocks in a ring, a
 //     K block being 128 keys x 64 values, a V block 8192 / DP keys x all values, 128-byte swizzle;
 //   * one thread issues the MMAs: S from shared memory, O with P as the operand in tensor memory
 //     (P overwrites its S, each softmax thread's within its own columns) and V with its values
@@ -16,9 +16,9 @@
 //     MMAs take 1.1. The threads of a row agree through one named barrier whether any score asks
 //     for a new maximum. Maxima, sums and O are 32 bits; P is rounded to the cache's 16 bits.
 // Head sizes above 128 run as pairs of blocks (cluster of 2, cta_group::2): an MMA then spans both, each
-// holding 128 of 256 rows in its tensor memory and half of K's keys and V's values in its shared memory.
-// One block alone has to bring 128 KB a step for 128 rows, and waited for it 3500 of 4900 cycles (7 TB/s
-// out of L2 over all SMs; prefill of 8192 tokens 684 us); a pair's block brings half of that.
+// holding 128 of 256 rows in its tensor memory and half of K's keys and V's values in its shared memory,
+// so that a step's 128 KB serve 256 rows as they do for smaller heads (prompt of 8192 tokens, 16/2 heads
+// of 256: 684 us with one block per 128 rows, 502 with pairs, the loads as they were then).
 //
 // With two row tiles the tensor core works on one while the softmax works on the other; with one
 // (head size 256, O takes half of tensor memory) S is double-buffered and QK of the next tile runs
@@ -28,8 +28,10 @@
 // which is rare after the first tiles: O is rescaled in tensor memory by the softmax threads
 // themselves, and no separate correction stage stands in the loop.
 //
-// Bound: at 2 * 128 * 128 * DP flops for 128 * 128 exponentials per product pair, the tensor core
-// and (head size 128) the 16 exponentials a clock an SM are about equally busy.
+// Bound: a step of 256 rows x 128 keys is 2048 cycles of MMA at head size 128 (in each block of a pair at
+// 256) and, at 16 exponentials a clock an SM, 2048 (1024) of exponentials. Measured 3700 cycles at 128,
+// the chain softmax -> weights -> O -> next scores of a row tile; 2350 at 256 (prompt of 8192 tokens
+// 394 us, 1.39 PFLOP/s).
 //
 // 8-bit caches: a launch before this one writes the visible keys and values out once as exact fp16 (an
 // int8 is; see attn_decode.cu, also for the scales: the key's multiplies the score, the value's the
@@ -71,8 +73,9 @@ struct ChunkShape {
   static constexpr int NB = I8 ? (DP == 64 ? 10 : 9) : DP == 64 ? 12 : 10;   // ring blocks
   static constexpr int TPR = 4 / NQ;                 // threads of a row in the softmax
   static constexpr int W = 128 / TPR;                // keys of a tile that one of them takes
-  static constexpr int Mma = 16, Load = 17;          // warps: softmax before, MMA issuer, TMA
-  static constexpr int Threads = 18 * 32;
+  static constexpr int Mma = 16, LoadK = 17, LoadV = 18;   // warps: softmax before, MMA issuer, TMA
+  static constexpr int Threads = 20 * 32;            // one warp idle: registers come in fours of warps
+
   static constexpr int Scales = I8 ? 8 * 1024 + 1024 : 0;   // K's and V's of 8 tiles; the rows' powers of two
   static constexpr int Smem = Q + NB * kBlock + 512 + 2048 + Scales;
   static_assert(Smem <= 232448, "shared memory");
@@ -91,7 +94,7 @@ struct ChunkCtl {
   uint64_t scales[8];             // 8-bit cache: the scales of tile j (mod 8) are there
   uint32_t tmem_base;
   int abort;
-  int page[4][8];                 // of the key tiles being loaded
+  int page[2][2][8];              // of the key tiles being loaded: K, V; this one's and the next's
 };
 static_assert(sizeof(ChunkCtl) <= 512, "control block");
 
@@ -327,21 +330,28 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
   const int page_mask = (1 << a.kv.page_log2) - 1;
   const int seen = row_lo(a, w, w.r0 / a.G);   // pages that end before the first key seen may be gone
 
-  if (warp == S::Load) {
+  if (warp == S::LoadK || warp == S::LoadV) {
     // ---------------------------------------------------------------------------- loads
-    // One elected thread, for the reason given at the MMA issuer: copies issued by several lanes are
-    // serialised through the uniform registers one by one, and the MMAs waited for them.
+    // One elected thread each for K and V, for the reason given at the MMA issuer: copies issued by several
+    // lanes are serialised through the uniform registers one by one, and the MMAs waited for them. Small
+    // pages are many copies (16 keys: 32 a step), so K's and V's are issued side by side.
     const int pool_rows = (a.kv.pages * a.kv.heads) << a.kv.page_log2;
     const int wide_row0 = I8 ? (b * a.kv.heads + h) * a.wide_len : 0;
     constexpr int KK = PAIR ? 64 : 128, KS = PAIR ? 2 : 1;   // keys and 64-value groups of a K block
     const int rk = I8 ? KK : min(1 << a.kv.page_log2, KK);   // keys of one K copy
     // 64-value groups of one copy: all of the block's where its keys are one copy too
     const int kg = copy_groups(a.D, rk == KK, KS), vg = copy_groups(a.D, gran == KB, B);
-    int q = 0, said = 0;
+    int said = 0, issued = 0;   // tiles whose scales, ring blocks whose copies were started
     bool ok = true;
+    const bool loads_v = warp == S::LoadV;
+    // first ring block of K or V of key tile j: K0 V0 K1 V1 .. with two row tiles, K0 K1 V0 K2 V1 .. with one
+    auto block_of = [&](bool v, int j) {
+      if (NQ == 2) return (2 * j + (v ? 1 : 0)) * B;
+      return v ? (j == tiles - 1 ? 2 * j + 1 : 2 * j + 2) * B : (j == 0 ? 0 : 2 * j - 1) * B;
+    };
     if (tiles > 0 && elect_one()) {
-      // The pages of a key tile (128 / page size, at least one) are looked up a tile ahead, and once for K and
-      // V: this thread's instructions, a few cycles each, are what a copy costs.
+      // The pages of a key tile (128 / page size, at least one) are looked up a tile ahead: a lookup right
+      // before its copies would cost an L2 round trip each time.
       const int shift = a.kv.page_log2, count = max(1, 128 >> shift), first_page = seen >> shift, last_page = (s1 - 1) >> shift;
       auto look = [&](int j, int i) {
         const int p = ((s0 + 128 * j) >> shift) + i;
@@ -349,14 +359,15 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
       };
       const uint32_t full0 = PAIR ? in_block(su32(&ctl->full[0]), 0) : su32(&ctl->full[0]), empty0 = su32(&ctl->empty[0]);
       const int part0 = a.D % 64 == 0 ? 0 : 64, part1 = a.D % 64 == 0;   // where a 64-value group stands in the map
-      int slot = 0, parity = 1;
+      int (*pages)[8] = ctl->page[loads_v ? 1 : 0];   // of this key tile and the next
       // K or V of key tile j
       auto load = [&](auto is_v, int j) {
         constexpr bool V = decltype(is_v)::value;
         constexpr int keys = V ? KB : KK, groups = V ? B : KS;
         const int k0 = s0 + 128 * j, step = V ? gran : rk, per = V ? vg : kg;
+        int slot = block_of(V, j) % NB, parity = block_of(V, j) / NB & 1 ^ 1;
         int next[8];
-        if (!I8 && !V && j + 1 < tiles) {
+        if (!I8 && j + 1 < tiles) {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             if (i < count) next[i] = look(j + 1, i);
@@ -386,42 +397,38 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
             const int k = k0 + key0 + i;
             int row = wide_row0 + k;
             if (!I8) {   // past the pool (zeros) where there is no key, or no page
-              const int page = ctl->page[j & 3][(key0 + i) >> shift];
+              const int page = pages[j & 1][(key0 + i) >> shift];
               row = k >= s1 || page < 0 || page >= a.kv.pages ? pool_rows : ((page * a.kv.heads + h) << shift) + (k & page_mask);
             }
 #pragma unroll 1
             for (int g = 0; g < groups; g += per)
               load_3d<PAIR>(dst + g * keys * 128 + i * 128, V ? &vmap : &kmap, part0 * (g0 + g), row, part1 * (g0 + g), bar);
           }
-          ++q;
+          issued = block_of(V, j) + c + 1;
           if (++slot == NB) {
             slot = 0;
             parity ^= 1;
           }
         }
-        if (!I8 && !V && j + 1 < tiles) {
+        if (!I8 && j + 1 < tiles) {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            if (i < count) ctl->page[(j + 1) & 3][i] = next[i];
+            if (i < count) pages[(j + 1) & 1][i] = next[i];
         }
         return true;
       };
-      using K_ = std::false_type;
-      using V_ = std::true_type;
       if (!I8)
-        for (int i = 0; i < count; ++i) ctl->page[0][i] = look(0, i);
-      // the MMAs' order: K0 V0 K1 V1 .. with two row tiles, K0 K1 V0 K2 V1 .. with one
-      ok = load(K_(), 0);
-      for (int j = 0; j < tiles && ok; ++j) {
-        if (NQ == 2) ok = load(V_(), j) && (j + 1 == tiles || load(K_(), j + 1));
-        else ok = (j + 1 == tiles || load(K_(), j + 1)) && load(V_(), j);
-      }
+        for (int i = 0; i < count; ++i) pages[0][i] = look(0, i);
+      if (loads_v)
+        for (int j = 0; j < tiles && ok; ++j) ok = load(std::true_type(), j);
+      else
+        for (int j = 0; j < tiles && ok; ++j) ok = load(std::false_type(), j);
     }
     __syncwarp();
     ok = __all_sync(0xffffffffu, ok);
-    q = __reduce_max_sync(0xffffffffu, q);
+    issued = __reduce_max_sync(0xffffffffu, issued);
     said = __reduce_max_sync(0xffffffffu, said);
-    if (ok && tail >= 0 && tiles > 0) {   // the whole warp zeroes what follows the last key in its copy
+    if (ok && loads_v && tail >= 0 && tiles > 0) {   // the whole warp zeroes what follows the last key in its copy
       const int kl = s0 + 128 * (tiles - 1), c = (tail - kl) / KB, at = (2 * tiles - 1) * B + c, kb = kl + c * KB;
       ok = __all_sync(0xffffffffu, chunk_wait(su32(PAIR ? &ctl->tail_here : &ctl->full[at % NB]), PAIR ? 0 : (at / NB) & 1, ctl));
       if (ok) {
@@ -442,7 +449,10 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
         const long long t0 = clock64();
         while (clock64() - t0 < 200000) {}
       }
-      for (int i = max(0, q - NB); !PAIR && i < q; ++i) chunk_drain(su32(&ctl->full[i % NB]), (i / NB) & 1);
+      for (int i = max(0, issued - NB); !PAIR && i < issued; ++i) {
+        const int j = i / B;
+        if (NQ == 2 && (j & 1) == (loads_v ? 1 : 0)) chunk_drain(su32(&ctl->full[i % NB]), (i / NB) & 1);
+      }
       if (I8)   // scales: at most 8 tiles' are under way; those waited for already answer at once
         for (int i = max(0, said - 8); i < said; ++i) chunk_drain(su32(&ctl->scales[i & 7]), (i >> 3) & 1);
     }
@@ -665,7 +675,7 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
       const uint32_t own = tmem + lanes + 128 * buf + W * part;
       const bool masked = k0 < all_lo || k0 + W > all_hi || missing;
       // The scores are read twice, 32 at a time, rather than held: 64 of them do not fit beside the
-      // weights in 96 registers (spilled: 591 us where this takes 247 on the three chunks; weighed
+      // weights in 96 registers (three chunks to 611 tokens over 8191: 247 us so, 591 spilled; weighed
       // before the maximum is agreed on, and again where it moves: 474 us).
       auto scores = [&](int c, float* s) {
         tmem_ld32(own + c, s);
@@ -985,9 +995,10 @@ void plan_attn_chunk(AttnArgs& a, int64_t max_new, int64_t max_len) {
   a.lo_mask = ~127;
   // One block an SM. Where the blocks do not fill the card, the keys are split for one round of blocks,
   // 256 keys at least: a split costs its start and, per row, its share of O written and read again
-  // (9 sequences of 5 drafts over 1024 keys, 18 blocks: 128 keys 20.5 us, 256 15.9, 512 18.3, whole 26;
-  // 64 tokens over 8000, 8 blocks: 256 33, 512 25.6, 1024 37). From a quarter of the card on rows are so
-  // many that a split has to take 2048 keys to pay (2048 tokens, 64 blocks: 1024 99 us, whole 69).
+  // (9 sequences of 5 drafts over 1024 keys, 18 blocks: 128 keys 22.3 us, 256 17.0, 512 21.6, whole 34;
+  // 64 tokens over 8000, 8 blocks in pairs: 256 35, 512 23.2, 1024 27.4). From a quarter of the card on
+  // rows are so many that a split has to take 2048 keys to pay (2048 tokens, 64 blocks: 1024 100 us, 2048
+  // 91, whole 71; two int8 chunks of 257 over 16385, 72 blocks: 4096 160, half 147, whole 235).
   int64_t keys = max_len;
   if (a.window && a.window + max_new + 128 < keys) keys = a.window + max_new + 128;
   const int64_t blocks = (int64_t)a.kv.seqs * a.kv.heads * a.row_blocks * (a.D > 128 ? 2 : 1);

@@ -19,8 +19,8 @@
 // into a ring of the warp's own, and with the 128-byte swizzle all of these reads are free of bank
 // conflicts. K and V are separate entries of the ring (a slot is refilled as soon as its half is
 // used), a warp waits for nobody but its copies, and the loads in flight cost no registers.
-// (cp.async by the lanes, 32 copies a lane and tile, measured 145 us where this takes the time given
-// at the launcher: the copies' addresses alone were half of a tile's instructions.)
+// (64 sequences of 800 to 8000 tokens, 16/2 heads of 256: 101 us, 5.7 TB/s; with cp.async by the lanes,
+// 32 copies a lane and tile whose addresses alone were half of the instructions, 145.)
 //
 // 8-bit caches: an int8 is exact in fp16 (1024 + u - 1152 with u = v + 128 placed in the mantissa),
 // so both products run in fp16 without loss, the scales outside: the key's into the score, the
