@@ -6,10 +6,12 @@
 // row p % page_size.
 //
 // All three are moved bytes: each thread owns 8 consecutive values of a head (one 16-byte load),
-// LPR = 2..32 lanes a row. In the half layout a value's partner sits half a rotary width away; it
-// is read a second time rather than shuffled (it hits L1, and needs no rule about where the halves
-// fall among the lanes). cos and sin belong to (token, pair) and serve every head, so a block takes
+// LPR = 2..32 lanes a row. In the half layout a value's partner sits half a rotary width away: a
+// lane holds 4 values and their 4 partners (two 8-byte loads), or, for few tokens and for widths that
+// are no multiple of 8, 8 values in a row and reads their partners beside them. cos and sin belong to (token, pair) and serve every head, so a block takes
 // one token and computes them once into shared memory, behind the value loads already in flight.
+#include <type_traits>
+
 #include "kv_dev.cuh"
 
 namespace vq2 {
@@ -64,6 +66,21 @@ __device__ __forceinline__ uint4 load_partner(const T* row, int i0, int rot, boo
   return r;
 }
 
+// The four values at p and the four `apart` values on.
+template <typename T>
+__device__ __forceinline__ uint4 load_fours(const T* p, int apart, bool vec) {
+  if (vec) {
+    const uint2 a = *reinterpret_cast<const uint2*>(p), b = *reinterpret_cast<const uint2*>(p + apart);
+    return make_uint4(a.x, a.y, b.x, b.y);
+  }
+  T t[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t[i] = p[i < 4 ? i : apart + i - 4];
+  uint4 r;
+  memcpy(&r, t, 16);
+  return r;
+}
+
 template <typename T>
 __device__ __forceinline__ void widen8(uint4 u, float (&f)[8]) {
 #pragma unroll
@@ -91,42 +108,105 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// (cos, sin) of the 8 values at i0 -- of their 4 pairs where neighbours are paired, else of each, the
-// sine's sign the value's side -- and the turn in 32 bits. Values past the rotary width: (1, 0).
-template <bool INTER>
+// Which 8 values of a row a lane holds, and where their partners are.
+enum class Hold {
+  kNeighbours,   // 8 in a row, paired with each other (also where nothing is turned)
+  kPartners,     // 8 in a row of the half layout, the partners loaded beside them: any rotary width
+  kSplit,        // half layout: 4 in a row and the 4 that pair with them, half a rotary width on
+};
+
+// (cos, sin) of a lane's 8 values -- of their 4 pairs, or with partners of each, the sine's sign the
+// value's side -- and the turn in 32 bits. Values past the rotary width: (1, 0).
+template <Hold HOLD>
 struct Turn {
-  float2 c[INTER ? 4 : 8];
-  __device__ __forceinline__ void load(int i0, int rot, const float2* cs) {
+  static constexpr int N = HOLD == Hold::kPartners ? 8 : 4;
+  float2 c[N];
+  __device__ __forceinline__ void load(int lane, int rot, const float2* cs) {
     const int h = rot >> 1;
 #pragma unroll
-    for (int j = 0; j < (INTER ? 4 : 8); ++j) {
-      const int e = INTER ? i0 + 2 * j : i0 + j;
-      c[j] = make_float2(1.f, 0.f);
-      if (e < rot) {
-        c[j] = cs[INTER ? e >> 1 : e < h ? e : e - h];
-        if (!INTER && e < h) c[j].y = -c[j].y;
-      }
+    for (int j = 0; j < N; ++j) {
+      const int e = lane * 8 + j;   // with partners
+      const int pair = HOLD == Hold::kPartners ? (e < h ? e : e < rot ? e - h : h) : lane * 4 + j;
+      c[j] = pair < h ? cs[pair] : make_float2(1.f, 0.f);
+      if (HOLD == Hold::kPartners && e < h) c[j].y = -c[j].y;
     }
   }
   __device__ __forceinline__ void apply(float (&x)[8], const float (&w)[8]) const {
-    if (INTER) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float a = x[2 * j], b = x[2 * j + 1];
-        x[2 * j] = a * c[j].x - b * c[j].y;
-        x[2 * j + 1] = b * c[j].x + a * c[j].y;
+    for (int j = 0; j < N; ++j) {
+      if (HOLD == Hold::kPartners) {
+        x[j] = x[j] * c[j].x + w[j] * c[j].y;
+      } else {
+        float &a = x[HOLD == Hold::kSplit ? j : 2 * j], &b = x[HOLD == Hold::kSplit ? j + 4 : 2 * j + 1];
+        const float a0 = a;
+        a = a0 * c[j].x - b * c[j].y;
+        b = b * c[j].x + a0 * c[j].y;
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = x[j] * c[j].x + w[j] * c[j].y;
     }
   }
 };
 
+// (cos, sin) * factor of each pair of token position pos (block-wide).
+__device__ __forceinline__ void fill_turns(const RopeArgs& a, int64_t pos, float2* cs) {
+  for (int i = threadIdx.x; i < (a.rot >> 1); i += blockDim.x) {
+    // The angle in turns in 64 bits, whole turns dropped before it is rounded: at position 10^5 the
+    // product rounded to 32 bits is off by up to 0.004 rad.
+    const double turns = (double)pos * (double)a.inv_freq[i] * 0.15915494309189533577;
+    float s, c;
+    sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
+    cs[i] = make_float2(c * a.factor, s * a.factor * a.sign);
+  }
+}
+
+// Token t's position and its place in the cache (block-wide): page * page_size + row, or -1.
+template <int MODE>
+__device__ __forceinline__ void place_of(const RopeArgs& a, int t, int64_t& pos, int64_t& slot) {
+  pos = 0;
+  slot = -1;
+  if (MODE == 0) {
+    pos = a.pos64 ? static_cast<const int64_t*>(a.positions)[t] : static_cast<const int32_t*>(a.positions)[t];
+    return;
+  }
+  const int b = sequence_of(a.kv, t);
+  if (b < 0) return;
+  int first, count;
+  sequence_rows(a.kv, b, first, count);
+  pos = (int64_t)a.kv.lens[b] - count + (t - first);
+  slot = slot_of(a.kv, b, pos);
+}
+
+// 8 values of a row held by 2^lanes_log2 lanes as int8, and the row's scale: amax / 127, 0 below 1e-30, NaN
+// where a value is not finite. Warp-wide; a lane that is not `mine` adds nothing.
+__device__ __forceinline__ uint2 quantise8(const float (&f)[8], bool mine, int lanes_log2, float& scale) {
+  float amax = 0.f;   // a NaN passes through
+  if (mine) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(f[j]));
+  }
+  for (int o = 1; o < (1 << lanes_log2); o <<= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  uint32_t o[2] = {0, 0};
+  scale = 0.f;
+  if (!(amax < INFINITY)) {
+    scale = __uint_as_float(0x7fc00000u);
+  } else if (amax >= 1e-30f) {
+    scale = __fdiv_rn(amax, 127.f);
+    const float inv = __fdiv_rn(127.f, amax);
+    // |x * inv| <= 127 (1 + 2^-23): no clamp. Adding 1.5 * 2^23 rounds to the nearest even integer and
+    // leaves it in the low byte.
+    uint32_t u[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u[j] = __float_as_uint(__fadd_rn(__fmul_rn(f[j], inv), 12582912.f));
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      o[j] = __byte_perm(__byte_perm(u[4 * j], u[4 * j + 1], 0x0040), __byte_perm(u[4 * j + 2], u[4 * j + 3], 0x0040), 0x5410);
+  }
+  return make_uint2(o[0], o[1]);
+}
+
 // MODE 0: rotary of q and k into contiguous outputs. MODE 1: rotary of q, k (rotated) and v into a
-// 16-bit cache. MODE 2: the same into an 8-bit cache. NIT rows per lane group. INTER: neighbours are
-// paired, and no partners are loaded (also where nothing is turned).
-template <typename T, int MODE, int NIT, bool INTER>
+// 16-bit cache. MODE 2: the same into an 8-bit cache. For few tokens: a row per lane group, its kind by its
+// number.
+template <typename T, int MODE, Hold HOLD>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
   __shared__ float2 cs[128];
   pdl_wait();
@@ -135,105 +215,141 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
   const int groups = blockDim.x >> a.lanes_log2;
   const int lane = threadIdx.x & ((1 << a.lanes_log2) - 1), g = threadIdx.x >> a.lanes_log2;
   const int rows_q = a.in[0].heads, rows_k = a.in[1].heads, rows = rows_q + rows_k * (MODE ? 2 : 1);
-  const int i0 = lane * 8;
-  const bool turning = a.inv_freq != nullptr;
+  const int i0 = lane * 8, r = blockIdx.y * groups + g;
+  const int kind = r < rows_q ? 0 : r < rows_q + rows_k ? 1 : 2;
+  const int h = kind == 0 ? r : kind == 1 ? r - rows_q : r - rows_q - rows_k;
+  const bool mine = r < rows && i0 < a.D, turning = a.inv_freq != nullptr, turned = turning && kind < 2 && i0 < a.rot;
 
-  uint4 x[NIT], w[INTER ? 1 : NIT];
-#pragma unroll
-  for (int n = 0; n < NIT; ++n) {
-    const int r = (blockIdx.y * NIT + n) * groups + g;
-    x[n] = make_uint4(0, 0, 0, 0);
-    if (!INTER) w[n] = make_uint4(0, 0, 0, 0);
-    if (r < rows && i0 < a.D) {
-      const int kind = r < rows_q ? 0 : r < rows_q + rows_k ? 1 : 2;
-      const RopeRows& in = a.in[kind];
-      const int h = kind == 0 ? r : kind == 1 ? r - rows_q : r - rows_q - rows_k;
-      const T* row = static_cast<const T*>(in.x) + t * in.ts + h * in.hs;
-      x[n] = load8(row + i0, in.vec);
-      if (!INTER && turning && kind < 2 && i0 < a.rot) w[n] = load_partner(row, i0, a.rot, in.vec);
-    }
+  uint4 x = make_uint4(0, 0, 0, 0), w = x;
+  if (mine) {   // ahead of the chain that finds the position
+    const RopeRows& in = a.in[kind];
+    const T* row = static_cast<const T*>(in.x) + t * in.ts + h * in.hs;
+    x = load8(row + i0, in.vec);
+    if (HOLD == Hold::kPartners && turned) w = load_partner(row, i0, a.rot, in.vec);
   }
-
-  int64_t pos = 0, slot = -1;  // slot: page * page_size + row, or -1 (token stored nowhere)
-  if (MODE == 0) {
-    pos = a.pos64 ? static_cast<const int64_t*>(a.positions)[t] : static_cast<const int32_t*>(a.positions)[t];
-  } else {
-    const int b = sequence_of(a.kv, t);
-    if (b >= 0) {
-      int first, count;
-      sequence_rows(a.kv, b, first, count);
-      pos = (int64_t)a.kv.lens[b] - count + (t - first);
-      slot = slot_of(a.kv, b, pos);
-    }
-  }
+  int64_t pos, slot;
+  place_of<MODE>(a, t, pos, slot);
+  Turn<HOLD> turn;
   if (turning) {
-    for (int i = threadIdx.x; i < (a.rot >> 1); i += blockDim.x) {
-      // The angle in turns in 64 bits, whole turns dropped before it is rounded: at position 10^5 the
-      // product rounded to 32 bits is off by up to 0.004 rad.
-      const double turns = (double)pos * (double)a.inv_freq[i] * 0.15915494309189533577;
-      float s, c;
-      sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
-      cs[i] = make_float2(c * a.factor, s * a.factor * a.sign);
+    fill_turns(a, pos, cs);
+    __syncthreads();
+    turn.load(lane, a.rot, cs);
+  }
+  float f[8], p[8];
+  widen8<T>(x, f);
+  if (turned) {
+    if (HOLD == Hold::kPartners) widen8<T>(w, p);
+    turn.apply(f, p);
+  }
+  if (MODE != 2 || kind == 0) {
+    if (mine && (MODE != 1 || kind == 0 || slot >= 0)) {
+      T* dst;
+      if (kind == 0) dst = static_cast<T*>(a.q_out) + ((int64_t)t * rows_q + h) * a.D;
+      else if (MODE == 0) dst = static_cast<T*>(a.k_out) + ((int64_t)t * rows_k + h) * a.D;
+      else dst = static_cast<T*>(const_cast<void*>(kind == 1 ? a.kv.k : a.kv.v)) + pool_row(a.kv, slot, h) * a.D;
+      *reinterpret_cast<uint4*>(dst + i0) = turned ? narrow8<T>(f) : x;
     }
+  }
+  if (MODE == 2) {   // rows of different kinds can share a warp, so every lane takes part
+    float scale;
+    const uint2 o = quantise8(f, mine, a.lanes_log2, scale);
+    if (kind == 0 || !mine || slot < 0) return;
+    const int64_t row = pool_row(a.kv, slot, h);
+    int8_t* dst = static_cast<int8_t*>(const_cast<void*>(kind == 1 ? a.kv.k : a.kv.v)) + row * a.D;
+    *reinterpret_cast<uint2*>(dst + i0) = o;
+    if (lane == 0) const_cast<float*>(kind == 1 ? a.kv.k_scale : a.kv.v_scale)[row] = scale;
+  }
+}
+
+// The same for many tokens, q, k and v one after the other: what a row is (turned or not, quantised or
+// not, where it goes) is then the same for a whole loop; choosing it per row took a third of the
+// instructions. In the half layout a lane holds both sides of its pairs (SPLIT), so that each value is
+// loaded and turned once. 40 registers, for the loads in flight that 6 blocks an SM hold; U rows at a
+// time, as many as fit them. B200, device time: rotary of 8191 tokens of 40 heads of 128 29.5 us (5.7
+// TB/s), half layout 32.3 (50.9 with the partners loaded beside the values, 42.8 so in these loops);
+// 11,731 tokens of 32 + 16 heads of 128 written in int8 and read back 70.8 us, half layout 75.1 (79.3 and
+// 114 with a row per lane group).
+template <typename T, int MODE, bool SPLIT>
+__global__ void __launch_bounds__(kRopeThreads, 6) rope_wide_kernel(const RopeArgs a) {
+  __shared__ float2 cs[128];
+  pdl_wait();
+  pdl_trigger();
+  const int t = blockIdx.x;
+  const int groups = blockDim.x >> a.lanes_log2;
+  const int lane = threadIdx.x & ((1 << a.lanes_log2) - 1), g = threadIdx.x >> a.lanes_log2;
+  const bool turning = a.inv_freq != nullptr, in_row = lane * 8 < a.D, in_rot = turning && lane * 8 < a.rot;
+  const int i0 = SPLIT && in_rot ? lane * 4 : lane * 8, apart = SPLIT && in_rot ? a.rot >> 1 : 4;
+
+  int64_t pos, slot;
+  place_of<MODE>(a, t, pos, slot);
+  if (turning) {
+    fill_turns(a, pos, cs);
     __syncthreads();
   }
-  // a lane has the same values of every row: one set of (cos, sin) in registers
-  Turn<INTER> turn;
-  if (turning) turn.load(i0, a.rot, cs);
+  Turn<SPLIT ? Hold::kSplit : Hold::kNeighbours> turn;
+  if (turning) turn.load(lane, a.rot, cs);
 
+  // rows of kind KIND: 0 q, 1 k, 2 v; U at a time
+  auto rows_of_kind = [&](auto kind_c, auto u_c) {
+    constexpr int KIND = decltype(kind_c)::value, U = decltype(u_c)::value;
+    const RopeRows& in = a.in[KIND];
+    const bool turned = KIND < 2 && in_rot;
+    const T* src = static_cast<const T*>(in.x) + t * in.ts + i0;
+    constexpr bool kPool = MODE != 0 && KIND > 0;
+    T* dst = kPool ? static_cast<T*>(const_cast<void*>(KIND == 1 ? a.kv.k : a.kv.v))
+                   : static_cast<T*>(KIND == 0 ? a.q_out : a.k_out) + (int64_t)t * in.heads * a.D;
+    const int64_t pool0 = kPool && slot >= 0 ? pool_row(a.kv, slot, 0) : 0;   // of head 0; the next head is a page of rows on
+    for (int h0 = g; h0 - g < in.heads; h0 += U * groups) {
+      uint4 x[U];
 #pragma unroll
-  for (int n = 0; n < NIT; ++n) {
-    const int r = (blockIdx.y * NIT + n) * groups + g;
-    const int kind = r < rows_q ? 0 : r < rows_q + rows_k ? 1 : 2;
-    const int h = kind == 0 ? r : kind == 1 ? r - rows_q : r - rows_q - rows_k;
-    const bool mine = r < rows && i0 < a.D;
-    float f[8], p[8];
-    widen8<T>(x[n], f);
-    const bool turned = turning && kind < 2 && i0 < a.rot;
-    if (turned) {
-      if (!INTER) widen8<T>(w[n], p);
-      turn.apply(f, p);
-    }
-    if (MODE != 2 || kind == 0) {
-      if (mine && (MODE != 1 || kind == 0 || slot >= 0)) {
-        T* dst;
-        if (kind == 0) dst = static_cast<T*>(a.q_out) + ((int64_t)t * rows_q + h) * a.D;
-        else if (MODE == 0) dst = static_cast<T*>(a.k_out) + ((int64_t)t * rows_k + h) * a.D;
-        else dst = static_cast<T*>(const_cast<void*>(kind == 1 ? a.kv.k : a.kv.v)) + pool_row(a.kv, slot, h) * a.D;
-        *reinterpret_cast<uint4*>(dst + i0) = turned ? narrow8<T>(f) : x[n];
+      for (int n = 0; n < U; ++n) {
+        const int h = h0 + n * groups;
+        x[n] = make_uint4(0, 0, 0, 0);
+        if (h < in.heads && in_row) {
+          if constexpr (SPLIT) x[n] = load_fours(src + h * in.hs, apart, in.vec);
+          else x[n] = load8(src + h * in.hs, in.vec);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < U; ++n) {
+        const int h = h0 + n * groups;
+        const bool mine = h < in.heads && in_row;
+        float f[8];
+        if (turned || (kPool && MODE == 2)) widen8<T>(x[n], f);
+        if (turned) turn.apply(f, f);
+        const int64_t row = kPool ? pool0 + ((int64_t)h << a.kv.page_log2) : h;
+        if (!kPool || MODE == 1) {
+          if (mine && (!kPool || slot >= 0)) {
+            if constexpr (SPLIT) {
+              T* to = dst + row * a.D + i0;
+              if (turned) x[n] = narrow8<T>(f);
+              *reinterpret_cast<uint2*>(to) = make_uint2(x[n].x, x[n].y);
+              *reinterpret_cast<uint2*>(to + apart) = make_uint2(x[n].z, x[n].w);
+            } else {
+              *reinterpret_cast<uint4*>(dst + row * a.D + i0) = turned ? narrow8<T>(f) : x[n];
+            }
+          }
+        } else {
+          float scale;
+          const uint2 o = quantise8(f, mine, a.lanes_log2, scale);
+          if (mine && slot >= 0) {
+            int8_t* to = reinterpret_cast<int8_t*>(dst) + row * a.D + i0;
+            if constexpr (SPLIT) {
+              *reinterpret_cast<uint32_t*>(to) = o.x;
+              *reinterpret_cast<uint32_t*>(to + apart) = o.y;
+            } else {
+              *reinterpret_cast<uint2*>(to) = o;
+            }
+            if (lane == 0) const_cast<float*>(KIND == 1 ? a.kv.k_scale : a.kv.v_scale)[row] = scale;
+          }
+        }
       }
     }
-    if (MODE == 2 && __any_sync(0xffffffffu, kind != 0)) {
-      // amax over the row's lanes, a NaN above all numbers. Rows of different kinds can share a warp, so
-      // every lane takes part.
-      float amax = 0.f;
-      if (mine) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(f[j]));
-      }
-      for (int o = 1; o < (1 << a.lanes_log2); o <<= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      if (kind == 0 || !mine || slot < 0) continue;
-      float scale = 0.f;
-      uint32_t o[2] = {0, 0};
-      if (!(amax < INFINITY)) scale = __uint_as_float(0x7fc00000u);
-      else if (amax >= 1e-30f) {
-        scale = __fdiv_rn(amax, 127.f);
-        const float inv = __fdiv_rn(127.f, amax);
-        // |x * inv| <= 127 (1 + 2^-23): no clamp. Adding 1.5 * 2^23 rounds to the nearest even integer
-        // and leaves it in the low byte.
-        uint32_t u[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) u[j] = __float_as_uint(__fadd_rn(__fmul_rn(f[j], inv), 12582912.f));
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          o[j] = __byte_perm(__byte_perm(u[4 * j], u[4 * j + 1], 0x0040), __byte_perm(u[4 * j + 2], u[4 * j + 3], 0x0040), 0x5410);
-      }
-      const int64_t row = pool_row(a.kv, slot, h);
-      int8_t* dst = static_cast<int8_t*>(const_cast<void*>(kind == 1 ? a.kv.k : a.kv.v)) + row * a.D;
-      *reinterpret_cast<uint2*>(dst + i0) = make_uint2(o[0], o[1]);
-      if (lane == 0) const_cast<float*>(kind == 1 ? a.kv.k_scale : a.kv.v_scale)[row] = scale;
-    }
-  }
+  };
+  using std::integral_constant;
+  rows_of_kind(integral_constant<int, 0>(), integral_constant<int, SPLIT ? 2 : 4>());
+  rows_of_kind(integral_constant<int, 1>(), integral_constant<int, 1>());
+  if (MODE != 0) rows_of_kind(integral_constant<int, 2>(), integral_constant<int, 1>());
 }
 
 struct ReadArgs {
@@ -308,24 +424,23 @@ template <typename T, int MODE>
 int launch_rope(const RopeArgs& a, int64_t T_, cudaStream_t st) {
   const int rows = a.in[0].heads + a.in[1].heads * (MODE ? 2 : 1);
   const int per = kRopeThreads >> a.lanes_log2;
+  const bool neighbours = a.interleaved || !a.inv_freq;
   // One row per lane group while the blocks are fewer than the card holds at once (2048 threads an
-  // SM): a lone token is spread over blocks. Then four, so that a block's
-  // table of cos and sin and its sequence lookup serve more rows; six in the 8-bit write, which
-  // instructions bound (11,731 tokens of 32 + 16 heads of 128: four rows 78 us, six 70, eight 75).
-  const int64_t blocks1 = T_ * ((rows + per - 1) / per);
-  const bool wide = blocks1 > (int64_t)sm_count() * 8;
-  const bool inter = a.interleaved || !a.inv_freq;
-  constexpr int kRows = MODE == 2 ? 6 : 4;
-  const int nit = !wide ? 1 : inter ? kRows : 4;
-  const int y = (rows + per * nit - 1) / (per * nit);
-  const int groups = (rows + y * nit - 1) / (y * nit);        // groups a block needs
-  const int threads = (((groups << a.lanes_log2) + 31) / 32) * 32;
-  const dim3 grid((unsigned)T_, (unsigned)y);
-  if (inter)
-    return wide ? launch_kernel(rope_kernel<T, MODE, kRows, true>, grid, dim3(threads), 0, st, a)
-                : launch_kernel(rope_kernel<T, MODE, 1, true>, grid, dim3(threads), 0, st, a);
-  return wide ? launch_kernel(rope_kernel<T, MODE, 4, false>, grid, dim3(threads), 0, st, a)
-              : launch_kernel(rope_kernel<T, MODE, 1, false>, grid, dim3(threads), 0, st, a);
+  // SM): a lone token is spread over blocks. Then a block a token, the rows of a kind in a loop; not
+  // where a half of the rotary width is no whole number of fours.
+  if (T_ * ((rows + per - 1) / per) <= (int64_t)sm_count() * 8 || (!neighbours && a.rot % 8)) {
+    const int y = (rows + per - 1) / per, groups = (rows + y - 1) / y;
+    const dim3 grid((unsigned)T_, (unsigned)y), block((((groups << a.lanes_log2) + 31) / 32) * 32);
+    return neighbours ? launch_kernel(rope_kernel<T, MODE, Hold::kNeighbours>, grid, block, 0, st, a)
+                      : launch_kernel(rope_kernel<T, MODE, Hold::kPartners>, grid, block, 0, st, a);
+  }
+  // four rows of the most numerous kind a lane group
+  const int most = a.in[0].heads > a.in[1].heads ? a.in[0].heads : a.in[1].heads;
+  int groups = (most + 3) / 4;
+  if (groups > per) groups = per;
+  const dim3 grid((unsigned)T_), block((((groups << a.lanes_log2) + 31) / 32) * 32);
+  return neighbours ? launch_kernel(rope_wide_kernel<T, MODE, false>, grid, block, 0, st, a)
+                    : launch_kernel(rope_wide_kernel<T, MODE, true>, grid, block, 0, st, a);
 }
 
 RopeRows rows_of(const void* x, int64_t ts, int64_t hs, int64_t heads) {

@@ -146,6 +146,25 @@ def test_rotary(dtype, interleaved, T, hq, hk, d, rot):
     assert torch.equal(same[0], got[0])
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("hq,hk,d,rot", [(9, 2, 256, 64), (4, 7, 16, 10), (5, 5, 48, 8), (3, 1, 16, 8), (12, 0, 112, 112)])
+def test_rotary_many_tokens_unaligned(interleaved, hq, hk, d, rot):
+    """More tokens than blocks at once, rows that start anywhere, widths that are no whole number of loads."""
+    T = 9001
+    big = randn(T, (hq + hk) * d + 1, seed=30)
+    q, k = big[:, 1:1 + hq * d].unflatten(1, (hq, d)), big[:, 1 + hq * d:].unflatten(1, (hk, d)) if hk else None
+    f = A.rope_frequencies(rot)[0].to(DEV)
+    pos = torch.arange(T, device=DEV) + 30000
+    for views in ((q, k), (q.contiguous(), k.contiguous() if hk else None)):
+        for x, y in zip(views, A.rotary(*views, pos, f, interleaved=interleaved)):
+            if x is None:
+                continue
+            want = turn64(x, pos, f, interleaved, 1.0)
+            want[..., rot:] = x[..., rot:].double()
+            assert ((y.double() - want).abs() <= EPS[x.dtype] * want.abs() + 4e-6 * x.double().abs().max()).all()
+            assert torch.equal(y[..., rot:], x[..., rot:])
+
+
 def test_rotary_strided_and_unaligned():
     big = randn(9, 7 * 64 + 3, seed=4)
     f = A.rope_frequencies(64)[0].to(DEV)
@@ -225,6 +244,32 @@ def test_cache_write_and_read(dtype, news, lens, hq, hkv, d, rot, page, int8):
     for got, pool, scale in zip((rk, rv), s.pools, s.scale):
         full = torch.cat([cache64(pool, scale, s.table, b, l) for b, l in enumerate(lens)])
         assert ((got.double() - full).abs() <= EPS[dtype] * full.abs()).all()
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("news,lens", [([3], [5]), ([1500, 0, 2001], [1500, 9, 4000])])
+@pytest.mark.parametrize("hq,hkv,d,rot", [(16, 2, 256, 64), (4, 3, 96, 28), (2, 2, 64, 64)])
+def test_cache_write_half_layout(int8, news, lens, hq, hkv, d, rot):
+    """The layout of `test_cache_write_and_read` is the neighbours'; here the halves', few tokens and many."""
+    page, dtype = 32, torch.float16
+    s = Setup(news, lens, hq, hkv, d, dtype, int8, page, seed=31, garbage=0.0)
+    q, k, v = (randn(sum(news), h, d, dtype=dtype, seed=32 + i) for i, h in enumerate((hq, hkv, hkv)))
+    f = A.rope_frequencies(rot)[0].to(DEV)
+    got_q = A.cache_write(k, v, *s.pools, s.table, s.lens, s.starts, k_scale=s.scale[0], v_scale=s.scale[1], q=q, inv_freq=f)
+    pos = torch.cat([torch.arange(l - n, l, device=DEV) for n, l in zip(news, lens)])
+    want_q, want_k = (turn64(x, pos, f, False) for x in (q, k))
+    assert ((got_q.double() - want_q).abs() <= EPS[dtype] * want_q.abs() + 4e-6 * q.double().abs().max()).all()
+    seq = torch.repeat_interleave(torch.arange(len(news), device=DEV), torch.tensor(news, device=DEV))
+    ids, off = s.table[seq, pos // page].long(), pos % page
+    for x, pool, scale in zip((want_k, v.double()), s.pools, s.scale):
+        have = pool[ids, :, off].double()
+        if int8:
+            step = x.abs().amax(-1) / 127
+            have_step = scale[ids, :, off].double()
+            assert ((have_step - step).abs() <= 1e-5 * step).all()
+            assert ((have * have_step[..., None] - x).abs() <= (0.5 + 2e-3) * step[..., None]).all()
+        else:
+            assert ((have - x).abs() <= EPS[dtype] * x.abs() + 4e-6 * x.abs().max()).all()
 
 
 def test_cache_write_int8_edges():
