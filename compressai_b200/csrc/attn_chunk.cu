@@ -245,6 +245,28 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+constexpr int kSorted = 32;   // sequences, at most, that blocks are ordered by
+
+// Which split this block is: over an 8-bit cache read again where it is needed rather than kept in a
+// register that spills (two int8 chunks 155 us kept, 147 so).
+__device__ __forceinline__ int this_split(const AttnArgs& a) {
+  uint32_t z;
+  asm volatile("mov.u32 %0, %%ctaid.z;" : "=r"(z));
+  return (int)(a.kv.seqs <= kSorted ? z / (uint32_t)a.kv.seqs : z);
+}
+
+// The sequence (of 32 at most) that stands at place n when they are ordered by length, longest first (warp-wide).
+__device__ __forceinline__ int nth_longest(const PagedKV& kv, int n, int lane) {
+  if (kv.seqs == 1) return 0;
+  const int len = lane < kv.seqs ? length_of(kv, lane) : -1;
+  int place = 0;
+  for (int i = 0; i < kv.seqs; ++i) {
+    const int l = __shfl_sync(0xffffffffu, len, i);
+    place += l > len || (l == len && i < lane);
+  }
+  return __ffs(__ballot_sync(0xffffffffu, lane < kv.seqs && place == n)) - 1;
+}
+
 // T: of queries and output. The products run in T, over an 8-bit cache in fp16.
 template <int DP, typename T, bool I8>
 __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
@@ -268,11 +290,15 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kMma = S::Mma, TPR = S::TPR, W = S::W;
-  // the last rows see the most keys: they go first
+  // Longest first, so that the last round of blocks is short: whole splits before what is left over, the
+  // longest sequence first, of its rows the last, which see the most keys (208 blocks of three sequences
+  // of 5659 to 8191 keys: 241 us in the sequences' order, 224 so).
   const int rank = PAIR ? blockIdx.x & 1 : 0;   // of a pair: which row tile, which half of K's keys and V's values
   const int bx = PAIR ? blockIdx.x >> 1 : blockIdx.x;
-  const int b = bx / a.row_blocks, rb = a.row_blocks - 1 - (bx - b * a.row_blocks);
-  const int split = blockIdx.y, h = blockIdx.z;
+  const bool sorted = a.kv.seqs <= kSorted;
+  const int nth = sorted ? blockIdx.z % a.kv.seqs : bx / a.row_blocks, split = sorted ? blockIdx.z / a.kv.seqs : blockIdx.z;
+  const int rb = a.row_blocks - 1 - (sorted ? bx : bx - nth * a.row_blocks), h = blockIdx.y;
+  const int b = sorted ? nth_longest(a.kv, nth, lane) : nth;
   const AttnRows w = attn_rows(a, b, rb);
   if (w.rows <= 0) return;
   int lo, hi;
@@ -846,14 +872,14 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
             const int t = token_of(rr, hd);
             if (rr < w.rows && c + 4 * k < a.D)
               *reinterpret_cast<float4*>(
-                  a.part_o + (((int64_t)(w.first + t) * a.hq + h * a.G + hd) * a.splits + split) * a.D + c + 4 * k) =
+                  a.part_o + (((int64_t)(w.first + t) * a.hq + h * a.G + hd) * a.splits + (I8 ? this_split(a) : split)) * a.D + c + 4 * k) =
                   *reinterpret_cast<const float4*>(mine_s + rl * 64 + ((k ^ (rl >> 1 & 3)) << 4));
           }
         }
       }
       const int64_t at = (int64_t)(w.first + tok) * a.hq + h * a.G + head;
       if (mine && part == 0) {
-        if (!alone) a.part_ml[at * a.splits + split] = make_float2(m, l);
+        if (!alone) a.part_ml[at * a.splits + (I8 ? this_split(a) : split)] = make_float2(m, l);
         else if (a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
       }
     }
@@ -974,7 +1000,9 @@ int launch(const AttnArgs& a, cudaStream_t st) {
   if (!make_pool_map(&kmap, I8 ? a.wide_k : a.kv.k, rows, a.D, kbox, copy_groups(a.D, kbox == KK, S::Pair ? 2 : 1), !I8 && a.q_bf16) ||
       !make_pool_map(&vmap, I8 ? a.wide_v : a.kv.v, rows, a.D, vbox, copy_groups(a.D, vbox == S::KB, S::B), !I8 && a.q_bf16))
     return VQ2_ERR_LAUNCH;
-  const dim3 grid((unsigned)(a.kv.seqs * a.row_blocks), (unsigned)a.splits, (unsigned)a.kv.heads);
+  const bool sorted = a.kv.seqs <= kSorted;
+  const dim3 grid((unsigned)(sorted ? a.row_blocks : a.kv.seqs * a.row_blocks), (unsigned)a.kv.heads,
+                  (unsigned)(sorted ? a.kv.seqs * a.splits : a.splits));
   if (S::Pair)
     return launch_cluster(kern, dim3(2 * grid.x, grid.y, grid.z), dim3(S::Threads), S::Smem, 2, st, a, kmap, vmap);
   return launch_kernel(kern, grid, dim3(S::Threads), S::Smem, st, a, kmap, vmap);
