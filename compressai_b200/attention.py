@@ -115,7 +115,11 @@ def paged_attention(q, k_pages, v_pages, table, lens, starts=None, *, k_scale=No
     is not 0; one that sees none gives zeros. Query head h reads key/value head h // (Hq / kv_heads). ``scale``
     defaults to D^-0.5. ``max_new`` and ``max_len`` bound every sequence's new tokens and length; the defaults (all of
     T, all that ``table`` has room for) are right and size the launch for more than may be needed. ``return_lse``:
-    also fp32 [T, Hq], the natural logarithm of each row's sum of exponentials (-inf where no key is seen)."""
+    also fp32 [T, Hq], the natural logarithm of each row's sum of exponentials (-inf where no key is seen).
+
+    A value that is not finite in a cached V row makes NaN, besides in the rows that see its token, in rows of the same
+    launch tile that do not (their weight of 0 is multiplied with it, as a masked dense product would). What lies past
+    a sequence's end or in pages that no sequence has may hold anything."""
     return (_host or _load()).paged_attention(q, k_pages, v_pages, table, k_scale, v_scale, lens, starts, scale, causal, window,
                                               max_new, max_len, return_lse)
 

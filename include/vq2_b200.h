@@ -662,6 +662,8 @@ VQ2_API int vq2_cache_read(const void* k_pages, const void* v_pages, int kv_dtyp
  * dtype; lse (may be NULL): fp32 [tokens, q_heads], the natural logarithm of the sum. max_new and
  * max_len bound every sequence's new tokens and length (larger is only slower). q: 16-byte aligned,
  * strides multiples of 8. workspace: vq2_paged_attention_workspace(...) bytes, 16-byte aligned.
+ * A value that is not finite in a cached V row can make NaN in rows that do not see its token too (0 x
+ * inf); what lies past a sequence's end or in unmapped pages may hold anything.
  */
 VQ2_API int64_t vq2_paged_attention_workspace(int64_t tokens, int64_t q_heads, int64_t kv_heads,
                                               int64_t head_size, int kv_dtype, int64_t seqs,

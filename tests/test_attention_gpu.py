@@ -359,6 +359,20 @@ def test_attention_pages_end_inside_tiles(page, d):
 
 
 @pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 64), (12, 3, 128), (4, 1, 256)])
+@pytest.mark.parametrize("seqs", [3, 32, 33])
+def test_attention_sequences_in_any_order(int8, hq, hkv, d, seqs):
+    """Lengths that rise and fall, equal ones among them, new tokens from none to all, up to and past 32 sequences."""
+    lens = [(37 * i * i + 11) % 530 + 1 for i in range(seqs)]
+    lens[-1] = lens[0]
+    news = [min(l, 0 if i % 7 == 3 else 40 + i) for i, l in enumerate(lens)]
+    s = Setup(news, lens, hq, hkv, d, torch.float16, int8, page=32, seed=40)
+    s.check(*s.run(return_lse=True))
+    from compressai_b200 import _lib
+    assert _lib.load().vq2_attention_status(0) == 0
+
+
+@pytest.mark.parametrize("int8", [False, True])
 def test_attention_rows_that_see_nothing(int8):
     """Empty sequences, more new tokens than the cache holds, and tokens of no sequence: zeros, lse -inf."""
     s = Setup([1, 1], [0, 20], 4, 2, 64, torch.float16, int8, seed=15)
