@@ -22,6 +22,7 @@ int64_t plan(AttnArgs& a, bool i8, int64_t max_new, int64_t max_len, bool& chunk
   chunked = max_new * a.G > (i8 ? 48 : 16) && (!i8 || wide_rows * a.D <= int64_t(1) << 30);
   if (chunked) plan_attn_chunk(a, max_new, max_len);
   else plan_attn_decode(a, max_new, max_len);
+  a.keys_end = 0x7fffffff;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     char* p = ws ? ws + at : nullptr;
@@ -33,7 +34,7 @@ int64_t plan(AttnArgs& a, bool i8, int64_t max_new, int64_t max_len, bool& chunk
     a.part_ml = reinterpret_cast<float2*>(take((int64_t)a.T * a.hq * a.splits * 8));
   }
   if (chunked && i8) {
-    a.wide_len = (int)wide_len;
+    a.wide_len = a.keys_end = (int)wide_len;
     a.wide_k = take(wide_rows * a.D * 2);
     a.wide_v = take(wide_rows * a.D * 2);
     a.wide_ks = reinterpret_cast<float*>(take(wide_rows * 4));

@@ -26,6 +26,7 @@ struct AttnArgs {
   void *wide_k, *wide_v;
   float *wide_ks, *wide_vs;
   int wide_len;
+  int keys_end;         // no key from here on is looked at: wide_len there, else past every position
 };
 
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -80,11 +81,12 @@ __device__ __forceinline__ int row_hi(const AttnArgs& a, const AttnRows& w, int 
   return a.causal ? max(0, min(w.len, w.len - w.count + i + 1)) : w.len;
 }
 
-// Keys that any row of the block sees, the start rounded down; no more than the splits cover.
+// Keys that any row of the block sees, the start rounded down; no more than the splits cover, and of a
+// widened cache no more than its copy holds, whatever lens says when the kernel runs.
 __device__ __forceinline__ void block_keys(const AttnArgs& a, const AttnRows& w, int& lo, int& hi) {
   lo = row_lo(a, w, w.r0 / a.G) & a.lo_mask;
   hi = w.rows > 0 ? row_hi(a, w, (w.r0 + w.rows - 1) / a.G) : 0;
-  hi = (int)min((int64_t)hi, lo + (int64_t)a.splits * a.chunk);
+  hi = (int)min((int64_t)min(hi, a.keys_end), lo + (int64_t)a.splits * a.chunk);
 }
 
 // Joins the splits of every row (launched after a kernel that left more than one).
