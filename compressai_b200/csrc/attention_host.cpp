@@ -134,7 +134,7 @@ Pools pools(PyObject* const* a, int dtype, int64_t heads, int64_t d, c10::Device
   p.table = static_cast<const int32_t*>(table.const_data_ptr());
   p.seqs = table.size(0);
   p.cols = table.size(1);
-  p.stride = std::max(table.stride(0), p.cols);
+  p.stride = table.stride(0);   // 0 where sequences share one row
   return p;
 }
 

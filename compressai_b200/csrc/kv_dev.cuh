@@ -28,7 +28,7 @@ inline int paged_kv(PagedKV& kv, const void* k, const void* v, int kv_dtype, con
   if (kv_dtype != VQ2_F16 && kv_dtype != VQ2_BF16 && kv_dtype != VQ2_I8) return VQ2_ERR_DTYPE;
   if ((kv_dtype == VQ2_I8) != (k_scale != nullptr) || (k_scale == nullptr) != (v_scale == nullptr)) return VQ2_ERR_ARG;
   if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)) || bad_head_size(D)) return VQ2_ERR_SHAPE;
-  if (pages < 1 || heads < 1 || heads > 4096 || seqs < 0 || seqs > 0x7ffffff || cols < 0 || table_stride < cols)
+  if (pages < 1 || heads < 1 || heads > 4096 || seqs < 0 || seqs > 0x7ffffff || cols < 0 || table_stride < 0)
     return VQ2_ERR_SHAPE;
   if (pages > 0x7fffffff / page_size || pages * page_size > 0x7fffffff / heads || cols > 0x7fffffff / page_size)
     return VQ2_ERR_SHAPE;  // a pool's rows and a sequence's positions are counted in 32 bits

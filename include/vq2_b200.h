@@ -608,7 +608,7 @@ VQ2_API int vq2_paged_moe_t1(const void* h, int h_dtype, int64_t top_k, const in
  * 16..256. Cache: k_pages, v_pages [pages, kv_heads, page_size, head_size] contiguous, page_size a
  * power of two 16..256; kv_dtype = dtype, or VQ2_I8 with fp32 k_scale, v_scale [pages, kv_heads,
  * page_size] (value = int8 * scale). table: int32 [seqs, table_cols] page ids (row stride
- * table_stride): position p of sequence b is row p % page_size of page table[b][p / page_size].
+ * table_stride; rows may overlap, 0: all sequences on the same row): position p of sequence b is row p % page_size of page table[b][p / page_size].
  * lens: int32 [seqs] tokens of each sequence in the cache, the new ones included. starts: int32
  * [seqs + 1], ascending: sequence b's new tokens are starts[b] .. starts[b + 1] - 1 and sit at
  * positions lens[b] - count .. lens[b] - 1; NULL: one new token per sequence (tokens = seqs).

@@ -33,3 +33,37 @@ def test_lengths_past_max_len_over_int8(hq, hkv, d, window):
         assert ((got - want).abs() <= (EPS[s.dtype] + 2e-5) * v.abs().max() + EPS[s.dtype] * want.abs()).all()
         seen = ~torch.isinf(want_lse)
         assert torch.equal(torch.isinf(have), ~seen) and ((have - want_lse).abs()[seen] <= 1e-4).all()
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("new", [1, 60])
+def test_tables_whose_rows_overlap(int8, new):
+    """Sequences on the same pages (one row expanded, with a second row elsewhere in memory behind it), rows that
+    start one page later each, one column of a wider table: as with a copy of the table."""
+    s = Setup([200], [200], 4, 2, 64, torch.float16, int8, page=16, seed=51, spare=6)
+    pool = s.pools[0].shape[0]
+    flat = torch.cat([s.table[0, :13], torch.arange(30, device=DEV, dtype=torch.int32) % pool])   # what follows names pages too
+    lens = torch.tensor([200, 77, 160], dtype=torch.int32, device=DEV)
+    q = randn(3 * new, 4, 64, dtype=torch.float16, seed=52)
+    starts = None if new == 1 else torch.tensor([0, new, 2 * new, 3 * new], dtype=torch.int32, device=DEV)
+    ends = torch.tensor([0, 90, 100, 180], dtype=torch.int32, device=DEV)
+    kw = dict(k_scale=s.scale[0], v_scale=s.scale[1])
+    zeroed = [p.masked_fill(p != p, 0) for p in s.pools]   # rows past 200 are in some of these sequences
+    if int8:
+        kw = {n: x.masked_fill(x != x, 0) for n, x in kw.items()}
+    for table in (flat[:13].expand(3, 13), flat.as_strided((3, 13), (1, 1)), flat.as_strided((3, 13), (7, 1))):
+        want, got = (A.paged_attention(q, *zeroed, t, lens, starts, **kw) for t in (table.contiguous(), table))
+        assert torch.equal(want, got) and torch.isfinite(got).all()
+        want, got = (A.cache_read(*zeroed, t, ends, 180, dtype=torch.float16, **kw) for t in (table.contiguous(), table))
+        assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+    k, v = randn(3, 2, 64, dtype=torch.float16, seed=53), randn(3, 2, 64, dtype=torch.float16, seed=54)
+    written = []
+    for table in (flat[:13].expand(3, 13).contiguous(), flat[:13].expand(3, 13)):
+        pools, sc = [p.clone() for p in zeroed], [None if x is None else x.clone() for x in (kw["k_scale"], kw["v_scale"])]
+        A.cache_write(k, v, *pools, table, lens, k_scale=sc[0], v_scale=sc[1])   # positions 199, 76, 159 of the same pages
+        written.append(pools + [x for x in sc if x is not None])
+    assert all(torch.equal(a, b) for a, b in zip(*written))
+    short = torch.tensor([9, 16, 3], dtype=torch.int32, device=DEV)
+    table = flat[:39].view(3, 13)[:, 4:5]
+    want, got = (A.paged_attention(q[:3], *zeroed, t, short, **kw) for t in (table.contiguous(), table))
+    assert torch.equal(want, got)
