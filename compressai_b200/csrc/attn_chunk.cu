@@ -669,6 +669,9 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
       ok = chunk_wait(su32(PAIR ? &ctl->q_here : &ctl->q_full), 0, ctl);
       scale *= undo_s[128 * i + 32 * quarter + lane];
     }
+    // Masked scores are -inf before they are scaled, and -inf * 0 is not -inf: a scale of 0 (or one that has
+    // underflowed) becomes the smallest number, which takes every finite score to less than 5e-7.
+    scale = fmaxf(scale, __int_as_float(1));
     // what the threads of this row leave for one another
     float* said = part_s + (warp - 4 * part) * 32 + lane;   // part p: said[128 * p]
     float m = -INFINITY, l = 0.f, vref = 0.f, vinv = 0.f;   // vref: a power of two above the V scales so far

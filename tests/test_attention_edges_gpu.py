@@ -67,3 +67,17 @@ def test_tables_whose_rows_overlap(int8, new):
     table = flat[:39].view(3, 13)[:, 4:5]
     want, got = (A.paged_attention(q[:3], *zeroed, t, short, **kw) for t in (table.contiguous(), table))
     assert torch.equal(want, got)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("scale", [0.0, -0.0, -0.2, 1e-44])
+def test_scales_of_zero_and_below(int8, dtype, d, scale):
+    """Uniform weights, and scores turned round, for few rows and many, hidden keys among the tiles' keys."""
+    few = Setup([1, 3], [1, 333], 4, 2, d, dtype, int8, page=16, seed=55)
+    many = Setup([70, 130], [200, 130], 8, 2, d, dtype, int8, page=16, seed=56)
+    for s in (few, many):
+        out, lse = s.run(scale=scale, return_lse=True)
+        s.check(out, lse, scale=scale)
+        s.check(s.run(scale=scale, window=40), scale=scale, window=40)
