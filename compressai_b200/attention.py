@@ -95,9 +95,10 @@ def rotary(q, k, positions, inv_freq, *, interleaved=False, factor=1.0, inverse=
 def cache_write(k, v, k_pages, v_pages, table, lens, starts=None, *, k_scale=None, v_scale=None, q=None, inv_freq=None,
                 interleaved=False, factor=1.0):
     """Write the new tokens' k and v [T, kv_heads, D] into the pools, in one launch. With ``inv_freq`` k is turned at
-    its position first, and ``q`` [T, Hq, D] with it: the turned q is returned (None without q). int8 pools: every
-    (token, head) row is quantised with its own scale, amax / 127, from the turned values in 32 bits; a row with an
-    infinity or a NaN reads back as NaN. Tokens whose position has no page in ``table`` are not stored."""
+    its position first, and ``q`` [T, Hq, D] with it: the turned q is returned (None without q; a token of no sequence
+    turns as at position 0). int8 pools: every (token, head) row is quantised with its own scale, amax / 127, from the
+    turned values in 32 bits; a row with an infinity or a NaN reads back as NaN. Tokens whose position has no page in
+    ``table`` are not stored."""
     return (_host or _load()).cache_write(k, v, k_pages, v_pages, table, k_scale, v_scale, lens, starts, q, inv_freq,
                                           interleaved, factor)
 
@@ -112,7 +113,8 @@ def paged_attention(q, k_pages, v_pages, table, lens, starts=None, *, k_scale=No
                     window=0, max_new=None, max_len=None, return_lse=False):
     """Attention of the new tokens q [T, Hq, D] over their sequences' cached keys and values (their own among them):
     [T, Hq, D]. A token at position p sees the keys l < lens, l <= p when ``causal``, l > p - window when ``window``
-    is not 0; one that sees none gives zeros. Query head h reads key/value head h // (Hq / kv_heads). ``scale``
+    is not 0; one that sees none gives zeros, and so do tokens of no sequence, before ``starts[0]`` and from
+    ``starts[-1]`` on (a step padded to a fixed size). Query head h reads key/value head h // (Hq / kv_heads). ``scale``
     defaults to D^-0.5. ``max_new`` and ``max_len`` bound every sequence's new tokens and length; the defaults (all of
     T, all that ``table`` has room for) are right and size the launch for more than may be needed. ``return_lse``:
     also fp32 [T, Hq], the natural logarithm of each row's sum of exponentials (-inf where no key is seen).

@@ -3,7 +3,7 @@
 //   o[t, h] = sum_l softmax_l(scale * q[t, h] . k[l, h / G]) v[l, h / G]
 //
 // over the keys l of t's sequence that t sees: l < len, l <= position(t) when causal, l >
-// position(t) - window when there is a window. A row that sees no key is zero (lse -inf).
+// position(t) - window when there is a window. A row that sees no key, and one of no sequence, is zero (lse -inf).
 #include "attn_dev.cuh"
 
 namespace vq2 {
@@ -41,6 +41,13 @@ int64_t plan(AttnArgs& a, bool i8, int64_t max_new, int64_t max_len, bool& chunk
     a.wide_vs = reinterpret_cast<float*>(take(wide_rows * 4));
   }
   return at;
+}
+
+// No sequence at all: every token is one of none.
+__global__ void __launch_bounds__(256) attn_blank_kernel(const AttnArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  blank_tokens(a, 0, a.T, blockIdx.x, gridDim.x);
 }
 
 bool bad_attn(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t seqs, int64_t max_new, int64_t max_len,
@@ -83,12 +90,12 @@ extern "C" int vq2_paged_attention(const void* q, int64_t q_token_stride, int64_
   int s = paged_kv(a.kv, k_pages, v_pages, kv_dtype, k_scale, v_scale, pages, kv_heads, page_size, head_size, table,
                    table_stride, table_cols, lens, starts, seqs);
   if (s != VQ2_OK) return s;
-  if (!q || !out || !lens) return VQ2_ERR_ARG;
+  if (!q || !out || (!lens && seqs > 0)) return VQ2_ERR_ARG;
   if ((dtype != VQ2_F16 && dtype != VQ2_BF16) || (kv_dtype != dtype && kv_dtype != VQ2_I8)) return VQ2_ERR_DTYPE;
   if (bad_attn(tokens, q_heads, kv_heads, seqs, max_new, max_len, window) || (!starts && tokens != seqs)) return VQ2_ERR_SHAPE;
   if (!aligned(q, 16) || q_token_stride % 8 || q_head_stride % 8 || !aligned(out, 16) || !aligned(workspace, 16))
     return VQ2_ERR_ALIGN;
-  if (tokens == 0 || seqs == 0) return VQ2_OK;
+  if (tokens == 0) return VQ2_OK;
   a.q = q;
   a.q_ts = q_token_stride;
   a.q_hs = q_head_stride;
@@ -102,12 +109,13 @@ extern "C" int vq2_paged_attention(const void* q, int64_t q_token_stride, int64_
   a.window = (int)window;
   a.out = out;
   a.lse = lse;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (seqs == 0) return launch_kernel(attn_blank_kernel, dim3(2 * sm_count()), dim3(256), 0, st, a);
   bool chunked;
   const bool i8 = kv_dtype == VQ2_I8;
   const int64_t bytes = plan(a, i8, starts ? max_new : 1, max_len, chunked, static_cast<char*>(workspace));
   if (bytes && (!workspace || workspace_bytes < bytes)) return VQ2_ERR_ARG;
   if ((int64_t)a.kv.seqs * a.row_blocks > 0x3fffffff) return VQ2_ERR_SHAPE;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
   s = chunked ? launch_attn_chunk(a, i8, st) : launch_attn_decode(a, i8, st);
   if (s != VQ2_OK || a.splits == 1) return s;
   return launch_attn_join(a, st);

@@ -300,6 +300,9 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
   const int rb = a.row_blocks - 1 - (sorted ? bx : bx - nth * a.row_blocks), h = blockIdx.y;
   const int b = sorted ? nth_longest(a.kv, nth, lane) : nth;
   const AttnRows w = attn_rows(a, b, rb);
+  if (!I8)   // the widening kernel's work there: registers are short here (two int8 chunks 160 us for 163)
+    blank_strays(a, w, b, ((rb * a.kv.heads + h) * a.splits + split) * (PAIR ? 2 : 1) + rank,
+                 a.row_blocks * a.kv.heads * a.splits * (PAIR ? 2 : 1));
   if (w.rows <= 0) return;
   int lo, hi;
   block_keys(a, w, lo, hi);
@@ -930,6 +933,7 @@ __global__ void __launch_bounds__(256) widen_kernel(const AttnArgs a) {
   AttnArgs all = a;
   all.rows_per_block = 0x7fffffff;
   const AttnRows w = attn_rows(all, b, 0);
+  blank_strays(a, w, b, blockIdx.x - b * a.kv.heads * per, a.kv.heads * per);
   if (w.rows <= 0) return;
   const int first = row_lo(a, w, 0) & a.lo_mask, end = min((w.len + 127) & ~127, a.wide_len);
   if (k0 + kWidenKeys <= first || k0 >= end) return;

@@ -497,7 +497,7 @@ extern "C" int vq2_cache_write(const void* q, int64_t q_token_stride, int64_t q_
   int s = paged_kv(a.kv, k_pages, v_pages, kv_dtype, k_scale, v_scale, pages, kv_heads, page_size, head_size, table,
                    table_stride, table_cols, lens, starts, seqs);
   if (s != VQ2_OK) return s;
-  if (!k || !v || !lens || (q_heads && (!q || !q_out))) return VQ2_ERR_ARG;
+  if (!k || !v || (!lens && seqs > 0) || (q_heads && (!q || !q_out))) return VQ2_ERR_ARG;
   if ((dtype != VQ2_F16 && dtype != VQ2_BF16) || (kv_dtype != dtype && kv_dtype != VQ2_I8)) return VQ2_ERR_DTYPE;
   if (tokens < 0 || tokens > 0x7fffffff || q_heads < 0 || q_heads > 4096 || bad_rotary(inv_freq, rot, head_size) ||
       (!starts && tokens != seqs))

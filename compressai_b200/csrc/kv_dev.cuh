@@ -24,7 +24,7 @@ inline bool bad_head_size(int64_t D) { return D < 16 || D > 256 || D % 16; }
 inline int paged_kv(PagedKV& kv, const void* k, const void* v, int kv_dtype, const float* k_scale, const float* v_scale,
                     int64_t pages, int64_t heads, int64_t page_size, int64_t D, const int32_t* table,
                     int64_t table_stride, int64_t cols, const int32_t* lens, const int32_t* starts, int64_t seqs) {
-  if (!k || !v || !table) return VQ2_ERR_ARG;
+  if (!k || !v || (!table && seqs > 0 && cols > 0)) return VQ2_ERR_ARG;   // an empty table may have no address
   if (kv_dtype != VQ2_F16 && kv_dtype != VQ2_BF16 && kv_dtype != VQ2_I8) return VQ2_ERR_DTYPE;
   if ((kv_dtype == VQ2_I8) != (k_scale != nullptr) || (k_scale == nullptr) != (v_scale == nullptr)) return VQ2_ERR_ARG;
   if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)) || bad_head_size(D)) return VQ2_ERR_SHAPE;

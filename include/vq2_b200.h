@@ -629,7 +629,7 @@ VQ2_API int vq2_rotary(const void* q, int64_t q_token_stride, int64_t q_head_str
 
 /*
  * Write the new tokens' k and v into their cache rows; with inv_freq (rot values) k, and q when
- * q_heads > 0, are turned first (q into q_out, contiguous). 8-bit cache: per (token, head)
+ * q_heads > 0, are turned first (q into q_out, contiguous; of a token of no sequence as at position 0). 8-bit cache: per (token, head)
  * scale = amax / 127 and int8 = round-to-even(x * (127 / amax)) of the turned values in 32 bits;
  * amax < 1e-30 stores zeros with scale 0, a row with an infinity or a NaN stores scale NaN. Tokens
  * without a page (a position outside the table, a page id outside the pool) are not stored.
@@ -658,7 +658,8 @@ VQ2_API int vq2_cache_read(const void* k_pages, const void* v_pages, int kv_dtyp
 /*
  * out[t, h] = sum_l softmax_l(scale * q[t, h] . k[l, h / (q_heads / kv_heads)]) v[l, ..] over the
  * keys l that token t sees: l < its sequence's length, l <= its position when causal, l > its
- * position - window when window > 0. A token that sees none gives zeros (lse -inf). out: contiguous,
+ * position - window when window > 0. A token that sees none, or that no sequence has (before starts[0],
+ * from starts[seqs] on), gives zeros (lse -inf). out: contiguous,
  * dtype; lse (may be NULL): fp32 [tokens, q_heads], the natural logarithm of the sum. max_new and
  * max_len bound every sequence's new tokens and length (larger is only slower). q: 16-byte aligned,
  * strides multiples of 8. workspace: vq2_paged_attention_workspace(...) bytes, 16-byte aligned.

@@ -81,3 +81,39 @@ def test_scales_of_zero_and_below(int8, dtype, d, scale):
         out, lse = s.run(scale=scale, return_lse=True)
         s.check(out, lse, scale=scale)
         s.check(s.run(scale=scale, window=40), scale=scale, window=40)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("hq,hkv,d,new", [(4, 2, 64, 3), (4, 2, 48, 40), (8, 2, 128, 40), (4, 1, 256, 40)])
+def test_tokens_of_no_sequence(int8, hq, hkv, d, new):
+    """A step padded in front and behind: zeros and -inf there, the sequences' rows right."""
+    s = Setup([new, new - 2], [300, new], hq, hkv, d, torch.bfloat16, int8, page=16, seed=57)
+    n, before, after = 2 * new - 2, 5, 900
+    q = torch.cat([randn(before, hq, d, seed=58), s.q, randn(after, hq, d, seed=59)])
+    torch.full((before + n + after, hq, d), float("nan"), dtype=torch.bfloat16, device=DEV)   # what the allocator hands out next
+    kw = dict(k_scale=s.scale[0], v_scale=s.scale[1], max_new=new, return_lse=True)
+    out, lse = A.paged_attention(q, *s.pools, s.table, s.lens, s.starts + before, **kw)
+    s.check(out[before:before + n], lse[before:before + n])
+    for part, l in ((out[:before], lse[:before]), (out[before + n:], lse[before + n:])):
+        assert (part == 0).all() and (l == -float("inf")).all()
+    for nothing in (torch.zeros(3, dtype=torch.int32, device=DEV), torch.full((3,), len(q) + 7, dtype=torch.int32, device=DEV)):
+        out, lse = A.paged_attention(q, *s.pools, s.table, s.lens, nothing, **kw)   # two sequences without a token here
+        assert (out == 0).all() and (lse == -float("inf")).all()
+    out, lse = A.paged_attention(q, *s.pools, s.table[:0], s.lens[:0], s.starts[:1], **kw)   # no sequences
+    assert (out == 0).all() and (lse == -float("inf")).all()
+    turned = A.cache_write(q[:, :hkv], q[:, :hkv], *s.pools, s.table[:0], s.lens[:0], s.starts[:1], q=q,
+                           **{n: kw[n] for n in ("k_scale", "v_scale")})
+    assert torch.equal(turned, q)
+    back = A.cache_read(*s.pools, s.table[:0], s.starts[:1], 9, **{n: kw[n] for n in ("k_scale", "v_scale")})
+    assert all((x == 0).all() and x.shape == (9, hkv, d) for x in back)
+
+
+def test_a_table_without_columns():
+    """Sequences that have no page yet: nothing to see, nothing stored."""
+    s = Setup([1, 1], [0, 0], 4, 2, 64, torch.float16, seed=60)
+    table = s.table[:, :0].contiguous()
+    before = [p.clone() for p in s.pools]
+    out, lse = A.paged_attention(s.q, *s.pools, table, s.lens, return_lse=True)
+    assert (out == 0).all() and (lse == -float("inf")).all()
+    A.cache_write(s.q[:, :2], s.q[:, :2], *s.pools, table, s.lens + 1)
+    assert all(torch.equal(a.nan_to_num(7), b.nan_to_num(7)) for a, b in zip(before, s.pools))
