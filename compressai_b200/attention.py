@@ -121,9 +121,19 @@ def paged_attention(q, k_pages, v_pages, table, lens, starts=None, *, k_scale=No
 
     A value that is not finite in a cached V row makes NaN, besides in the rows that see its token, in rows of the same
     launch tile that do not (their weight of 0 is multiplied with it, as a masked dense product would). What lies past
-    a sequence's end or in pages that no sequence has may hold anything."""
+    a sequence's end or in pages that no sequence has may hold anything.
+
+    A call returns before its kernels have run; ``check_status`` says whether any of them gave up (NaN in its rows)."""
     return (_host or _load()).paged_attention(q, k_pages, v_pages, table, k_scale, v_scale, lens, starts, scale, causal, window,
                                               max_new, max_len, return_lse)
+
+
+def check_status(device=None):
+    """Wait for the device and raise VQ2Error if a ``paged_attention`` on it, on any stream, gave up a wait since this
+    was last called: the kernels wait for their own copies about 2 s at most, then leave NaN in the rows they were at.
+    For where a program synchronises anyway."""
+    with torch.cuda.device(device):
+        _lib.check(_lib.load().vq2_attention_status(1), "vq2_paged_attention")
 
 
 class PagedKVCache:

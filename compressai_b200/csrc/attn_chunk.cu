@@ -46,7 +46,7 @@
 // read: the copy's coordinate is put past the pool, which fills zeros).
 //
 // Every wait is bounded by the SM clock (about 2 s): one that gives up raises the abort flag and
-// vq2_attention_status, every role leaves its loop, copies and MMAs in flight are drained.
+// vq2_attention_status, every role leaves its loop, copies and MMAs in flight are drained, the rows are NaN.
 #include <atomic>
 #include <type_traits>
 
@@ -829,65 +829,64 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
     if (ok && !leave && tiles > 0) ok = __all_sync(0xffffffffu, chunk_wait(su32(&ctl->o_full[i]), 0, ctl));
     said[128 * part] = l;
     ok = !any_of(bar, 32 * TPR, !ok || leave);
-    if (ok) {
-      tc_fence_after();
-      l = 0.f;
+    tc_fence_after();
+    l = 0.f;
 #pragma unroll
-      for (int p = 0; p < TPR; ++p) l += said[128 * p];
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      // 16 values of 32 rows at a time through 2 KB of the tile's queries, which nobody reads any more:
-      // a row's 16 values then go out as whole sectors.
-      unsigned char* mine_s = sm + i * S::QC * kBlock + (warp - 4 * TPR * i) * 2048;
+    for (int p = 0; p < TPR; ++p) l += said[128 * p];
+    if (!ok) l = __int_as_float(0x7fffffff);   // gave up: the rows come out as NaN
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    // 16 values of 32 rows at a time through 2 KB of the tile's queries, which nobody reads any more:
+    // a row's 16 values then go out as whole sectors.
+    unsigned char* mine_s = sm + i * S::QC * kBlock + (warp - 4 * TPR * i) * 2048;
 #pragma unroll 1
-      for (int c = part * (DP / TPR); c < (part + 1) * (DP / TPR); c += 16) {
-        float o[16];
+    for (int c = part * (DP / TPR); c < (part + 1) * (DP / TPR); c += 16) {
+      float o[16];
+      __syncwarp();
+      if (tiles > 0) tmem_ld16(o_col + c, o);
+      else
+#pragma unroll
+        for (int k = 0; k < 16; ++k) o[k] = 0.f;
+      const float by = (alone ? inv : 1.f) * (I8 ? vref : 1.f);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) o[k] *= by;
+      if (alone) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          *reinterpret_cast<uint4*>(mine_s + lane * 32 + ((k ^ (lane >> 2 & 1)) << 4)) =
+              make_uint4(pack2<T>(o[8 * k], o[8 * k + 1]), pack2<T>(o[8 * k + 2], o[8 * k + 3]),
+                         pack2<T>(o[8 * k + 4], o[8 * k + 5]), pack2<T>(o[8 * k + 6], o[8 * k + 7]));
         __syncwarp();
-        if (tiles > 0) tmem_ld16(o_col + c, o);
-        else
 #pragma unroll
-          for (int k = 0; k < 16; ++k) o[k] = 0.f;
-        const float by = (alone ? inv : 1.f) * (I8 ? vref : 1.f);
+        for (int n = 0; n < 2; ++n) {
+          const int rl = 16 * n + (lane >> 1), k = lane & 1, rr = 128 * tile + 32 * quarter + rl;
+          int hd;
+          const int t = token_of(rr, hd);
+          if (rr < w.rows && c + 8 * k < a.D)
+            *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + ((int64_t)(w.first + t) * a.hq + h * a.G + hd) * a.D + c + 8 * k) =
+                *reinterpret_cast<const uint4*>(mine_s + rl * 32 + ((k ^ (rl >> 2 & 1)) << 4));
+        }
+      } else {
 #pragma unroll
-        for (int k = 0; k < 16; ++k) o[k] *= by;
-        if (alone) {
+        for (int k = 0; k < 4; ++k)
+          *reinterpret_cast<float4*>(mine_s + lane * 64 + ((k ^ (lane >> 1 & 3)) << 4)) =
+              make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+        __syncwarp();
 #pragma unroll
-          for (int k = 0; k < 2; ++k)
-            *reinterpret_cast<uint4*>(mine_s + lane * 32 + ((k ^ (lane >> 2 & 1)) << 4)) =
-                make_uint4(pack2<T>(o[8 * k], o[8 * k + 1]), pack2<T>(o[8 * k + 2], o[8 * k + 3]),
-                           pack2<T>(o[8 * k + 4], o[8 * k + 5]), pack2<T>(o[8 * k + 6], o[8 * k + 7]));
-          __syncwarp();
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            const int rl = 16 * n + (lane >> 1), k = lane & 1, rr = 128 * tile + 32 * quarter + rl;
-            int hd;
-            const int t = token_of(rr, hd);
-            if (rr < w.rows && c + 8 * k < a.D)
-              *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + ((int64_t)(w.first + t) * a.hq + h * a.G + hd) * a.D + c + 8 * k) =
-                  *reinterpret_cast<const uint4*>(mine_s + rl * 32 + ((k ^ (rl >> 2 & 1)) << 4));
-          }
-        } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            *reinterpret_cast<float4*>(mine_s + lane * 64 + ((k ^ (lane >> 1 & 3)) << 4)) =
-                make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-          __syncwarp();
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const int rl = 8 * n + (lane >> 2), k = lane & 3, rr = 128 * tile + 32 * quarter + rl;
-            int hd;
-            const int t = token_of(rr, hd);
-            if (rr < w.rows && c + 4 * k < a.D)
-              *reinterpret_cast<float4*>(
-                  a.part_o + (((int64_t)(w.first + t) * a.hq + h * a.G + hd) * a.splits + (I8 ? this_split(a) : split)) * a.D + c + 4 * k) =
-                  *reinterpret_cast<const float4*>(mine_s + rl * 64 + ((k ^ (rl >> 1 & 3)) << 4));
-          }
+        for (int n = 0; n < 4; ++n) {
+          const int rl = 8 * n + (lane >> 2), k = lane & 3, rr = 128 * tile + 32 * quarter + rl;
+          int hd;
+          const int t = token_of(rr, hd);
+          if (rr < w.rows && c + 4 * k < a.D)
+            *reinterpret_cast<float4*>(
+                a.part_o + (((int64_t)(w.first + t) * a.hq + h * a.G + hd) * a.splits + (I8 ? this_split(a) : split)) * a.D + c + 4 * k) =
+                *reinterpret_cast<const float4*>(mine_s + rl * 64 + ((k ^ (rl >> 1 & 3)) << 4));
         }
       }
-      const int64_t at = (int64_t)(w.first + tok) * a.hq + h * a.G + head;
-      if (mine && part == 0) {
-        if (!alone) a.part_ml[at * a.splits + (I8 ? this_split(a) : split)] = make_float2(m, l);
-        else if (a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
-      }
+    }
+    const int64_t at = (int64_t)(w.first + tok) * a.hq + h * a.G + head;
+    if (mine && part == 0) {
+      if (!alone) a.part_ml[at * a.splits + (I8 ? this_split(a) : split)] = make_float2(m, l);
+      else if (a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
     }
   }
 

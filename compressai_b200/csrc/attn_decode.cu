@@ -464,8 +464,11 @@ __global__ void __launch_bounds__(DecodeShape<DP, NT, I8>::kWarps * 32, DecodeSh
       }
     step();
   }
-  if (!ok)   // copies under way have landed before the ring's memory is used for anything else
+  if (!ok) {   // copies under way have landed before the ring's memory is used for anything else
     for (int i = max(0, put - S::kSlots); i < put; ++i) copy_wait(bar0 + 8 * (i % S::kSlots), (i / S::kSlots) & 1);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) l[i][0] = l[i][1] = __int_as_float(0x7fffffff);   // the rows come out as NaN
+  }
   __syncthreads();   // every warp is done with its ring: O takes its place
 
   // ---- join the warps: maximum, then sums relative to it

@@ -222,4 +222,6 @@ def _decode(model, ids, steps, warmup, cache, seqs):
         nxt = out.logits[:, -1].argmax(-1, keepdim=True)
     e1.record()
     e1.synchronize()
+    if cache is not None:
+        attention.check_status(dev)
     return e0.elapsed_time(e1) / 1e3 / steps, nxt

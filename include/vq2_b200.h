@@ -677,8 +677,10 @@ VQ2_API int vq2_paged_attention(const void* q, int64_t q_token_stride, int64_t q
                                 const int32_t* lens, const int32_t* starts, int64_t seqs, int64_t max_new,
                                 int64_t max_len, float scale, int causal, int64_t window, void* out,
                                 float* lse, void* workspace, int64_t workspace_bytes, void* stream);
-/* Sticky status word of vq2_paged_attention's tensor-core kernel: VQ2_ERR_TIMEOUT once a bounded
- * on-chip wait gave up (its output is then not valid); cleared when reset is non-zero. Synchronises. */
+/* Sticky status of the current device's vq2_paged_attention kernels, one for all streams: VQ2_ERR_TIMEOUT
+ * once a bounded on-chip wait gave up (its block's rows of out and lse are then NaN), VQ2_ERR_ALIGN should
+ * a block's shared memory start off its line (its rows are not written); cleared when reset is non-zero.
+ * Synchronises. */
 VQ2_API int vq2_attention_status(int reset);
 
 #ifdef __cplusplus

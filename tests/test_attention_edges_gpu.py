@@ -117,3 +117,10 @@ def test_a_table_without_columns():
     assert (out == 0).all() and (lse == -float("inf")).all()
     A.cache_write(s.q[:, :2], s.q[:, :2], *s.pools, table, s.lens + 1)
     assert all(torch.equal(a.nan_to_num(7), b.nan_to_num(7)) for a, b in zip(before, s.pools))
+
+
+def test_check_status():
+    s = Setup([1, 70], [20, 300], 8, 2, 128, torch.bfloat16, seed=61)
+    s.run()
+    A.check_status()
+    A.check_status("cuda:0")
