@@ -192,18 +192,25 @@ class PagedKVCache:
             host = host.pin_memory()
         t = host.to(self.device, non_blocking=True)
         one = all(c == 1 for c in counts)
-        self.batch = dict(lens=t[:B], starts=None if one else t[B:2 * B + 1], table=t[2 * B + 1:].view(B, cols),
+        self.batch = dict(counts=list(counts), lens=t[:B], starts=None if one else t[B:2 * B + 1], table=t[2 * B + 1:].view(B, cols),
                           max_new=max(counts, default=0), max_len=max(lens, default=0))
+
+    def _batch(self, tokens):
+        if self.batch is None:
+            raise RuntimeError("no batch: begin says which sequences the tokens belong to")
+        if tokens != sum(self.batch["counts"]):
+            raise ValueError(f"the batch has {sum(self.batch['counts'])} new tokens; got {tokens}")
+        return self.batch
 
     def write(self, layer, k, v, *, q=None, inv_freq=None, interleaved=False, factor=1.0):
         """``cache_write`` of the batch's tokens into a layer."""
-        b = self.batch
+        b = self._batch(k.shape[0])
         return cache_write(k, v, *self.pools[layer], b["table"], b["lens"], b["starts"], k_scale=self.scales[layer][0],
                            v_scale=self.scales[layer][1], q=q, inv_freq=inv_freq, interleaved=interleaved, factor=factor)
 
     def attend(self, layer, q, *, scale=None, causal=True, window=0):
         """``paged_attention`` of the batch's tokens over a layer."""
-        b = self.batch
+        b = self._batch(q.shape[0])
         return paged_attention(q, *self.pools[layer], b["table"], b["lens"], b["starts"], k_scale=self.scales[layer][0],
                                v_scale=self.scales[layer][1], scale=scale, causal=causal, window=window,
                                max_new=b["max_new"], max_len=b["max_len"])

@@ -46,3 +46,18 @@ def test_int8_pools_have_scales():
     c = cache(dtype=torch.int8)
     assert c.pools[1][0].dtype == torch.int8 and c.scales[1][1].shape == (6, 1, 16)
     assert cache(dtype=torch.float16).scales[0] == (None, None)
+
+
+def test_tokens_are_the_batch_s():
+    """A write of fewer tokens than begun would leave rows that later steps read unwritten: refused ahead of the kernels."""
+    c = cache()
+    x = torch.zeros(5, 1, 16, dtype=torch.bfloat16)
+    for call in (lambda: c.write(0, x, x), lambda: c.attend(0, x)):
+        with pytest.raises(RuntimeError, match="begin"):
+            call()
+    a, b = c.add(), c.add()
+    for counts in ([4, 0], [5, 1]):
+        c.begin([a, b], counts)
+        for call in (lambda: c.write(0, x, x), lambda: c.attend(0, x)):
+            with pytest.raises(ValueError, match="new tokens"):
+                call()
