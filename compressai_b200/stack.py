@@ -148,14 +148,36 @@ def build_vq2_moe_model(config=None, device="cuda", seed=0, group=None, max_toke
 
 class PagedAttention(nn.Module):
     """Drop-in for Qwen3_5MoeAttention: its projections, norms and output gate, around one fused launch
-    that turns q and k and writes k and v into the paged cache, and the attention over it."""
+    that turns q and k and writes k and v into the paged cache, and the attention over it.
+
+    Positions, lengths and what a token sees are the cache's: its ``begin`` comes before every forward of the model,
+    with hidden_states' [sequences, tokens]. Position ids and the transformers cache (which holds the other layers'
+    states) are not read; a padding mask is refused. Inference only: no gradients pass."""
 
     def __init__(self, attn, cache, layer, inv_freq):
         super().__init__()
         self.attn, self.cache, self.layer, self.inv_freq = attn, cache, layer, inv_freq
+        self.served = None   # the batch of the last forward
+
+    def check(self, lead, mask):
+        batch = self.cache.batch
+        if batch is None or batch is self.served:
+            raise RuntimeError("cache.begin comes before every forward of a model on the paged cache: it says which "
+                               "sequences the tokens belong to")
+        if batch["counts"] != [lead[-1]] * (lead.numel() // lead[-1] if lead[-1] else 0):
+            raise ValueError(f"cache.begin counted {batch['counts']} new tokens; the forward has {tuple(lead)}")
+        if mask is not None:
+            sees = mask if mask.dtype == torch.bool else mask >= 0 if mask.is_floating_point() else mask > 0
+            q, k = sees.shape[-2:]
+            plain = sees if sees.dim() == 2 else sees == torch.ones(q, k, dtype=torch.bool, device=sees.device).tril(k - q)
+            if not plain.all():
+                raise ValueError("a mask that is not the causal one: the paged cache has no padding (begin takes each "
+                                 "sequence's own number of tokens)")
 
     def forward(self, hidden_states, position_embeddings=None, attention_mask=None, past_key_values=None, **kwargs):
         a, lead = self.attn, hidden_states.shape[:-1]
+        self.check(lead, attention_mask)
+        self.served = self.cache.batch
         q, gate = a.q_proj(hidden_states).reshape(lead.numel(), -1, 2 * a.head_dim).chunk(2, dim=-1)
         q = a.q_norm(q)
         k = a.k_norm(a.k_proj(hidden_states).reshape(lead.numel(), -1, a.head_dim))

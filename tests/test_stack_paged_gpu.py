@@ -63,3 +63,24 @@ def test_paged_greedy_decode(dtype):
     with pytest.raises(MemoryError):
         stack.decode(model, batch=9, prompt_len=20, steps=1, warmup=0, cache=cache)
     assert len(cache.free) == 8
+
+
+@torch.no_grad()
+def test_model_refuses_padding_and_a_forward_without_begin():
+    model = small_model(6)
+    cache = stack.use_paged_attention(model, pages=8, page_size=16)
+    ids = torch.randint(0, 1024, (2, 6), device=DEV)
+    with pytest.raises(RuntimeError, match="begin"):
+        model(input_ids=ids)
+    seqs = [cache.add(), cache.add()]
+    mask = torch.ones(2, 6, dtype=torch.long, device=DEV)
+    mask[0, :2] = 0
+    cache.begin(seqs, [6, 6])
+    with pytest.raises(ValueError, match="mask"):
+        model(input_ids=ids, attention_mask=mask)
+    want = model(input_ids=ids, attention_mask=torch.ones_like(mask)).logits
+    with pytest.raises(RuntimeError, match="begin"):
+        model(input_ids=ids)
+    again = [cache.add(), cache.add()]
+    cache.begin(again, [6, 6])
+    assert torch.equal(model(input_ids=ids).logits, want)
