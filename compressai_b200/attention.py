@@ -169,7 +169,8 @@ class PagedKVCache:
 
     def begin(self, seqs, counts):
         """The next calls' tokens are ``counts[i]`` new ones of sequence ``seqs[i]``, in this order. Pages are taken
-        for all of them or, with a MemoryError, for none."""
+        for all of them or, with a MemoryError, for none. The tokens count from here on: where a step fails before
+        every layer has written them, ``cancel`` takes them back."""
         if len(seqs) != len(counts) or len(set(seqs)) != len(seqs) or any(c < 0 for c in counts):
             raise ValueError("seqs are different sequences, counts their numbers of new tokens")
         P = self.page_size
@@ -182,6 +183,14 @@ class PagedKVCache:
         for s, n, k in zip(seqs, lens, need):
             self.pages[s] += [self.free.pop() for _ in range(k)]
             self.lengths[s] = n
+        self.batch = dict(seqs=list(seqs), counts=list(counts))
+        try:
+            self.batch.update(self._tables(lens, counts, seqs))
+        except BaseException:
+            self.cancel()
+            raise
+
+    def _tables(self, lens, counts, seqs):
         B, cols = len(seqs), max([len(self.pages[s]) for s in seqs] + [1])
         starts = [0]
         for c in counts:
@@ -192,8 +201,20 @@ class PagedKVCache:
             host = host.pin_memory()
         t = host.to(self.device, non_blocking=True)
         one = all(c == 1 for c in counts)
-        self.batch = dict(counts=list(counts), lens=t[:B], starts=None if one else t[B:2 * B + 1], table=t[2 * B + 1:].view(B, cols),
-                          max_new=max(counts, default=0), max_len=max(lens, default=0))
+        return dict(lens=t[:B], starts=None if one else t[B:2 * B + 1], table=t[2 * B + 1:].view(B, cols),
+                    max_new=max(counts, default=0), max_len=max(lens, default=0))
+
+    def cancel(self):
+        """Take back the last ``begin``: its tokens, and the pages that they alone needed (for sequences not released since)."""
+        if self.batch is None:
+            raise RuntimeError("no batch to take back")
+        for s, c in reversed(list(zip(self.batch["seqs"], self.batch["counts"]))):
+            if s in self.pages:
+                self.lengths[s] -= c
+                keep = -(-self.lengths[s] // self.page_size)
+                self.free += reversed(self.pages[s][keep:])
+                del self.pages[s][keep:]
+        self.batch = None
 
     def _batch(self, tokens):
         if self.batch is None:

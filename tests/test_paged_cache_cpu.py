@@ -61,3 +61,36 @@ def test_tokens_are_the_batch_s():
         for call in (lambda: c.write(0, x, x), lambda: c.attend(0, x)):
             with pytest.raises(ValueError, match="new tokens"):
                 call()
+
+
+def test_a_failed_step_is_taken_back():
+    """Begun again after a step that failed, the same tokens stand at the same positions on the same pages."""
+    c = cache()
+    a, b = c.add(), c.add()
+    c.begin([a, b], [16, 3])
+    before = (list(c.free), dict(c.lengths), {s: list(p) for s, p in c.pages.items()})
+    c.begin([b, a], [20, 1])
+    lens, table = c.batch["lens"].tolist(), c.batch["table"].tolist()
+    c.cancel()
+    assert before == (c.free, c.lengths, c.pages) and c.batch is None
+    c.begin([b, a], [20, 1])
+    assert c.batch["lens"].tolist() == lens and c.batch["table"].tolist() == table
+    c.release(b)
+    c.cancel()
+    assert c.lengths == {a: 16} and len(c.free) == 5
+    with pytest.raises(RuntimeError):
+        c.cancel()
+
+
+def test_a_begin_that_fails_late_changes_nothing(monkeypatch):
+    c = cache()
+    a = c.add()
+    c.begin([a], [10])
+    before = (list(c.free), dict(c.lengths), {s: list(p) for s, p in c.pages.items()})
+
+    def full(*args):
+        raise torch.OutOfMemoryError("full")
+    monkeypatch.setattr(c, "_tables", full)
+    with pytest.raises(torch.OutOfMemoryError):
+        c.begin([a], [30])
+    assert before == (c.free, c.lengths, c.pages) and c.batch is None
