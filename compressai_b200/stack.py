@@ -189,18 +189,20 @@ class PagedAttention(nn.Module):
 
 def use_paged_attention(model, pages, page_size=64, max_len=32768, dtype=torch.bfloat16):
     """Replace the model's full-attention layers by PagedAttention over one new PagedKVCache (returned):
-    ``pages`` pages of ``page_size`` tokens, bf16 or int8."""
+    ``pages`` pages of ``page_size`` tokens, bf16 or int8. A model that has a paged cache already gets the new one in
+    its place."""
     cfg = model.config
     dev = next(model.parameters()).device
     layers = [m for m in model.model.layers if hasattr(m, "self_attn")]
+    plain = [m.self_attn.attn if isinstance(m.self_attn, PagedAttention) else m.self_attn for m in layers]
     cache = attention.PagedKVCache(len(layers), pages, cfg.num_key_value_heads, cfg.head_dim, page_size=page_size,
                                    max_len=max_len, dtype=dtype, device=dev)
     rope = cfg.rope_parameters
     if rope.get("rope_type", "default") != "default":
         raise ValueError(f"rotary type {rope['rope_type']!r}: build inv_freq with attention.rope_frequencies")
     inv_freq, _ = attention.rope_frequencies(int(cfg.head_dim * rope.get("partial_rotary_factor", 1.0)), rope["rope_theta"])
-    for i, m in enumerate(layers):
-        m.self_attn = PagedAttention(m.self_attn, cache, i, inv_freq.to(dev))
+    for i, (m, attn) in enumerate(zip(layers, plain)):
+        m.self_attn = PagedAttention(attn, cache, i, inv_freq.to(dev))
     return cache
 
 

@@ -1,10 +1,12 @@
 """What the paged attention layer refuses before it launches anything (no device needed)."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 import torch.nn as nn
 
 from compressai_b200.attention import PagedKVCache
-from compressai_b200.stack import PagedAttention
+from compressai_b200.stack import PagedAttention, use_paged_attention
 
 
 class Reached(Exception):
@@ -64,3 +66,25 @@ def test_padding_masks_are_refused_and_causal_ones_taken(q, k):
             m, _, _ = layer(2, [q, q])
             with pytest.raises(error):
                 m(hidden_states=torch.zeros(2, q, 8), attention_mask=mask)
+
+
+class Model(nn.Module):
+    """As much of a stack as use_paged_attention looks at."""
+
+    def __init__(self, **rope):
+        super().__init__()
+        self.weight = nn.Parameter(torch.zeros(1))
+        self.config = SimpleNamespace(num_key_value_heads=1, head_dim=64,
+                                      rope_parameters={"rope_theta": 10000.0, "partial_rotary_factor": 0.25, **rope})
+        self.model = nn.Module()
+        self.model.layers = nn.ModuleList([nn.Module(), nn.Module()])
+        self.model.layers[1].self_attn = Attn()
+
+
+def test_a_second_cache_takes_the_place_of_the_first():
+    m = Model()
+    attn = m.model.layers[1].self_attn
+    use_paged_attention(m, pages=4)
+    cache = use_paged_attention(m, pages=6, page_size=16, dtype=torch.int8)
+    layer = m.model.layers[1].self_attn
+    assert layer.attn is attn and layer.cache is cache and len(cache.free) == 6 and not hasattr(m.model.layers[0], "self_attn")
