@@ -154,9 +154,9 @@ class PagedAttention(nn.Module):
     with hidden_states' [sequences, tokens]. Position ids and the transformers cache (which holds the other layers'
     states) are not read; a padding mask is refused. Inference only: no gradients pass."""
 
-    def __init__(self, attn, cache, layer, inv_freq):
+    def __init__(self, attn, cache, layer, inv_freq, factor=1.0):
         super().__init__()
-        self.attn, self.cache, self.layer, self.inv_freq = attn, cache, layer, inv_freq
+        self.attn, self.cache, self.layer, self.inv_freq, self.factor = attn, cache, layer, inv_freq, factor
         self.served = None   # the batch of the last forward
 
     def check(self, lead, mask):
@@ -182,27 +182,29 @@ class PagedAttention(nn.Module):
         q = a.q_norm(q)
         k = a.k_norm(a.k_proj(hidden_states).reshape(lead.numel(), -1, a.head_dim))
         v = a.v_proj(hidden_states).reshape(lead.numel(), -1, a.head_dim)
-        q = self.cache.write(self.layer, k, v, q=q, inv_freq=self.inv_freq)
+        q = self.cache.write(self.layer, k, v, q=q, inv_freq=self.inv_freq, factor=self.factor)
         o = self.cache.attend(self.layer, q, scale=a.scaling)
         return a.o_proj((o * torch.sigmoid(gate)).reshape(*lead, -1)), None
 
 
-def use_paged_attention(model, pages, page_size=64, max_len=32768, dtype=torch.bfloat16):
+def use_paged_attention(model, pages, page_size=64, max_len=32768, dtype=torch.bfloat16, inv_freq=None, factor=1.0):
     """Replace the model's full-attention layers by PagedAttention over one new PagedKVCache (returned):
     ``pages`` pages of ``page_size`` tokens, bf16 or int8. A model that has a paged cache already gets the new one in
-    its place."""
+    its place. ``inv_freq``, ``factor``: what attention.rope_frequencies gives, for a model whose configuration
+    stretches its context (yarn, llama3, ..); without them the configuration's plain frequencies."""
     cfg = model.config
     dev = next(model.parameters()).device
     layers = [m for m in model.model.layers if hasattr(m, "self_attn")]
     plain = [m.self_attn.attn if isinstance(m.self_attn, PagedAttention) else m.self_attn for m in layers]
+    if inv_freq is None:
+        rope = cfg.rope_parameters
+        if rope.get("rope_type", "default") != "default":
+            raise ValueError(f"rotary type {rope['rope_type']!r}: give inv_freq and factor from attention.rope_frequencies")
+        inv_freq, factor = attention.rope_frequencies(int(cfg.head_dim * rope.get("partial_rotary_factor", 1.0)), rope["rope_theta"])
     cache = attention.PagedKVCache(len(layers), pages, cfg.num_key_value_heads, cfg.head_dim, page_size=page_size,
                                    max_len=max_len, dtype=dtype, device=dev)
-    rope = cfg.rope_parameters
-    if rope.get("rope_type", "default") != "default":
-        raise ValueError(f"rotary type {rope['rope_type']!r}: build inv_freq with attention.rope_frequencies")
-    inv_freq, _ = attention.rope_frequencies(int(cfg.head_dim * rope.get("partial_rotary_factor", 1.0)), rope["rope_theta"])
     for i, (m, attn) in enumerate(zip(layers, plain)):
-        m.self_attn = PagedAttention(attn, cache, i, inv_freq.to(dev))
+        m.self_attn = PagedAttention(attn, cache, i, inv_freq.to(dev), factor)
     return cache
 
 

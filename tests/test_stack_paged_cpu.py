@@ -5,7 +5,7 @@ import pytest
 import torch
 import torch.nn as nn
 
-from compressai_b200.attention import PagedKVCache
+from compressai_b200.attention import PagedKVCache, rope_frequencies
 from compressai_b200.stack import PagedAttention, use_paged_attention
 
 
@@ -88,3 +88,15 @@ def test_a_second_cache_takes_the_place_of_the_first():
     cache = use_paged_attention(m, pages=6, page_size=16, dtype=torch.int8)
     layer = m.model.layers[1].self_attn
     assert layer.attn is attn and layer.cache is cache and len(cache.free) == 6 and not hasattr(m.model.layers[0], "self_attn")
+
+
+def test_stretched_rotary_is_given():
+    m = Model(rope_type="yarn", factor=8.0)
+    with pytest.raises(ValueError, match="inv_freq"):
+        use_paged_attention(m, pages=4)
+    assert isinstance(m.model.layers[1].self_attn, Attn)
+    f, factor = rope_frequencies(16, 10000.0, {"type": "yarn", "factor": 8.0, "original": 4096})
+    use_paged_attention(m, pages=4, inv_freq=f, factor=factor)
+    layer = m.model.layers[1].self_attn
+    assert torch.equal(layer.inv_freq, f) and layer.factor == factor != 1.0
+    use_paged_attention(Model(), pages=4)

@@ -84,3 +84,20 @@ def test_model_refuses_padding_and_a_forward_without_begin():
     again = [cache.add(), cache.add()]
     cache.begin(again, [6, 6])
     assert torch.equal(model(input_ids=ids).logits, want)
+
+
+@torch.no_grad()
+def test_stretched_rotary_reaches_the_layer():
+    """Frequencies and factor given are those that the keys are stored with."""
+    model = small_model(7)
+    f, factor = stack.attention.rope_frequencies(32, 10000.0, {"type": "yarn", "factor": 8.0, "original": 64})
+    cache = stack.use_paged_attention(model, pages=4, page_size=16, inv_freq=f, factor=factor)
+    seen = []
+    layer = model.model.layers[3].self_attn
+    hook = layer.attn.k_norm.register_forward_hook(lambda m, args, out: seen.append(out.clone()))
+    seq = cache.add()
+    cache.begin([seq], [16])
+    model(input_ids=torch.randint(0, 1024, (1, 16), device=DEV))
+    hook.remove()
+    want, _ = stack.attention.rotary(seen[0], None, torch.arange(16, device=DEV), f.to(DEV), factor=factor)
+    assert torch.equal(cache.pools[0][0][cache.pages[seq][0]].transpose(0, 1), want)
