@@ -76,7 +76,7 @@ struct ChunkShape {
   static constexpr int Mma = 16, LoadK = 17, LoadV = 18;   // warps: softmax before, MMA issuer, TMA
   static constexpr int Threads = 20 * 32;            // one warp idle: registers come in fours of warps
 
-  static constexpr int Scales = I8 ? 8 * 1024 + 1024 : 0;   // K's and V's of 8 tiles; the rows' powers of two
+  static constexpr int Scales = I8 ? 8 * 1024 + 1024 + 2048 : 0;   // K's and V's of 8 tiles; the rows' powers of two; a word a softmax thread
   static constexpr int Smem = Q + NB * kBlock + 512 + 2048 + Scales;
   static_assert(Smem <= 232448, "shared memory");
   static constexpr uint32_t O0 = 256;                // first TMEM column of O; S buffers at 0 and 128
@@ -282,6 +282,7 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
   float* part_s = reinterpret_cast<float*>(ring + NB * kBlock + 512);   // a word of each softmax thread
   float* scale_s = part_s + 512;      // 8-bit: [8 tiles][K 128, V 128], then what undoes each row's power of two
   float* undo_s = scale_s + 8 * 256;
+  float* vmax_s = undo_s + 256;
   pdl_wait();
   pdl_trigger();
   if (su32(sm) & 1023) {   // the swizzle needs it; the only shared memory here, so it starts a 1024-byte line
@@ -677,7 +678,7 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
     scale = fmaxf(scale, __int_as_float(1));
     // what the threads of this row leave for one another
     float* said = part_s + (warp - 4 * part) * 32 + lane;   // part p: said[128 * p]
-    float m = -INFINITY, l = 0.f, vref = 0.f, vinv = 0.f;   // vref: a power of two above the V scales so far
+    float m = -INFINITY, l = 0.f, vref = 0.f, vinv = 0.f;   // vref: a power of two above the V scales that the row has seen
     uint64_t l2 = pair(0.f, 0.f), l3 = l2;
     auto page_at = [&](int k) { return lane < W / 16 && k + 16 * lane < s1 ? table[(k + 16 * lane) >> a.kv.page_log2] : 0; };
     int page = page_at(s0 + W * part);   // a tile ahead
@@ -692,15 +693,32 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
         ok = ok && chunk_wait(su32(&ctl->scales[j & 7]), (j >> 3) & 1, ctl);
         ks = scale_s + (j & 7) * 256 + W * part;
         vs = ks + 128;
-        const float4 f = *reinterpret_cast<const float4*>(scale_s + (j & 7) * 256 + 128 + 4 * lane);
-        // the largest of the tile; a NaN or an infinity (a value that was stored as such) sets no reference
+        // the largest of the tile's keys that the row sees (a hidden one's scale must not cost the row bits), where
+        // some are hidden of this thread's part of them; a NaN or an infinity (a value that was stored as such) sets
+        // no reference
+        const float* tile_vs = scale_s + (j & 7) * 256 + 128;
+        const int tile0 = s0 + 128 * j;
         uint32_t x = 0;
+        if (tile0 >= all_lo && tile0 + 128 <= all_hi) {
+          const float4 f = *reinterpret_cast<const float4*>(tile_vs + 4 * lane);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t y = __float_as_uint((&f.x)[e]);
-          if (y < 0x7f800000u) x = max(x, y);
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t y = __float_as_uint((&f.x)[e]);
+            if (y < 0x7f800000u) x = max(x, y);
+          }
+          x = __reduce_max_sync(0xffffffffu, x);
+        } else {
+#pragma unroll 4
+          for (int k = 0; k < W; k += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(vs + k);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t y = __float_as_uint((&f.x)[e]);
+              if (y < 0x7f800000u && k0 + k + e >= klo && k0 + k + e < khi) x = max(x, y);
+            }
+          }
         }
-        vmax = __uint_as_float(__reduce_max_sync(0xffffffffu, x));
+        vmax = __uint_as_float(x);
       }
       ok = __all_sync(0xffffffffu, ok && chunk_wait(su32(&ctl->s_full[buf]), (NQ == 2 ? j : j >> 1) & 1, ctl));
       tc_fence_after();
@@ -743,15 +761,20 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
       // One that gave up waiting says so here, so that all leave together.
       if (any_of(bar, 32 * TPR, mx > m + 8.f || vmax > vref || !ok)) {
         said[128 * part] = mx;
+        float* said_v = vmax_s + (said - part_s);
+        if (I8) said_v[128 * part] = vmax;
         leave = any_of(bar, 32 * TPR, !ok);
         if (leave) break;
         float all = mx;
 #pragma unroll
-        for (int q = 0; q < TPR; ++q) all = fmaxf(all, said[128 * q]);
+        for (int q = 0; q < TPR; ++q) {
+          all = fmaxf(all, said[128 * q]);
+          if (I8) vmax = fmaxf(vmax, said_v[128 * q]);
+        }
         const float mn = fmaxf(m, all), by = mn == -INFINITY ? 1.f : ex2(m - mn);
         float undo = 1.f;
-        if (I8 && vmax > vref) {   // at most 2^120 or so: its inverse is a normal number too
-          const float ref = fminf(__uint_as_float((__float_as_uint(vmax) & 0x7f800000u) + 0x00800000u), 1.3e36f);
+        if (I8 && vmax > vref) {
+          const float ref = above(vmax);
           undo = vref / ref;
           vref = ref;
           vinv = 1.f / ref;

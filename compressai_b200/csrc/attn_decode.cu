@@ -24,8 +24,8 @@
 //
 // 8-bit caches: an int8 is exact in fp16 (1024 + u - 1152 with u = v + 128 placed in the mantissa),
 // so both products run in fp16 without loss, the scales outside: the key's into the score, the
-// value's into P, relative to a power of two at least the largest seen (vref) so that P stays in
-// fp16's range. bf16 queries become fp16 by a power of two per row, exact down to 2^-28 of the
+// value's into P, relative to a power of two above the largest that the row has seen (vref) so that P
+// stays in fp16's range. bf16 queries become fp16 by a power of two per row, exact down to 2^-28 of the
 // row's largest value.
 //
 // Rescaling is lazy: m moves only when a score passes it by 8 powers of two, so P is at most 256 --
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(DecodeShape<DP, NT, I8>::kWarps * 32, DecodeSh
   // keys that every row sees need no mask
   const int all_lo = row_lo(a, w, (w.r0 + w.rows - 1) / a.G), all_hi = row_hi(a, w, w.r0 / a.G);
 
-  float o[NT][DP / 16][4], m[NT][2], base[NT][2], l[NT][2], vref = 0.f, vinv = 0.f;
+  float o[NT][DP / 16][4], m[NT][2], base[NT][2], l[NT][2], vref[NT][2];
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
 #pragma unroll
@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(DecodeShape<DP, NT, I8>::kWarps * 32, DecodeSh
       for (int c = 0; c < 4; ++c) o[i][j][c] = 0.f;
     m[i][0] = m[i][1] = -INFINITY;
     base[i][0] = base[i][1] = 0.f;   // m, or 0 while no key has been seen
-    l[i][0] = l[i][1] = 0.f;
+    l[i][0] = l[i][1] = vref[i][0] = vref[i][1] = 0.f;
   }
 
   // this lane's chunks in a piece: K rows g, g + 8 (1024 bytes on), V rows 2t, 2t + 1 (and 8 on)
@@ -335,6 +335,11 @@ __global__ void __launch_bounds__(DecodeShape<DP, NT, I8>::kWarps * 32, DecodeSh
     const bool whole = k0 >= all_lo && k0 + S::kKeys <= all_hi && k0 + S::kKeys <= s1 && !none;
     float ks[S::kU][2], vs[S::kU][2];
     bool high = false;
+    float vlow = INFINITY;   // what every row's vref covers
+    if (I8) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) vlow = fminf(vlow, fminf(vref[i][0], vref[i][1]));
+    }
 #pragma unroll
     for (int u = 0; u < S::kU; ++u) {
 #pragma unroll
@@ -346,7 +351,7 @@ __global__ void __launch_bounds__(DecodeShape<DP, NT, I8>::kWarps * 32, DecodeSh
           asm volatile("ld.shared.f32 %0, [%1];" : "=f"(vs[u][e]) : "r"(at + 4 * S::kKeys));
           // what lies past the keys, or on a page that does not exist, is no scale
           if (!whole && (((none >> u) & 1) || k0 + 16 * u + g + 8 * e >= s1)) vs[u][e] = 0.f;
-          high |= vs[u][e] > vref;
+          high |= vs[u][e] > vlow;
         }
       }
 #pragma unroll
@@ -364,22 +369,6 @@ __global__ void __launch_bounds__(DecodeShape<DP, NT, I8>::kWarps * 32, DecodeSh
     }
     if (++scale_slot == S::kScaleSlots) scale_slot = 0;
     if (__any_sync(0xffffffffu, high)) {
-      float by[NT][2], undo = 1.f;
-      if (I8) {
-        float x = vs[0][0];
-#pragma unroll
-        for (int u = 0; u < S::kU; ++u) x = fmaxf(x, fmaxf(vs[u][0], vs[u][1]));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-        if (x > vref) {
-          // the power of two above it; at most 2^120 or so, its inverse is a normal number too
-          const float ref = fminf(__uint_as_float((__float_as_uint(x) & 0x7f800000u) + 0x00800000u), 1.3e36f);
-          undo = vref / ref;
-          vref = ref;
-          vinv = 1.f / ref;
-        }
-      }
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -390,15 +379,32 @@ __global__ void __launch_bounds__(DecodeShape<DP, NT, I8>::kWarps * 32, DecodeSh
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          float undo = 1.f;
+          if (I8) {   // of the keys that the row sees: a hidden one's scale must not cost it bits
+            float y = 0.f;
+#pragma unroll
+            for (int u = 0; u < S::kU; ++u)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (s[u][i][0][c + 2 * e] != -INFINITY) y = fmaxf(y, vs[u][e]);
+            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
+            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
+            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
+            if (y > vref[i][c]) {
+              const float ref = above(y);
+              undo = vref[i][c] / ref;
+              vref[i][c] = ref;
+            }
+          }
           const float mn = fmaxf(m[i][c], x);
-          by[i][c] = mn == -INFINITY ? 1.f : ex2(m[i][c] - mn);
+          const float by = mn == -INFINITY ? 1.f : ex2(m[i][c] - mn);
           m[i][c] = mn;
           base[i][c] = mn == -INFINITY ? 0.f : mn;
-          l[i][c] *= by[i][c];
+          l[i][c] *= by;
 #pragma unroll
           for (int j = 0; j < DP / 16; ++j) {
-            o[i][j][c] *= by[i][c] * undo;
-            o[i][j][c + 2] *= by[i][c] * undo;
+            o[i][j][c] *= by * undo;
+            o[i][j][c + 2] *= by * undo;
           }
         }
     }
@@ -416,6 +422,8 @@ __global__ void __launch_bounds__(DecodeShape<DP, NT, I8>::kWarps * 32, DecodeSh
           l[i][c & 1] += p[c];
           if (I8) {
             const bool hidden = !whole && p[c] == 0.f;   // a masked key's scale may be anything
+            // 1 / vref, a power of two (2^127 where no scale but 0 has been seen)
+            const float vinv = __int_as_float(0x7f000000 - __float_as_int(vref[i][c & 1]));
             p[c] = hidden ? 0.f : p[c] * (vs[u][c >> 1] * vinv);
           }
         }
@@ -484,7 +492,6 @@ __global__ void __launch_bounds__(DecodeShape<DP, NT, I8>::kWarps * 32, DecodeSh
     }
   float* acc = reinterpret_cast<float*>(sm);   // [warp][row][DP + 4]
   constexpr int LD = DP + 4;
-  const float undo = I8 ? vref : 1.f;
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -494,7 +501,7 @@ __global__ void __launch_bounds__(DecodeShape<DP, NT, I8>::kWarps * 32, DecodeSh
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float2* dst = reinterpret_cast<float2*>(acc + (warp * NT * 8 + 8 * i + 2 * t + c) * LD + d);
-        *dst = make_float2(o[i][j][c] * undo, o[i][j][c + 2] * undo);
+        *dst = make_float2(o[i][j][c] * (I8 ? vref[i][c] : 1.f), o[i][j][c + 2] * (I8 ? vref[i][c] : 1.f));
       }
     }
   __syncthreads();

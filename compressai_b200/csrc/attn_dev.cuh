@@ -37,6 +37,12 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// The power of two above a positive V scale, which the weights of an 8-bit cache are relative to. 2^126 at most,
+// so that its inverse is a normal number too (a scale above overflows with any value beyond 2 anyway).
+__device__ __forceinline__ float above(float scale) {
+  return __uint_as_float(min((__float_as_uint(scale) & 0x7f800000u) + 0x00800000u, 0x7e800000u));
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if (std::is_same<T, __half>::value) {

@@ -124,3 +124,30 @@ def test_check_status():
     s.run()
     A.check_status()
     A.check_status("cuda:0")
+
+
+def check_rows(s, out, scale, causal=True, window=0):
+    """Every row within its own bound: u * sum p |v| for the weights' rounding and 32-bit work, u |out| for its own."""
+    at = 0
+    for b, (n, l) in enumerate(zip(s.news, s.lens_list)):
+        k, v = (cache64(p, x, s.table, b, l) for p, x in zip(s.pools, s.scale))
+        q, pos = s.q[at:at + n], torch.arange(l - n, l, device=DEV)
+        want, sizes = (attend64(q, k, y, pos, scale, causal, window)[0] for y in (v, v.abs()))
+        off = (out[at:at + n].double() - want).abs()
+        assert (off <= (EPS[s.dtype] + 2e-5) * sizes + EPS[s.dtype] * want.abs()).all(), (b, (off / sizes).max().item())
+        at += n
+
+
+@pytest.mark.parametrize("by", [1e4, 1e8, 1e30])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 64), (4, 2, 128), (4, 1, 256)])
+@pytest.mark.parametrize("new", [4, 70])
+def test_int8_values_of_hidden_keys_cost_nothing(by, hq, hkv, d, new):
+    """A token with a far larger V row, later than some rows or out of their window: the rows that do not see it are as
+    exact as ever."""
+    s = Setup([new, 1], [300, 200], hq, hkv, d, torch.float16, int8=True, page=16, seed=62)
+    for b, key in ((0, 298), (1, 161)):
+        s.scale[1][s.table[b, key // 16].long(), :, key % 16] *= by
+    out = s.run(window=30)   # sequence 0: hidden from all rows but the last two; sequence 1: 9 keys before its window
+    rows = torch.arange(new - 2)
+    s.q, s.news, s.lens_list = torch.cat([s.q[rows], s.q[new:]]), [new - 2, 1], [298, 200]
+    check_rows(s, torch.cat([out[rows], out[new:]]), d ** -0.5, window=30)
