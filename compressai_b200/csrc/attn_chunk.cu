@@ -24,7 +24,7 @@
 // (head size 256, O takes half of tensor memory) S is double-buffered and QK of the next tile runs
 // under the softmax.
 //
-// The running maximum moves only when a score passes it by 8 powers of two (P is then at most 256),
+// The running maximum moves only when a score passes it by 8 powers of two (P is at most 256; fp16: 2^15),
 // which is rare after the first tiles: O is rescaled in tensor memory by the softmax threads
 // themselves, and no separate correction stage stands in the loop.
 //
@@ -276,6 +276,9 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
   constexpr int NQ = S::NQ, B = S::B, KB = S::KB, NB = S::NB;
   constexpr bool PAIR = S::Pair;
   constexpr bool BF = std::is_same<M, __nv_bfloat16>::value;
+  // fp16 weights: 2^7 larger than in bf16, up to 2^15, so that those down to 2^-32 of the largest (2^-25 otherwise)
+  // are more than 0: over 200,000 keys together they can outweigh a rounding. Taken back where splits are joined.
+  constexpr float kLift = BF ? 0.f : 7.f, kDrop = BF ? 1.f : 1.f / 128.f;
   extern __shared__ __align__(1024) unsigned char sm[];
   unsigned char* ring = sm + S::Q;
   ChunkCtl* ctl = reinterpret_cast<ChunkCtl*>(ring + NB * kBlock);
@@ -679,7 +682,6 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
     // what the threads of this row leave for one another
     float* said = part_s + (warp - 4 * part) * 32 + lane;   // part p: said[128 * p]
     float m = -INFINITY, l = 0.f, vref = 0.f, vinv = 0.f;   // vref: a power of two above the V scales that the row has seen
-    uint64_t l2 = pair(0.f, 0.f), l3 = l2;
     auto page_at = [&](int k) { return lane < W / 16 && k + 16 * lane < s1 ? table[(k + 16 * lane) >> a.kv.page_log2] : 0; };
     int page = page_at(s0 + W * part);   // a tile ahead
     for (int j = 0; j < tiles && !leave; ++j) {
@@ -759,7 +761,7 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
       }
       const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
       // One that gave up waiting says so here, so that all leave together.
-      if (any_of(bar, 32 * TPR, mx > m + 8.f || vmax > vref || !ok)) {
+      if (any_of(bar, 32 * TPR, mx > m + (8.f + kLift) || vmax > vref || !ok)) {
         said[128 * part] = mx;
         float* said_v = vmax_s + (said - part_s);
         if (I8) said_v[128 * part] = vmax;
@@ -771,7 +773,7 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
           all = fmaxf(all, said[128 * q]);
           if (I8) vmax = fmaxf(vmax, said_v[128 * q]);
         }
-        const float mn = fmaxf(m, all), by = mn == -INFINITY ? 1.f : ex2(m - mn);
+        const float mn = fmaxf(m, all - kLift), by = mn == -INFINITY ? 1.f : ex2(m - mn);
         float undo = 1.f;
         if (I8 && vmax > vref) {
           const float ref = above(vmax);
@@ -780,8 +782,7 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
           vinv = 1.f / ref;
         }
         m = mn;
-        l2 = fma2(l2, pair(by, by), pair(0.f, 0.f));
-        l3 = fma2(l3, pair(by, by), pair(0.f, 0.f));
+        l *= by;
         if (j > 0) {
           // scores of tile j follow the product of tile j - 1 (two row tiles) or j - 2 (one)
           if (NQ == 1) {
@@ -803,6 +804,8 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
       const float base = m == -INFINITY ? 0.f : m;
       const uint64_t scale2 = pair(scale, scale), base2 = pair(-base, -base);
       const uint64_t vinv2 = pair(vinv, vinv);
+      // The tile's sum by itself: beside a running sum of 1, weights of 2^-25 would vanish one by one.
+      uint64_t l2 = pair(0.f, 0.f);
       auto weigh = [&](auto hides, int c) {   // hides: some keys of the tile are masked
         float s[32];
         uint32_t p[16];
@@ -812,8 +815,7 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
           const float2 x = unpair(fma2(pair(s[k], s[k + 1]), scale2, base2));
           const float2 z = unpair(fma2(pair(s[k + 2], s[k + 3]), scale2, base2));
           uint64_t y = pair(ex2(x.x), ex2(x.y)), w = pair(ex2(z.x), ex2(z.y));
-          l2 = add2(l2, y);
-          l3 = add2(l3, w);
+          l2 = add2(l2, add2(y, w));
           if (I8) {
             const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(vs + c + k);
             y = mul2(y, mul2(f.x, vinv2));
@@ -836,6 +838,8 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
         if (I8 && masked) weigh(std::true_type(), c);
         else weigh(std::false_type(), c);
       }
+      const float2 l01 = unpair(l2);
+      l += l01.x + l01.y;
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -843,10 +847,6 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
         if (PAIR) mbar_arrive_cluster_relaxed(in_block(su32(&ctl->p_full[buf]), 0));
         else mbar_arrive(su32(&ctl->p_full[buf]));
       }
-    }
-    {
-      const float2 x = unpair(l2), y = unpair(l3);
-      l = (x.x + x.y) + (y.x + y.y);
     }
     // ---- the rows' output, or their share of it
     if (ok && !leave && tiles > 0) ok = __all_sync(0xffffffffu, chunk_wait(su32(&ctl->o_full[i]), 0, ctl));
@@ -869,7 +869,7 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
       else
 #pragma unroll
         for (int k = 0; k < 16; ++k) o[k] = 0.f;
-      const float by = (alone ? inv : 1.f) * (I8 ? vref : 1.f);
+      const float by = (alone ? inv : kDrop) * (I8 ? vref : 1.f);
 #pragma unroll
       for (int k = 0; k < 16; ++k) o[k] *= by;
       if (alone) {
@@ -908,7 +908,7 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
     }
     const int64_t at = (int64_t)(w.first + tok) * a.hq + h * a.G + head;
     if (mine && part == 0) {
-      if (!alone) a.part_ml[at * a.splits + (I8 ? this_split(a) : split)] = make_float2(m, l);
+      if (!alone) a.part_ml[at * a.splits + (I8 ? this_split(a) : split)] = make_float2(m + kLift, l * kDrop);
       else if (a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
     }
   }

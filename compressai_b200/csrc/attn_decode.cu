@@ -28,8 +28,8 @@
 // stays in fp16's range. bf16 queries become fp16 by a power of two per row, exact down to 2^-28 of the
 // row's largest value.
 //
-// Rescaling is lazy: m moves only when a score passes it by 8 powers of two, so P is at most 256 --
-// in range for fp16 -- and the usual step has no shuffles beyond one vote. P is rounded to the
+// Rescaling is lazy: m moves only when a score passes it by 8 powers of two, so P is at most 256 (fp16:
+// 2^15, see kLift) and the usual step has no shuffles beyond one vote. P is rounded to the
 // cache's 16 bits (fp16 for int8) for the second product; maxima, sums and O are 32 bits.
 #include <atomic>
 #include <type_traits>
@@ -108,6 +108,9 @@ __global__ void __launch_bounds__(DecodeShape<DP, NT, I8>::kWarps * 32, DecodeSh
     attn_decode_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using S = DecodeShape<DP, NT, I8>;
   using M = typename std::conditional<I8, __half, T>::type;  // type of the products
+  // fp16 weights: 2^7 larger than in bf16, so that those down to 2^-32 of the largest are more than 0
+  constexpr bool kHalf = std::is_same<M, __half>::value;
+  constexpr float kLift = kHalf ? 7.f : 0.f, kDrop = kHalf ? 1.f / 128.f : 1.f;
   extern __shared__ unsigned char decode_raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(decode_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* q_s = sm + (S::kRing > S::kJoin ? S::kRing : S::kJoin);
@@ -364,7 +367,7 @@ __global__ void __launch_bounds__(DecodeShape<DP, NT, I8>::kWarps * 32, DecodeSh
             if (((none >> u) & 1) || key >= s1 || key < klo[i][c & 1] || key >= khi[i][c & 1]) v = -INFINITY;
           }
           s[u][i][0][c] = v;
-          high |= v > m[i][c & 1] + 8.f;
+          high |= v > m[i][c & 1] + (8.f + kLift);
         }
     }
     if (++scale_slot == S::kScaleSlots) scale_slot = 0;
@@ -396,7 +399,7 @@ __global__ void __launch_bounds__(DecodeShape<DP, NT, I8>::kWarps * 32, DecodeSh
               vref[i][c] = ref;
             }
           }
-          const float mn = fmaxf(m[i][c], x);
+          const float mn = fmaxf(m[i][c], x - kLift);
           const float by = mn == -INFINITY ? 1.f : ex2(m[i][c] - mn);
           m[i][c] = mn;
           base[i][c] = mn == -INFINITY ? 0.f : mn;
@@ -488,7 +491,7 @@ __global__ void __launch_bounds__(DecodeShape<DP, NT, I8>::kWarps * 32, DecodeSh
       x += __shfl_xor_sync(0xffffffffu, x, 4);
       x += __shfl_xor_sync(0xffffffffu, x, 8);
       x += __shfl_xor_sync(0xffffffffu, x, 16);
-      if (g == 0) ml_s[warp][8 * i + 2 * t + c] = make_float2(m[i][c], x);
+      if (g == 0) ml_s[warp][8 * i + 2 * t + c] = make_float2(m[i][c] + kLift, x * kDrop);
     }
   float* acc = reinterpret_cast<float*>(sm);   // [warp][row][DP + 4]
   constexpr int LD = DP + 4;
@@ -501,7 +504,8 @@ __global__ void __launch_bounds__(DecodeShape<DP, NT, I8>::kWarps * 32, DecodeSh
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float2* dst = reinterpret_cast<float2*>(acc + (warp * NT * 8 + 8 * i + 2 * t + c) * LD + d);
-        *dst = make_float2(o[i][j][c] * (I8 ? vref[i][c] : 1.f), o[i][j][c + 2] * (I8 ? vref[i][c] : 1.f));
+        const float by = kDrop * (I8 ? vref[i][c] : 1.f);
+        *dst = make_float2(o[i][j][c] * by, o[i][j][c + 2] * by);
       }
     }
   __syncthreads();

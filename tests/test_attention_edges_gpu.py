@@ -2,6 +2,8 @@
 small, tables that share rows, scales of 0 and below, tokens of no sequence, values far apart in size.
 
 Bounds as in test_attention_gpu.py: outputs round once to 16 bits (u), the softmax weights once more."""
+import math
+
 import pytest
 import torch
 
@@ -151,3 +153,30 @@ def test_int8_values_of_hidden_keys_cost_nothing(by, hq, hkv, d, new):
     rows = torch.arange(new - 2)
     s.q, s.news, s.lens_list = torch.cat([s.q[rows], s.q[new:]]), [new - 2, 1], [298, 200]
     check_rows(s, torch.cat([out[rows], out[new:]]), d ** -0.5, window=30)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_many_small_weights_beside_a_large_one(int8, dtype):
+    """One key outweighs each of 200,000 others by 2^26: together they are 0.3 % of the sum, and all of the output."""
+    new, h, d, page, keys = 4096, 10, 64, 256, 200_000
+    kind = torch.int8 if int8 else dtype
+    k = torch.zeros(2, h, page, d, dtype=kind, device=DEV)
+    v = torch.full_like(k, 64 if int8 else 1)
+    k[0, :, 0, 0] = 104 if int8 else 26
+    v[0, :, 0] = 0
+    scale = [torch.full((2, h, page), by, device=DEV) for by in (0.25, 2.0 ** -6)] if int8 else [None, None]
+    table = torch.ones(1, -(-keys // page), dtype=torch.int32, device=DEV)
+    table[0, 0] = 0
+    lens = torch.tensor([keys], dtype=torch.int32, device=DEV)
+    for n in (new, 1):
+        q = torch.zeros(n, h, d, dtype=dtype, device=DEV)
+        q[..., 0] = 1
+        starts = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+        out, lse = A.paged_attention(q, k, v, table, lens, starts, k_scale=scale[0], v_scale=scale[1], scale=math.log(2.0),
+                                     causal=False, return_lse=True)
+        rest = (keys - 1) * 2.0 ** -26
+        want = rest / (1 + rest)
+        # weights and output rounded once each, relative to themselves; 1e-3 and 1e-4 for the 32-bit sums of 200,000 terms
+        assert ((out.double() - want).abs() <= (2 * EPS[dtype] + 1e-3) * want).all()
+        assert ((lse.double() - (26 * math.log(2) + math.log1p(rest))).abs() <= 1e-4).all()
