@@ -18,7 +18,8 @@ int64_t plan(AttnArgs& a, bool i8, int64_t max_new, int64_t max_len, bool& chunk
   // first, from 49 rows on (the same, 32 rows: 96 us here, 156 there; 16/2 heads of 256: 63 and 88). Its
   // fp16 copy of an 8-bit cache is kept to 4 GB; past that (a batch of very long sequences) the decode
   // kernel reads the 8 bits again after all.
-  const int64_t wide_len = (max_len + 127) & ~int64_t(127), wide_rows = a.kv.seqs * (int64_t)a.kv.heads * wide_len;
+  // A bound of 0 leaves it one tile: a launch of no blocks is an error.
+  const int64_t wide_len = max_len ? (max_len + 127) & ~int64_t(127) : 128, wide_rows = a.kv.seqs * (int64_t)a.kv.heads * wide_len;
   chunked = max_new * a.G > (i8 ? 48 : 16) && (!i8 || wide_rows * a.D <= int64_t(1) << 30);
   if (chunked) plan_attn_chunk(a, max_new, max_len);
   else plan_attn_decode(a, max_new, max_len);

@@ -180,3 +180,14 @@ def test_many_small_weights_beside_a_large_one(int8, dtype):
         # weights and output rounded once each, relative to themselves; 1e-3 and 1e-4 for the 32-bit sums of 200,000 terms
         assert ((out.double() - want).abs() <= (2 * EPS[dtype] + 1e-3) * want).all()
         assert ((lse.double() - (26 * math.log(2) + math.log1p(rest))).abs() <= 1e-4).all()
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("new", [2, 70])
+def test_nothing_cached_at_all(int8, new):
+    """New tokens whose sequences have no key and no page, the bound on lengths 0: zeros."""
+    s = Setup([new, 1], [0, 0], 4, 2, 64, torch.float16, int8, seed=63)
+    for table, kw in ((s.table, dict(max_len=0)), (s.table[:, :0].contiguous(), {})):
+        out, lse = A.paged_attention(s.q, *s.pools, table, s.lens, s.starts, k_scale=s.scale[0], v_scale=s.scale[1],
+                                     return_lse=True, **kw)
+        assert (out == 0).all() and (lse == -float("inf")).all()
