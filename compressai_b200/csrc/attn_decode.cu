@@ -130,8 +130,8 @@ __global__ void __launch_bounds__(DecodeShape<DP, NT, I8>::kWarps * 32, DecodeSh
   if (w.rows <= 0) return;
   int lo, hi;
   block_keys(a, w, lo, hi);
-  const int s0 = lo + split * a.chunk, s1 = min(hi, s0 + a.chunk);
-  if (split > 0 && s0 >= hi) {   // split 0 stays: it writes the rows that see nothing
+  const int s0 = lo + split * a.chunk, s1 = s0 + min(a.chunk, hi - s0);   // no sum past 2^31
+  if (split > 0 && (int64_t)split * a.chunk >= hi - lo) {   // split 0 stays: it writes the rows that see nothing
     if (!I8) strays();
     return;
   }
@@ -556,7 +556,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
   sequence_rows(a.kv, b, first, count);
   block_keys(a, attn_rows(a, b, ((t - first) * a.G + hq % a.G) / a.rows_per_block), lo, hi);
   if (hi - lo <= a.chunk) return;   // written already
-  const int n = min(256, (hi - lo + a.chunk - 1) / a.chunk);
+  const int n = min(256, (hi - lo - 1) / a.chunk + 1);
   const int64_t at = (int64_t)t * a.hq + hq;
   // the weight of each split: one a thread
   const int i = threadIdx.x;
@@ -624,7 +624,7 @@ __global__ void __launch_bounds__(256) attn_join_rows_kernel(const AttnArgs a) {
   sequence_rows(a.kv, b, first, count);
   block_keys(a, attn_rows(a, b, ((t - first) * a.G + hq % a.G) / a.rows_per_block), lo, hi);
   if (hi - lo <= a.chunk) return;   // written already
-  const int n = min(32, (hi - lo + a.chunk - 1) / a.chunk);
+  const int n = min(32, (hi - lo - 1) / a.chunk + 1);
   const int64_t at = (int64_t)t * a.hq + hq;
   const float2 x = lane < n ? a.part_ml[at * a.splits + lane] : make_float2(-INFINITY, 0.f);
   float top = x.x;

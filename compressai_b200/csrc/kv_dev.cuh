@@ -30,8 +30,8 @@ inline int paged_kv(PagedKV& kv, const void* k, const void* v, int kv_dtype, con
   if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)) || bad_head_size(D)) return VQ2_ERR_SHAPE;
   if (pages < 1 || heads < 1 || heads > 4096 || seqs < 0 || seqs > 0x7ffffff || cols < 0 || table_stride < 0)
     return VQ2_ERR_SHAPE;
-  if (pages > 0x7fffffff / page_size || pages * page_size > 0x7fffffff / heads || cols > 0x7fffffff / page_size)
-    return VQ2_ERR_SHAPE;  // a pool's rows and a sequence's positions are counted in 32 bits
+  if (pages > 0x7fffffff / page_size || pages * page_size > 0x7fffffff / heads || cols > 0x7fffff00 / page_size)
+    return VQ2_ERR_SHAPE;  // a pool's rows and a sequence's positions, and the 255 after them, are counted in 32 bits
   if (!aligned(k, 16) || !aligned(v, 16) || !aligned(k_scale, 16) || !aligned(v_scale, 16)) return VQ2_ERR_ALIGN;
   int l = 4;
   while ((1 << l) < page_size) ++l;

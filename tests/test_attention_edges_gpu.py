@@ -191,3 +191,20 @@ def test_nothing_cached_at_all(int8, new):
         out, lse = A.paged_attention(s.q, *s.pools, table, s.lens, s.starts, k_scale=s.scale[0], v_scale=s.scale[1],
                                      return_lse=True, **kw)
         assert (out == 0).all() and (lse == -float("inf")).all()
+
+
+def test_the_longest_sequence():
+    """2^31 - 256 positions on two pages: the last page, on which all the weight lies, is read."""
+    cols, d = (2 ** 31 - 256) // 256, 16
+    k = torch.zeros(2, 1, 256, d, dtype=torch.float16, device=DEV)
+    v = torch.ones_like(k)
+    k[1, :, :, 0], v[1] = 10, 3
+    table = torch.zeros(1, cols, dtype=torch.int32, device=DEV)
+    table[0, -1] = 1
+    q = torch.full((1, 1, d), 4.0, dtype=torch.float16, device=DEV)
+    lens = torch.tensor([2 ** 31 - 256], dtype=torch.int32, device=DEV)
+    out, lse = A.paged_attention(q, k, v, table, lens, scale=1.0, return_lse=True)
+    # e^40 * 256 against 2^31: the rest is 4e-11 of it
+    assert (out == 3).all() and abs(lse.item() - 40 - math.log(256)) <= 1e-4
+    with pytest.raises(ValueError):
+        A.cache_read(k, v, table.new_zeros(1, cols + 1), torch.zeros(2, dtype=torch.int32, device=DEV), 1)
