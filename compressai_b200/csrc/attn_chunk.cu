@@ -644,8 +644,7 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
               }
 #pragma unroll
               for (int o = 1; o < DP / 8; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-              int up = 0;
-              if (big > 1e-30f && big < 1e30f) up = 13 - ilogbf(big);
+              const int up = fp16_lift(big);
               const float by = __int_as_float((127 + up) << 23);
               back = __int_as_float((127 - up) << 23);
 #pragma unroll

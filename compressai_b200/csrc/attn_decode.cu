@@ -228,9 +228,7 @@ __global__ void __launch_bounds__(DecodeShape<DP, NT, I8>::kWarps * 32, DecodeSh
           }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // largest value into [2^13, 2^14); exponents of the row's largest outside +-100 stay as they are
-        int e = 0;
-        if (top > 1e-30f && top < 1e30f) e = 13 - ilogbf(top);
+        const int e = fp16_lift(top);
         const float by = __int_as_float((127 + e) << 23);
         back = __int_as_float((127 - e) << 23);
 #pragma unroll

@@ -43,6 +43,12 @@ __device__ __forceinline__ float above(float scale) {
   return __uint_as_float(min((__float_as_uint(scale) & 0x7f800000u) + 0x00800000u, 0x7e800000u));
 }
 
+// The exponent that brings a bf16 row whose largest magnitude is `top` into fp16, to 2^13 .. 2^14, and back: its
+// power of two and the inverse are normal numbers. 0 where there is nothing to bring, or no finite number.
+__device__ __forceinline__ int fp16_lift(float top) {
+  return top > 0.f && top < INFINITY ? min(13 - ilogbf(top), 126) : 0;
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if (std::is_same<T, __half>::value) {

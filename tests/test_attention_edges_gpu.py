@@ -208,3 +208,14 @@ def test_the_longest_sequence():
     assert (out == 3).all() and abs(lse.item() - 40 - math.log(256)) <= 1e-4
     with pytest.raises(ValueError):
         A.cache_read(k, v, table.new_zeros(1, cols + 1), torch.zeros(2, dtype=torch.int32, device=DEV), 1)
+
+
+@pytest.mark.parametrize("new", [1, 70])
+@pytest.mark.parametrize("d", [64, 256])
+@pytest.mark.parametrize("size", [1e34, 1e31, 1e-31, 1e-38])
+def test_int8_with_queries_of_any_size(size, d, new):
+    """bf16 queries from the smallest normal numbers to the largest, the scale set against them."""
+    s = Setup([new], [300], 4, 1, d, torch.bfloat16, int8=True, page=16, seed=64)
+    s.q = (s.q.float().clamp(-4, 4) * size).bfloat16()
+    scale = d ** -0.5 / size
+    check_rows(s, s.run(scale=scale), scale)
