@@ -148,9 +148,10 @@ class PagedKVCache:
                  device="cuda"):
         if pages < 1 or layers < 1 or max_len < 1:
             raise ValueError("layers, pages and max_len are at least 1")
-        self.page_size, self.max_len, self.device = page_size, max_len, torch.device(device)
+        self.page_size, self.max_len = page_size, max_len
         shape = (pages, kv_heads, page_size, head_size)
         self.pools = [tuple(torch.empty(shape, dtype=dtype, device=device) for _ in range(2)) for _ in range(layers)]
+        self.device = self.pools[0][0].device   # with its index: the current device may change
         self.scales = [tuple(torch.empty(shape[:3], device=device) for _ in range(2)) if dtype == torch.int8 else (None, None)
                        for _ in range(layers)]
         self.free = list(range(pages - 1, -1, -1))

@@ -219,3 +219,11 @@ def test_int8_with_queries_of_any_size(size, d, new):
     s.q = (s.q.float().clamp(-4, 4) * size).bfloat16()
     scale = d ** -0.5 / size
     check_rows(s, s.run(scale=scale), scale)
+
+
+def test_a_cache_stays_on_its_device():
+    """Named without an index, the device is the one that was current when the pools were made."""
+    c = A.PagedKVCache(1, 2, 1, 16, page_size=16)
+    assert c.device == c.pools[0][0].device == torch.device("cuda", torch.cuda.current_device())
+    c.begin([c.add()], [3])
+    assert c.batch["table"].device == c.device
