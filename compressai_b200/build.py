@@ -26,6 +26,7 @@ BUILD = os.path.join(PKG, "_build")
 LIBDIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIBDIR, "libvq2_b200.so")
 HOST = os.path.join(LIBDIR, "_attention_host.so")
+HOST_STAMP = os.path.join(BUILD, "attention_host.key")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-fvisibility=hidden",
@@ -64,13 +65,29 @@ def _compile(src, force):
     return obj, log
 
 
+def _host_key():
+    """What the host module is compiled against, beside the sources: the interpreter's ABI and torch's."""
+    import sysconfig
+
+    import torch
+    return f"{sysconfig.get_config_var('EXT_SUFFIX')} torch {torch.__version__}"
+
+
+def _host_stale(src):
+    try:
+        with open(HOST_STAMP) as f:
+            return f.read() != _host_key() or _stale(HOST, src)
+    except FileNotFoundError:
+        return True
+
+
 def _build_host(force):
-    """lib/_attention_host.so: a CPython module over torch's C++ headers."""
+    """lib/_attention_host.so: a CPython module over torch's C++ headers; rebuilt when torch changes too."""
     import sysconfig
 
     import torch
     src = os.path.join(CSRC, "attention_host.cpp")
-    if not force and not _stale(HOST, src):
+    if not force and not _host_stale(src):
         return HOST
     root = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(nvcc()))
@@ -85,6 +102,8 @@ def _build_host(force):
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed for {src}:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, HOST)
+    with open(HOST_STAMP, "w") as f:
+        f.write(_host_key())
     return HOST
 
 
