@@ -227,3 +227,27 @@ def test_a_cache_stays_on_its_device():
     assert c.device == c.pools[0][0].device == torch.device("cuda", torch.cuda.current_device())
     c.begin([c.add()], [3])
     assert c.batch["table"].device == c.device
+
+
+@pytest.mark.parametrize("dtype,int8,new", [(torch.float16, False, 4), (torch.bfloat16, False, 2), (torch.float16, True, 12),
+                                            (torch.bfloat16, True, 5)])
+@pytest.mark.parametrize("hq,hkv,d", [(16, 4, 256), (8, 8, 64), (8, 2, 96), (12, 3, 128)])
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 21), (False, 0), (False, 40)])
+def test_few_new_tokens_of_several_positions(dtype, int8, new, hq, hkv, d, causal, window):
+    """Drafts: rows of several tokens in one block of the kernel for few rows (16 rows, over int8 48), ragged."""
+    news = [new, 1, 0, max(1, new - 1), new]
+    s = Setup(news, [new, 40, 9, 333, 1500], hq, hkv, d, dtype, int8, page=16, seed=65)
+    out, lse = s.run(causal=causal, window=window, max_new=new, max_len=1500, return_lse=True)
+    s.check(out, lse, causal=causal, window=window)
+
+
+@pytest.mark.parametrize("window", [0, 50])
+def test_int8_with_a_table_too_wide_to_widen(window):
+    """Room for more keys than the fp16 copy of an int8 cache may hold (2^30 values): many rows go to the kernel for
+    few, as many blocks of them as it takes."""
+    s = Setup([150, 1, 40], [700, 333, 40], 8, 2, 256, torch.bfloat16, int8=True, page=256, seed=66)
+    wide = torch.full((3, 2800), -1, dtype=torch.int32, device=DEV)   # 3 * 2 * 2800 * 256 * 256 > 2^30
+    wide[:, :s.table.shape[1]] = s.table
+    s.table = wide
+    out, lse = s.run(window=window, return_lse=True)
+    s.check(out, lse, window=window)
