@@ -9,6 +9,8 @@ int32 ``[seqs + 1]`` says where its new tokens begin in q, k and v (None: one ne
 stay on the device; a call reads them when its kernels run, so a CUDA graph replays with whatever
 they hold then. ``PagedKVCache`` keeps them for a program that has no allocator of its own.
 
+Nothing here is recorded by autograd: rotary's gradient is its ``inverse``, the rest is for inference.
+
 The reference leaves these blocks to the transformers modules (vq2/load_and_test_full_35b.py:124-223),
 whose cache is concatenated anew every step.
 """
@@ -116,7 +118,8 @@ def paged_attention(q, k_pages, v_pages, table, lens, starts=None, *, k_scale=No
     is not 0; one that sees none gives zeros, and so do tokens of no sequence, before ``starts[0]`` and from
     ``starts[-1]`` on (a step padded to a fixed size). Query head h reads key/value head h // (Hq / kv_heads). ``scale``
     defaults to D^-0.5. ``max_new`` and ``max_len`` bound every sequence's new tokens and length; the defaults (all of
-    T, all that ``table`` has room for) are right and size the launch for more than may be needed. ``return_lse``:
+    T, all that ``table`` has room for) are right and size the launch for more than may be needed; of a sequence past
+    them, keys from ``max_len`` on may be left out and rows from ``max_new`` on hold anything. ``return_lse``:
     also fp32 [T, Hq], the natural logarithm of each row's sum of exponentials (-inf where no key is seen).
 
     A value that is not finite in a cached V row makes NaN, besides in the rows that see its token, in rows of the same
@@ -142,7 +145,8 @@ class PagedKVCache:
     calls ``write`` and ``attend`` once a layer; ``release`` gives a sequence's pages back.
 
     ``dtype`` is that of q, k and v, or torch.int8, which quantises what is written. The tables are kept on
-    the host and go to the device in one copy a step."""
+    the host and go to the device in one copy a step, as new tensors: a captured step would replay with the ones it
+    was captured with (keep tables of your own for that)."""
 
     def __init__(self, layers, pages, kv_heads, head_size, *, page_size=64, max_len=32768, dtype=torch.bfloat16,
                  device="cuda"):

@@ -31,7 +31,7 @@
 // Bound: a step of 256 rows x 128 keys is 2048 cycles of MMA at head size 128 (in each block of a pair at
 // 256) and, at 16 exponentials a clock an SM, 2048 (1024) of exponentials. Measured 3700 cycles at 128,
 // the chain softmax -> weights -> O -> next scores of a row tile; 2350 at 256 (prompt of 8192 tokens
-// 394 us, 1.39 PFLOP/s).
+// 401 us, 1.37 PFLOP/s).
 //
 // 8-bit caches: a launch before this one writes the visible keys and values out once as exact fp16 (an
 // int8 is; see attn_decode.cu, also for the scales: the key's multiplies the score, the value's the

@@ -661,7 +661,8 @@ VQ2_API int vq2_cache_read(const void* k_pages, const void* v_pages, int kv_dtyp
  * position - window when window > 0. A token that sees none, or that no sequence has (before starts[0],
  * from starts[seqs] on), gives zeros (lse -inf). out: contiguous,
  * dtype; lse (may be NULL): fp32 [tokens, q_heads], the natural logarithm of the sum. max_new and
- * max_len bound every sequence's new tokens and length (larger is only slower). q: 16-byte aligned,
+ * max_len bound every sequence's new tokens and length (larger is only slower; of a sequence past them, keys
+ * from max_len on may be left out and rows from max_new on are not written); without starts max_new is 1. q: 16-byte aligned,
  * strides multiples of 8. workspace: vq2_paged_attention_workspace(...) bytes, 16-byte aligned.
  * A value that is not finite in a cached V row can make NaN in rows that do not see its token too (0 x
  * inf); what lies past a sequence's end or in unmapped pages may hold anything.
