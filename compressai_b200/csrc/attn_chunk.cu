@@ -305,8 +305,8 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
   const int b = sorted ? nth_longest(a.kv, nth, lane) : nth;
   const AttnRows w = attn_rows(a, b, rb);
   if (!I8)   // the widening kernel's work there: registers are short here (two int8 chunks 160 us for 163)
-    blank_strays(a, w, b, ((rb * a.kv.heads + h) * a.splits + split) * (PAIR ? 2 : 1) + rank,
-                 a.row_blocks * a.kv.heads * a.splits * (PAIR ? 2 : 1));
+    blank_strays(a, w, b, (((int64_t)rb * a.kv.heads + h) * a.splits + split) * (PAIR ? 2 : 1) + rank,
+                 (int64_t)a.row_blocks * a.kv.heads * a.splits * (PAIR ? 2 : 1));
   if (w.rows <= 0) return;
   int lo, hi;
   block_keys(a, w, lo, hi);

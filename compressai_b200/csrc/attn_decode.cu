@@ -125,7 +125,9 @@ __global__ void __launch_bounds__(DecodeShape<DP, NT, I8>::kWarps * 32, DecodeSh
   const AttnRows w = attn_rows(a, b, rb);
   // Behind the first copies where registers allow it: ahead of them it takes 0.2 of 8.8 us of a lone sequence's
   // step; over an 8-bit cache (128 registers) it spills there (four long sequences 143 us for 141).
-  auto strays = [&] { blank_strays(a, w, b, (rb * a.kv.heads + h) * a.splits + split, a.row_blocks * a.kv.heads * a.splits); };
+  auto strays = [&] {
+    blank_strays(a, w, b, ((int64_t)rb * a.kv.heads + h) * a.splits + split, (int64_t)a.row_blocks * a.kv.heads * a.splits);
+  };
   if (I8 || w.rows <= 0) strays();
   if (w.rows <= 0) return;
   int lo, hi;

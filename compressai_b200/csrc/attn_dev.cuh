@@ -103,15 +103,15 @@ __device__ __forceinline__ void block_keys(const AttnArgs& a, const AttnRows& w,
 
 // Zeros, lse -inf, for `rows` rows (token, head) of `vecs` 16-byte pieces: part `part` of `parts` blocks. Not
 // inlined: a launch that has no such rows then does not fetch these instructions.
-static __device__ __noinline__ void blank(uint4* out, float* lse, int64_t rows, int vecs, int part, int parts) {
-  const int64_t i0 = (int64_t)part * blockDim.x + threadIdx.x, step = (int64_t)parts * blockDim.x;
+static __device__ __noinline__ void blank(uint4* out, float* lse, int64_t rows, int vecs, int64_t part, int64_t parts) {
+  const int64_t i0 = part * blockDim.x + threadIdx.x, step = parts * blockDim.x;
   for (int64_t i = i0; i < rows * vecs; i += step) out[i] = make_uint4(0, 0, 0, 0);
   if (lse)
     for (int64_t i = i0; i < rows; i += step) lse[i] = -INFINITY;
 }
 
 // The tokens [from, to).
-__device__ __forceinline__ void blank_tokens(const AttnArgs& a, int from, int to, int part, int parts) {
+__device__ __forceinline__ void blank_tokens(const AttnArgs& a, int from, int to, int64_t part, int64_t parts) {
   const int64_t row = (int64_t)from * a.hq;
   blank(reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row * a.D), a.lse ? a.lse + row : nullptr,
         (int64_t)(to - from) * a.hq, a.D >> 3, part, parts);
@@ -119,7 +119,7 @@ __device__ __forceinline__ void blank_tokens(const AttnArgs& a, int from, int to
 
 // Tokens of no sequence (a step padded to a fixed size): the first sequence's blocks blank those before its
 // tokens, the last one's those after, each its share.
-__device__ __forceinline__ void blank_strays(const AttnArgs& a, const AttnRows& w, int b, int part, int parts) {
+__device__ __forceinline__ void blank_strays(const AttnArgs& a, const AttnRows& w, int b, int64_t part, int64_t parts) {
   const bool before = b == 0 && w.first > 0, after = b == a.kv.seqs - 1 && w.first + w.count < a.T;
   if (!before && !after) return;
   if (before) blank_tokens(a, 0, w.first, part, parts);
