@@ -310,8 +310,8 @@ __global__ void __launch_bounds__(ChunkShape<DP, I8>::Threads, 1)
   if (w.rows <= 0) return;
   int lo, hi;
   block_keys(a, w, lo, hi);
-  const int s0 = lo + split * a.chunk, s1 = s0 + min(a.chunk, hi - s0);   // no sum past 2^31
   if (split > 0 && (int64_t)split * a.chunk >= hi - lo) return;  // split 0 stays: it writes the rows that see nothing
+  const int s0 = lo + split * a.chunk, s1 = s0 + min(a.chunk, hi - s0);   // no sum past 2^31
   const bool alone = hi - lo <= a.chunk;
   const int tiles = s1 > s0 ? (s1 - s0 + 127) >> 7 : 0;
   const int nq = NQ == 2 && w.rows > 128 ? 2 : 1;  // row tiles in use

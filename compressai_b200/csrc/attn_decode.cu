@@ -132,11 +132,11 @@ __global__ void __launch_bounds__(DecodeShape<DP, NT, I8>::kWarps * 32, DecodeSh
   if (w.rows <= 0) return;
   int lo, hi;
   block_keys(a, w, lo, hi);
-  const int s0 = lo + split * a.chunk, s1 = s0 + min(a.chunk, hi - s0);   // no sum past 2^31
   if (split > 0 && (int64_t)split * a.chunk >= hi - lo) {   // split 0 stays: it writes the rows that see nothing
     if (!I8) strays();
     return;
   }
+  const int s0 = lo + split * a.chunk, s1 = s0 + min(a.chunk, hi - s0);   // no sum past 2^31
   const bool alone = hi - lo <= a.chunk;
   const int tiles = s1 > s0 ? (s1 - s0 + S::kKeys - 1) / S::kKeys : 0;
 

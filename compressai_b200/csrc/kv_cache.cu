@@ -8,8 +8,9 @@
 // All three are moved bytes: each thread owns 8 consecutive values of a head (one 16-byte load),
 // LPR = 2..32 lanes a row. In the half layout a value's partner sits half a rotary width away: a
 // lane holds 4 values and their 4 partners (two 8-byte loads), or, for few tokens and for widths that
-// are no multiple of 8, 8 values in a row and reads their partners beside them. cos and sin belong to (token, pair) and serve every head, so a block takes
-// one token and computes them once into shared memory, behind the value loads already in flight.
+// are no multiple of 8, 8 values in a row and reads their partners beside them. cos and sin belong to
+// (token, pair) and serve every head, so a block takes one token and computes them once into shared
+// memory, behind the value loads already in flight.
 #include <type_traits>
 
 #include "kv_dev.cuh"
