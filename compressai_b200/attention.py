@@ -1,9 +1,11 @@
 """What stands between a decoder layer's q/k/v projections and its output projection: rotary
-positions, a paged key/value cache (16-bit, or 8-bit with a scale per token and head) and attention
+positions, a paged key/value cache (16-bit, 8-bit with a scale per token and head, or 4-bit) and attention
 of new tokens over it -- one token per sequence while decoding, chunks or whole prompts before that.
 
 Tensors. A cache layer is two pools ``[pages, kv_heads, page_size, head_size]`` (int8 ones with two
-fp32 scale tensors ``[pages, kv_heads, page_size]``); ``table`` int32 ``[seqs, cols]`` names the pages
+fp32 scale tensors ``[pages, kv_heads, page_size]``; 4-bit ones, of head sizes that are multiples of 32, as
+uint8 ``[.., head_size / 2]`` with two uint8 scale tensors ``[pages, kv_heads, page_size / 16, 4 + groups, 16]``,
+``groups`` of 64 values a head: ``empty_pool`` makes either); ``table`` int32 ``[seqs, cols]`` names the pages
 of each sequence, ``lens`` int32 ``[seqs]`` counts its tokens, the new ones included, and ``starts``
 int32 ``[seqs + 1]`` says where its new tokens begin in q, k and v (None: one new token each). They
 stay on the device; a call reads them when its kernels run, so a CUDA graph replays with whatever
@@ -79,11 +81,25 @@ def _load():
         spec = importlib.util.spec_from_file_location("_attention_host", path)
         mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(mod)
-        names = ("vq2_rotary", "vq2_cache_write", "vq2_cache_read", "vq2_paged_attention", "vq2_paged_attention_workspace")
+        names = ("vq2_rotary", "vq2_cache_write", "vq2_cache_read", "vq2_paged_attention", "vq2_paged_attention_workspace",
+                 "vq2_copy_pages")
         mod.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names}, _lib.check,
                  torch.OutOfMemoryError)
         _host = mod
     return _host
+
+
+def empty_pool(pages, kv_heads, page_size, head_size, dtype=torch.bfloat16, device="cuda"):
+    """(pool, scales) of one layer's K or V, their contents not set; scales are None for fp16 and bf16. ``dtype``
+    torch.int8 or torch.int4 makes a quantised one (4 bits: two values a byte, uint8)."""
+    shape = (pages, kv_heads, page_size, head_size)
+    if dtype == torch.int4:
+        if head_size % 32 or page_size % 16:
+            raise ValueError(f"a 4-bit cache has heads of a multiple of 32 values and pages of one of 16 rows; got {head_size}, {page_size}")
+        return (torch.empty(*shape[:3], head_size // 2, dtype=torch.uint8, device=device),
+                torch.empty(pages, kv_heads, page_size // 16, 4 + -(-head_size // 64), 16, dtype=torch.uint8, device=device))
+    scale = torch.empty(shape[:3], device=device) if dtype == torch.int8 else None
+    return torch.empty(shape, dtype=dtype, device=device), scale
 
 
 def rotary(q, k, positions, inv_freq, *, interleaved=False, factor=1.0, inverse=False):
@@ -99,15 +115,17 @@ def cache_write(k, v, k_pages, v_pages, table, lens, starts=None, *, k_scale=Non
     """Write the new tokens' k and v [T, kv_heads, D] into the pools, in one launch. With ``inv_freq`` k is turned at
     its position first, and ``q`` [T, Hq, D] with it: the turned q is returned (None without q; a token of no sequence
     turns as at position 0). int8 pools: every (token, head) row is quantised with its own scale, amax / 127, from the
-    turned values in 32 bits; a row with an infinity or a NaN reads back as NaN. Tokens whose position has no page in
-    ``table`` are not stored."""
+    turned values in 32 bits; a row with an infinity or a NaN reads back as NaN. 4-bit pools (uint8): a row's scale is
+    amax / 7; each 64 of its values share a factor, their amax over the row's, rounded up to 8 bits (e4m3), and
+    become integers from -7 to 7, to the nearest, ties away from zero: off by half of factor * scale at most. Tokens
+    whose position has no page in ``table`` are not stored."""
     return (_host or _load()).cache_write(k, v, k_pages, v_pages, table, k_scale, v_scale, lens, starts, q, inv_freq,
                                           interleaved, factor)
 
 
 def cache_read(k_pages, v_pages, table, starts, total, *, k_scale=None, v_scale=None, dtype=None):
     """Whole sequences back out of the pools: (k, v) [total, kv_heads, D], sequence b's first starts[b+1] - starts[b]
-    positions from row starts[b] on. ``dtype``: of the result for int8 pools (default bf16)."""
+    positions from row starts[b] on. ``dtype``: of the result for int8 and 4-bit pools (default bf16)."""
     return (_host or _load()).cache_read(k_pages, v_pages, table, k_scale, v_scale, starts, total, dtype)
 
 
@@ -131,6 +149,33 @@ def paged_attention(q, k_pages, v_pages, table, lens, starts=None, *, k_scale=No
                                               max_new, max_len, return_lse)
 
 
+def copy_pages(pools, src, dst):
+    """In every one of ``pools`` (contiguous tensors [pages, ..], of any type, a page a multiple of 16 bytes: K and V of
+    all layers with their scales, say) page ``dst[i]`` becomes what page ``src[i]`` is, in one launch. ``src`` and ``dst``:
+    int32 on the pools' device, read when the kernel runs (ids outside the pools copy nothing), or lists, which are
+    checked: pages in ``dst`` are different ones and none is in ``src``. Where a tensor breaks that, such a page
+    holds bytes of any of its sources."""
+    if not isinstance(src, torch.Tensor) or not isinstance(dst, torch.Tensor):
+        src, dst = ([int(p) for p in x] for x in (src, dst))
+        if not pools:
+            return
+        pages = pools[0].shape[0]
+        if len(src) != len(dst) or len(set(dst)) != len(dst) or set(dst) & set(src):
+            raise ValueError("src and dst name as many pages each, those in dst different ones, none of them in src")
+        if any(not 0 <= p < pages for p in src + dst):
+            raise ValueError(f"the pools have pages 0 to {pages - 1}")
+        src, dst = _ints([src, dst], pools[0].device)
+    (_host or _load()).copy_pages(pools, src, dst)
+
+
+def _ints(lists, device):
+    """Lists of integers as int32 tensors on a device, in one copy that does not wait."""
+    host = torch.tensor([v for x in lists for v in x], dtype=torch.int32)
+    if device.type == "cuda":
+        host = host.pin_memory()
+    return host.to(device, non_blocking=True).split([len(x) for x in lists])
+
+
 def check_status(device=None):
     """Wait for the device and raise VQ2Error if a ``paged_attention`` on it, on any stream, gave up a wait since this
     was last called: the kernels wait for their own copies about 2 s at most, then leave NaN in the rows they were at.
@@ -144,21 +189,26 @@ class PagedKVCache:
     has which page. A program ``add``s sequences, says with ``begin`` how many tokens each one adds, and then
     calls ``write`` and ``attend`` once a layer; ``release`` gives a sequence's pages back.
 
-    ``dtype`` is that of q, k and v, or torch.int8, which quantises what is written. The tables are kept on
+    ``fork`` makes a sequence that goes on from another one's tokens, on the same pages: whole pages stay shared, a
+    partly filled one is copied (in all layers at once) when one of those that share it writes on. ``truncate`` takes a
+    sequence's last tokens back, ``compact`` moves the pages in use to the front of the pools, and ``resize``
+    gives the pools another size. These belong between steps: they end the batch that ``begin`` has set.
+
+    ``dtype`` is that of q, k and v, or torch.int8 or torch.int4, which quantise what is written. The tables are kept on
     the host and go to the device in one copy a step, as new tensors: a captured step would replay with the ones it
-    was captured with (keep tables of your own for that)."""
+    was captured with (keep tables of your own for that). Page copies run on the current stream, as the step's calls do."""
 
     def __init__(self, layers, pages, kv_heads, head_size, *, page_size=64, max_len=32768, dtype=torch.bfloat16,
                  device="cuda"):
         if pages < 1 or layers < 1 or max_len < 1:
             raise ValueError("layers, pages and max_len are at least 1")
         self.page_size, self.max_len = page_size, max_len
-        shape = (pages, kv_heads, page_size, head_size)
-        self.pools = [tuple(torch.empty(shape, dtype=dtype, device=device) for _ in range(2)) for _ in range(layers)]
+        made = [[empty_pool(pages, kv_heads, page_size, head_size, dtype, device) for _ in range(2)] for _ in range(layers)]
+        self.pools = [(k[0], v[0]) for k, v in made]
+        self.scales = [(k[1], v[1]) for k, v in made]
         self.device = self.pools[0][0].device   # with its index: the current device may change
-        self.scales = [tuple(torch.empty(shape[:3], device=device) for _ in range(2)) if dtype == torch.int8 else (None, None)
-                       for _ in range(layers)]
         self.free = list(range(pages - 1, -1, -1))
+        self.users = [0] * pages                # sequences on each page
         self.pages, self.lengths = {}, {}
         self._next, self.batch = 0, None
 
@@ -168,9 +218,86 @@ class PagedKVCache:
         self.pages[self._next], self.lengths[self._next] = [], 0
         return self._next
 
+    def fork(self, seq):
+        """A new sequence's id, with the tokens of ``seq`` and on its pages."""
+        pages, length = self.pages[seq], self.lengths[seq]
+        self.batch = None
+        new = self.add()
+        self.pages[new], self.lengths[new] = list(pages), length
+        for p in pages:
+            self.users[p] += 1
+        return new
+
     def release(self, seq):
-        self.free += reversed(self.pages.pop(seq))
+        self._give_back(self.pages.pop(seq))
         del self.lengths[seq]
+
+    def truncate(self, seq, length):
+        """Keep the first ``length`` tokens of a sequence; the pages of the others go back (drafts that were not taken)."""
+        if not 0 <= length <= self.lengths[seq]:
+            raise ValueError(f"the sequence has {self.lengths[seq]} tokens; {length} cannot be kept")
+        self.batch = None
+        keep = -(-length // self.page_size)
+        self._give_back(self.pages[seq][keep:])
+        del self.pages[seq][keep:]
+        self.lengths[seq] = length
+
+    def compact(self):
+        """Move the pages in use to ids 0 .. n - 1, as few of them as that takes, in one launch; returns n."""
+        n = sum(1 for u in self.users if u)
+        to = iter([p for p in range(n) if not self.users[p]])
+        moves = {p: next(to) for p in range(n, len(self.users)) if self.users[p]}
+        self.batch = None
+        if moves:
+            self._copy(*_ints([list(moves), list(moves.values())], self.device))
+        for pages in self.pages.values():
+            pages[:] = [moves.get(p, p) for p in pages]
+        for old, new in moves.items():
+            self.users[new], self.users[old] = self.users[old], 0
+        self.free = list(range(len(self.users) - 1, n - 1, -1))
+        return n
+
+    def resize(self, pages):
+        """Pools of ``pages`` pages, the ones in use compacted into them; memory is taken and given back a pool at a time.
+        Where it runs out on the way, more pages than before are not had, fewer are."""
+        n = sum(1 for u in self.users if u)
+        if pages < max(n, 1):
+            raise ValueError(f"{n} pages are in use: {pages} do not hold them")
+        self.compact()
+        size = min(pages, len(self.users))
+
+        def moved(x):
+            y = x.new_empty(pages, *x.shape[1:])
+            y[:n].copy_(x[:n])
+            return y
+        try:
+            for kept in (self.pools, self.scales):
+                for i, (k, v) in enumerate(kept):
+                    if k is not None:
+                        kept[i] = (moved(k), v)
+                        del k
+                        kept[i] = (kept[i][0], moved(v))
+                    del v
+            size = pages
+        finally:
+            for kept in (self.pools, self.scales):   # all of one size, also where memory ran out on the way
+                kept[:] = [tuple(x if x is None else x[:size] for x in pair) for pair in kept]
+            self.users = self.users[:n] + [0] * (size - n)
+            self.free = list(range(size - 1, n - 1, -1))
+
+    def _give_back(self, pages):
+        for p in reversed(pages):
+            self.users[p] -= 1
+            if not self.users[p]:
+                self.free.append(p)
+
+    def _take(self):
+        p = self.free.pop()
+        self.users[p] = 1
+        return p
+
+    def _copy(self, src, dst):
+        copy_pages([x for both in (self.pools, self.scales) for pair in both for x in pair if x is not None], src, dst)
 
     def begin(self, seqs, counts):
         """The next calls' tokens are ``counts[i]`` new ones of sequence ``seqs[i]``, in this order. Pages are taken
@@ -183,30 +310,43 @@ class PagedKVCache:
         if max(lens, default=0) > self.max_len:
             raise ValueError(f"a sequence of {max(lens)} tokens: this cache's are at most {self.max_len}")
         need = [-(-n // P) - len(self.pages[s]) for s, n in zip(seqs, lens)]
-        if sum(need) > len(self.free):
-            raise MemoryError(f"{sum(need)} pages are needed, {len(self.free)} are free")
+        # partly filled pages that other sequences are on too: all but the last of these write on in a copy
+        own, left = [], {}
+        for s, c in zip(seqs, counts):
+            if c and self.lengths[s] % P:
+                p = self.pages[s][-1]
+                left[p] = left.get(p, self.users[p]) - 1
+                if left[p]:
+                    own.append(s)
+        if sum(need) + len(own) > len(self.free):
+            raise MemoryError(f"{sum(need) + len(own)} pages are needed, {len(self.free)} are free")
+        moves = []
+        for s in own:
+            old, new = self.pages[s][-1], self._take()
+            self.pages[s][-1] = new
+            self.users[old] -= 1
+            moves.append((s, old, new))
         for s, n, k in zip(seqs, lens, need):
-            self.pages[s] += [self.free.pop() for _ in range(k)]
+            self.pages[s] += [self._take() for _ in range(k)]
             self.lengths[s] = n
-        self.batch = dict(seqs=list(seqs), counts=list(counts))
+        self.batch = dict(seqs=list(seqs), counts=list(counts), moves=moves)
         try:
-            self.batch.update(self._tables(lens, counts, seqs))
+            self.batch.update(self._tables(lens, counts, seqs, moves))
+            if moves:
+                self._copy(self.batch["src"], self.batch["dst"])
         except BaseException:
             self.cancel()
             raise
 
-    def _tables(self, lens, counts, seqs):
+    def _tables(self, lens, counts, seqs, moves):
         B, cols = len(seqs), max([len(self.pages[s]) for s in seqs] + [1])
         starts = [0]
         for c in counts:
             starts.append(starts[-1] + c)
-        flat = lens + starts + [p for s in seqs for p in self.pages[s] + [-1] * (cols - len(self.pages[s]))]
-        host = torch.tensor(flat, dtype=torch.int32)
-        if self.device.type == "cuda":
-            host = host.pin_memory()
-        t = host.to(self.device, non_blocking=True)
+        lens_t, starts_t, src, dst, table = _ints([lens, starts, [m[1] for m in moves], [m[2] for m in moves], [
+            p for s in seqs for p in self.pages[s] + [-1] * (cols - len(self.pages[s]))]], self.device)
         one = all(c == 1 for c in counts)
-        return dict(lens=t[:B], starts=None if one else t[B:2 * B + 1], table=t[2 * B + 1:].view(B, cols),
+        return dict(lens=lens_t, starts=None if one else starts_t, table=table.view(B, cols), src=src, dst=dst,
                     max_new=max(counts, default=0), max_len=max(lens, default=0))
 
     def cancel(self):
@@ -217,8 +357,13 @@ class PagedKVCache:
             if s in self.pages:
                 self.lengths[s] -= c
                 keep = -(-self.lengths[s] // self.page_size)
-                self.free += reversed(self.pages[s][keep:])
+                self._give_back(self.pages[s][keep:])
                 del self.pages[s][keep:]
+        for s, old, new in reversed(self.batch["moves"]):
+            if s in self.pages and self.users[old]:   # else its copy is the only one by now
+                self.pages[s][-1] = old
+                self.users[old] += 1
+                self._give_back([new])
         self.batch = None
 
     def _batch(self, tokens):

@@ -11,7 +11,7 @@ namespace {
 
 // Which kernel, the splits of the keys and the workspace they and a widened 8-bit cache take: a function
 // of shapes and bounds alone. Points into `ws` where it is given; returns its bytes.
-int64_t plan(AttnArgs& a, bool i8, int64_t max_new, int64_t max_len, bool& chunked, char* ws) {
+int64_t plan(AttnArgs& a, int bits, int64_t max_new, int64_t max_len, bool& chunked, char* ws) {
   // Rows that share a key: the decode kernel holds 16 and would read the keys again for more; from there
   // on the tensor-core kernel takes over (16 sequences of 4000 tokens, 32/8 heads of 128: 16 rows 60 us
   // here, 20 to 40 rows 63 us there; 32 rows here took 100). Over an 8-bit cache, which it has to widen
@@ -20,8 +20,9 @@ int64_t plan(AttnArgs& a, bool i8, int64_t max_new, int64_t max_len, bool& chunk
   // kernel reads the 8 bits again after all.
   // A bound of 0 leaves it one tile: a launch of no blocks is an error.
   const int64_t wide_len = max_len ? (max_len + 127) & ~int64_t(127) : 128, wide_rows = a.kv.seqs * (int64_t)a.kv.heads * wide_len;
-  chunked = max_new * a.G > (i8 ? 48 : 16) && (!i8 || wide_rows * a.D <= int64_t(1) << 30);
+  chunked = max_new * a.G > (bits < 16 ? 48 : 16) && (bits == 16 || wide_rows * a.D <= int64_t(1) << 30);
   if (chunked) plan_attn_chunk(a, max_new, max_len);
+  else if (bits == 4) plan_attn_decode4(a, max_new, max_len);
   else plan_attn_decode(a, max_new, max_len);
   a.keys_end = 0x7fffffff;
   int64_t at = 0;
@@ -34,7 +35,7 @@ int64_t plan(AttnArgs& a, bool i8, int64_t max_new, int64_t max_len, bool& chunk
     a.part_o = reinterpret_cast<float*>(take((int64_t)a.T * a.hq * a.splits * a.D * 4));
     a.part_ml = reinterpret_cast<float2*>(take((int64_t)a.T * a.hq * a.splits * 8));
   }
-  if (chunked && i8) {
+  if (chunked && bits < 16) {
     a.wide_len = a.keys_end = (int)wide_len;
     a.wide_k = take(wide_rows * a.D * 2);
     a.wide_v = take(wide_rows * a.D * 2);
@@ -50,6 +51,8 @@ __global__ void __launch_bounds__(256) attn_blank_kernel(const AttnArgs a) {
   pdl_trigger();
   blank_tokens(a, 0, a.T, blockIdx.x, gridDim.x);
 }
+
+int bits_of(int kv_dtype) { return kv_dtype == VQ2_I4 ? 4 : kv_dtype == VQ2_I8 ? 8 : 16; }
 
 bool bad_attn(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t seqs, int64_t max_new, int64_t max_len,
               int64_t window) {
@@ -76,7 +79,7 @@ extern "C" int64_t vq2_paged_attention_workspace(int64_t tokens, int64_t q_heads
   a.G = a.hq / a.kv.heads;
   a.window = (int)window;
   bool chunked;
-  return tokens && seqs ? plan(a, kv_dtype == VQ2_I8, max_new, max_len, chunked, nullptr) : 0;
+  return tokens && seqs ? plan(a, bits_of(kv_dtype), max_new, max_len, chunked, nullptr) : 0;
 }
 
 extern "C" int vq2_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype,
@@ -92,7 +95,8 @@ extern "C" int vq2_paged_attention(const void* q, int64_t q_token_stride, int64_
                    table_stride, table_cols, lens, starts, seqs);
   if (s != VQ2_OK) return s;
   if (!q || !out || (!lens && seqs > 0)) return VQ2_ERR_ARG;
-  if ((dtype != VQ2_F16 && dtype != VQ2_BF16) || (kv_dtype != dtype && kv_dtype != VQ2_I8)) return VQ2_ERR_DTYPE;
+  if ((dtype != VQ2_F16 && dtype != VQ2_BF16) || (kv_dtype != dtype && kv_dtype != VQ2_I8 && kv_dtype != VQ2_I4))
+    return VQ2_ERR_DTYPE;
   if (bad_attn(tokens, q_heads, kv_heads, seqs, max_new, max_len, window) || (!starts && tokens != seqs)) return VQ2_ERR_SHAPE;
   if (!aligned(q, 16) || q_token_stride % 8 || q_head_stride % 8 || !aligned(out, 16) || !aligned(workspace, 16))
     return VQ2_ERR_ALIGN;
@@ -113,11 +117,11 @@ extern "C" int vq2_paged_attention(const void* q, int64_t q_token_stride, int64_
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (seqs == 0) return launch_kernel(attn_blank_kernel, dim3(2 * sm_count()), dim3(256), 0, st, a);
   bool chunked;
-  const bool i8 = kv_dtype == VQ2_I8;
-  const int64_t bytes = plan(a, i8, starts ? max_new : 1, max_len, chunked, static_cast<char*>(workspace));
+  const int bits = bits_of(kv_dtype);
+  const int64_t bytes = plan(a, bits, starts ? max_new : 1, max_len, chunked, static_cast<char*>(workspace));
   if (bytes && (!workspace || workspace_bytes < bytes)) return VQ2_ERR_ARG;
   if ((int64_t)a.kv.seqs * a.row_blocks > 0x3fffffff) return VQ2_ERR_SHAPE;
-  s = chunked ? launch_attn_chunk(a, i8, st) : launch_attn_decode(a, i8, st);
+  s = chunked ? launch_attn_chunk(a, bits, st) : bits == 4 ? launch_attn_decode4(a, st) : launch_attn_decode(a, bits == 8, st);
   if (s != VQ2_OK || a.splits == 1) return s;
   return launch_attn_join(a, st);
 }

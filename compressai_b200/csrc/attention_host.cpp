@@ -15,6 +15,7 @@
 #include <sstream>
 #include <stdexcept>
 #include <string>
+#include <vector>
 
 #include "vq2_b200.h"
 
@@ -25,6 +26,7 @@ decltype(&vq2_cache_write) f_write;
 decltype(&vq2_cache_read) f_read;
 decltype(&vq2_paged_attention) f_attention;
 decltype(&vq2_paged_attention_workspace) f_workspace;
+decltype(&vq2_copy_pages) f_copy;
 PyObject *check_status, *out_of_memory;   // _lib.check(status, name); torch.OutOfMemoryError
 
 struct Refused : std::runtime_error {
@@ -62,7 +64,7 @@ int truth(PyObject* o) {
 }
 
 int code(at::ScalarType t) {
-  return t == at::kHalf ? VQ2_F16 : t == at::kBFloat16 ? VQ2_BF16 : t == at::kChar ? VQ2_I8 : -1;
+  return t == at::kHalf ? VQ2_F16 : t == at::kBFloat16 ? VQ2_BF16 : t == at::kChar ? VQ2_I8 : t == at::kByte ? VQ2_I4 : -1;
 }
 
 void on_cuda(const at::Tensor& t) {
@@ -92,7 +94,7 @@ const int32_t* ints(const at::Tensor& x, const char* name, int64_t n, c10::Devic
 
 struct Pools {
   void *k, *v;
-  float *ks = nullptr, *vs = nullptr;
+  float *ks = nullptr, *vs = nullptr;   // 4 bits: the address of bytes
   int kind;
   int64_t pages, heads, page, d, stride, cols, seqs;
   const int32_t* table;
@@ -105,14 +107,14 @@ Pools pools(PyObject* const* a, int dtype, int64_t heads, int64_t d, c10::Device
   Pools p;
   p.kind = code(k.scalar_type());
   if (p.kind < 0 || v.scalar_type() != k.scalar_type())
-    refuse("pools hold fp16, bf16 or int8, both the same; got ", k.scalar_type(), " and ", v.scalar_type());
+    refuse("pools hold fp16, bf16, int8 or (uint8) two 4-bit values a byte, both the same; got ", k.scalar_type(), " and ", v.scalar_type());
   if (k.dim() != 4 || k.sizes() != v.sizes() || !k.is_contiguous() || !v.is_contiguous())
     refuse("pools must be contiguous [pages, kv_heads, page_size, head_size], k and v alike; got ", k.sizes(), " and ", v.sizes());
   if (k.device() != dev || v.device() != dev) refuse("pools on ", k.device(), " and ", v.device(), ", tokens on ", dev);
   p.pages = k.size(0);
   p.heads = k.size(1);
   p.page = k.size(2);
-  p.d = k.size(3);
+  p.d = k.size(3) * (p.kind == VQ2_I4 ? 2 : 1);
   if (p.kind == VQ2_I8) {
     for (const at::Tensor* s : {ks, vs})
       if (!s || s->scalar_type() != at::kFloat || s->dim() != 3 || s->size(0) != p.pages || s->size(1) != p.heads ||
@@ -120,8 +122,16 @@ Pools pools(PyObject* const* a, int dtype, int64_t heads, int64_t d, c10::Device
         refuse("int8 pools need contiguous fp32 k_scale and v_scale [pages, kv_heads, page_size]");
     p.ks = static_cast<float*>(ks->data_ptr());
     p.vs = static_cast<float*>(vs->data_ptr());
+  } else if (p.kind == VQ2_I4) {
+    if (p.d % 32 || p.page % 16) refuse("4-bit pools have heads of a multiple of 32 values and pages of one of 16 rows; got ", k.sizes());
+    for (const at::Tensor* s : {ks, vs})
+      if (!s || s->scalar_type() != at::kByte || s->dim() != 5 || s->size(0) != p.pages || s->size(1) != p.heads ||
+          s->size(2) != p.page / 16 || s->size(3) != 4 + (p.d + 63) / 64 || s->size(4) != 16 || !s->is_contiguous() || s->device() != dev)
+        refuse("4-bit pools need contiguous uint8 k_scale and v_scale [pages, kv_heads, page_size / 16, 4 + ceil(head_size / 64), 16]");
+    p.ks = static_cast<float*>(ks->data_ptr());
+    p.vs = static_cast<float*>(vs->data_ptr());
   } else if (ks || vs) {
-    refuse("scales go with int8 pools only");
+    refuse("scales go with int8 and 4-bit pools only");
   } else if (dtype >= 0 && p.kind != dtype) {
     refuse("pools hold ", k.scalar_type(), ", which is not the tokens' type");
   }
@@ -240,7 +250,7 @@ PyObject* cache_read(PyObject* const* a) {
   const at::Tensor& k_pages = tensor(a[0], "k_pages");
   on_cuda(k_pages);
   const auto dev = k_pages.device();
-  at::ScalarType t = k_pages.scalar_type() == at::kChar ? at::kBFloat16 : k_pages.scalar_type();
+  at::ScalarType t = k_pages.scalar_type() == at::kChar || k_pages.scalar_type() == at::kByte ? at::kBFloat16 : k_pages.scalar_type();
   if (a[7] != Py_None) {
     if (!THPDtype_Check(a[7])) refuse("dtype must be a torch dtype");
     t = reinterpret_cast<THPDtype*>(a[7])->scalar_type;
@@ -302,6 +312,33 @@ PyObject* paged_attention(PyObject* const* a) {
   return pair(THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(lse)));
 }
 
+// pools, src, dst -> None
+PyObject* copy_pages(PyObject* const* a) {
+  if (!PyList_Check(a[0]) && !PyTuple_Check(a[0])) refuse("pools must be a list or tuple of tensors");
+  const Py_ssize_t n_pools = PySequence_Fast_GET_SIZE(a[0]);
+  const at::Tensor &src = tensor(a[1], "src"), &dst = tensor(a[2], "dst");
+  on_cuda(src);
+  const auto dev = src.device();
+  if (src.dim() != 1) refuse("src must be a vector of page ids; got ", src.sizes());
+  const int64_t n = src.size(0);
+  const int32_t *sp = ints(src, "src", n, dev), *dp = ints(dst, "dst", n, dev);
+  std::vector<vq2_page_pool> pools(n_pools);
+  int64_t pages = 0;
+  for (Py_ssize_t i = 0; i < n_pools; ++i) {
+    const at::Tensor& x = tensor(PySequence_Fast_GET_ITEM(a[0], i), "a pool");
+    if (x.device() != dev || x.dim() < 1 || !x.is_contiguous() || (i && x.size(0) != pages))
+      refuse("pools must be contiguous [pages, ..], of the same number of pages, on ", dev, "; got ", x.sizes(), " on ", x.device());
+    pages = x.size(0);
+    const int64_t bytes = pages ? static_cast<int64_t>(x.nbytes()) / pages : 0;
+    if (bytes % 16 || reinterpret_cast<uintptr_t>(x.const_data_ptr()) % 16)
+      refuse("a page must be a multiple of 16 bytes and start on one; got ", bytes, " bytes");
+    pools[i] = {x.data_ptr(), bytes};
+  }
+  const c10::cuda::CUDAGuard guard(dev);
+  if (n && pages) check(f_copy(pools.data(), n_pools, pages, sp, dp, n, current_stream(dev)), "vq2_copy_pages");
+  return none();
+}
+
 // No C++ exception leaves an entry of the module.
 template <PyObject* (*F)(PyObject* const*), Py_ssize_t N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -336,7 +373,8 @@ PyObject* bind(PyObject*, PyObject* args) {
   f_read = reinterpret_cast<decltype(f_read)>(of("vq2_cache_read"));
   f_attention = reinterpret_cast<decltype(f_attention)>(of("vq2_paged_attention"));
   f_workspace = reinterpret_cast<decltype(f_workspace)>(of("vq2_paged_attention_workspace"));
-  if (!f_rotary || !f_write || !f_read || !f_attention || !f_workspace) {
+  f_copy = reinterpret_cast<decltype(f_copy)>(of("vq2_copy_pages"));
+  if (!f_rotary || !f_write || !f_read || !f_attention || !f_workspace || !f_copy) {
     PyErr_SetString(PyExc_ValueError, "an entry point's address is missing");
     return nullptr;
   }
@@ -349,6 +387,7 @@ PyObject* bind(PyObject*, PyObject* args) {
 
 #define ENTRY(name, n) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(entry<name, n>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {ENTRY(rotary, 7), ENTRY(cache_write, 13), ENTRY(cache_read, 8), ENTRY(paged_attention, 14),
+                         ENTRY(copy_pages, 3),
                          {"bind", bind, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_attention_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

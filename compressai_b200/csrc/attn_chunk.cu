@@ -945,6 +945,7 @@ constexpr int kWidenKeys = 64;
 // [seqs, heads, wide_len] beside them; zeros past a sequence's end (to the next 128 keys) and where a
 // page does not exist. 64 keys a block; bound by memory (a key of 256 values: 516 bytes read, 1032
 // written).
+template <int BITS>
 __global__ void __launch_bounds__(256) widen_kernel(const AttnArgs a) {
   pdl_wait();
   pdl_trigger();
@@ -970,8 +971,14 @@ __global__ void __launch_bounds__(256) widen_kernel(const AttnArgs a) {
     }
     row_s[threadIdx.x] = row;
     const int64_t at = (int64_t)bh * a.wide_len + k;
-    a.wide_ks[at] = row < 0 ? 0.f : a.kv.k_scale[row];
-    a.wide_vs[at] = row < 0 ? 0.f : a.kv.v_scale[row];
+    if (BITS == 8) {
+      a.wide_ks[at] = row < 0 ? 0.f : a.kv.k_scale[row];
+      a.wide_vs[at] = row < 0 ? 0.f : a.kv.v_scale[row];
+    } else {
+      const Scale4 places(a.D);
+      a.wide_ks[at] = row < 0 ? 0.f : *reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(a.kv.k_scale) + places.row(row));
+      a.wide_vs[at] = row < 0 ? 0.f : *reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(a.kv.v_scale) + places.row(row));
+    }
   }
   __syncthreads();
   // 256 / pieces keys a round; the loads of two rounds, K's and V's, go out together
@@ -985,15 +992,31 @@ __global__ void __launch_bounds__(256) widen_kernel(const AttnArgs a) {
       const int key = k + (i >> 1) * per_round, row = key < kWidenKeys ? row_s[key] : -1;
       const char* src = static_cast<const char*>(i & 1 ? a.kv.v : a.kv.k);
       x[i] = make_uint4(0, 0, 0, 0);
-      if (row >= 0) x[i] = *reinterpret_cast<const uint4*>(src + (int64_t)row * a.D + 16 * p);
+      if (row < 0) continue;
+      if (BITS == 8) {
+        x[i] = *reinterpret_cast<const uint4*>(src + (int64_t)row * a.D + 16 * p);
+      } else {   // 16 codes, their factor
+        const uint2 c = *reinterpret_cast<const uint2*>(src + (int64_t)row * (a.D >> 1) + 8 * p);
+        const uint8_t* scales = reinterpret_cast<const uint8_t*>(i & 1 ? a.kv.v_scale : a.kv.k_scale);
+        x[i] = make_uint4(c.x, c.y, scales[Scale4(a.D).factor(row, p >> 2)], 0);
+      }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int key = k + (i >> 1) * per_round;
       if (key >= kWidenKeys) continue;
       uint4 y[2];
+      if (BITS == 4) {   // code * factor: 7 bits at most, exact
+        const __half2 u = __float2half2_rn(e4m3_value(x[i].z)), bias = __float2half2_rn(1032.f);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t w = (&x[i].x)[j >> 2] >> (8 * (j & 3)), c = 0x64006400u | (w & 15u) | (w & 0xf0u) << 12;   // 1024 + code + 8
+          const __half2 v = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&c), bias), u);
+          (&y[j >> 2].x)[j & 3] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+      }
+#pragma unroll
+      for (int j = 0; BITS == 8 && j < 4; ++j) {
         const uint32_t u = (&x[i].x)[j] ^ 0x80808080u;   // offset binary
         (&y[j >> 1].x)[2 * (j & 1)] = bytes_f16(u, 0x4140);
         (&y[j >> 1].x)[2 * (j & 1) + 1] = bytes_f16(u, 0x4342);
@@ -1069,10 +1092,10 @@ void plan_attn_chunk(AttnArgs& a, int64_t max_new, int64_t max_len) {
   if (a.splits < 1) a.splits = 1;
 }
 
-int launch_attn_chunk(const AttnArgs& a, bool i8, cudaStream_t st) {
-  if (i8) {
+int launch_attn_chunk(const AttnArgs& a, int bits, cudaStream_t st) {
+  if (bits < 16) {
     const int64_t blocks = (int64_t)a.kv.seqs * a.kv.heads * (a.wide_len / kWidenKeys);
-    const int s = launch_kernel(widen_kernel, dim3((unsigned)blocks), dim3(256), 0, st, a);
+    const int s = launch_kernel(bits == 8 ? widen_kernel<8> : widen_kernel<4>, dim3((unsigned)blocks), dim3(256), 0, st, a);
     if (s != VQ2_OK) return s;
     return a.q_bf16 ? launch_shape<__nv_bfloat16, true>(a, st) : launch_shape<__half, true>(a, st);
   }

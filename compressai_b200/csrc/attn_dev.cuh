@@ -22,7 +22,7 @@ struct AttnArgs {
   int chunk, splits, rows_per_block, row_blocks, lo_mask;
   float* part_o;        // [T * hq, splits, D]: weighted sums of V relative to the maximum
   float2* part_ml;      // [T * hq, splits]: (maximum score in powers of two, sum of weights)
-  // 8-bit cache, many rows: the visible keys and values as fp16 [seqs, heads, wide_len, D], their scales
+  // 8-bit and 4-bit caches, many rows: the visible keys and values as fp16 [seqs, heads, wide_len, D], their scales
   void *wide_k, *wide_v;
   float *wide_ks, *wide_vs;
   int wide_len;
@@ -132,7 +132,10 @@ int launch_attn_join(const AttnArgs& a, cudaStream_t st);
 // chunk, splits, rows_per_block, row_blocks and lo_mask.
 int launch_attn_decode(const AttnArgs& a, bool i8, cudaStream_t st);
 void plan_attn_decode(AttnArgs& a, int64_t max_new, int64_t max_len);
-int launch_attn_chunk(const AttnArgs& a, bool i8, cudaStream_t st);
+// Few rows over a 4-bit cache (attn_decode4.cu).
+int launch_attn_decode4(const AttnArgs& a, cudaStream_t st);
+void plan_attn_decode4(AttnArgs& a, int64_t max_new, int64_t max_len);
+int launch_attn_chunk(const AttnArgs& a, int bits, cudaStream_t st);
 void plan_attn_chunk(AttnArgs& a, int64_t max_new, int64_t max_len);
 int attn_chunk_status(int reset);   // its part of vq2_attention_status
 

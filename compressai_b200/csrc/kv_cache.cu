@@ -1,4 +1,4 @@
-// Rotary positions, and the paged key/value cache: written (rotary of q and k fused, 8-bit
+// Rotary positions, and the paged key/value cache: written (rotary of q and k fused, 8-bit or 4-bit
 // quantisation optional) and read back.
 //
 // Pools are [pages, kv_heads, page_size, head] so that a (page, head) pair is one contiguous piece
@@ -204,8 +204,99 @@ __device__ __forceinline__ uint2 quantise8(const float (&f)[8], bool mine, int l
   return make_uint2(o[0], o[1]);
 }
 
+// A 4-bit group's factor (e4m3, as a byte and as a number): its largest magnitude over the row's, rounded up so that
+// no value passes 7 steps. 2^-9 at least unless the group is 0.
+__device__ __forceinline__ uint32_t factor_of(float group, float row, float& u) {
+  const float r = __fdiv_rn(group, row);
+  const uint32_t b = r >= 0.015625f ? ((__float_as_uint(r) + 0xfffffu) >> 20) - 960u : (uint32_t)ceilf(r * 512.f);
+  u = e4m3_value(b);
+  return b;
+}
+
+// What turns a value of such a group into its code, -7..7. The nearest integer to 7 x / (row * u), a tie away from
+// zero: a share of 2^-20 more lifts every tie, and no quotient of 16-bit values (a tie is 2^-16 away if it is not
+// met) over it, so that one multiplication rounds as an exact division would.
+__device__ __forceinline__ float steps_per_one(float row, float u) {
+  return u == 0.f ? 0.f : __fdiv_rn(7.f + 7.f / 1048576.f, __fmul_rn(row, u));
+}
+
+// Four codes, plus 8, in the low half of the result.
+__device__ __forceinline__ uint32_t codes4(const float* f, float per) {
+  uint32_t r = 0;   // adding 1.5 * 2^23 + 8 rounds to an integer and leaves it in the low bits
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r |= (__float_as_uint(__fadd_rn(__fmul_rn(f[j], per), 12582920.f)) & 15u) << (4 * j);
+  return r;
+}
+
+struct Row4 {
+  uint32_t codes;   // of the lane's 8 values
+  float scale;      // of the row
+};
+
+// 8 values of a row held by 2^lanes_log2 lanes as 4-bit codes, with the row's scale; `put(group, byte)` stores a factor
+// (by the lanes that have a group to store). The first four values are row elements e0 .., the other four e1 ..;
+// SPLIT: not one after the other, and of two groups perhaps. Warp-wide; a lane that is not `mine` adds nothing.
+template <bool SPLIT, typename Put>
+__device__ __forceinline__ Row4 quantise4(const float (&f)[8], bool mine, int lanes_log2, int lane, int e0, int e1, int groups,
+                                          Put put) {
+  float m0 = 0.f, m1 = 0.f;   // a NaN passes through
+  if (mine) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      m0 = max_nan(m0, fabsf(f[j]));
+      m1 = max_nan(m1, fabsf(f[4 + j]));
+    }
+  }
+  const int lanes = 1 << lanes_log2, g0 = e0 >> 6, g1 = e1 >> 6;
+  float of0, of1, row;   // the largest magnitude of the fours' groups, of the row
+  float of[4];           // SPLIT: of every group
+  if (SPLIT) {
+    of0 = of1 = row = 0.f;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      of[g] = 0.f;
+      if (g >= groups) continue;
+      float m = max_nan(g0 == g ? m0 : 0.f, g1 == g ? m1 : 0.f);
+      for (int o = 1; o < lanes; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+      of[g] = m;
+      row = max_nan(row, m);
+      if (g0 == g) of0 = m;
+      if (g1 == g) of1 = m;
+    }
+  } else {
+    of0 = max_nan(m0, m1);
+    for (int o = 1; o < lanes && o < 8; o <<= 1) of0 = max_nan(of0, __shfl_xor_sync(0xffffffffu, of0, o));
+    of1 = row = of0;
+    for (int o = 8; o < lanes; o <<= 1) row = max_nan(row, __shfl_xor_sync(0xffffffffu, row, o));
+  }
+  Row4 r = {0x88888888u, 0.f};   // zeros
+  const bool bad = !(row < INFINITY), some = !bad && row >= 1e-30f;
+  if (bad) r.scale = __uint_as_float(0x7fc00000u);
+  if (some) {
+    r.scale = __fdiv_rn(row, 7.f);
+    float u0, u1;
+    const uint32_t b0 = factor_of(of0, row, u0);
+    if (SPLIT) {
+      factor_of(of1, row, u1);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float u;
+        if (g < groups && lane == g) put(g, factor_of(of[g], row, u));
+      }
+      r.codes = codes4(f, steps_per_one(row, u0)) | codes4(f + 4, steps_per_one(row, u1)) << 16;
+    } else {
+      if (!(lane & 7)) put(g0, b0);
+      const float per = steps_per_one(row, u0);
+      r.codes = codes4(f, per) | codes4(f + 4, per) << 16;
+    }
+  } else if (SPLIT ? lane < groups : !(lane & 7)) {
+    put(SPLIT ? lane : g0, bad ? 0x38u : 0u);   // a finite factor beside a scale of NaN
+  }
+  return r;
+}
+
 // MODE 0: rotary of q and k into contiguous outputs. MODE 1: rotary of q, k (rotated) and v into a
-// 16-bit cache. MODE 2: the same into an 8-bit cache. For few tokens: a row per lane group, its kind by its
+// 16-bit cache. MODE 2: the same into an 8-bit cache, MODE 3: into a 4-bit one. For few tokens: a row per lane group, its kind by its
 // number.
 template <typename T, int MODE, Hold HOLD>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
@@ -242,7 +333,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
     if (HOLD == Hold::kPartners) widen8<T>(w, p);
     turn.apply(f, p);
   }
-  if (MODE != 2 || kind == 0) {
+  if (MODE < 2 || kind == 0) {
     if (mine && (MODE != 1 || kind == 0 || slot >= 0)) {
       T* dst;
       if (kind == 0) dst = static_cast<T*>(a.q_out) + ((int64_t)t * rows_q + h) * a.D;
@@ -259,6 +350,19 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
     int8_t* dst = static_cast<int8_t*>(const_cast<void*>(kind == 1 ? a.kv.k : a.kv.v)) + row * a.D;
     *reinterpret_cast<uint2*>(dst + i0) = o;
     if (lane == 0) const_cast<float*>(kind == 1 ? a.kv.k_scale : a.kv.v_scale)[row] = scale;
+  }
+  if (MODE == 3) {
+    const bool stored = kind > 0 && mine && slot >= 0;
+    const Scale4 places(a.D);
+    const int64_t row = stored ? pool_row(a.kv, slot, h) : 0;
+    uint8_t* scales = reinterpret_cast<uint8_t*>(const_cast<float*>(kind == 1 ? a.kv.k_scale : a.kv.v_scale));
+    const Row4 o = quantise4<false>(f, mine, a.lanes_log2, lane, i0, i0 + 4, places.groups, [&](int group, uint32_t b) {
+      if (stored) scales[places.factor(row, group)] = (uint8_t)b;
+    });
+    if (!stored) return;
+    uint8_t* dst = static_cast<uint8_t*>(const_cast<void*>(kind == 1 ? a.kv.k : a.kv.v)) + row * (a.D >> 1);
+    *reinterpret_cast<uint32_t*>(dst + (i0 >> 1)) = o.codes;
+    if (lane == 0) *reinterpret_cast<float*>(scales + places.row(row)) = o.scale;
   }
 }
 
@@ -316,7 +420,7 @@ __global__ void __launch_bounds__(kRopeThreads, 6) rope_wide_kernel(const RopeAr
         const int h = h0 + n * groups;
         const bool mine = h < in.heads && in_row;
         float f[8];
-        if (turned || (kPool && MODE == 2)) widen8<T>(x[n], f);
+        if (turned || (kPool && MODE >= 2)) widen8<T>(x[n], f);
         if (turned) turn.apply(f, f);
         const int64_t row = kPool ? pool0 + ((int64_t)h << a.kv.page_log2) : h;
         if (!kPool || MODE == 1) {
@@ -329,6 +433,23 @@ __global__ void __launch_bounds__(kRopeThreads, 6) rope_wide_kernel(const RopeAr
             } else {
               *reinterpret_cast<uint4*>(dst + row * a.D + i0) = turned ? narrow8<T>(f) : x[n];
             }
+          }
+        } else if constexpr (MODE == 3) {
+          const bool stored = mine && slot >= 0;
+          const Scale4 places(a.D);
+          uint8_t* scales = reinterpret_cast<uint8_t*>(const_cast<float*>(KIND == 1 ? a.kv.k_scale : a.kv.v_scale));
+          const Row4 o = quantise4<SPLIT>(f, mine, a.lanes_log2, lane, i0, i0 + apart, places.groups, [&](int group, uint32_t b) {
+            if (stored) scales[places.factor(row, group)] = (uint8_t)b;
+          });
+          if (stored) {
+            uint8_t* to = reinterpret_cast<uint8_t*>(dst) + row * (a.D >> 1) + (i0 >> 1);
+            if constexpr (SPLIT) {
+              *reinterpret_cast<uint16_t*>(to) = (uint16_t)o.codes;
+              *reinterpret_cast<uint16_t*>(to + (apart >> 1)) = (uint16_t)(o.codes >> 16);
+            } else {
+              *reinterpret_cast<uint32_t*>(to) = o.codes;
+            }
+            if (lane == 0) *reinterpret_cast<float*>(scales + places.row(row)) = o.scale;
           }
         } else {
           float scale;
@@ -361,7 +482,7 @@ struct ReadArgs {
 };
 
 // Row (token, head) per lane group, K and V together; NIT rows per group, their loads in flight at once.
-template <typename T, bool I8, int NIT>
+template <typename T, int BITS, int NIT>
 __global__ void __launch_bounds__(kRopeThreads) cache_read_kernel(const ReadArgs a) {
   pdl_wait();
   pdl_trigger();
@@ -385,7 +506,16 @@ __global__ void __launch_bounds__(kRopeThreads) cache_read_kernel(const ReadArgs
     const int64_t slot = slot_of(a.kv, b, t - a.kv.starts[b]);
     if (slot < 0) continue;
     const int64_t row = pool_row(a.kv, slot, h), e = row * a.D + i0;
-    if (I8) {
+    if (BITS == 4) {
+      const Scale4 places(a.D);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const uint8_t* scales = reinterpret_cast<const uint8_t*>(c ? a.kv.v_scale : a.kv.k_scale);
+        x[n][c].x = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(c ? a.kv.v : a.kv.k) + (e >> 1));
+        x[n][c].y = scales[places.factor(row, i0 >> 6)];
+        s[n][c] = *reinterpret_cast<const float*>(scales + places.row(row));
+      }
+    } else if (BITS == 8) {
       const uint2 k = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(a.kv.k) + e);
       const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(a.kv.v) + e);
       x[n][0] = make_uint4(k.x, k.y, 0, 0);
@@ -404,7 +534,13 @@ __global__ void __launch_bounds__(kRopeThreads) cache_read_kernel(const ReadArgs
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       uint4 y = x[n][c];
-      if (I8) {
+      if (BITS == 4) {
+        const float step = e4m3_value(x[n][c].y) * s[n][c];
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = (float)((int)(x[n][c].x >> (4 * j) & 15) - 8) * step;
+        y = narrow8<T>(f);
+      } else if (BITS == 8) {
         float f[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = (float)(int8_t)((&x[n][c].x)[j >> 2] >> (8 * (j & 3))) * s[n][c];
@@ -499,7 +635,8 @@ extern "C" int vq2_cache_write(const void* q, int64_t q_token_stride, int64_t q_
                    table_stride, table_cols, lens, starts, seqs);
   if (s != VQ2_OK) return s;
   if (!k || !v || (!lens && seqs > 0) || (q_heads && (!q || !q_out))) return VQ2_ERR_ARG;
-  if ((dtype != VQ2_F16 && dtype != VQ2_BF16) || (kv_dtype != dtype && kv_dtype != VQ2_I8)) return VQ2_ERR_DTYPE;
+  if ((dtype != VQ2_F16 && dtype != VQ2_BF16) || (kv_dtype != dtype && kv_dtype != VQ2_I8 && kv_dtype != VQ2_I4))
+    return VQ2_ERR_DTYPE;
   if (tokens < 0 || tokens > 0x7fffffff || q_heads < 0 || q_heads > 4096 || bad_rotary(inv_freq, rot, head_size) ||
       (!starts && tokens != seqs))
     return VQ2_ERR_SHAPE;
@@ -517,6 +654,8 @@ extern "C" int vq2_cache_write(const void* q, int64_t q_token_stride, int64_t q_
   a.D = (int)head_size;
   a.lanes_log2 = lanes_log2(a.D);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (kv_dtype == VQ2_I4)
+    return dtype == VQ2_F16 ? launch_rope<__half, 3>(a, tokens, st) : launch_rope<__nv_bfloat16, 3>(a, tokens, st);
   if (kv_dtype == VQ2_I8)
     return dtype == VQ2_F16 ? launch_rope<__half, 2>(a, tokens, st) : launch_rope<__nv_bfloat16, 2>(a, tokens, st);
   return dtype == VQ2_F16 ? launch_rope<__half, 1>(a, tokens, st) : launch_rope<__nv_bfloat16, 1>(a, tokens, st);
@@ -532,7 +671,8 @@ extern "C" int vq2_cache_read(const void* k_pages, const void* v_pages, int kv_d
                    table_stride, table_cols, nullptr, starts, seqs);
   if (s != VQ2_OK) return s;
   if (!starts || !k_out || !v_out) return VQ2_ERR_ARG;
-  if ((out_dtype != VQ2_F16 && out_dtype != VQ2_BF16) || (kv_dtype != out_dtype && kv_dtype != VQ2_I8)) return VQ2_ERR_DTYPE;
+  if ((out_dtype != VQ2_F16 && out_dtype != VQ2_BF16) || (kv_dtype != out_dtype && kv_dtype != VQ2_I8 && kv_dtype != VQ2_I4))
+    return VQ2_ERR_DTYPE;
   if (total < 0 || total > 0x7fffffff) return VQ2_ERR_SHAPE;
   if (!aligned(k_out, 16) || !aligned(v_out, 16)) return VQ2_ERR_ALIGN;
   if (total == 0) return VQ2_OK;
@@ -547,9 +687,13 @@ extern "C" int vq2_cache_read(const void* k_pages, const void* v_pages, int kv_d
   if (blocks > 0x7fffffff) return VQ2_ERR_SHAPE;
   const dim3 grid((unsigned)blocks), block(kRopeThreads);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool half = out_dtype == VQ2_F16;
+  if (kv_dtype == VQ2_I4)
+    return half ? launch_kernel(cache_read_kernel<__half, 4, NIT>, grid, block, 0, st, a)
+                : launch_kernel(cache_read_kernel<__nv_bfloat16, 4, NIT>, grid, block, 0, st, a);
   if (kv_dtype == VQ2_I8)
-    return out_dtype == VQ2_F16 ? launch_kernel(cache_read_kernel<__half, true, NIT>, grid, block, 0, st, a)
-                                : launch_kernel(cache_read_kernel<__nv_bfloat16, true, NIT>, grid, block, 0, st, a);
-  return out_dtype == VQ2_F16 ? launch_kernel(cache_read_kernel<__half, false, NIT>, grid, block, 0, st, a)
-                              : launch_kernel(cache_read_kernel<__nv_bfloat16, false, NIT>, grid, block, 0, st, a);
+    return half ? launch_kernel(cache_read_kernel<__half, 8, NIT>, grid, block, 0, st, a)
+                : launch_kernel(cache_read_kernel<__nv_bfloat16, 8, NIT>, grid, block, 0, st, a);
+  return half ? launch_kernel(cache_read_kernel<__half, 16, NIT>, grid, block, 0, st, a)
+              : launch_kernel(cache_read_kernel<__nv_bfloat16, 16, NIT>, grid, block, 0, st, a);
 }

@@ -9,8 +9,8 @@
 namespace vq2 {
 
 struct PagedKV {
-  const void *k, *v;             // [pages, heads, page_size, D] 16-bit or int8
-  const float *k_scale, *v_scale;  // int8: [pages, heads, page_size]
+  const void *k, *v;             // [pages, heads, page_size, D] 16-bit, int8 or (two a byte) 4-bit
+  const float *k_scale, *v_scale;  // int8: [pages, heads, page_size]; 4-bit: records of 16 rows, see Scale4
   const int32_t* table;          // [seqs, cols] page ids, row stride table_stride
   const int32_t* lens;           // [seqs] tokens in the cache, the new ones among them
   const int32_t* starts;         // [seqs + 1] first new token of each sequence; null: one token each
@@ -25,9 +25,11 @@ inline int paged_kv(PagedKV& kv, const void* k, const void* v, int kv_dtype, con
                     int64_t pages, int64_t heads, int64_t page_size, int64_t D, const int32_t* table,
                     int64_t table_stride, int64_t cols, const int32_t* lens, const int32_t* starts, int64_t seqs) {
   if (!k || !v || (!table && seqs > 0 && cols > 0)) return VQ2_ERR_ARG;   // an empty table may have no address
-  if (kv_dtype != VQ2_F16 && kv_dtype != VQ2_BF16 && kv_dtype != VQ2_I8) return VQ2_ERR_DTYPE;
-  if ((kv_dtype == VQ2_I8) != (k_scale != nullptr) || (k_scale == nullptr) != (v_scale == nullptr)) return VQ2_ERR_ARG;
-  if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)) || bad_head_size(D)) return VQ2_ERR_SHAPE;
+  if (kv_dtype != VQ2_F16 && kv_dtype != VQ2_BF16 && kv_dtype != VQ2_I8 && kv_dtype != VQ2_I4) return VQ2_ERR_DTYPE;
+  if ((kv_dtype == VQ2_I8 || kv_dtype == VQ2_I4) != (k_scale != nullptr) || (k_scale == nullptr) != (v_scale == nullptr)) return VQ2_ERR_ARG;
+  if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)) || bad_head_size(D) ||
+      (kv_dtype == VQ2_I4 && D % 32))
+    return VQ2_ERR_SHAPE;
   if (pages < 1 || heads < 1 || heads > 4096 || seqs < 0 || seqs > 0x7ffffff || cols < 0 || table_stride < 0)
     return VQ2_ERR_SHAPE;
   if (pages > 0x7fffffff / page_size || pages * page_size > 0x7fffffff / heads || cols > 0x7fffff00 / page_size)
@@ -38,6 +40,22 @@ inline int paged_kv(PagedKV& kv, const void* k, const void* v, int kv_dtype, con
   kv = {k, v, k_scale, v_scale, table, lens, starts, table_stride, (int32_t)pages, (int32_t)heads, l, (int32_t)cols,
         (int32_t)seqs};
   return VQ2_OK;
+}
+
+// Scales of a 4-bit cache: a record for each 16 rows of the pool (rows as pool_row counts them), fp32 [16] and then
+// e4m3 [groups][16], the factor of each 64 values. code * factor is exact in fp16 (3 + 4 bits), so that the
+// products run on exact values and the row's scale stays outside in 32 bits, as an int8 row's does.
+struct Scale4 {
+  int groups;
+  __host__ __device__ explicit Scale4(int D) : groups((D + 63) >> 6) {}
+  __host__ __device__ int record() const { return 64 + 16 * groups; }
+  __device__ int64_t row(int64_t r) const { return (r >> 4) * record() + 4 * (r & 15); }
+  __device__ int64_t factor(int64_t r, int group) const { return (r >> 4) * record() + 64 + 16 * group + (r & 15); }
+};
+
+// What an e4m3 byte without a sign stands for.
+__device__ __forceinline__ float e4m3_value(uint32_t b) {
+  return b < 8 ? (float)b * 0.001953125f : __uint_as_float((b + 960) << 20);
 }
 
 // Sequences whose new tokens end at or before token t. Block-wide (every thread calls it): one

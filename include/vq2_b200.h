@@ -45,6 +45,7 @@ extern "C" {
 #define VQ2_BF16 1
 #define VQ2_F32 2
 #define VQ2_I8 3  /* quantised key/value pages only */
+#define VQ2_I4 4  /* the same in 4 bits, two values a byte */
 
 /* ABI version of this header (bumped on any signature change). */
 VQ2_API int vq2_abi_version(void);
@@ -607,7 +608,11 @@ VQ2_API int vq2_paged_moe_t1(const void* h, int h_dtype, int64_t top_k, const in
  * fp16 or bf16 (dtype), strides in elements, last dimension contiguous; head_size a multiple of 16,
  * 16..256. Cache: k_pages, v_pages [pages, kv_heads, page_size, head_size] contiguous, page_size a
  * power of two 16..256; kv_dtype = dtype, or VQ2_I8 with fp32 k_scale, v_scale [pages, kv_heads,
- * page_size] (value = int8 * scale). table: int32 [seqs, table_cols] page ids (row stride
+ * page_size] (value = int8 * scale), or VQ2_I4 (head_size a multiple of 32) with k_pages, v_pages
+ * [pages, kv_heads, page_size, head_size / 2] bytes -- value 2i of a row in the low half of byte i, 2i + 1 in the
+ * high half, each an integer -7..7 plus 8 -- and k_scale, v_scale the address of [pages, kv_heads,
+ * page_size / 16, 4 + groups, 16] bytes, groups = ceil(head_size / 64): for 16 rows their fp32 scales, then of each
+ * 64 values (the last group may have 32) 16 factors in e4m3 (value = integer * factor * scale). table: int32 [seqs, table_cols] page ids (row stride
  * table_stride; rows may overlap, 0: all sequences on the same row): position p of sequence b is row p % page_size of page table[b][p / page_size].
  * lens: int32 [seqs] tokens of each sequence in the cache, the new ones included. starts: int32
  * [seqs + 1], ascending: sequence b's new tokens are starts[b] .. starts[b + 1] - 1 and sit at
@@ -631,7 +636,9 @@ VQ2_API int vq2_rotary(const void* q, int64_t q_token_stride, int64_t q_head_str
  * Write the new tokens' k and v into their cache rows; with inv_freq (rot values) k, and q when
  * q_heads > 0, are turned first (q into q_out, contiguous; of a token of no sequence as at position 0). 8-bit cache: per (token, head)
  * scale = amax / 127 and int8 = round-to-even(x * (127 / amax)) of the turned values in 32 bits;
- * amax < 1e-30 stores zeros with scale 0, a row with an infinity or a NaN stores scale NaN. Tokens
+ * amax < 1e-30 stores zeros with scale 0, a row with an infinity or a NaN stores scale NaN. 4-bit cache: per
+ * (token, head) scale = amax / 7; per group factor = its own amax / the row's, rounded up to e4m3 (at least 2^-9
+ * unless it is 0); the nearest integer to x / (scale * factor), of two the one further from zero. Tokens
  * without a page (a position outside the table, a page id outside the pool) are not stored.
  */
 VQ2_API int vq2_cache_write(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t q_heads,
@@ -683,6 +690,21 @@ VQ2_API int vq2_paged_attention(const void* q, int64_t q_token_stride, int64_t q
  * a block's shared memory start off its line (its rows are not written); cleared when reset is non-zero.
  * Synchronises. */
 VQ2_API int vq2_attention_status(int reset);
+
+/*
+ * Copy pages within pools that share page ids (no reference counterpart: the reference has no paged key/value
+ * cache): of every pool, page dst[i] becomes what page src[i] is, i = 0 .. n - 1. pools: HOST array; a pool is `pages`
+ * pages of page_bytes bytes, one after the other (16-byte aligned, page_bytes a multiple of 16, at most 2^30). src,
+ * dst: device int32 [n], read when the kernel runs; a pair with an id outside the pool copies nothing. All pairs are
+ * copied at once: a page that is named twice in dst, or in src and in dst, holds bytes of any of its sources
+ * after.
+ */
+typedef struct vq2_page_pool {
+  void* base;
+  int64_t page_bytes;
+} vq2_page_pool;
+VQ2_API int vq2_copy_pages(const vq2_page_pool* pools, int64_t n_pools, int64_t pages, const int32_t* src,
+                           const int32_t* dst, int64_t n, void* stream);
 
 #ifdef __cplusplus
 }
