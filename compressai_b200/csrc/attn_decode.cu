@@ -775,6 +775,6 @@ extern "C" int vq2_attention_status(int reset) {
     vq2::set_last_cuda_error(e);
     return VQ2_ERR_LAUNCH;
   }
-  const int other = vq2::attn_chunk_status(reset);
-  return v > other ? v : other;
+  for (const int other : {vq2::attn_chunk_status(reset), vq2::attn_decode4_status(reset)}) v = v > other ? v : other;
+  return v;
 }

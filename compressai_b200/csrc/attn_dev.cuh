@@ -137,6 +137,7 @@ int launch_attn_decode4(const AttnArgs& a, cudaStream_t st);
 void plan_attn_decode4(AttnArgs& a, int64_t max_new, int64_t max_len);
 int launch_attn_chunk(const AttnArgs& a, int bits, cudaStream_t st);
 void plan_attn_chunk(AttnArgs& a, int64_t max_new, int64_t max_len);
-int attn_chunk_status(int reset);   // its part of vq2_attention_status
+int attn_chunk_status(int reset);   // their parts of vq2_attention_status
+int attn_decode4_status(int reset);
 
 }  // namespace vq2
