@@ -35,6 +35,13 @@ int64_t plan(AttnArgs& a, int bits, int64_t max_new, int64_t max_len, bool& chun
     a.part_o = reinterpret_cast<float*>(take((int64_t)a.T * a.hq * a.splits * a.D * 4));
     a.part_ml = reinterpret_cast<float2*>(take((int64_t)a.T * a.hq * a.splits * 8));
   }
+  if (!chunked && bits == 4) {
+    a.segments = reinterpret_cast<int2*>(take((int64_t)a.kv.seqs * a.row_blocks * a.kv.heads * 8));
+    if (a.whole != 0x7fffffff) {
+      a.part_o = reinterpret_cast<float*>(take((int64_t)a.blocks * 2 * a.rows_per_block * a.D * 4));
+      a.part_ml = reinterpret_cast<float2*>(take((int64_t)a.blocks * 2 * a.rows_per_block * 8));
+    }
+  }
   if (chunked && bits < 16) {
     a.wide_len = a.keys_end = (int)wide_len;
     a.wide_k = take(wide_rows * a.D * 2);

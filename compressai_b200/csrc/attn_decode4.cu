@@ -62,18 +62,52 @@ __device__ __forceinline__ uint32_t lds1(uint32_t addr) {
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
                                     float c0, float c1, float c2, float c3) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  mma(d, a0, a1, a2, a3, b0, b1, d[0], d[1], d[2], d[3]);
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same value in a register of its own: an MMA takes its operands from registers in a row, and would have equal ones
+// copied there each time.
+__device__ __forceinline__ float apart(float v) {
+  float r;
+  asm volatile("mov.b32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t apart(uint32_t v) {
+  uint32_t r;
+  asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
+}
+
+__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;   // codes of an even byte, as numbers 2^-24 and 16 2^-24
+
+// The codes of bytes 0 and 2 (odd: 1 and 3) of w as two fp16 numbers each: low ones by 2^-24, high ones by 16 2^-24. Integer
+// instructions run at half rate: the second mask of the odd bytes is a subtraction.
+__device__ __forceinline__ void two_codes(bool odd, uint32_t w, uint32_t& low, uint32_t& high) {
+  if (odd) {
+    const uint32_t both = __byte_perm(w, 0, 0x4341);
+    low = both & kLow;
+    high = hsub2(both, low);
+  } else {
+    low = w & kLow;
+    high = w & kHigh;
+  }
 }
 
 // Two e4m3 bytes (the low two of w) as fp16.
@@ -87,37 +121,149 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// Shapes of one variant. DP: head size rounded up (values past D are zeros); NT: 8-row tiles.
-template <int DP, int NT>
+// Shapes of one variant. G: groups of a row (codes past D are zeros); NT: 8-row tiles.
+template <int G, int NT>
 struct Shape4 {
-  static constexpr int kRow = DP / 2;                   // bytes of a key's codes
-  static constexpr int kG = DP / 64;                    // groups
-  static constexpr int kU = DP == 64 ? 4 : 2;          // 16-key tiles a step
-  static constexpr int kKeys = 16 * kU;
-  static constexpr int kHalf = kKeys * kRow;            // K or V of a step
   static constexpr int kWarps = 4;
-  static constexpr int kPerSm = NT == 2 ? 2 : DP == 256 ? 3 : 4;   // blocks an SM, as registers allow
-  static constexpr int kRecords = kU * (64 + 16 * kG);  // scales of a half, at most
-  static constexpr int kFit = (224 * 1024 / kPerSm - 10240) / (kWarps * (kHalf + kRecords));
-  static constexpr int kSlots = kFit > 8 ? 8 : kFit;
-  static constexpr int kRing = kWarps * kSlots * kHalf;
-  static constexpr int kJoin = kWarps * NT * 8 * (DP + 4) * 4;   // the warps' O, over the ring
-  static constexpr int kQ = NT * kG * 1024;             // query fragments
-  static constexpr int kScaleSlots = kSlots / 2 + 1;    // steps under way
-  static constexpr int kScales = kWarps * kScaleSlots * 2 * kRecords;
-  static constexpr int kSmem = 1024 + (kRing > kJoin ? kRing : kJoin) + kQ + kScales;
-  static_assert(kSlots >= 3, "a half in use, two in flight");
-  static_assert(kScaleSlots * kU <= 32, "bits of the pages that are gone");
+  static constexpr int kRow = G > 2 ? 128 : 32 * G;     // bytes of a key's codes in shared memory
+  static constexpr int kU = G > 2 ? 2 : 4;              // 16-key tiles of a warp a step
+  static constexpr int kKeys = 16 * kU * kWarps;        // of a step
+  static constexpr int kHalf = kKeys * kRow;            // K or V of a step
+  static constexpr int kRecord = 64 + 16 * G;           // scales of 16 keys
+  static constexpr int kScales = kKeys / 16 * kRecord;
+  static constexpr int kStages = 2;                       // steps under way
+  static constexpr int kPerSm = NT == 2 ? 2 : 3;        // blocks an SM, as registers allow
+  static constexpr int kQ = NT * G * 1024;              // query fragments
+  static constexpr int kRing = kStages * 2 * kHalf;
+  static constexpr int kWidth = 64 * G + 4;             // of a row of O
+  static constexpr int kJoin = kWarps * NT * 8 * kWidth * 4;   // the warps' O, over the ring
+  // (three blocks an SM: 76 KB each, static and reserved memory of 2.5 KB included)
+  static constexpr int kSmem = 1024 + (kRing > kJoin ? kRing : kJoin) + kStages * 2 * kScales + kQ;
+  static_assert(kPerSm * (kSmem + 2560) <= 228 * 1024, "blocks an SM");
 };
 
 // The key of a tile that stands in row r (0..7) of the MMA's first 8; 8 on, that of row r + 8. Rows 0..3, rows 4..7,
 // the even ones and the odd ones are each on four different 32-byte places of shared memory.
-template <int DP>
+template <int ROW>
 __device__ __forceinline__ int key_of_row(int r) {
   const int place = (r & 3) ^ (r >> 2), other = r >> 2;
-  if (DP == 256) return 2 * place + other;
-  if (DP == 128) return (place & 1) | other << 1 | (place & 2) << 1;
+  if (ROW == 128) return 2 * place + other;
+  if (ROW == 64) return (place & 1) | other << 1 | (place & 2) << 1;
   return place + 4 * other;
+}
+
+// Work is counted in units of a block step. Every pair (block of rows, key/value head) has its keys' units, at least one, and,
+// where a block's share of all units is four or more, two for its start and its end. The launch's blocks take equal shares in
+// order, so that lengths of any kind fill the card evenly; what a block has of one pair is a segment. Only pairs of more than
+// a.whole units are split.
+struct Place {
+  int64_t x;     // units before the pair
+  int item, h;   // block of rows (sequence by sequence), head
+  int k;         // the pair's units before this one, its start not counted
+};
+struct Share {
+  int64_t of;    // a block's
+  int start;     // units of a pair's start
+};
+
+// (Not inlined, as what follows: run a few times a block, they would push the loop out of the instruction cache.)
+template <int UNIT>
+__device__ __noinline__ int units_of(const AttnArgs& a, int item) {
+  const int b = a.row_blocks == 1 ? item : item / a.row_blocks;
+  const AttnRows w = attn_rows(a, b, item - b * a.row_blocks);
+  if (w.rows <= 0) return 0;
+  int lo, hi;
+  block_keys(a, w, lo, hi);
+  return hi > lo ? (hi - lo - 1) / UNIT + 1 : 1;
+}
+
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
+  return (x | y) >> 31 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y);
+}
+
+// Where this block's units start and end (block-wide, 128 threads; false: it has none). Each thread counts a run of the
+// items; the runs' sums are added up, and the thread whose run a boundary falls in finds it there.
+template <int UNIT>
+__device__ __noinline__ bool my_units(const AttnArgs& a, Place* ends, int64_t* sums, Share& share) {
+  const int items = a.kv.seqs * a.row_blocks, run = (items + 127) >> 7, i0 = min(items, (int)threadIdx.x * run), i1 = min(items, i0 + run);
+  int64_t units = 0;
+  int pairs = 0, last = 0;
+#pragma unroll 1
+  for (int i = i0; i < i1; ++i) {
+    last = units_of<UNIT>(a, i);
+    units += last;
+    pairs += last > 0;
+  }
+  // up to this thread: units, items with rows
+  int64_t upto_u = units, upto_p = pairs;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, upto_u, o), z = __shfl_up_sync(0xffffffffu, upto_p, o);
+    if ((threadIdx.x & 31) >= o) {
+      upto_u += y;
+      upto_p += z;
+    }
+  }
+  if ((threadIdx.x & 31) == 31) {
+    sums[2 * (threadIdx.x >> 5)] = upto_u;
+    sums[2 * (threadIdx.x >> 5) + 1] = upto_p;
+  }
+  __syncthreads();
+  int64_t total_u = 0, total_p = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i < (int)(threadIdx.x >> 5)) {
+      upto_u += sums[2 * i];
+      upto_p += sums[2 * i + 1];
+    }
+    total_u += sums[2 * i];
+    total_p += sums[2 * i + 1];
+  }
+  share.start = total_u * a.kv.heads >= 4 * (int64_t)gridDim.x ? 2 : 0;
+  const int64_t total = (total_u + share.start * total_p) * a.kv.heads, mine = (units + share.start * pairs) * a.kv.heads,
+                upto = (upto_u + share.start * upto_p) * a.kv.heads;
+  share.of = quotient(total + gridDim.x - 1, gridDim.x);
+  if (blockIdx.x * share.of >= total) return false;
+#pragma unroll 1
+  for (int e = 0; e < 2; ++e) {
+    const int64_t x = (blockIdx.x + e) * share.of;
+    if (x >= total) {
+      if (threadIdx.x == 0) ends[e] = {total, items, 0, 0};
+    } else if (x >= upto - mine && x < upto) {
+      Place p = {upto - mine, i0, 0, 0};
+      int n;   // of a pair
+#pragma unroll 1
+      for (;; ++p.item) {
+        n = run == 1 ? last : units_of<UNIT>(a, p.item);
+        if (n == 0) continue;
+        n += share.start;
+        if (x < p.x + (int64_t)n * a.kv.heads) break;
+        p.x += (int64_t)n * a.kv.heads;
+      }
+      p.h = (int)quotient(x - p.x, n);
+      p.x += (int64_t)p.h * n;
+      p.k = max(0, (int)(x - p.x) - share.start);
+      n -= share.start;
+      if (n <= a.whole) {   // whole: the nearer end
+        if (2 * p.k >= n) {
+          p.x += n + share.start;
+          if (++p.h == a.kv.heads) {
+            p.h = 0;
+            do ++p.item; while (p.item < items && units_of<UNIT>(a, p.item) == 0);
+          }
+        }
+        p.k = 0;
+      }
+      ends[e] = p;
+    }
+  }
+  __syncthreads();
+  return ends[0].item != ends[1].item || ends[0].h != ends[1].h || ends[0].k != ends[1].k;
+}
+
+// How many blocks, from that with unit x on, have the n units from there on.
+__device__ __noinline__ int blocks_of(int64_t x, int n, int64_t share) {
+  return (int)(quotient(x + n - 1, share) - quotient(x, share)) + 1;
 }
 
 constexpr long long kWaitCycles = 4000000000LL;  // ~2 s at 1.965 GHz
@@ -133,136 +279,160 @@ __device__ __forceinline__ bool copy_wait(uint32_t bar, uint32_t parity) {
   return true;
 }
 
-template <int DP, int NT, typename T>
-__global__ void __launch_bounds__(Shape4<DP, NT>::kWarps * 32, Shape4<DP, NT>::kPerSm)
-    attn_decode4_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
-  using S = Shape4<DP, NT>;
-  constexpr int G = S::kG, U = S::kU, ROW = S::kRow;
+template <int G, int NT, typename T>
+__global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPerSm)
+    attn_decode4_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+  using S = Shape4<G, NT>;
+  constexpr int U = S::kU, ROW = S::kRow, UNIT = S::kKeys, ST = S::kStages, REC = S::kRecord;
   // weights 2^7 larger than the maximum asks for, so that those down to 2^-32 of the largest are more than 0
   constexpr float kLift = 7.f, kDrop = 1.f / 128.f;
-  constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
   extern __shared__ unsigned char decode4_raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(decode4_raw) + 1023) & ~uintptr_t(1023));
-  unsigned char* q_s = sm + (S::kRing > S::kJoin ? S::kRing : S::kJoin);
-  __shared__ uint64_t bars[S::kWarps][S::kSlots];
-  __shared__ float2 ml_s[S::kWarps][NT * 8];
-  __shared__ float qexp_s[NT * 8], qsum_s[NT * 8][G];
+  unsigned char* q_s = sm + (S::kRing > S::kJoin ? S::kRing : S::kJoin) + ST * 2 * S::kScales;
+  __shared__ uint64_t full[ST], empty[ST];
+  __shared__ uint32_t gone_s[ST];               // the boxes whose pages are not in the pool
+  __shared__ float2 red[S::kWarps][NT * 8];
+  __shared__ float qexp_s[NT * 8], qtop_s[G][NT * 8];
+  __shared__ float4 start_s[NT][G][4];
+  __shared__ uint4 ones_s[2];                   // A of the MMA that sums a group's weights, in the row of its number and in others
+  __shared__ Place ends[2];
+  __shared__ int64_t sums[8];
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int split = blockIdx.y, h = blockIdx.z;
-  const int b = blockIdx.x / a.row_blocks, rb = blockIdx.x - b * a.row_blocks;
-  const AttnRows w = attn_rows(a, b, rb);
-  blank_strays(a, w, b, ((int64_t)rb * a.kv.heads + h) * a.splits + split, (int64_t)a.row_blocks * a.kv.heads * a.splits);
-  if (w.rows <= 0) return;
-  int lo, hi;
-  block_keys(a, w, lo, hi);
-  if (split > 0 && (int64_t)split * a.chunk >= hi - lo) return;   // split 0 stays: it writes the rows that see nothing
-  const int s0 = lo + split * a.chunk, s1 = s0 + min(a.chunk, hi - s0);   // no sum past 2^31
-  const bool alone = hi - lo <= a.chunk;
-  const int tiles = s1 > s0 ? (s1 - s0 + S::kKeys - 1) / S::kKeys : 0;
-
-  // ---- the warp's ring: halves K0 V0 K1 V1 .. of its steps warp, warp + kWarps, ..
-  const int groups = (a.D + 63) >> 6, record = 64 + 16 * groups;   // bytes of 16 keys' scales
-  const uint32_t q_sm = su32(q_s), ring = su32(sm) + warp * S::kSlots * S::kHalf, bar0 = su32(&bars[warp][0]);
-  const uint32_t scales = q_sm + S::kQ + warp * S::kScaleSlots * 2 * S::kRecords;
-  const int32_t* table = a.kv.table + b * a.kv.table_stride;
-  const int page_mask = (1 << a.kv.page_log2) - 1, seen = row_lo(a, w, w.r0 / a.G);
-  const int halves = tiles > warp ? 2 * ((tiles - warp + S::kWarps - 1) / S::kWarps) : 0;
-  auto key_of = [&](int i) { return s0 + S::kKeys * (warp + S::kWarps * i); };   // first key of the warp's step i
-  // A copy is min(page, step) keys: this lane's, and the key it starts at.
-  const int box_keys = min(1 << a.kv.page_log2, S::kKeys), sub = lane * box_keys;
-  const bool copies = sub < S::kKeys;
-  auto page_of = [&](int i) {   // of this lane's copy; -1 where there is none or its keys are past
-    const int k = key_of(i) + (copies ? sub : 0);
-    return 2 * i < halves && k < s1 && (k | page_mask) >= seen ? table[k >> a.kv.page_log2] : -1;
-  };
-  if (lane == 0) {
-    for (int i = 0; i < S::kSlots; ++i) mbar_init(bar0 + 8 * i, 1);
+  const uint32_t ring = su32(sm), scales = su32(q_s) - ST * 2 * S::kScales, q_sm = su32(q_s), full0 = su32(full), empty0 = su32(empty);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(full0 + 8 * i, 1);
+      mbar_init(empty0 + 8 * i, S::kWarps);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async();
   }
-  __syncwarp();
-  // gone: bit U i + u of 32 says that the page of tile u of step i is not in the pool: no such keys
-  uint32_t gone = 0;
-  int ahead = page_of(0), row = 0;   // page of the lane's next copy; pool row of its present one
-  int put = 0, put_slot = 0, put_scale = 0;   // next half to fetch, its slot, its step's place for scales
-  auto fetch = [&]() {
-    if (put >= halves) return;
-    const int i = put >> 1;
-    const uint32_t bar = bar0 + 8 * put_slot;
-    if (!(put & 1)) {
-      const bool there = ahead >= 0 && ahead < a.kv.pages;
-      const uint32_t out = __ballot_sync(0xffffffffu, !there);
-      const int k = key_of(i);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {   // of the lane whose copy holds tile u
-        const uint32_t bit = (out >> (16 * u / box_keys)) & 1;
-        const int at = (U * i + u) & 31;
-        gone = (gone & ~(1u << at)) | (bit << at);
-      }
-      // a page that exists stands in for one that does not
-      row = (((there ? ahead : 0) * a.kv.heads + h) << a.kv.page_log2) + ((k + sub) & page_mask);
-      ahead = page_of(i + 1);
-      if (lane == 0) mbar_arrive_tx(bar, S::kHalf + 2 * U * record);
-      __syncwarp();
-      if (copies) {
-        const uint32_t dst = scales + put_scale * 2 * S::kRecords + (sub >> 4) * record;
-        const int64_t from = (int64_t)(row >> 4) * record;
-        const int bytes = (box_keys >> 4) * record;
-        bulk_load(dst, reinterpret_cast<const unsigned char*>(a.kv.k_scale) + from, bytes, bar);
-        bulk_load(dst + S::kRecords, reinterpret_cast<const unsigned char*>(a.kv.v_scale) + from, bytes, bar);
-      }
-      if (++put_scale == S::kScaleSlots) put_scale = 0;
-    } else {
-      if (lane == 0) mbar_arrive_tx(bar, S::kHalf);
-      __syncwarp();
-    }
-    if (copies) tma_load_2d(ring + put_slot * S::kHalf + sub * ROW, put & 1 ? &vmap : &kmap, 0, row, bar);
-    ++put;
-    if (++put_slot == S::kSlots) put_slot = 0;
+  if (threadIdx.x < 2) ones_s[threadIdx.x] = threadIdx.x ? make_uint4(0, 0, 0, 0) : make_uint4(0x00080008u, 0u, 0x00080008u, 0u);
+  Share share;
+  const bool any = my_units<UNIT>(a, ends, sums, share);
+  const Place end = ends[1];
+  const int page_mask = (1 << a.kv.page_log2) - 1;
+  // A copy is a box of min(page, step) keys; a step's are found by a lane each and issued by one thread of the warp whose turn it is.
+  const int box_keys = min(1 << a.kv.page_log2, S::kKeys), boxes = S::kKeys / box_keys, box_record = (box_keys >> 4) * REC;
+  // this lane's places: K's key (another 8 on), V's keys of the MMA's rows 2t, 2t + 1 (others 8 on); 32 bytes a group
+  auto swizzled = [](int key, int byte) {
+    const int x = ROW == 128 ? key & 7 : ROW == 64 ? (key >> 1) & 3 : 0;
+    return (uint32_t)(key * ROW + (byte ^ (x << 4)));
   };
-#pragma unroll 1
-  for (int j = 0; j < S::kSlots; ++j) fetch();
+  const int kkey = key_of_row<ROW>(g), vkey0 = key_of_row<ROW>(2 * t), vkey1 = key_of_row<ROW>(2 * t + 1);
+  const uint32_t kx = swizzled(kkey, 8 * t), vx[2] = {swizzled(vkey0, 4 * g), swizzled(vkey1, 4 * g)};
+  // the factors of V's two keys out of the four bytes that both are in
+  const uint32_t vword = vkey0 & 4, vsel = (uint32_t)(vkey0 & 3) | (uint32_t)(vkey1 & 3) << 4;
+  uint32_t done = 0;              // steps of the segments so far
+  uint32_t mine = 0xffffffffu;    // the last step that this warp fetched
+  bool lost = false, ok = true;   // a wait of this warp, none of the block's has given up
 
-  // ---- queries as B fragments, in the order of K's codes: of a group's 16 values of lane t, word w holds 8 w .. 8 w + 7,
-  // and its MMA j takes values 2 j, 2 j + 4 and 2 j + 1, 2 j + 5 (these by 16)
-  for (int i = warp; i < NT; i += S::kWarps) {
-    const int r = w.r0 + 8 * i + g;
-    const bool ok = 8 * i + g < w.rows;
-    const T* src = static_cast<const T*>(a.q);
-    if (ok) src += (w.first + r / a.G) * a.q_ts + (h * a.G + r % a.G) * a.q_hs;
-    uint4 v[G][2];
-    float top = 0.f;
+  int item = ends[0].item, h = ends[0].h, unit0 = ends[0].k;
+  int64_t x = ends[0].x;
+#pragma unroll 1
+  for (bool more = any; more;) {   // ---- a segment
+    const int b = a.row_blocks == 1 ? item : item / a.row_blocks;
+    const AttnRows w = attn_rows(a, b, item - b * a.row_blocks);
+    int lo, hi;
+    block_keys(a, w, lo, hi);
+    const int n_units = hi > lo ? (hi - lo - 1) / UNIT + 1 : 1;
+    const int take = (item == end.item && h == end.h ? end.k : n_units) - unit0;
+    const int s0 = lo + unit0 * UNIT, s1 = (int)min((int64_t)hi, s0 + (int64_t)take * UNIT);
+    const bool alone = take == n_units;
+    if (unit0 == 0 && threadIdx.x == 0)   // for the joining launch: who has this pair
+      a.segments[(int64_t)item * a.kv.heads + h] = make_int2(blockIdx.x, alone ? 1 : blocks_of(x + share.start, n_units, share.of));
+    const int32_t* table = a.kv.table + b * a.kv.table_stride;
+    const int seen = row_lo(a, w, w.r0 / a.G);
+    const int steps = ok && s1 > s0 ? (s1 - s0 + S::kKeys - 1) / S::kKeys : 0;
+    const uint32_t first = done;   // the segment's first step
+    // The queries first, ahead of the copies that fill the memory's queues: a group of 8 rows a warp, 16 values a lane.
+    constexpr int QW = (NT * G + 3) / 4;
+    uint4 qv[QW][2];
 #pragma unroll
-    for (int k = 0; k < G; ++k)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int d = 64 * k + 16 * t + 8 * c;
-        v[k][c] = make_uint4(0, 0, 0, 0);
-        if (ok && d < a.D) v[k][c] = *reinterpret_cast<const uint4*>(src + d);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = unpack2<T>((&v[k][c].x)[j]);
-          top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+    for (int p = 0; p < QW; ++p) {
+      const int e = warp + 4 * p, i = e / G, r = 8 * i + g, d = 64 * (e % G) + 16 * t;
+      qv[p][0] = qv[p][1] = make_uint4(0, 0, 0, 0);
+      if (e < NT * G && r < w.rows && d < a.D) {
+        const int tok = (w.r0 + r) / a.G;
+        const uint4* from = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(w.first + tok) * a.q_ts +
+                                                           (int64_t)(h * a.G + w.r0 + r - tok * a.G) * a.q_hs + d);
+        qv[p][0] = from[0];
+        qv[p][1] = from[1];
+      }
+    }
+    // page of the lane's box of step i; -1 where there is none or its keys are past
+    auto page_of = [&](int i) {
+      const int k = s0 + S::kKeys * i + lane * box_keys;
+      return lane < boxes && i < steps && k < s1 && (k | page_mask) >= seen ? table[k >> a.kv.page_log2] : -1;
+    };
+    int turn = (warp - (int)first) & 3;   // the segment's step that this warp fetches next
+    int ahead = page_of(turn);
+    auto fetch = [&]() {
+      const uint32_t step = first + turn, st = step % ST, bar = full0 + 8 * st;
+      if (step >= ST) lost |= !copy_wait(empty0 + 8 * st, (step / ST - 1) & 1);
+      if (__any_sync(0xffffffffu, lost)) return;
+      const bool there = ahead >= 0 && ahead < a.kv.pages;
+      const uint32_t out = __ballot_sync(0xffffffffu, lane < boxes && !there);
+      // a page that exists stands in for one that does not
+      const int rows = (((there ? ahead : 0) * a.kv.heads + h) << a.kv.page_log2) + ((s0 + S::kKeys * turn + lane * box_keys) & page_mask);
+      mine = step;
+      turn += 4;
+      ahead = page_of(turn);
+#pragma unroll 1
+      for (int c = 0; c < boxes; ++c) {
+        const int row = __shfl_sync(0xffffffffu, rows, c);
+        if (elect_one()) {
+          if (c == 0) {
+            *reinterpret_cast<volatile uint32_t*>(&gone_s[st]) = out;
+            mbar_arrive_tx(bar, 2 * (S::kHalf + S::kScales));
+          }
+          const uint32_t to = ring + st * 2 * S::kHalf + c * box_keys * ROW, to_s = scales + st * 2 * S::kScales + c * box_record;
+          const int64_t from = (int64_t)(row >> 4) * REC;
+          tma_load_2d(to, &kmap, 0, row, bar);
+          bulk_load(to_s, reinterpret_cast<const unsigned char*>(a.kv.k_scale) + from, box_record, bar);
+          tma_load_2d(to + S::kHalf, &vmap, 0, row, bar);
+          bulk_load(to_s + S::kScales, reinterpret_cast<const unsigned char*>(a.kv.v_scale) + from, box_record, bar);
         }
       }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const int e = fp16_lift(top);
-    const float by = __int_as_float((127 + e) << 23);
-    if (t == 0) qexp_s[8 * i + g] = __int_as_float((127 - e) << 23);
+    };
+    if (turn < min(ST, steps)) fetch();
+
+    // ---- queries as B fragments, in the order of K's codes: of a group's 16 values of lane t, word w holds 8 w .. 8 w + 7,
+    // and its MMA j takes values 2 j, 2 j + 4 and 2 j + 1, 2 j + 5 (these by 16)
 #pragma unroll
-    for (int k = 0; k < G; ++k) {
+    for (int p = 0; p < QW; ++p) {
+      float top = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float2 f = unpack2<T>((&qv[p][j >> 2].x)[j & 3]);
+        top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int e = warp + 4 * p;
+      if (t == 0 && e < NT * G) qtop_s[e % G][8 * (e / G) + g] = top;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int p = 0; p < QW; ++p) {
+      const int n = warp + 4 * p, i = n / G, k = n % G;
+      if (n >= NT * G) break;
+      float top = 0.f;
+#pragma unroll
+      for (int c = 0; c < G; ++c) top = fmaxf(top, qtop_s[c][8 * i + g]);
+      const int e = fp16_lift(top);
+      const float by = __int_as_float((127 + e) << 23);
       float sum = 0.f;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float f[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float2 x = unpack2<T>((&v[k][c].x)[j]);
-          f[2 * j] = x.x * by;
-          f[2 * j + 1] = x.y * by;
+          const float2 y = unpack2<T>((&qv[p][c].x)[j]);
+          f[2 * j] = y.x * by;
+          f[2 * j + 1] = y.y * by;
         }
         uint4 o;
 #pragma unroll
@@ -271,330 +441,449 @@ __global__ void __launch_bounds__(Shape4<DP, NT>::kWarps * 32, Shape4<DP, NT>::k
           const uint32_t b1 = pack2<__half>(f[2 * j + 1] * 0.0625f, f[2 * j + 5] * 0.0625f);
           (&o.x)[2 * j] = b0;
           (&o.x)[2 * j + 1] = b1;
-          const float2 x = unpack2<__half>(b0), y = unpack2<__half>(b1);
-          sum += (x.x + x.y) + 16.f * (y.x + y.y);
+          const float2 y = unpack2<__half>(b0), z = unpack2<__half>(b1);
+          sum += (y.x + y.y) + 16.f * (z.x + z.y);
         }
-        *reinterpret_cast<uint4*>(q_s + ((i * G + k) * 2 + c) * 512 + lane * 16) = o;
+        *reinterpret_cast<uint4*>(q_s + (n * 2 + c) * 512 + lane * 16) = o;
       }
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      if (t == 0) qsum_s[8 * i + g][k] = sum * (-8.f / 16777216.f);
+      if (t == 0) {   // what a group's sum starts at, as the MMA's four of the lanes with row 8 i + g
+        float* to = reinterpret_cast<float*>(&start_s[i][k][g >> 1]) + (g & 1);
+        to[0] = to[2] = sum * (-8.f / 16777216.f);
+        if (k == 0) qexp_s[8 * i + g] = __int_as_float((127 - e) << 23);
+      }
     }
-  }
-  __syncthreads();
+    __syncthreads();
 
-  // ---- this lane's two rows of each tile (columns 2t, 2t + 1 of S^T): what they see
-  int klo[NT][2], khi[NT][2];
-  float sc[NT][2], start[NT][G][2];   // start: what a group's sum starts at
+    // ---- this lane's two rows of each tile (columns 2t, 2t + 1 of S^T): what they see
+    int klo[NT][2], khi[NT][2];
+    float sc[NT][2];
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
+    for (int i = 0; i < NT; ++i)
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int r = 8 * i + 2 * t + c;
-      const bool ok = r < w.rows;
-      const int tok = (w.r0 + (ok ? r : 0)) / a.G;
-      klo[i][c] = row_lo(a, w, tok);
-      khi[i][c] = ok ? row_hi(a, w, tok) : 0;
-      sc[i][c] = a.scale_log2 * qexp_s[r];
-#pragma unroll
-      for (int k = 0; k < G; ++k) start[i][k][c] = qsum_s[r][k];
-    }
-  // keys that every row sees need no mask
-  const int all_lo = row_lo(a, w, (w.r0 + w.rows - 1) / a.G), all_hi = row_hi(a, w, w.r0 / a.G);
+      for (int c = 0; c < 2; ++c) {
+        const int r = 8 * i + 2 * t + c;
+        const bool there = r < w.rows;
+        const int tok = (w.r0 + (there ? r : 0)) / a.G;
+        klo[i][c] = row_lo(a, w, tok);
+        khi[i][c] = there ? row_hi(a, w, tok) : 0;
+        sc[i][c] = a.scale_log2 * qexp_s[r];
+      }
+    // keys that every row sees need no mask
+    const int all_lo = row_lo(a, w, (w.r0 + w.rows - 1) / a.G), all_hi = min(s1, row_hi(a, w, w.r0 / a.G));
 
-  // o: sums over the codes plus 8, of values d (0, 1) and, 16 times as large, d + 1 (2, 3); oc: row k of it, 8 2^-24 times the
-  // weights of group k
-  float o[NT][DP / 16][4], oc[NT][4], m[NT][2], base[NT][2], l[NT][2], vref[NT][2];
+    // o: sums over the codes plus 8 of values d (0, 1) and (2, 3) d + 1, these 16 times as large, in odd tiles with those of d
+    // added; oc: in row k 8 2^-24 times the weights of group k
+    float o[NT][4 * G][4], oc[NT][4], m[NT][2], l[NT][2], vref[NT][2];
 #pragma unroll
-  for (int i = 0; i < NT; ++i) {
+    for (int i = 0; i < NT; ++i) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 4; ++c) {
 #pragma unroll
-      for (int j = 0; j < DP / 16; ++j) o[i][j][c] = 0.f;
-      oc[i][c] = 0.f;
+        for (int j = 0; j < 4 * G; ++j) o[i][j][c] = 0.f;
+        oc[i][c] = 0.f;
+      }
+      m[i][0] = m[i][1] = -INFINITY;
+      l[i][0] = l[i][1] = vref[i][0] = vref[i][1] = 0.f;
     }
-    m[i][0] = m[i][1] = -INFINITY;
-    base[i][0] = base[i][1] = 0.f;   // m, or 0 while no key has been seen
-    l[i][0] = l[i][1] = vref[i][0] = vref[i][1] = 0.f;
-  }
 
-  // this lane's places: K's key (another 8 on), V's keys of the MMA's rows 2t, 2t + 1 (others 8 on); 32 bytes a group
-  auto swizzled = [](int key, int byte) {
-    const int x = DP == 256 ? key & 7 : DP == 128 ? (key >> 1) & 3 : 0;
-    return (uint32_t)(key * ROW + (byte ^ (x << 4)));
-  };
-  const int kkey = key_of_row<DP>(g), vkey0 = key_of_row<DP>(2 * t), vkey1 = key_of_row<DP>(2 * t + 1);
-  const uint32_t kx = swizzled(kkey, 8 * t), vx[2] = {swizzled(vkey0, 4 * g), swizzled(vkey1, 4 * g)};
-  // the factors of V's two keys out of the four bytes that both are in
-  const uint32_t vword = vkey0 & 4, vsel = (uint32_t)(vkey0 & 3) | (uint32_t)(vkey1 & 3) << 4;
-  int slot = 0, phase = 0, scale_slot = 0;
-  bool ok = true;
-  auto step = [&]() {   // the half in `slot` is used up: refill it, go to the next
-    __syncwarp();
-    fetch();
-    if (++slot == S::kSlots) {
-      slot = 0;
-      phase ^= 1;
-    }
-  };
-  for (int n = 0; 2 * n < halves; ++n) {
-    ok = __all_sync(0xffffffffu, copy_wait(bar0 + 8 * slot, phase));
-    if (!ok) break;
-    uint32_t src = ring + slot * S::kHalf;
-    const uint32_t k_rec = scales + scale_slot * 2 * S::kRecords, v_rec = k_rec + S::kRecords;
-    if (++scale_slot == S::kScaleSlots) scale_slot = 0;
-    // ---- S^T = K Q^T, a group's sum times its factor
-    float s[U][NT][4];
+#pragma unroll 1
+    for (int n = 0; n < steps; ++n) {
+      const uint32_t step = first + n, st = step % ST;
+      lost |= !copy_wait(full0 + 8 * st, (step / ST) & 1);
+      if (__any_sync(0xffffffffu, lost)) break;
+      const uint32_t src = ring + st * 2 * S::kHalf + warp * U * 16 * ROW;
+      const uint32_t k_rec = scales + st * 2 * S::kScales + warp * U * REC, v_rec = k_rec + S::kScales;
+      // ---- S^T = K Q^T, a group's sum times its factor
+      float s[U][NT][4];
 #pragma unroll
-    for (int k = 0; k < G; ++k) {
-      uint4 q[NT][2];
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) q[i][c] = lds16(q_sm + ((i * G + k) * 2 + c) * 512 + lane * 16);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const uint32_t at = src + u * 16 * ROW + (kx ^ (32 * k));
-        const uint2 x = lds8(at), y = lds8(at + 8 * ROW);
-        float f0 = 0.f, f1 = 0.f;   // factors, by 2^-8: their bits as fp16's
-        if (k < groups) {
-          const uint32_t fa = k_rec + u * record + 64 + 16 * k + kkey;
-          const uint32_t two = (lds1(fa) | lds1(fa + 8) << 16) << 7;
-          const float2 f = unpack2<__half>(two);
-          f0 = f.x;
-          f1 = f.y;
-        }
+      for (int k = 0; k < G; ++k) {
+        uint4 q[NT][2];
+        float4 start[NT];
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          float acc[4];
+          start[i] = start_s[i][k][t];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) q[i][c] = lds16(q_sm + ((i * G + k) * 2 + c) * 512 + lane * 16);
+        }
+        uint2 kc[U], kd[U];
+        float2 f[U];   // factors, by 2^-8: their bits as fp16's
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const uint32_t at = src + u * 16 * ROW + (kx ^ (32 * k)), fa = k_rec + u * REC + 64 + 16 * k + kkey;
+          kc[u] = lds8(at);
+          kd[u] = lds8(at + 8 * ROW);
+          f[u] = unpack2<__half>((lds1(fa) | lds1(fa + 8) << 16) << 7);
+        }
+        // the tiles side by side: a sum's next MMA does not wait for the one before
+        float acc[U][NT][4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            uint32_t a0, a1, a2, a3;
+            two_codes(c & 1, c & 2 ? kc[u].y : kc[u].x, a0, a2);
+            two_codes(c & 1, c & 2 ? kd[u].y : kd[u].x, a1, a3);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+              const uint32_t b0 = c & 1 ? q[i][c >> 1].z : q[i][c >> 1].x, b1 = c & 1 ? q[i][c >> 1].w : q[i][c >> 1].y;
+              if (c == 0) mma(acc[u][i], a0, a1, a2, a3, b0, b1, start[i].x, start[i].y, start[i].z, start[i].w);
+              else mma(acc[u][i], a0, a1, a2, a3, b0, b1);
+            }
+          }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const float by = c < 2 ? f[u].x : f[u].y;
+              s[u][i][c] = k ? fmaf(acc[u][i][c], by, s[u][i][c]) : acc[u][i][c] * by;
+            }
+      }
+      float vs[U][2];   // V's row scales
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float ks[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t at = u * REC + 4 * (kkey + 8 * e);
+          ks[e] = lds_f32(k_rec + at);
+          vs[u][e] = lds_f32(v_rec + at);
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[u][i][c] = s[u][i][c] * 4294967296.f * (sc[i][c & 1] * ks[c >> 1]);   // 2^24 of the codes, 2^8 of the factors
+      }
+      // ---- masks
+      const int k0 = s0 + n * S::kKeys + warp * U * 16;
+      const uint32_t gone = *reinterpret_cast<volatile uint32_t*>(&gone_s[st]);
+      uint32_t hidden = 0;   // the masked ones of this lane's weights
+      if (!(k0 >= all_lo && k0 + 16 * U <= all_hi && !gone)) {
+        static_assert(U * NT * 4 <= 32, "bits of hidden");
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int left = (gone >> (16 * (warp * U + u) / box_keys)) & 1 ? 0 : s1 - k0 - 16 * u;   // keys of the tile that there are
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (kkey + 8 * e >= left) vs[u][e] = 0.f;   // what lies past them is no scale
+#pragma unroll
+          for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int key = kkey + 8 * (c >> 1), p = k0 + 16 * u + key;
+              if (key >= left || p < klo[i][c & 1] || p >= khi[i][c & 1]) {
+                s[u][i][c] = -INFINITY;
+                hidden |= 1u << ((u * NT + i) * 4 + c);
+              }
+            }
+          // nor a factor: 0 * NaN would not be 0 (a group's 16 in the lanes 4 k .. 4 k + 3)
+          if (lane < 4 * G) {
+            const uint32_t at = v_rec + u * REC + 64 + 4 * lane;
+            const int in = left - 4 * (lane & 3);
+            if (in < 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(in > 0 ? lds4(at) & ((1u << (8 * in)) - 1) : 0u) : "memory");
+          }
+        }
+        fence_proxy_async();   // ahead of the copy that takes this place next
+        __syncwarp();
+      }
+      // ---- the running maximum, and the V scale that weights are relative to
+      bool high = false;
+      float vlow = INFINITY;   // what every row's vref covers
+#pragma unroll
+      for (int i = 0; i < NT; ++i) vlow = fminf(vlow, fminf(vref[i][0], vref[i][1]));
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        high |= vs[u][0] > vlow || vs[u][1] > vlow;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) high |= s[u][i][c] > m[i][c & 1] + (8.f + kLift);
+      }
+      if (__any_sync(0xffffffffu, high)) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const uint32_t xw = c ? x.y : x.x, yw = c ? y.y : y.x, xs = xw >> 8, ys = yw >> 8;
-            const float s0_ = start[i][k][0], s1_ = start[i][k][1];
-            if (c == 0) mma(acc, xw & kLow, yw & kLow, xw & kHigh, yw & kHigh, q[i][c].x, q[i][c].y, s0_, s1_, s0_, s1_);
-            else mma(acc, xw & kLow, yw & kLow, xw & kHigh, yw & kHigh, q[i][c].x, q[i][c].y);
-            mma(acc, xs & kLow, ys & kLow, xs & kHigh, ys & kHigh, q[i][c].z, q[i][c].w);
+            float top = -INFINITY, y = 0.f;   // y: of the keys that the row sees: a hidden one's scale must not cost it bits
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                top = fmaxf(top, s[u][i][c + 2 * e]);
+                if (s[u][i][c + 2 * e] != -INFINITY) y = fmaxf(y, vs[u][e]);
+              }
+#pragma unroll
+            for (int f = 4; f <= 16; f <<= 1) {
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, f));
+              y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, f));
+            }
+            float undo = 1.f;
+            if (y > vref[i][c]) {
+              const float ref = above(y);
+              undo = vref[i][c] / ref;
+              vref[i][c] = ref;
+            }
+            const float mn = fmaxf(m[i][c], top - kLift);
+            const float by = mn == -INFINITY ? 1.f : ex2(m[i][c] - mn);
+            m[i][c] = mn;
+            l[i][c] *= by;
+#pragma unroll
+            for (int j = 0; j < 4 * G; ++j) {
+              o[i][j][c] *= by * undo;
+              o[i][j][c + 2] *= by * undo;
+            }
+            oc[i][c] *= by * undo;
           }
-#pragma unroll
-          for (int c = 0; c < 4; ++c) s[u][i][c] = k ? fmaf(acc[c], c < 2 ? f0 : f1, s[u][i][c]) : acc[c] * (c < 2 ? f0 : f1);
-        }
       }
-    }
-    // ---- scores, masks
-    const int k0 = key_of(n);
-    const uint32_t none = (gone >> (U * n & 31)) & ((1u << U) - 1);
-    const bool whole = k0 >= all_lo && k0 + S::kKeys <= all_hi && k0 + S::kKeys <= s1 && !none;
-    float vs[U][2];
-    bool high = false;
-    float vlow = INFINITY;   // what every row's vref covers
+      // ---- P^T: columns summed, then turned into B fragments
+      uint32_t p0[U][NT], p1[U][NT];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) vlow = fminf(vlow, fminf(vref[i][0], vref[i][1]));
+      for (int i = 0; i < NT; ++i) {
+        // 1 / vref, a power of two (2^127 where no scale but 0 has been seen); m, or 0 while no key has been seen
+        const float vinv[2] = {__int_as_float(0x7f000000 - __float_as_int(vref[i][0])), __int_as_float(0x7f000000 - __float_as_int(vref[i][1]))};
+        const float base[2] = {m[i][0] == -INFINITY ? 0.f : m[i][0], m[i][1] == -INFINITY ? 0.f : m[i][1]};
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float ks[2];
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint32_t at = u * record + 4 * (kkey + 8 * e);
-        ks[e] = lds_f32(k_rec + at);
-        vs[u][e] = lds_f32(v_rec + at);
-        // what lies past the keys, or on a page that does not exist, is no scale
-        if (!whole && (((none >> u) & 1) || k0 + 16 * u + kkey + 8 * e >= s1)) vs[u][e] = 0.f;
-        high |= vs[u][e] > vlow;
-      }
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float v = s[u][i][c] * 4294967296.f * (sc[i][c & 1] * ks[c >> 1]);   // 2^24 of the codes, 2^8 of the factors
-          if (!whole) {
-            const int key = k0 + 16 * u + kkey + 8 * (c >> 1);
-            if (((none >> u) & 1) || key >= s1 || key < klo[i][c & 1] || key >= khi[i][c & 1]) v = -INFINITY;
+          for (int c = 0; c < 4; ++c) {
+            const float p = ex2(s[u][i][c] - base[c & 1]);
+            l[i][c & 1] += p;
+            s[u][i][c] = p * (vs[u][c >> 1] * vinv[c & 1]);
           }
-          s[u][i][c] = v;
-          high |= v > m[i][c & 1] + (8.f + kLift);
-        }
-    }
-    if (__any_sync(0xffffffffu, high)) {
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float x = -INFINITY, y = 0.f;   // y: of the keys that the row sees: a hidden one's scale must not cost it bits
+        if (hidden) {   // a masked key's scale may be anything: 0 * inf, 0 * NaN
 #pragma unroll
           for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              x = fmaxf(x, s[u][i][c + 2 * e]);
-              if (s[u][i][c + 2 * e] != -INFINITY) y = fmaxf(y, vs[u][e]);
+            for (int c = 0; c < 4; ++c)
+              if (hidden >> ((u * NT + i) * 4 + c) & 1) s[u][i][c] = 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          p0[u][i] = transpose8x8(pack2<__half>(s[u][i][0], s[u][i][1]));
+          p1[u][i] = transpose8x8(pack2<__half>(s[u][i][2], s[u][i][3]));
+        }
+      }
+      // ---- O^T += V^T P^T, P times the group's factors
+#pragma unroll
+      for (int k = 0; k < G; ++k) {
+        const uint4 ones = lds16(su32(&ones_s[g == k ? 0 : 1]));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const uint32_t fa = v_rec + u * REC + 64 + 16 * k + vword;
+          const uint32_t f01 = factors_f16(__byte_perm(lds4(fa), 0, vsel)), f89 = factors_f16(__byte_perm(lds4(fa + 8), 0, vsel));
+          const uint32_t at = src + S::kHalf + u * 16 * ROW, b0 = at + (vx[0] ^ (32 * k)), b1 = at + (vx[1] ^ (32 * k));
+          const uint32_t w0 = lds4(b0), w1 = lds4(b1), w2 = lds4(b0 + 8 * ROW), w3 = lds4(b1 + 8 * ROW);
+          uint32_t f0[NT], f1[NT];
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            f0[i] = hmul2(p0[u][i], f01);
+            f1[i] = hmul2(p1[u][i], f89);
+            mma(oc[i], ones.x, ones.y, ones.z, ones.w, f0[i], f1[i]);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {   // values 2 j and 2 j + 1 of each lane's 8
+            uint32_t y = __byte_perm(w0, w1, j < 2 ? 0x5410 : 0x7632), z = __byte_perm(w2, w3, j < 2 ? 0x5410 : 0x7632);
+            if (j & 1) {   // the odd bytes: their high codes with the low ones
+              y = __byte_perm(y, 0, 0x4341);
+              z = __byte_perm(z, 0, 0x4341);
             }
 #pragma unroll
-          for (int f = 4; f <= 16; f <<= 1) {
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, f));
-            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, f));
+            for (int i = 0; i < NT; ++i) mma(o[i][4 * k + j], y & kLow, j & 1 ? y : y & kHigh, z & kLow, j & 1 ? z : z & kHigh, f0[i], f1[i]);
           }
-          float undo = 1.f;
-          if (y > vref[i][c]) {
-            const float ref = above(y);
-            undo = vref[i][c] / ref;
-            vref[i][c] = ref;
-          }
-          const float mn = fmaxf(m[i][c], x - kLift);
-          const float by = mn == -INFINITY ? 1.f : ex2(m[i][c] - mn);
-          m[i][c] = mn;
-          base[i][c] = mn == -INFINITY ? 0.f : mn;
-          l[i][c] *= by;
-#pragma unroll
-          for (int j = 0; j < DP / 16; ++j) {
-            o[i][j][c] *= by * undo;
-            o[i][j][c + 2] *= by * undo;
-          }
-          oc[i][c] *= by * undo;
-        }
-    }
-    step();
-    // ---- P^T: columns summed, then turned into B fragments
-    uint32_t p0[U][NT], p1[U][NT];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        float p[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          p[c] = ex2(s[u][i][c] - base[i][c & 1]);
-          l[i][c & 1] += p[c];
-          const bool hidden = !whole && p[c] == 0.f;   // a masked key's scale may be anything
-          // 1 / vref, a power of two (2^127 where no scale but 0 has been seen)
-          const float vinv = __int_as_float(0x7f000000 - __float_as_int(vref[i][c & 1]));
-          p[c] = hidden ? 0.f : p[c] * (vs[u][c >> 1] * vinv);
-        }
-        p0[u][i] = transpose8x8(pack2<__half>(p[0], p[1]));
-        p1[u][i] = transpose8x8(pack2<__half>(p[2], p[3]));
-      }
-    ok = __all_sync(0xffffffffu, copy_wait(bar0 + 8 * slot, phase));
-    if (!ok) break;
-    src = ring + slot * S::kHalf;
-    // ---- O^T += V^T P^T, P times the group's factors
-#pragma unroll
-    for (int k = 0; k < G; ++k) {
-      if (k >= groups) continue;   // values past D
-      const uint32_t ones = g == k ? 0x00080008u : 0u;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const uint32_t fa = v_rec + u * record + 64 + 16 * k + vword;
-        uint32_t f01 = factors_f16(__byte_perm(lds4(fa), 0, vsel)), f89 = factors_f16(__byte_perm(lds4(fa + 8), 0, vsel));
-        if (!whole) {   // factors past the keys may be anything, and 0 * NaN is not 0
-          const int left = (none >> u) & 1 ? 0 : s1 - (k0 + 16 * u);
-          f01 &= (vkey0 < left ? 0xffffu : 0u) | (vkey1 < left ? 0xffff0000u : 0u);
-          f89 &= (vkey0 + 8 < left ? 0xffffu : 0u) | (vkey1 + 8 < left ? 0xffff0000u : 0u);
-        }
-        const uint32_t at = src + u * 16 * ROW, b0 = at + (vx[0] ^ (32 * k)), b1 = at + (vx[1] ^ (32 * k));
-        const uint32_t w0 = lds4(b0), w1 = lds4(b1), w2 = lds4(b0 + 8 * ROW), w3 = lds4(b1 + 8 * ROW);
-        uint32_t f0[NT], f1[NT];
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          f0[i] = hmul2(p0[u][i], f01);
-          f1[i] = hmul2(p1[u][i], f89);
-          mma(oc[i], ones, 0u, ones, 0u, f0[i], f1[i]);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {   // values 2 j and 2 j + 1 of each lane's 8
-          uint32_t x = __byte_perm(w0, w1, j < 2 ? 0x5410 : 0x7632), y = __byte_perm(w2, w3, j < 2 ? 0x5410 : 0x7632);
-          if (j & 1) {
-            x >>= 8;
-            y >>= 8;
-          }
-#pragma unroll
-          for (int i = 0; i < NT; ++i) mma(o[i][4 * k + j], x & kLow, x & kHigh, y & kLow, y & kHigh, f0[i], f1[i]);
         }
       }
+      __syncwarp();   // the stage is used up
+      if (lane == 0) mbar_arrive(empty0 + 8 * st);
+      if (turn == n + ST && turn < steps) fetch();
     }
-    step();
-  }
-  if (!ok) {   // copies under way have landed before the ring's memory is used for anything else
-    for (int i = max(0, put - S::kSlots); i < put; ++i) copy_wait(bar0 + 8 * (i % S::kSlots), (i / S::kSlots) & 1);
+    done += steps;
+    if (__syncthreads_or(lost)) {   // copies under way have landed before the ring's memory is used for anything else
+      ok = false;
+      if (mine != 0xffffffffu) copy_wait(full0 + 8 * (mine % ST), (mine / ST) & 1);
+      __syncthreads();
 #pragma unroll
-    for (int i = 0; i < NT; ++i) l[i][0] = l[i][1] = __int_as_float(0x7fffffff);   // the rows come out as NaN
-  }
-  __syncthreads();   // every warp is done with its ring: O takes its place
+      for (int i = 0; i < NT; ++i) l[i][0] = l[i][1] = __int_as_float(0x7fffffff);   // the rows come out as NaN
+    } else if (!ok) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) l[i][0] = l[i][1] = __int_as_float(0x7fffffff);
+    }
 
-  // ---- join the warps: maximum, then sums relative to it
+    // ---- join the warps: maximum, then sums relative to it
+    constexpr float kUnit = 16777216.f * kDrop;   // 2^24 of the codes
+    constexpr int LD = S::kWidth;
+    float* acc = reinterpret_cast<float*>(sm);    // [warp][row][64 G + 4]
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      float x = l[i][c];
-      x += __shfl_xor_sync(0xffffffffu, x, 4);
-      x += __shfl_xor_sync(0xffffffffu, x, 8);
-      x += __shfl_xor_sync(0xffffffffu, x, 16);
-      if (g == 0) ml_s[warp][8 * i + 2 * t + c] = make_float2(m[i][c] + kLift, x * kDrop);
-    }
-  float* acc = reinterpret_cast<float*>(sm);   // [warp][row][DP + 4]
-  constexpr int LD = DP + 4;
-#pragma unroll
-  for (int i = 0; i < NT; ++i)
-#pragma unroll
-    for (int k = 0; k < G; ++k)
+    for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const float less = __shfl_sync(0xffffffffu, oc[i][c], 4 * k + t);   // row k, this column
-        const float by = kDrop * vref[i][c];
+        float y = l[i][c];
+        y += __shfl_xor_sync(0xffffffffu, y, 4);
+        y += __shfl_xor_sync(0xffffffffu, y, 8);
+        y += __shfl_xor_sync(0xffffffffu, y, 16);
+        if (g == 0) red[warp][8 * i + 2 * t + c] = make_float2(m[i][c] + kLift, y * kDrop);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int d = 64 * k + 8 * g + 2 * j;
-          float2* dst = reinterpret_cast<float2*>(acc + (warp * NT * 8 + 8 * i + 2 * t + c) * LD + d);
-          *dst = make_float2((o[i][4 * k + j][c] - less) * 16777216.f * by, (o[i][4 * k + j][c + 2] * 0.0625f - less) * 16777216.f * by);
+        for (int k = 0; k < G; ++k) {
+          const float less = __shfl_sync(0xffffffffu, oc[i][c], 4 * k + t);   // row k, this column
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float low = o[i][4 * k + j][c], high = o[i][4 * k + j][c + 2];
+            *reinterpret_cast<float2*>(acc + (warp * NT * 8 + 8 * i + 2 * t + c) * LD + 64 * k + 8 * g + 2 * j) =
+                make_float2((low - less) * kUnit * vref[i][c], ((j & 1 ? high - low : high) * 0.0625f - less) * kUnit * vref[i][c]);
+          }
         }
       }
-  __syncthreads();
-  const int vecs = a.D >> 2;
-  for (int e = threadIdx.x; e < w.rows * vecs; e += blockDim.x) {
-    const int r = e / vecs, d = (e - r * vecs) * 4;
-    float top = -INFINITY, sum = 0.f;
+    __syncthreads();
+#pragma unroll 1
+    for (int e = threadIdx.x; e < w.rows * (16 * G); e += S::kWarps * 32) {
+      const int r = e / (16 * G), d = e % (16 * G) * 4;
+      if (d >= a.D) continue;
+      float top = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int k = 0; k < S::kWarps; ++k) top = fmaxf(top, ml_s[k][r].x);
-    const float base = top == -INFINITY ? 0.f : top;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = 0; k < S::kWarps; ++k) top = fmaxf(top, red[k][r].x);
+      const float base = top == -INFINITY ? 0.f : top;
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int k = 0; k < S::kWarps; ++k) {
-      const float by = ex2(ml_s[k][r].x - base);
-      const float4 y = *reinterpret_cast<const float4*>(acc + (k * NT * 8 + r) * LD + d);
-      sum += ml_s[k][r].y * by;
-      x.x += y.x * by;
-      x.y += y.y * by;
-      x.z += y.z * by;
-      x.w += y.w * by;
+      for (int k = 0; k < S::kWarps; ++k) {
+        const float by = ex2(red[k][r].x - base);
+        const float4 z = *reinterpret_cast<const float4*>(acc + (k * NT * 8 + r) * LD + d);
+        sum += red[k][r].y * by;
+        y.x += z.x * by;
+        y.y += z.y * by;
+        y.z += z.z * by;
+        y.w += z.w * by;
+      }
+      if (alone) {
+        const int row = w.r0 + r;
+        const int64_t at = (int64_t)(w.first + row / a.G) * a.hq + h * a.G + row % a.G;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at * a.D + d) =
+            make_uint2(pack2<T>(y.x * inv, y.y * inv), pack2<T>(y.z * inv, y.w * inv));
+        if (a.lse && d == 0) a.lse[at] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * kLn2;
+      } else {
+        // a block has at most one segment that a pair starts with and does not end with, and one that it goes on with
+        const int64_t at = ((int64_t)blockIdx.x * 2 + (unit0 == 0)) * a.rows_per_block + r;
+        *reinterpret_cast<float4*>(a.part_o + at * a.D + d) = y;
+        if (d == 0) a.part_ml[at] = make_float2(top, sum);
+      }
     }
-    const int row = w.r0 + r;
-    const int64_t at = (int64_t)(w.first + row / a.G) * a.hq + h * a.G + row % a.G;
-    if (alone) {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      const uint2 y = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
-      *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at * a.D + d) = y;
-      if (a.lse && d == 0) a.lse[at] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * kLn2;
-    } else {
-      *reinterpret_cast<float4*>(a.part_o + (at * a.splits + split) * a.D + d) = x;
-      if (d == 0) a.part_ml[at * a.splits + split] = make_float2(top, sum);
+    more = unit0 + take == n_units;   // the pair ends here
+    if (more) {
+      x += n_units + share.start;
+      unit0 = 0;
+      if (++h == a.kv.heads) {
+        h = 0;
+        do ++item; while (item < a.kv.seqs * a.row_blocks && units_of<UNIT>(a, item) == 0);
+      }
+      more = item != end.item || h != end.h || end.k != 0;
     }
+    if (more) {
+      fence_proxy_async();   // the ring's memory goes back to the copies
+      __syncthreads();
+    }
+  }
+  if (a.kv.starts) {   // tokens of no sequence
+    const int first = max(0, min(a.kv.starts[0], a.T)), past = max(first, min(a.kv.starts[a.kv.seqs], a.T));
+    if (first > 0) blank_tokens(a, 0, first, blockIdx.x, gridDim.x);
+    if (past < a.T) blank_tokens(a, past, a.T, blockIdx.x, gridDim.x);
   }
 }
 
-// A pool's codes [rows, D / 2] as boxes of `keys` rows x DP / 2 bytes, swizzled over the row; bytes past D / 2 read as zeros.
-bool make_code_map(CUtensorMap* map, const void* base, const AttnArgs& a, int DP, int keys) {
+// Joins the segments of a row (token, head) that has more than one: a block takes 4 * LANES of its values, LANES threads of
+// them for each of 256 / LANES shares of the segments; the shares are then added in order.
+template <typename T, int LANES>
+__global__ void __launch_bounds__(256) attn_join4_kernel(const __grid_constant__ AttnArgs a) {
+  __shared__ float4 acc[256];
+  __shared__ float red[8], sum_s[256 / LANES];
+  // Of what is read ahead of the wait nothing is written by the launch before, and that one has waited for all before it.
+  const int t = blockIdx.x, hq = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = sequence_of(a.kv, t);
+  int64_t row = -1, pair = 0;
+  if (b >= 0) {
+    row = (int64_t)(t - attn_rows(a, b, 0).first) * a.G + hq % a.G;
+    if (row >= (int64_t)a.row_blocks * a.rows_per_block) row = -1;   // past max_new
+  }
+  int r = 0;
+  if (row >= 0) {
+    const int rb = (int)row / a.rows_per_block;
+    r = (int)row - rb * a.rows_per_block;
+    if (r >= attn_rows(a, b, rb).rows) row = -1;
+    pair = ((int64_t)b * a.row_blocks + rb) * a.kv.heads + hq / a.G;
+  }
+  pdl_wait();   // by every block: what follows this launch takes its end for the end of the one before too
+  pdl_trigger();
+  if (row < 0) return;
+  const int2 seg = a.segments[pair];
+  if (seg.y <= 1) return;   // written already
+  // part of segment i: the first one's is its block's second
+  auto part = [&](int i) { return ((int64_t)(seg.x + i) * 2 + (i == 0)) * a.rows_per_block + r; };
+  float top = -INFINITY;
+  for (int i = threadIdx.x; i < seg.y; i += 256) top = fmaxf(top, a.part_ml[part(i)].x);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) red[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 8; ++k) top = fmaxf(top, red[k]);
+  const float base = top == -INFINITY ? 0.f : top;
+  constexpr int kShares = 256 / LANES;
+  const int share = threadIdx.x / LANES, d = 4 * (blockIdx.z * LANES + threadIdx.x % LANES);
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+#pragma unroll 4
+  for (int i = share; i < seg.y; i += kShares) {
+    const int64_t p = part(i);
+    const float2 ml = a.part_ml[p];
+    const float by = ex2(ml.x - base);
+    sum += ml.y * by;
+    if (d < a.D) {
+      const float4 z = *reinterpret_cast<const float4*>(a.part_o + p * a.D + d);
+      y.x += z.x * by;
+      y.y += z.y * by;
+      y.z += z.z * by;
+      y.w += z.w * by;
+    }
+  }
+  acc[threadIdx.x] = y;
+  if (threadIdx.x % LANES == 0) sum_s[share] = sum;
+  __syncthreads();
+  if (share) return;
+  sum = sum_s[0];
+#pragma unroll
+  for (int k = 1; k < kShares; ++k) {
+    sum += sum_s[k];
+    const float4 z = acc[LANES * k + threadIdx.x];
+    y.x += z.x;
+    y.y += z.y;
+    y.z += z.z;
+    y.w += z.w;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int64_t at = (int64_t)t * a.hq + hq;
+  if (d < a.D)
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at * a.D + d) =
+        make_uint2(pack2<T>(y.x * inv, y.y * inv), pack2<T>(y.z * inv, y.w * inv));
+  if (a.lse && d == 0) a.lse[at] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * kLn2;
+}
+
+// A pool's codes [rows, D / 2] as boxes of `keys` rows x `row` bytes, swizzled over the row; bytes past D / 2 read as zeros.
+bool make_code_map(CUtensorMap* map, const void* base, const AttnArgs& a, int row, int keys) {
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(a.D / 2), (static_cast<cuuint64_t>(a.kv.pages) * a.kv.heads) << a.kv.page_log2};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(a.D / 2)};
-  const cuuint32_t boxes[2] = {static_cast<cuuint32_t>(DP / 2), static_cast<cuuint32_t>(keys)};
+  const cuuint32_t boxes[2] = {static_cast<cuuint32_t>(row), static_cast<cuuint32_t>(keys)};
   const cuuint32_t es[2] = {1, 1};
   return encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, boxes, es,
                      CU_TENSOR_MAP_INTERLEAVE_NONE,
-                     DP == 256 ? CU_TENSOR_MAP_SWIZZLE_128B : DP == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                     row == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : row == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE,
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DP, int NT, typename T>
-int launch(const AttnArgs& a, cudaStream_t st) {
-  using S = Shape4<DP, NT>;
-  auto kern = attn_decode4_kernel<DP, NT, T>;
+template <int G, int NT, typename T>
+int launch(AttnArgs a, cudaStream_t st) {
+  using S = Shape4<G, NT>;
+  auto kern = attn_decode4_kernel<G, NT, T>;
   static std::atomic<uint64_t> done{0};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -607,52 +896,71 @@ int launch(const AttnArgs& a, cudaStream_t st) {
     }
     done.fetch_or(bit);
   }
-  const dim3 grid((unsigned)(a.kv.seqs * a.row_blocks), (unsigned)a.splits, (unsigned)a.kv.heads);
   CUtensorMap kmap, vmap;
   const int keys = S::kKeys < 1 << a.kv.page_log2 ? S::kKeys : 1 << a.kv.page_log2;
-  if (!make_code_map(&kmap, a.kv.k, a, DP, keys) || !make_code_map(&vmap, a.kv.v, a, DP, keys)) return VQ2_ERR_LAUNCH;
-  return launch_kernel(kern, grid, dim3(S::kWarps * 32), S::kSmem, st, a, kmap, vmap);
+  a.lo_mask = ~(keys - 1);   // a box lies in a page
+  if (!make_code_map(&kmap, a.kv.k, a, S::kRow, keys) || !make_code_map(&vmap, a.kv.v, a, S::kRow, keys)) return VQ2_ERR_LAUNCH;
+  return launch_kernel(kern, dim3((unsigned)a.blocks), dim3(S::kWarps * 32), S::kSmem, st, a, kmap, vmap);
+}
+
+// f(shape, groups, row tiles) of the variant for `a`.
+template <typename F>
+auto with_shape(const AttnArgs& a, F f) {
+  using std::integral_constant;
+  auto rows = [&](auto groups) {
+    return a.rows_per_block == 8 ? f(groups, integral_constant<int, 1>()) : f(groups, integral_constant<int, 2>());
+  };
+  if (a.D > 192) return rows(integral_constant<int, 4>());
+  if (a.D > 128) return rows(integral_constant<int, 3>());
+  return a.D > 64 ? rows(integral_constant<int, 2>()) : rows(integral_constant<int, 1>());
 }
 
 template <typename T>
 int launch_shape(const AttnArgs& a, cudaStream_t st) {
-  const int nt = a.rows_per_block / 8;
-  if (a.D > 128) return nt == 1 ? launch<256, 1, T>(a, st) : launch<256, 2, T>(a, st);
-  if (a.D > 64) return nt == 1 ? launch<128, 1, T>(a, st) : launch<128, 2, T>(a, st);
-  return nt == 1 ? launch<64, 1, T>(a, st) : launch<64, 2, T>(a, st);
+  return with_shape(a, [&](auto g, auto nt) { return launch<decltype(g)::value, decltype(nt)::value, T>(a, st); });
 }
 
 }  // namespace
 
 void plan_attn_decode4(AttnArgs& a, int64_t max_new, int64_t max_len) {
-  // As plan_attn_decode, in pieces of 64 keys: a step's, which a page holds whole or in whole parts.
   const int64_t rows = max_new * a.G;
   const int nt = rows <= 8 ? 1 : 2;
   a.rows_per_block = 8 * nt;
   a.row_blocks = (int)((rows + 8 * nt - 1) / (8 * nt));
   if (a.row_blocks < 1) a.row_blocks = 1;
-  a.lo_mask = ~63;
-  const int64_t step = a.D > 128 ? 128 : 256;
+  a.splits = 1;
+  a.chunk = 0x7fffffff;
+  int unit = 0, per_sm = 0;
+  with_shape(a, [&](auto g, auto nt) {
+    using S = Shape4<decltype(g)::value, decltype(nt)::value>;
+    unit = S::kKeys;
+    per_sm = S::kPerSm;
+    return 0;
+  });
   int64_t keys = max_len;
-  if (a.window && a.window + max_new + 64 < keys) keys = a.window + max_new + 64;
-  keys += 63;   // the first key is rounded down by up to 63
-  const int64_t blocks = (int64_t)a.kv.seqs * a.kv.heads * a.row_blocks;
-  const int64_t fill = (keys * blocks * 2 + 3 * sm_count() - 1) / (3 * sm_count());
-  int64_t chunk = fill < 768 ? fill : 768;
-  const int64_t least = (keys + 63) / 64 < fill ? (keys + 63) / 64 : fill;
-  if (chunk < least) chunk = least;
-  if (chunk < step) chunk = step;
-  if (chunk < (keys + 255) / 256) chunk = (keys + 255) / 256;   // what the joining kernel takes
-  if (keys <= 2 * step + 63) chunk = keys;
-  chunk = (chunk + 63) & ~int64_t(63);
-  a.chunk = (int)chunk;
-  a.splits = (int)((keys + chunk - 1) / chunk);
-  if (a.splits < 1) a.splits = 1;
+  if (a.window && a.window + max_new < keys) keys = a.window + max_new;
+  // the first key is rounded down by less than a unit
+  const int64_t units = (keys + unit - 2) / unit + 1, pairs = (int64_t)a.kv.seqs * a.row_blocks * a.kv.heads;
+  const int64_t room = (int64_t)sm_count() * per_sm;
+  a.blocks = (int)(pairs >= room || units >= room || pairs * units >= room ? room : pairs * units);
+  // Two units stay whole: a joining launch and two starts cost more than they take (see the figures above). Where none is
+  // longer, by the caller's bounds, nothing is split and no joining launch follows.
+  a.whole = units <= 2 ? 0x7fffffff : 2;
 }
 
 int launch_attn_decode4(const AttnArgs& a, cudaStream_t st) {
   if (!encode_fn()) return VQ2_ERR_LAUNCH;
-  return a.q_bf16 ? launch_shape<__nv_bfloat16>(a, st) : launch_shape<__half>(a, st);
+  const int s = a.q_bf16 ? launch_shape<__nv_bfloat16>(a, st) : launch_shape<__half>(a, st);
+  if (s != VQ2_OK || a.whole == 0x7fffffff) return s;
+  // Few rows of many segments: 64 values a block, 16 segments read at once; else whole rows.
+  const int lanes = (int64_t)a.T * a.hq < 2 * sm_count() || a.D <= 64 ? 16 : a.D <= 128 ? 32 : 64;
+  const dim3 grid((unsigned)a.T, (unsigned)a.hq, (unsigned)((a.D + 4 * lanes - 1) / (4 * lanes)));
+  auto join = [&](auto type) {
+    using T = decltype(type);
+    return launch_kernel(lanes == 16 ? attn_join4_kernel<T, 16> : lanes == 32 ? attn_join4_kernel<T, 32> : attn_join4_kernel<T, 64>,
+                         grid, dim3(256), 0, st, a);
+  };
+  return a.q_bf16 ? join(__nv_bfloat16()) : join(__half());
 }
 
 int attn_decode4_status(int reset) {

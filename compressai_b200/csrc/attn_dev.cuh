@@ -22,6 +22,10 @@ struct AttnArgs {
   int chunk, splits, rows_per_block, row_blocks, lo_mask;
   float* part_o;        // [T * hq, splits, D]: weighted sums of V relative to the maximum
   float2* part_ml;      // [T * hq, splits]: (maximum score in powers of two, sum of weights)
+  // 4-bit cache, few rows: blocks of the launch, each with two parts of rows_per_block rows; for each (block of rows, head)
+  // the first block that has it and how many have. whole: units of keys that are not split.
+  int blocks, whole;
+  int2* segments;       // [seqs * row_blocks, heads]
   // 8-bit and 4-bit caches, many rows: the visible keys and values as fp16 [seqs, heads, wide_len, D], their scales
   void *wide_k, *wide_v;
   float *wide_ks, *wide_vs;

@@ -436,6 +436,23 @@ def test_sizes_of_q_and_v(scale_of, new):
     assert torch.isfinite(got).all() and ((got - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("new", [1, 20])
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 128), (4, 1, 256), (16, 1, 64)])
+def test_scales_of_hidden_keys(hq, hkv, d, new):
+    """What a window or a later position hides has no say, whatever the size of its values beside those of the keys seen."""
+    window, l = 30, 300
+    s = Setup([new], [l], hq, hkv, d, torch.bfloat16, page=256, seed=4)
+    for which, seen in ((0, 1.0), (1, 2.0 ** -90)):
+        x = torch.randn(s.pools[which].shape[0], hkv, 256, d, generator=gen(which), device=DEV)
+        pos = torch.full((x.shape[0], 256), -1, device=DEV)
+        for j in range(2):
+            pos[s.table[0, j].long()] = torch.arange(256 * j, 256 * j + 256, device=DEV)
+        last = l - new - window + 1   # positions that no row sees
+        x *= torch.where(pos < last, 2.0 ** (100 if which else 30), torch.where(pos < l, seen, 2.0 ** 90))[:, None, :, None]
+        fill(s.pools[which], s.scales[which], x.to(torch.bfloat16))
+    s.check(s.run(window=window, max_new=new), window=window)
+
+
 def test_graph_streams_and_strides():
     s = Setup([1, 1, 1], [100, 300, 17], 8, 2, 128, torch.bfloat16, page=16, seed=1)
     want = s.run(starts=None, max_len=400)
