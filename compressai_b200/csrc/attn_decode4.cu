@@ -297,6 +297,8 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
   __shared__ uint4 ones_s[2];                   // A of the MMA that sums a group's weights, in the row of its number and in others
   __shared__ Place ends[2];
   __shared__ int64_t sums[8];
+  if (threadIdx.x < 2)   // constant: ahead of the wait
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(threadIdx.x ? &vmap : &kmap)) : "memory");
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;

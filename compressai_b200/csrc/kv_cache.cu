@@ -13,7 +13,7 @@
 // memory, behind the value loads already in flight.
 #include <type_traits>
 
-#include "kv_dev.cuh"
+#include "kv4_dev.cuh"
 
 namespace vq2 {
 namespace {
@@ -99,13 +99,6 @@ __device__ __forceinline__ uint4 narrow8(const float (&f)[8]) {
   for (int i = 0; i < 8; ++i) t[i] = from_f32<T>(f[i]);
   uint4 r;
   memcpy(&r, t, 16);
-  return r;
-}
-
-// Maximum that a NaN passes through.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 
@@ -204,30 +197,6 @@ __device__ __forceinline__ uint2 quantise8(const float (&f)[8], bool mine, int l
   return make_uint2(o[0], o[1]);
 }
 
-// A 4-bit group's factor (e4m3, as a byte and as a number): its largest magnitude over the row's, rounded up so that
-// no value passes 7 steps. 2^-9 at least unless the group is 0.
-__device__ __forceinline__ uint32_t factor_of(float group, float row, float& u) {
-  const float r = __fdiv_rn(group, row);
-  const uint32_t b = r >= 0.015625f ? ((__float_as_uint(r) + 0xfffffu) >> 20) - 960u : (uint32_t)ceilf(r * 512.f);
-  u = e4m3_value(b);
-  return b;
-}
-
-// What turns a value of such a group into its code, -7..7. The nearest integer to 7 x / (row * u), a tie away from
-// zero: a share of 2^-20 more lifts every tie, and no quotient of 16-bit values (a tie is 2^-16 away if it is not
-// met) over it, so that one multiplication rounds as an exact division would.
-__device__ __forceinline__ float steps_per_one(float row, float u) {
-  return u == 0.f ? 0.f : __fdiv_rn(7.f + 7.f / 1048576.f, __fmul_rn(row, u));
-}
-
-// Four codes, plus 8, in the low half of the result.
-__device__ __forceinline__ uint32_t codes4(const float* f, float per) {
-  uint32_t r = 0;   // adding 1.5 * 2^23 + 8 rounds to an integer and leaves it in the low bits
-#pragma unroll
-  for (int j = 0; j < 4; ++j) r |= (__float_as_uint(__fadd_rn(__fmul_rn(f[j], per), 12582920.f)) & 15u) << (4 * j);
-  return r;
-}
-
 struct Row4 {
   uint32_t codes;   // of the lane's 8 values
   float scale;      // of the row
@@ -270,27 +239,23 @@ __device__ __forceinline__ Row4 quantise4(const float (&f)[8], bool mine, int la
     for (int o = 8; o < lanes; o <<= 1) row = max_nan(row, __shfl_xor_sync(0xffffffffu, row, o));
   }
   Row4 r = {0x88888888u, 0.f};   // zeros
-  const bool bad = !(row < INFINITY), some = !bad && row >= 1e-30f;
-  if (bad) r.scale = __uint_as_float(0x7fc00000u);
-  if (some) {
-    r.scale = __fdiv_rn(row, 7.f);
-    float u0, u1;
-    const uint32_t b0 = factor_of(of0, row, u0);
-    if (SPLIT) {
-      factor_of(of1, row, u1);
+  uint32_t byte;
+  const float per0 = quantiser4(of0, row, byte, r.scale);
+  if (SPLIT) {
+    uint32_t other;
+    float same;
+    const float per1 = quantiser4(of1, row, other, same);
+    const float g[8] = {f[0] * per0, f[1] * per0, f[2] * per0, f[3] * per0, f[4] * per1, f[5] * per1, f[6] * per1, f[7] * per1};
+    r.codes = row >= 1e-30f && row < INFINITY ? codes8(g, 1.f) : r.codes;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        float u;
-        if (g < groups && lane == g) put(g, factor_of(of[g], row, u));
+    for (int k = 0; k < 4; ++k)
+      if (k < groups && lane == k) {
+        quantiser4(of[k], row, other, same);
+        put(k, other);
       }
-      r.codes = codes4(f, steps_per_one(row, u0)) | codes4(f + 4, steps_per_one(row, u1)) << 16;
-    } else {
-      if (!(lane & 7)) put(g0, b0);
-      const float per = steps_per_one(row, u0);
-      r.codes = codes4(f, per) | codes4(f + 4, per) << 16;
-    }
-  } else if (SPLIT ? lane < groups : !(lane & 7)) {
-    put(SPLIT ? lane : g0, bad ? 0x38u : 0u);   // a finite factor beside a scale of NaN
+  } else {
+    if (per0 != 0.f) r.codes = codes8(f, per0);
+    if (!(lane & 7)) put(g0, byte);
   }
   return r;
 }
@@ -506,16 +471,7 @@ __global__ void __launch_bounds__(kRopeThreads) cache_read_kernel(const ReadArgs
     const int64_t slot = slot_of(a.kv, b, t - a.kv.starts[b]);
     if (slot < 0) continue;
     const int64_t row = pool_row(a.kv, slot, h), e = row * a.D + i0;
-    if (BITS == 4) {
-      const Scale4 places(a.D);
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint8_t* scales = reinterpret_cast<const uint8_t*>(c ? a.kv.v_scale : a.kv.k_scale);
-        x[n][c].x = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(c ? a.kv.v : a.kv.k) + (e >> 1));
-        x[n][c].y = scales[places.factor(row, i0 >> 6)];
-        s[n][c] = *reinterpret_cast<const float*>(scales + places.row(row));
-      }
-    } else if (BITS == 8) {
+    if (BITS == 8) {
       const uint2 k = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(a.kv.k) + e);
       const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(a.kv.v) + e);
       x[n][0] = make_uint4(k.x, k.y, 0, 0);
@@ -534,13 +490,7 @@ __global__ void __launch_bounds__(kRopeThreads) cache_read_kernel(const ReadArgs
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       uint4 y = x[n][c];
-      if (BITS == 4) {
-        const float step = e4m3_value(x[n][c].y) * s[n][c];
-        float f[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = (float)((int)(x[n][c].x >> (4 * j) & 15) - 8) * step;
-        y = narrow8<T>(f);
-      } else if (BITS == 8) {
+      if (BITS == 8) {
         float f[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = (float)(int8_t)((&x[n][c].x)[j >> 2] >> (8 * (j & 3))) * s[n][c];
@@ -654,6 +604,8 @@ extern "C" int vq2_cache_write(const void* q, int64_t q_token_stride, int64_t q_
   a.D = (int)head_size;
   a.lanes_log2 = lanes_log2(a.D);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (kv_dtype == VQ2_I4 && !inv_freq && !q_heads)
+    return launch_store4(a.kv, k, k_token_stride, k_head_stride, v, v_token_stride, v_head_stride, dtype == VQ2_F16, tokens, head_size, st);
   if (kv_dtype == VQ2_I4)
     return dtype == VQ2_F16 ? launch_rope<__half, 3>(a, tokens, st) : launch_rope<__nv_bfloat16, 3>(a, tokens, st);
   if (kv_dtype == VQ2_I8)
@@ -676,6 +628,7 @@ extern "C" int vq2_cache_read(const void* k_pages, const void* v_pages, int kv_d
   if (total < 0 || total > 0x7fffffff) return VQ2_ERR_SHAPE;
   if (!aligned(k_out, 16) || !aligned(v_out, 16)) return VQ2_ERR_ALIGN;
   if (total == 0) return VQ2_OK;
+  if (kv_dtype == VQ2_I4) return launch_load4(a.kv, k_out, v_out, out_dtype == VQ2_F16, total, head_size, static_cast<cudaStream_t>(stream));
   a.k_out = k_out;
   a.v_out = v_out;
   a.total = total;
@@ -688,9 +641,6 @@ extern "C" int vq2_cache_read(const void* k_pages, const void* v_pages, int kv_d
   const dim3 grid((unsigned)blocks), block(kRopeThreads);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool half = out_dtype == VQ2_F16;
-  if (kv_dtype == VQ2_I4)
-    return half ? launch_kernel(cache_read_kernel<__half, 4, NIT>, grid, block, 0, st, a)
-                : launch_kernel(cache_read_kernel<__nv_bfloat16, 4, NIT>, grid, block, 0, st, a);
   if (kv_dtype == VQ2_I8)
     return half ? launch_kernel(cache_read_kernel<__half, 8, NIT>, grid, block, 0, st, a)
                 : launch_kernel(cache_read_kernel<__nv_bfloat16, 8, NIT>, grid, block, 0, st, a);
