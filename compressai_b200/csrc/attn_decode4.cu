@@ -6,26 +6,41 @@
 //   S^T [16 keys x 8 rows] = K Q^T,   P = 2^(S - m),   O^T [D x 8 rows] += V^T P^T
 //
 // with mma.m16n8k16 and its own running maximum m and sum; warps, and blocks that split a long sequence, are joined at
-// the end. HBM bounds it (half of int8's bytes) as long as the codes become operands in few instructions:
+// the end. HBM bounds it (half of int8's bytes) as long as the codes become operands in few instructions, and they still
+// set the pace: 270 a warp for 16 keys of 128 values, K and V.
 //
 //   * A code's bits c in the low end of a 16-bit float are the number c 2^-24 (and one place of four further up,
-//     16 c 2^-24), exactly: a mask takes two codes out of a word and they are an operand register. Four masks and one
-//     shift serve the 8 codes of a word; no conversion, no subtraction.
+//     16 c 2^-24), exactly: a mask takes two codes out of a word and they are an operand register. The 8 codes of a word take
+//     five integer instructions (which run at half rate) and, for K, a subtraction; no conversion.
 //   * What the 16 stands for is put right where it is free: in K in the queries' operand (half of it is divided by 16),
 //     in V in the rows of O that such codes end in.
 //   * The 8 in every code: K's sums start at -8 sum q, and V's gets -8 sum P of each group at the end, summed by one more
 //     MMA a group into the row of the group's number, from the same rounded weights.
-//   * K's factors multiply a group's sum (4 numbers a lane), V's multiply the weights (2 registers a group): both of
-//     them once for 16 keys x 64 values.
+//   * K's factors multiply a group's sum (4 numbers a lane), V's the weights ahead of their rounding: both of them once for
+//     16 keys x 64 values.
 //
 // Where the codes are: a K operand wants 16 values of a group in the four lanes of a key's row, a V operand 8 in each
 // of the eight lanes g: lane (g, t) reads the 8 bytes t of a group from keys of number g and the 4 bytes g from keys of
 // number 2t, 2t + 1. With TMA's swizzle (none where a row is 32 bytes) all of these reads are free of bank conflicts if the
-// keys are numbered as `key_of_row` does. (4 sequences to 100,003, 32/8 heads of 128, B200.)
+// keys are numbered as `key_of_row` does.
+//
+// A step's K, V and scales (256 keys; 128 for heads above 128) come for the block's four warps together, issued by one thread
+// of the warp whose turn it is, two steps under way. Lengths are ragged and the split of a long sequence is worth a few
+// steps only where blocks are all equally long, so the launch has as many blocks as the card holds at once (3 an SM) and each
+// finds its equal share of all keys from the lengths, see `my_units`.
 //
 // Queries become fp16 by a power of two per row, exact down to 2^-24 of the row's largest value; the weights are fp16,
-// relative to a power of two above the row scales of V that the row sees, and rounded once more with the factor. Maxima,
-// sums and O are 32 bits. Rescaling is lazy, see attn_decode.cu.
+// relative to a power of two above the row scales of V that the row sees. Maxima, sums and O are 32 bits. Rescaling is lazy, see
+// attn_decode.cu.
+//
+// Measured (B200, one graph): 64 sequences of 800 to 8000, 16/2 heads of 256 (154 MB) 48.8 us, 4 sequences to 100,003, 32/8 heads
+// of 128 (372 MB) 86.8. What it took: a warp a row, 32 bits, 1667 and 3483; the MMAs, a ring a warp and splits of 768
+// keys 65.8 and 134; splits of 1536 keys 54 and 109, of 4800 117 and 116; equal shares 71 and 93, with the queries loaded ahead of
+// the copies and by all warps (6 us a segment before) 57 and 92, with a pair's start counted as two units 48.7 and 85.7. Left out:
+// one tile less a warp and step for 4 blocks an SM (58 and 98.7: spills, and a step's fixed cost), four steps under way (53 and
+// 95), P through shared memory and a group of O a warp (66 and 114: two barriers' waits), the last warp done with a step
+// fetching the next (49 and 92), groups and tiles in rolled loops (73 and 120). Pages of 16 keys instead of 256: 102 and 79 us
+// at the second (16 times the copies).
 #include <atomic>
 #include <type_traits>
 
@@ -71,19 +86,6 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// The same value in a register of its own: an MMA takes its operands from registers in a row, and would have equal ones
-// copied there each time.
-__device__ __forceinline__ float apart(float v) {
-  float r;
-  asm volatile("mov.b32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-__device__ __forceinline__ uint32_t apart(uint32_t v) {
-  uint32_t r;
-  asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(v));
-  return r;
-}
-
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -116,11 +118,6 @@ __device__ __forceinline__ uint32_t factors_f16(uint32_t w) {
   asm("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(w));
   return r;
 }
-__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
-  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-
 // Shapes of one variant. G: groups of a row (codes past D are zeros); NT: 8-row tiles.
 template <int G, int NT>
 struct Shape4 {
@@ -325,8 +322,6 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
   };
   const int kkey = key_of_row<ROW>(g), vkey0 = key_of_row<ROW>(2 * t), vkey1 = key_of_row<ROW>(2 * t + 1);
   const uint32_t kx = swizzled(kkey, 8 * t), vx[2] = {swizzled(vkey0, 4 * g), swizzled(vkey1, 4 * g)};
-  // the factors of V's two keys out of the four bytes that both are in
-  const uint32_t vword = vkey0 & 4, vsel = (uint32_t)(vkey0 & 3) | (uint32_t)(vkey1 & 3) << 4;
   uint32_t done = 0;              // steps of the segments so far
   uint32_t mine = 0xffffffffu;    // the last step that this warp fetched
   bool lost = false, ok = true;   // a wait of this warp, none of the block's has given up
@@ -640,8 +635,7 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
             oc[i][c] *= by * undo;
           }
       }
-      // ---- P^T: columns summed, then turned into B fragments
-      uint32_t p0[U][NT], p1[U][NT];
+      // ---- P^T: columns summed, weights relative to the V scale
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         // 1 / vref, a power of two (2^127 where no scale but 0 has been seen); m, or 0 while no key has been seen
@@ -662,27 +656,23 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
             for (int c = 0; c < 4; ++c)
               if (hidden >> ((u * NT + i) * 4 + c) & 1) s[u][i][c] = 0.f;
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          p0[u][i] = transpose8x8(pack2<__half>(s[u][i][0], s[u][i][1]));
-          p1[u][i] = transpose8x8(pack2<__half>(s[u][i][2], s[u][i][3]));
-        }
       }
-      // ---- O^T += V^T P^T, P times the group's factors
+      // ---- O^T += V^T P^T. P times the group's factors is rounded once and turned into B fragments: a rounding before and
+      // one after the factor is 1.5 times the error of 32 bits rounded at the end where the output is fp16 (1.4 so; 2 instructions of 88)
 #pragma unroll
       for (int k = 0; k < G; ++k) {
         const uint4 ones = lds16(su32(&ones_s[g == k ? 0 : 1]));
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const uint32_t fa = v_rec + u * REC + 64 + 16 * k + vword;
-          const uint32_t f01 = factors_f16(__byte_perm(lds4(fa), 0, vsel)), f89 = factors_f16(__byte_perm(lds4(fa + 8), 0, vsel));
+          const uint32_t fa = v_rec + u * REC + 64 + 16 * k;
+          const float2 f = unpack2<__half>(factors_f16(lds1(fa + kkey) | lds1(fa + kkey + 8) << 8));
           const uint32_t at = src + S::kHalf + u * 16 * ROW, b0 = at + (vx[0] ^ (32 * k)), b1 = at + (vx[1] ^ (32 * k));
           const uint32_t w0 = lds4(b0), w1 = lds4(b1), w2 = lds4(b0 + 8 * ROW), w3 = lds4(b1 + 8 * ROW);
           uint32_t f0[NT], f1[NT];
 #pragma unroll
           for (int i = 0; i < NT; ++i) {
-            f0[i] = hmul2(p0[u][i], f01);
-            f1[i] = hmul2(p1[u][i], f89);
+            f0[i] = transpose8x8(pack2<__half>(s[u][i][0] * f.x, s[u][i][1] * f.x));
+            f1[i] = transpose8x8(pack2<__half>(s[u][i][2] * f.y, s[u][i][3] * f.y));
             mma(oc[i], ones.x, ones.y, ones.z, ones.w, f0[i], f1[i]);
           }
 #pragma unroll
