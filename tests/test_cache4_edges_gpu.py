@@ -247,13 +247,12 @@ def test_refusals():
         A.paged_attention(s.q, s.pools[0], s.pools[1].to(torch.int8), s.table, s.lens, **kw)
 
 
-@pytest.mark.parametrize("dtype", [torch.int4])
-def test_the_stack_decodes_on_it(dtype):
+def test_the_stack_decodes_on_it():
     """Greedy decode of the small stack twice: the same ids, every page back."""
     from compressai_b200 import stack
     from test_stack_paged_gpu import small_model
     model = small_model(5)
-    cache = stack.use_paged_attention(model, pages=8, page_size=16, dtype=dtype)
+    cache = stack.use_paged_attention(model, pages=8, page_size=16, dtype=torch.int4)
     t1, ids1 = stack.decode(model, batch=3, prompt_len=20, steps=3, warmup=1, seed=9, cache=cache)
     t2, ids2 = stack.decode(model, batch=3, prompt_len=20, steps=3, warmup=1, seed=9, cache=cache)
     assert t1 > 0 and torch.equal(ids1, ids2) and len(cache.free) == 8 and not cache.pages

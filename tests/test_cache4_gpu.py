@@ -405,16 +405,16 @@ def test_pages_that_do_not_exist_hide_their_keys(new):
 
 def test_a_row_that_is_not_finite():
     """Its NaN reaches the rows that see it, and those alone."""
-    d, T = 64, 40
+    d, T = 64, 200
     pools, table, lens, starts = one_sequence(T, 1, d, 16)
     x = torch.randn(T, 1, d, generator=gen(0), device=DEV).half()
-    x[30, 0, 3] = math.inf
+    x[150, 0, 3] = math.inf
     A.cache_write(x, x, pools[0][0], pools[1][0], table, lens, starts, k_scale=pools[0][1], v_scale=pools[1][1])
     q = torch.randn(T, 1, d, generator=gen(1), device=DEV).half()
-    for lo, hi in ((0, 40), (24, 40)):   # chunk, decode kernel
-        at = torch.tensor([0, hi - lo], dtype=torch.int32, device=DEV)
-        out = A.paged_attention(q[lo:hi], pools[0][0], pools[1][0], table, lens, at, k_scale=pools[0][1], v_scale=pools[1][1])
-        assert torch.equal(out.isnan().any(-1).any(-1), torch.arange(lo, hi, device=DEV) >= 30)
+    for lo in (0, 140, 199):   # the kernel for many rows, for few, one
+        at = torch.tensor([0, T - lo], dtype=torch.int32, device=DEV)
+        out = A.paged_attention(q[lo:], pools[0][0], pools[1][0], table, lens, at, k_scale=pools[0][1], v_scale=pools[1][1])
+        assert torch.equal(out.isnan().any(-1).any(-1), torch.arange(lo, T, device=DEV) >= 150)
 
 
 @pytest.mark.parametrize("scale_of", [2.0 ** -100, 2.0 ** 60])
