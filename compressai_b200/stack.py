@@ -15,8 +15,8 @@ is built without materialising its dense weights, then
   * norms, the DeltaNet convolution / decay parameters and the rotary tables stay the reference's
     PyTorch modules, initialised here.
 
-``use_paged_attention`` then gives the full-attention layers this library's rotary, paged cache (bf16 or
-int8) and attention in place of the transformers cache, and ``decode(..., cache=...)`` decodes with it.
+``use_paged_attention`` then gives the full-attention layers this library's rotary, paged cache (bf16, int8
+or 4-bit) and attention in place of the transformers cache, and ``decode(..., cache=...)`` decodes with it.
 """
 import math
 
@@ -189,7 +189,7 @@ class PagedAttention(nn.Module):
 
 def use_paged_attention(model, pages, page_size=64, max_len=32768, dtype=torch.bfloat16, inv_freq=None, factor=1.0):
     """Replace the model's full-attention layers by PagedAttention over one new PagedKVCache (returned):
-    ``pages`` pages of ``page_size`` tokens, bf16 or int8. A model that has a paged cache already gets the new one in
+    ``pages`` pages of ``page_size`` tokens, bf16, torch.int8 or torch.int4. A model that has a paged cache already gets the new one in
     its place. ``inv_freq``, ``factor``: what attention.rope_frequencies gives, for a model whose configuration
     stretches its context (yarn, llama3, ..); without them the configuration's plain frequencies."""
     cfg = model.config
