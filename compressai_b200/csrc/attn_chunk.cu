@@ -33,8 +33,8 @@
 // the chain softmax -> weights -> O -> next scores of a row tile; 2350 at 256 (prompt of 8192 tokens
 // 401 us, 1.37 PFLOP/s).
 //
-// 8-bit caches: a launch before this one writes the visible keys and values out once as exact fp16 (an
-// int8 is; see attn_decode.cu, also for the scales: the key's multiplies the score, the value's the
+// 8-bit and 4-bit caches: a launch before this one writes the visible keys and values out once as exact fp16 (an
+// int8 is, and a 4-bit code times its factor; see attn_decode.cu, also for the scales: the key's multiplies the score, the value's the
 // weight, relative to a power of two), in order and without pages, and this kernel reads those. Every
 // block of rows would convert the same keys again: warps that did so inside this kernel, beside the
 // softmax, took 4700 cycles an operand tile (two chunks of 257 tokens over 16385, 34 blocks a
@@ -941,8 +941,8 @@ bool make_pool_map(CUtensorMap* map, const void* base, int64_t rows, int D, int 
 
 constexpr int kWidenKeys = 64;
 
-// The visible keys and values of an 8-bit cache as fp16 integers [seqs, heads, wide_len, D], their scales
-// [seqs, heads, wide_len] beside them; zeros past a sequence's end (to the next 128 keys) and where a
+// The visible keys and values of an 8-bit cache as fp16 integers [seqs, heads, wide_len, D] (of a 4-bit one: times their groups'
+// factors), their scales [seqs, heads, wide_len] beside them; zeros past a sequence's end (to the next 128 keys) and where a
 // page does not exist. 64 keys a block; bound by memory (a key of 256 values: 516 bytes read, 1032
 // written).
 template <int BITS>
@@ -1006,13 +1006,20 @@ __global__ void __launch_bounds__(256) widen_kernel(const AttnArgs a) {
       const int key = k + (i >> 1) * per_round;
       if (key >= kWidenKeys) continue;
       uint4 y[2];
-      if (BITS == 4) {   // code * factor: 7 bits at most, exact
-        const __half2 u = __float2half2_rn(e4m3_value(x[i].z)), bias = __float2half2_rn(1032.f);
+      if (BITS == 4) {
+        // code * factor: 7 bits at most, exact, and so is (1024 + code + 8) * factor - 1032 * factor (1032 = 8 * 129, times 15 at most)
+        const __half2 u = __float2half2_rn(e4m3_value(x[i].z)), bias = __float2half2_rn(-1032.f * e4m3_value(x[i].z));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t w = (&x[i].x)[j >> 2] >> (8 * (j & 3)), c = 0x64006400u | (w & 15u) | (w & 0xf0u) << 12;   // 1024 + code + 8
-          const __half2 v = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&c), bias), u);
-          (&y[j >> 2].x)[j & 3] = *reinterpret_cast<const uint32_t*>(&v);
+        for (int j = 0; j < 2; ++j) {
+          uint32_t v[4];   // values k and k + 4
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t c = ((j ? x[i].y : x[i].x) >> (4 * k) & 0x000f000fu) | 0x64006400u;
+            const __half2 f = __hfma2(*reinterpret_cast<const __half2*>(&c), u, bias);
+            v[k] = *reinterpret_cast<const uint32_t*>(&f);
+          }
+          y[j] = make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632),
+                            __byte_perm(v[2], v[3], 0x7632));
         }
       }
 #pragma unroll
@@ -1022,8 +1029,13 @@ __global__ void __launch_bounds__(256) widen_kernel(const AttnArgs a) {
         (&y[j >> 1].x)[2 * (j & 1) + 1] = bytes_f16(u, 0x4342);
       }
       uint4* to = reinterpret_cast<uint4*>(static_cast<unsigned char*>(i & 1 ? a.wide_v : a.wide_k) + (out0 + (int64_t)key * a.D) * 2);
-      to[0] = y[0];
-      to[1] = y[1];
+      if (BITS == 4 && !(reinterpret_cast<uintptr_t>(to) & 31)) {   // one access of 32 bytes: two of 16 each touch half of every sector
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                     ::"l"(to), "r"(y[0].x), "r"(y[0].y), "r"(y[0].z), "r"(y[0].w), "r"(y[1].x), "r"(y[1].y), "r"(y[1].z), "r"(y[1].w) : "memory");
+      } else {
+        to[0] = y[0];
+        to[1] = y[1];
+      }
     }
   }
 }

@@ -277,3 +277,25 @@ def test_two_graphs_and_an_eager_call_between():
     b.check(outs[1])
     assert torch.equal(eager, outs[1])
     A.check_status()
+
+
+@pytest.mark.parametrize("off", [0, 16])
+def test_a_workspace_on_any_16_bytes(off):
+    """The C entry point asks for 16-byte alignment of its workspace, no more."""
+    import ctypes
+
+    from compressai_b200 import _lib
+    s = Setup([120], [300], 4, 2, 128, torch.float16, page=16, seed=3)
+    lib = _lib.load()
+    kind, T = _lib.VQ2_I4, 120
+    bytes_ = lib.vq2_paged_attention_workspace(T, 4, 2, 128, kind, 1, T, 300, 0)
+    ws = torch.empty(bytes_ + 64, dtype=torch.uint8, device=DEV)
+    out = torch.empty(T, 4, 128, dtype=torch.float16, device=DEV)
+    p = ctypes.c_void_p
+    n = s.pools[0].shape[0]
+    _lib.check(lib.vq2_paged_attention(
+        p(s.q.data_ptr()), 512, 128, _lib.VQ2_F16, T, 4, p(s.pools[0].data_ptr()), p(s.pools[1].data_ptr()), kind,
+        p(s.scales[0].data_ptr()), p(s.scales[1].data_ptr()), n, 2, 16, 128, p(s.table.data_ptr()), s.table.stride(0), s.table.shape[1],
+        p(s.lens.data_ptr()), p(s.starts.data_ptr()), 1, T, 300, 128 ** -0.5, 1, 0, p(out.data_ptr()), None, p(ws.data_ptr() + off),
+        bytes_, p(torch.cuda.current_stream().cuda_stream)), "vq2_paged_attention")
+    s.check(out)
