@@ -935,9 +935,11 @@ void plan_attn_decode4(AttnArgs& a, int64_t max_new, int64_t max_len) {
   const int64_t units = (keys + unit - 2) / unit + 1, pairs = (int64_t)a.kv.seqs * a.row_blocks * a.kv.heads;
   const int64_t room = (int64_t)sm_count() * per_sm;
   a.blocks = (int)(pairs >= room || units >= room || pairs * units >= room ? room : pairs * units);
-  // Two units stay whole: a joining launch and two starts cost more than they take (see the figures above). Where none is
-  // longer, by the caller's bounds, nothing is split and no joining launch follows.
-  a.whole = units <= 2 ? 0x7fffffff : 2;
+  // Pairs of two units stay whole: a joining launch and a second start cost more than they take. Where no pair is longer, by the
+  // caller's bounds, nothing is split and no joining launch follows; with pairs for a quarter of the blocks, where none is
+  // longer than eight (32 sequences of 1100, 32/8 heads of 128: split 24.8 us, whole 22.5; 64 of 500, 16/2 of 256: 21.9, 20.6;
+  // 8 of 600, 16/2 of 256, 16 pairs: 12.2, 16.9).
+  a.whole = units <= (4 * pairs >= room ? 8 : 2) ? 0x7fffffff : 2;
 }
 
 int launch_attn_decode4(const AttnArgs& a, cudaStream_t st) {
