@@ -7,7 +7,7 @@
 //
 // with mma.m16n8k16 and its own running maximum m and sum; warps, and blocks that split a long sequence, are joined at
 // the end. HBM bounds it (half of int8's bytes) as long as the codes become operands in few instructions, and they still
-// set the pace: 270 a warp for 16 keys of 128 values, K and V.
+// set the pace: 280 a warp for 16 keys of 128 values, K and V.
 //
 //   * A code's bits c in the low end of a 16-bit float are the number c 2^-24 (and one place of four further up,
 //     16 c 2^-24), exactly: a mask takes two codes out of a word and they are an operand register. The 8 codes of a word take
@@ -118,6 +118,7 @@ __device__ __forceinline__ uint32_t factors_f16(uint32_t w) {
   asm("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(w));
   return r;
 }
+
 // Shapes of one variant. G: groups of a row (codes past D are zeros); NT: 8-row tiles.
 template <int G, int NT>
 struct Shape4 {
@@ -128,7 +129,7 @@ struct Shape4 {
   static constexpr int kHalf = kKeys * kRow;            // K or V of a step
   static constexpr int kRecord = 64 + 16 * G;           // scales of 16 keys
   static constexpr int kScales = kKeys / 16 * kRecord;
-  static constexpr int kStages = 2;                       // steps under way
+  static constexpr int kStages = 2;                     // steps under way
   static constexpr int kPerSm = NT == 2 ? 2 : 3;        // blocks an SM, as registers allow
   static constexpr int kQ = NT * G * 1024;              // query fragments
   static constexpr int kRing = kStages * 2 * kHalf;
