@@ -24,23 +24,23 @@
 // number 2t, 2t + 1. With TMA's swizzle (none where a row is 32 bytes) all of these reads are free of bank conflicts if the
 // keys are numbered as `key_of_row` does.
 //
-// A step's K, V and scales (256 keys; 128 for heads above 128) come for the block's four warps together, issued by one thread
-// of the warp whose turn it is, two steps under way. Lengths are ragged and the split of a long sequence is worth a few
-// steps only where blocks are all equally long, so the launch has as many blocks as the card holds at once (3 an SM) and each
-// finds its equal share of all keys from the lengths, see `my_units`.
+// A warp's 64 keys of a step (32 for heads above 128), K, V and scales, come into a ring of its own, two steps under way,
+// issued by one of its threads; it waits for nobody but its copies. Lengths are ragged, and starts and ends cost a block as
+// much as a few steps, so the launch has as many blocks as the card holds at once (3 an SM) and each finds its equal share of all
+// keys from the lengths, see `my_units`.
 //
 // Queries become fp16 by a power of two per row, exact down to 2^-24 of the row's largest value; the weights are fp16,
 // relative to a power of two above the row scales of V that the row sees. Maxima, sums and O are 32 bits. Rescaling is lazy, see
 // attn_decode.cu.
 //
-// Measured (B200, one graph): 64 sequences of 800 to 8000, 16/2 heads of 256 (154 MB) 48.8 us, 4 sequences to 100,003, 32/8 heads
-// of 128 (372 MB) 86.8. What it took: a warp a row, 32 bits, 1667 and 3483; the MMAs, a ring a warp and splits of 768
-// keys 65.8 and 134; splits of 1536 keys 54 and 109, of 4800 117 and 116; equal shares 71 and 93, with the queries loaded ahead of
-// the copies and by all warps (6 us a segment before) 57 and 92, with a pair's start counted as two units 48.7 and 85.7. Left out:
-// one tile less a warp and step for 4 blocks an SM (58 and 98.7: spills, and a step's fixed cost), four steps under way (53 and
-// 95), P through shared memory and a group of O a warp (66 and 114: two barriers' waits), the last warp done with a step
-// fetching the next (49 and 92), groups and tiles in rolled loops (73 and 120). Pages of 16 keys instead of 256: 102 and 79 us
-// at the second (16 times the copies).
+// Measured (B200, one graph): 64 sequences of 800 to 8000, 16/2 heads of 256 (154 MB) 47.5 us, 4 sequences to 100,003, 32/8 heads
+// of 128 in pages of 32 (372 MB) 81.3; pages of 16 87.4, of 64 and more 79.7. What it took: a warp a row, 32 bits, 1667 and
+// 3483; the MMAs, splits of 768 keys, K and V fetched by halves 65.8 and 134; whole steps, masks in a branch 60 and 115; splits of
+// 1536 keys 54 and 109, of 4800 117 and 116; equal shares 71 and 93, with the queries loaded ahead of the copies and by all warps
+// (6 us a segment before) 57 and 92, with a pair's start counted as two units 48.7 and 85.7, these with the copies for a block's four
+// warps by one thread. Left out: one tile less a warp and step for 4 blocks an SM (58 and 98.7: spills, and a step's fixed
+// cost), P through shared memory and a group of O a warp (66 and 114: two barriers' waits), the last warp done with a block's
+// step fetching the next (49 and 92), groups and tiles in rolled loops (73 and 120).
 #include <atomic>
 #include <type_traits>
 
@@ -150,7 +150,7 @@ __device__ __forceinline__ int key_of_row(int r) {
   return place + 4 * other;
 }
 
-// Work is counted in units of a block step. Every pair (block of rows, key/value head) has its keys' units, at least one, and,
+// Work is counted in units of a block step (a step of each warp). Every pair (block of rows, key/value head) has its keys' units, at least one, and,
 // where a block's share of all units is four or more, two for its start and its end. The launch's blocks take equal shares in
 // order, so that lengths of any kind fill the card evenly; what a block has of one pair is a segment. Only pairs of more than
 // a.whole units are split.
@@ -287,8 +287,7 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
   extern __shared__ unsigned char decode4_raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(decode4_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* q_s = sm + (S::kRing > S::kJoin ? S::kRing : S::kJoin) + ST * 2 * S::kScales;
-  __shared__ uint64_t full[ST], empty[ST];
-  __shared__ uint32_t gone_s[ST];               // the boxes whose pages are not in the pool
+  __shared__ uint64_t full[S::kWarps][ST];
   __shared__ float2 red[S::kWarps][NT * 8];
   __shared__ float qexp_s[NT * 8], qtop_s[G][NT * 8];
   __shared__ float4 start_s[NT][G][4];
@@ -300,12 +299,9 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const uint32_t ring = su32(sm), scales = su32(q_s) - ST * 2 * S::kScales, q_sm = su32(q_s), full0 = su32(full), empty0 = su32(empty);
+  const uint32_t ring = su32(sm), scales = su32(q_s) - ST * 2 * S::kScales, q_sm = su32(q_s), full0 = su32(&full[warp][0]);
   if (threadIdx.x == 0) {
-    for (int i = 0; i < ST; ++i) {
-      mbar_init(full0 + 8 * i, 1);
-      mbar_init(empty0 + 8 * i, S::kWarps);
-    }
+    for (int i = 0; i < ST * S::kWarps; ++i) mbar_init(full0 + 8 * i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async();
   }
@@ -314,8 +310,8 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
   const bool any = my_units<UNIT>(a, ends, sums, share);
   const Place end = ends[1];
   const int page_mask = (1 << a.kv.page_log2) - 1;
-  // A copy is a box of min(page, step) keys; a step's are found by a lane each and issued by one thread of the warp whose turn it is.
-  const int box_keys = min(1 << a.kv.page_log2, S::kKeys), boxes = S::kKeys / box_keys, box_record = (box_keys >> 4) * REC;
+  // A copy is a box of the warp's keys of a step, as many as a page has; boxes are found by a lane each and issued by one thread.
+  const int box_keys = min(1 << a.kv.page_log2, 16 * U), boxes = 16 * U / box_keys, box_record = (box_keys >> 4) * REC;
   // this lane's places: K's key (another 8 on), V's keys of the MMA's rows 2t, 2t + 1 (others 8 on); 32 bytes a group
   auto swizzled = [](int key, int byte) {
     const int x = ROW == 128 ? key & 7 : ROW == 64 ? (key >> 1) & 3 : 0;
@@ -324,7 +320,6 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
   const int kkey = key_of_row<ROW>(g), vkey0 = key_of_row<ROW>(2 * t), vkey1 = key_of_row<ROW>(2 * t + 1);
   const uint32_t kx = swizzled(kkey, 8 * t), vx[2] = {swizzled(vkey0, 4 * g), swizzled(vkey1, 4 * g)};
   uint32_t done = 0;              // steps of the segments so far
-  uint32_t mine = 0xffffffffu;    // the last step that this warp fetched
   bool lost = false, ok = true;   // a wait of this warp, none of the block's has given up
 
   int item = ends[0].item, h = ends[0].h, unit0 = ends[0].k;
@@ -360,33 +355,30 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
         qv[p][1] = from[1];
       }
     }
-    // page of the lane's box of step i; -1 where there is none or its keys are past
+    // page of the lane's box of step i; -1 where there is none or its keys are past (looked up a step ahead)
     auto page_of = [&](int i) {
-      const int k = s0 + S::kKeys * i + lane * box_keys;
+      const int k = s0 + S::kKeys * i + 16 * U * warp + lane * box_keys;
       return lane < boxes && i < steps && k < s1 && (k | page_mask) >= seen ? table[k >> a.kv.page_log2] : -1;
     };
-    int turn = (warp - (int)first) & 3;   // the segment's step that this warp fetches next
-    int ahead = page_of(turn);
+    int put = 0;   // the segment's step that the warp fetches next
+    uint32_t gone = 0;   // a byte a stage: the boxes whose pages are not in the pool
+    int ahead = page_of(0);
     auto fetch = [&]() {
-      const uint32_t step = first + turn, st = step % ST, bar = full0 + 8 * st;
-      if (step >= ST) lost |= !copy_wait(empty0 + 8 * st, (step / ST - 1) & 1);
-      if (__any_sync(0xffffffffu, lost)) return;
+      if (put >= steps) return;
+      const uint32_t step = first + put, st = step % ST, bar = full0 + 8 * st;
       const bool there = ahead >= 0 && ahead < a.kv.pages;
       const uint32_t out = __ballot_sync(0xffffffffu, lane < boxes && !there);
       // a page that exists stands in for one that does not
-      const int rows = (((there ? ahead : 0) * a.kv.heads + h) << a.kv.page_log2) + ((s0 + S::kKeys * turn + lane * box_keys) & page_mask);
-      mine = step;
-      turn += 4;
-      ahead = page_of(turn);
+      const int rows = (((there ? ahead : 0) * a.kv.heads + h) << a.kv.page_log2) + ((s0 + S::kKeys * put + 16 * U * warp + lane * box_keys) & page_mask);
+      gone &= ~(0xffu << (8 * st));
+      gone |= out << (8 * st);
+      ahead = page_of(++put);
 #pragma unroll 1
       for (int c = 0; c < boxes; ++c) {
         const int row = __shfl_sync(0xffffffffu, rows, c);
         if (elect_one()) {
-          if (c == 0) {
-            *reinterpret_cast<volatile uint32_t*>(&gone_s[st]) = out;
-            mbar_arrive_tx(bar, 2 * (S::kHalf + S::kScales));
-          }
-          const uint32_t to = ring + st * 2 * S::kHalf + c * box_keys * ROW, to_s = scales + st * 2 * S::kScales + c * box_record;
+          if (c == 0) mbar_arrive_tx(bar, 2 * (S::kHalf + S::kScales) / S::kWarps);
+          const uint32_t to = ring + st * 2 * S::kHalf + (16 * U * warp + c * box_keys) * ROW, to_s = scales + st * 2 * S::kScales + warp * U * REC + c * box_record;
           const int64_t from = (int64_t)(row >> 4) * REC;
           tma_load_2d(to, &kmap, 0, row, bar);
           bulk_load(to_s, reinterpret_cast<const unsigned char*>(a.kv.k_scale) + from, box_record, bar);
@@ -395,7 +387,8 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
         }
       }
     };
-    if (turn < min(ST, steps)) fetch();
+#pragma unroll 1
+    for (int i = 0; i < ST; ++i) fetch();
 
     // ---- queries as B fragments, in the order of K's codes: of a group's 16 values of lane t, word w holds 8 w .. 8 w + 7,
     // and its MMA j takes values 2 j, 2 j + 4 and 2 j + 1, 2 j + 5 (these by 16)
@@ -557,13 +550,13 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
       }
       // ---- masks
       const int k0 = s0 + n * S::kKeys + warp * U * 16;
-      const uint32_t gone = *reinterpret_cast<volatile uint32_t*>(&gone_s[st]);
+      const uint32_t out = gone >> (8 * st) & 0xffu;
       uint32_t hidden = 0;   // the masked ones of this lane's weights
-      if (!(k0 >= all_lo && k0 + 16 * U <= all_hi && !gone)) {
+      if (!(k0 >= all_lo && k0 + 16 * U <= all_hi && !out)) {
         static_assert(U * NT * 4 <= 32, "bits of hidden");
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int left = (gone >> (16 * (warp * U + u) / box_keys)) & 1 ? 0 : s1 - k0 - 16 * u;   // keys of the tile that there are
+          const int left = (out >> (16 * u / box_keys)) & 1 ? 0 : s1 - k0 - 16 * u;   // keys of the tile that there are
 #pragma unroll
           for (int e = 0; e < 2; ++e)
             if (kkey + 8 * e >= left) vs[u][e] = 0.f;   // what lies past them is no scale
@@ -689,13 +682,12 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
         }
       }
       __syncwarp();   // the stage is used up
-      if (lane == 0) mbar_arrive(empty0 + 8 * st);
-      if (turn == n + ST && turn < steps) fetch();
+      fetch();
     }
     done += steps;
     if (__syncthreads_or(lost)) {   // copies under way have landed before the ring's memory is used for anything else
       ok = false;
-      if (mine != 0xffffffffu) copy_wait(full0 + 8 * (mine % ST), (mine / ST) & 1);
+      for (uint32_t i = first + max(0, put - ST); i < first + put; ++i) copy_wait(full0 + 8 * (i % ST), (i / ST) & 1);
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < NT; ++i) l[i][0] = l[i][1] = __int_as_float(0x7fffffff);   // the rows come out as NaN
@@ -890,7 +882,7 @@ int launch(AttnArgs a, cudaStream_t st) {
     done.fetch_or(bit);
   }
   CUtensorMap kmap, vmap;
-  const int keys = S::kKeys < 1 << a.kv.page_log2 ? S::kKeys : 1 << a.kv.page_log2;
+  const int keys = 16 * S::kU < 1 << a.kv.page_log2 ? 16 * S::kU : 1 << a.kv.page_log2;
   a.lo_mask = ~(keys - 1);   // a box lies in a page
   if (!make_code_map(&kmap, a.kv.k, a, S::kRow, keys) || !make_code_map(&vmap, a.kv.v, a, S::kRow, keys)) return VQ2_ERR_LAUNCH;
   return launch_kernel(kern, dim3((unsigned)a.blocks), dim3(S::kWarps * 32), S::kSmem, st, a, kmap, vmap);
