@@ -37,8 +37,8 @@
 // of 128 in pages of 32 (372 MB) 81.3; pages of 16 87.4, of 64 and more 79.7. What it took: a warp a row, 32 bits, 1667 and
 // 3483; the MMAs, splits of 768 keys, K and V fetched by halves 65.8 and 134; whole steps, masks in a branch 60 and 115; splits of
 // 1536 keys 54 and 109, of 4800 117 and 116; equal shares 71 and 93, with the queries loaded ahead of the copies and by all warps
-// (6 us a segment before) 57 and 92, with a pair's start counted as two units 48.7 and 85.7, these with the copies for a block's four
-// warps by one thread. Left out: one tile less a warp and step for 4 blocks an SM (58 and 98.7: spills, and a step's fixed
+// (6 us a segment before) 57 and 92, with a pair's start counted as two units 48.7 and 85.7 (these with the copies for a block's four
+// warps by one thread). Left out: one tile less a warp and step for 4 blocks an SM (59 and 93.5: spills, and a step's fixed
 // cost), P through shared memory and a group of O a warp (66 and 114: two barriers' waits), the last warp done with a block's
 // step fetching the next (49 and 92), groups and tiles in rolled loops (73 and 120).
 #include <atomic>
