@@ -612,7 +612,8 @@ VQ2_API int vq2_paged_moe_t1(const void* h, int h_dtype, int64_t top_k, const in
  * [pages, kv_heads, page_size, head_size / 2] bytes -- value 2i of a row in the low half of byte i, 2i + 1 in the
  * high half, each an integer -7..7 plus 8 -- and k_scale, v_scale the address of [pages, kv_heads,
  * page_size / 16, 4 + groups, 16] bytes, groups = ceil(head_size / 64): for 16 rows their fp32 scales, then of each
- * 64 values (the last group may have 32) 16 factors in e4m3 (value = integer * factor * scale). table: int32 [seqs, table_cols] page ids (row stride
+ * 64 values (the last group may have 32) 16 factors in e4m3, from 0 to 1 (larger
+ * ones pass the range of the kernels' 16-bit products): value = integer * factor * scale, scales not negative. table: int32 [seqs, table_cols] page ids (row stride
  * table_stride; rows may overlap, 0: all sequences on the same row): position p of sequence b is row p % page_size of page table[b][p / page_size].
  * lens: int32 [seqs] tokens of each sequence in the cache, the new ones included. starts: int32
  * [seqs + 1], ascending: sequence b's new tokens are starts[b] .. starts[b + 1] - 1 and sit at
