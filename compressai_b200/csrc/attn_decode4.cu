@@ -14,8 +14,9 @@
 //     five integer instructions (which run at half rate) and, for K, a subtraction; no conversion.
 //   * What the 16 stands for is put right where it is free: in K in the queries' operand (half of it is divided by 16),
 //     in V in the rows of O that such codes end in.
-//   * The 8 in every code: K's sums start at -8 sum q, and V's gets -8 sum P of each group at the end, summed by one more
-//     MMA a group into the row of the group's number, from the same rounded weights.
+//   * The 8 in every code: K's sums, of 64 products each, start at -8 sum q. V's sums run over all keys of a warp, and an MMA's
+//     addition is off by up to 2^-22 of its largest operand, to zero's side: with the 8 left in, sums of positive numbers only, 56
+//     sequences of 131,072 keys came out 12 % off (524,288: 35 %). So V's operand has it taken away, a subtraction a register.
 //   * K's factors multiply a group's sum (4 numbers a lane), V's the weights ahead of their rounding: both of them once for
 //     16 keys x 64 values.
 //
@@ -98,6 +99,7 @@ __device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
 }
 
 constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;   // codes of an even byte, as numbers 2^-24 and 16 2^-24
+constexpr uint32_t k8 = 0x00080008u;                          // 8 2^-24
 
 // The codes of bytes 0 and 2 (odd: 1 and 3) of w as two fp16 numbers each: low ones by 2^-24, high ones by 16 2^-24. Integer
 // instructions run at half rate: the second mask of the odd bytes is a subtraction.
@@ -291,7 +293,6 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
   __shared__ float2 red[S::kWarps][NT * 8];
   __shared__ float qexp_s[NT * 8], qtop_s[G][NT * 8];
   __shared__ float4 start_s[NT][G][4];
-  __shared__ uint4 ones_s[2];                   // A of the MMA that sums a group's weights, in the row of its number and in others
   __shared__ Place ends[2];
   __shared__ int64_t sums[8];
   if (threadIdx.x < 2)   // constant: ahead of the wait
@@ -305,7 +306,6 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async();
   }
-  if (threadIdx.x < 2) ones_s[threadIdx.x] = threadIdx.x ? make_uint4(0, 0, 0, 0) : make_uint4(0x00080008u, 0u, 0x00080008u, 0u);
   Share share;
   const bool any = my_units<UNIT>(a, ends, sums, share);
   const Place end = ends[1];
@@ -464,17 +464,14 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
     // keys that every row sees need no mask
     const int all_lo = row_lo(a, w, (w.r0 + w.rows - 1) / a.G), all_hi = min(s1, row_hi(a, w, w.r0 / a.G));
 
-    // o: sums over the codes plus 8 of values d (0, 1) and (2, 3) d + 1, these 16 times as large, in odd tiles with those of d
-    // added; oc: in row k 8 2^-24 times the weights of group k
-    float o[NT][4 * G][4], oc[NT][4], m[NT][2], l[NT][2], vref[NT][2];
+    // o: sums over the codes of values d (0, 1) and (2, 3) d + 1, these 16 times as large, in odd tiles with those of d added
+    float o[NT][4 * G][4], m[NT][2], l[NT][2], vref[NT][2];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 4; ++c)
 #pragma unroll
         for (int j = 0; j < 4 * G; ++j) o[i][j][c] = 0.f;
-        oc[i][c] = 0.f;
-      }
       m[i][0] = m[i][1] = -INFINITY;
       l[i][0] = l[i][1] = vref[i][0] = vref[i][1] = 0.f;
     }
@@ -626,7 +623,6 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
               o[i][j][c] *= by * undo;
               o[i][j][c + 2] *= by * undo;
             }
-            oc[i][c] *= by * undo;
           }
       }
       // ---- P^T: columns summed, weights relative to the V scale
@@ -655,7 +651,6 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
       // one after the factor is 1.5 times the error of 32 bits rounded at the end where the output is fp16 (1.4 so; 2 instructions of 88)
 #pragma unroll
       for (int k = 0; k < G; ++k) {
-        const uint4 ones = lds16(su32(&ones_s[g == k ? 0 : 1]));
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const uint32_t fa = v_rec + u * REC + 64 + 16 * k;
@@ -667,7 +662,6 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
           for (int i = 0; i < NT; ++i) {
             f0[i] = transpose8x8(pack2<__half>(s[u][i][0] * f.x, s[u][i][1] * f.x));
             f1[i] = transpose8x8(pack2<__half>(s[u][i][2] * f.y, s[u][i][3] * f.y));
-            mma(oc[i], ones.x, ones.y, ones.z, ones.w, f0[i], f1[i]);
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {   // values 2 j and 2 j + 1 of each lane's 8
@@ -676,8 +670,10 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
               y = __byte_perm(y, 0, 0x4341);
               z = __byte_perm(z, 0, 0x4341);
             }
+            const uint32_t y0 = hsub2(y & kLow, k8), y1 = hsub2(j & 1 ? y : y & kHigh, j & 1 ? k8 + k8 * 16 : k8 * 16);
+            const uint32_t z0 = hsub2(z & kLow, k8), z1 = hsub2(j & 1 ? z : z & kHigh, j & 1 ? k8 + k8 * 16 : k8 * 16);
 #pragma unroll
-            for (int i = 0; i < NT; ++i) mma(o[i][4 * k + j], y & kLow, j & 1 ? y : y & kHigh, z & kLow, j & 1 ? z : z & kHigh, f0[i], f1[i]);
+            for (int i = 0; i < NT; ++i) mma(o[i][4 * k + j], y0, y1, z0, z1, f0[i], f1[i]);
           }
         }
       }
@@ -710,15 +706,13 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
         y += __shfl_xor_sync(0xffffffffu, y, 16);
         if (g == 0) red[warp][8 * i + 2 * t + c] = make_float2(m[i][c] + kLift, y * kDrop);
 #pragma unroll
-        for (int k = 0; k < G; ++k) {
-          const float less = __shfl_sync(0xffffffffu, oc[i][c], 4 * k + t);   // row k, this column
+        for (int k = 0; k < G; ++k)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float low = o[i][4 * k + j][c], high = o[i][4 * k + j][c + 2];
             *reinterpret_cast<float2*>(acc + (warp * NT * 8 + 8 * i + 2 * t + c) * LD + 64 * k + 8 * g + 2 * j) =
-                make_float2((low - less) * kUnit * vref[i][c], ((j & 1 ? high - low : high) * 0.0625f - less) * kUnit * vref[i][c]);
+                make_float2(low * kUnit * vref[i][c], (j & 1 ? high - low : high) * 0.0625f * kUnit * vref[i][c]);
           }
-        }
       }
     __syncthreads();
 #pragma unroll 1
