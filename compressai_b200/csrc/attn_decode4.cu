@@ -13,12 +13,14 @@
 //     16 c 2^-24), exactly: a mask takes two codes out of a word and they are an operand register. The 8 codes of a word take
 //     five integer instructions (which run at half rate) and, for K, a subtraction; no conversion.
 //   * What the 16 stands for is put right where it is free: in K in the queries' operand (half of it is divided by 16),
-//     in V in the rows of O that such codes end in.
+//     in V in what such codes are multiplied by.
 //   * The 8 in every code: K's sums, of 64 products each, start at -8 sum q. V's sums run over all keys of a warp, and an MMA's
 //     addition is off by up to 2^-22 of its largest operand, to zero's side: with the 8 left in, sums of positive numbers only, 56
-//     sequences of 131,072 keys came out 12 % off (524,288: 35 %). So V's operand has it taken away, a subtraction a register.
-//   * K's factors multiply a group's sum (4 numbers a lane), V's the weights ahead of their rounding: both of them once for
-//     16 keys x 64 values.
+//     sequences of 131,072 keys came out 12 % off (524,288: 35 %). So V's operand has it taken away.
+//   * K's factors multiply a group's sum (4 numbers a lane). V's multiply its operand, in the multiply-add that takes the 8 away:
+//     code * factor is exact in 16 bits. (On the weights, ahead of their rounding, they cost less: 88.3 us for 92.3. But a factor goes
+//     down to 2^-9 and took up to 9 bits of what fp16 has for small weights: beside a key of 2^20 times their weight
+//     a group with factors of 2^-8 came out 4 % off in bf16; now 0.2 %, the output's own rounding.)
 //
 // Where the codes are: a K operand wants 16 values of a group in the four lanes of a key's row, a V operand 8 in each
 // of the eight lanes g: lane (g, t) reads the 8 bytes t of a group from keys of number g and the 4 bytes g from keys of
@@ -30,7 +32,7 @@
 // much as a few steps, so the launch has as many blocks as the card holds at once (3 an SM) and each finds its equal share of all
 // keys from the lengths, see `my_units`.
 //
-// Queries become fp16 by a power of two per row, exact down to 2^-24 of the row's largest value; the weights are fp16,
+// Queries become fp16 by a power of two per row, exact down to 2^-24 of the row's largest value; the weights are rounded to fp16 once,
 // relative to a power of two above the row scales of V that the row sees. Maxima, sums and O are 32 bits. Rescaling is lazy, see
 // attn_decode.cu.
 //
@@ -97,9 +99,16 @@ __device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
   const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&c));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
 
 constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;   // codes of an even byte, as numbers 2^-24 and 16 2^-24
-constexpr uint32_t k8 = 0x00080008u;                          // 8 2^-24
 
 // The codes of bytes 0 and 2 (odd: 1 and 3) of w as two fp16 numbers each: low ones by 2^-24, high ones by 16 2^-24. Integer
 // instructions run at half rate: the second mask of the odd bytes is a subtraction.
@@ -284,7 +293,8 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
     attn_decode4_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using S = Shape4<G, NT>;
   constexpr int U = S::kU, ROW = S::kRow, UNIT = S::kKeys, ST = S::kStages, REC = S::kRecord;
-  // weights 2^7 larger than the maximum asks for, so that those down to 2^-32 of the largest are more than 0
+  // weights 2^7 larger than the maximum asks for, so that those down to 2^-32 of the largest are more than 0 (of keys whose V scale
+  // is the largest; 2^-32 over its share of that otherwise)
   constexpr float kLift = 7.f, kDrop = 1.f / 128.f;
   extern __shared__ unsigned char decode4_raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(decode4_raw) + 1023) & ~uintptr_t(1023));
@@ -318,6 +328,7 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
     return (uint32_t)(key * ROW + (byte ^ (x << 4)));
   };
   const int kkey = key_of_row<ROW>(g), vkey0 = key_of_row<ROW>(2 * t), vkey1 = key_of_row<ROW>(2 * t + 1);
+  const uint32_t vkeys = vkey0 | vkey1 << 4;   // as bytes of 8 factors
   const uint32_t kx = swizzled(kkey, 8 * t), vx[2] = {swizzled(vkey0, 4 * g), swizzled(vkey1, 4 * g)};
   uint32_t done = 0;              // steps of the segments so far
   bool lost = false, ok = true;   // a wait of this warp, none of the block's has given up
@@ -464,7 +475,7 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
     // keys that every row sees need no mask
     const int all_lo = row_lo(a, w, (w.r0 + w.rows - 1) / a.G), all_hi = min(s1, row_hi(a, w, w.r0 / a.G));
 
-    // o: sums over the codes of values d (0, 1) and (2, 3) d + 1, these 16 times as large, in odd tiles with those of d added
+    // o: sums of values d (0, 1) and d + 1 (2, 3)
     float o[NT][4 * G][4], m[NT][2], l[NT][2], vref[NT][2];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
@@ -647,33 +658,35 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
               if (hidden >> ((u * NT + i) * 4 + c) & 1) s[u][i][c] = 0.f;
         }
       }
-      // ---- O^T += V^T P^T. P times the group's factors is rounded once and turned into B fragments: a rounding before and
-      // one after the factor is 1.5 times the error of 32 bits rounded at the end where the output is fp16 (1.4 so; 2 instructions of 88)
+      // ---- O^T += V^T P^T, P rounded and turned into B fragments
+      uint32_t p0[U][NT], p1[U][NT];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          p0[u][i] = transpose8x8(pack2<__half>(s[u][i][0], s[u][i][1]));
+          p1[u][i] = transpose8x8(pack2<__half>(s[u][i][2], s[u][i][3]));
+        }
 #pragma unroll
       for (int k = 0; k < G; ++k) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const uint32_t fa = v_rec + u * REC + 64 + 16 * k;
-          const float2 f = unpack2<__half>(factors_f16(lds1(fa + kkey) | lds1(fa + kkey + 8) << 8));
+          // factors of keys 2t, 2t + 1 and of those 8 on; code * factor comes out 2^-9 times as large, a code of 2^-24 times
+          // 2^15 factor: none of it is lost, as factors are multiples of 2^-9
+          const uint4 fw = lds16(v_rec + u * REC + 64 + 16 * k);
+          const uint32_t fy = factors_f16(__byte_perm(fw.x, fw.y, vkeys)), fz = factors_f16(__byte_perm(fw.z, fw.w, vkeys));
+          const uint32_t yl = hmul2(fy, 0x78007800u), yh = hmul2(fy, 0x68006800u), y8 = hmul2(fy, 0xa400a400u);   // 2^15, 2^11, -2^-6 (8 codes)
+          const uint32_t zl = hmul2(fz, 0x78007800u), zh = hmul2(fz, 0x68006800u), z8 = hmul2(fz, 0xa400a400u);
           const uint32_t at = src + S::kHalf + u * 16 * ROW, b0 = at + (vx[0] ^ (32 * k)), b1 = at + (vx[1] ^ (32 * k));
           const uint32_t w0 = lds4(b0), w1 = lds4(b1), w2 = lds4(b0 + 8 * ROW), w3 = lds4(b1 + 8 * ROW);
-          uint32_t f0[NT], f1[NT];
-#pragma unroll
-          for (int i = 0; i < NT; ++i) {
-            f0[i] = transpose8x8(pack2<__half>(s[u][i][0] * f.x, s[u][i][1] * f.x));
-            f1[i] = transpose8x8(pack2<__half>(s[u][i][2] * f.y, s[u][i][3] * f.y));
-          }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {   // values 2 j and 2 j + 1 of each lane's 8
-            uint32_t y = __byte_perm(w0, w1, j < 2 ? 0x5410 : 0x7632), z = __byte_perm(w2, w3, j < 2 ? 0x5410 : 0x7632);
-            if (j & 1) {   // the odd bytes: their high codes with the low ones
-              y = __byte_perm(y, 0, 0x4341);
-              z = __byte_perm(z, 0, 0x4341);
-            }
-            const uint32_t y0 = hsub2(y & kLow, k8), y1 = hsub2(j & 1 ? y : y & kHigh, j & 1 ? k8 + k8 * 16 : k8 * 16);
-            const uint32_t z0 = hsub2(z & kLow, k8), z1 = hsub2(j & 1 ? z : z & kHigh, j & 1 ? k8 + k8 * 16 : k8 * 16);
+            uint32_t y0, y1, z0, z1;
+            two_codes(j & 1, __byte_perm(w0, w1, j < 2 ? 0x5410 : 0x7632), y0, y1);
+            two_codes(j & 1, __byte_perm(w2, w3, j < 2 ? 0x5410 : 0x7632), z0, z1);
 #pragma unroll
-            for (int i = 0; i < NT; ++i) mma(o[i][4 * k + j], y0, y1, z0, z1, f0[i], f1[i]);
+            for (int i = 0; i < NT; ++i)
+              mma(o[i][4 * k + j], hfma2(y0, yl, y8), hfma2(y1, yh, y8), hfma2(z0, zl, z8), hfma2(z1, zh, z8), p0[u][i], p1[u][i]);
           }
         }
       }
@@ -693,7 +706,7 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
     }
 
     // ---- join the warps: maximum, then sums relative to it
-    constexpr float kUnit = 16777216.f * kDrop;   // 2^24 of the codes
+    constexpr float kUnit = 512.f * kDrop;        // 2^9 of code * factor
     constexpr int LD = S::kWidth;
     float* acc = reinterpret_cast<float*>(sm);    // [warp][row][64 G + 4]
 #pragma unroll
@@ -708,11 +721,9 @@ __global__ void __launch_bounds__(Shape4<G, NT>::kWarps * 32, Shape4<G, NT>::kPe
 #pragma unroll
         for (int k = 0; k < G; ++k)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float low = o[i][4 * k + j][c], high = o[i][4 * k + j][c + 2];
+          for (int j = 0; j < 4; ++j)
             *reinterpret_cast<float2*>(acc + (warp * NT * 8 + 8 * i + 2 * t + c) * LD + 64 * k + 8 * g + 2 * j) =
-                make_float2(low * kUnit * vref[i][c], (j & 1 ? high - low : high) * 0.0625f * kUnit * vref[i][c]);
-          }
+                make_float2(o[i][4 * k + j][c] * kUnit * vref[i][c], o[i][4 * k + j][c + 2] * kUnit * vref[i][c]);
       }
     __syncthreads();
 #pragma unroll 1

@@ -53,3 +53,44 @@ def test_sums_over_many_keys(L, seqs, new, d):
     tol = 2.0 ** -11 * want.abs() + 2.0 ** -25 + sums
     assert sums < 0.05 * want.abs().max()   # the bound says something
     assert ((got.double() - want).abs() <= tol).all(), ((got.double() - want).abs() - tol).max().item()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("new", [1, 3, 100])
+@pytest.mark.parametrize("d,factors", [(128, [0, 8]), (128, [9, 0]), (256, [0, 4, 6, 9]), (96, [2, 7])])
+@pytest.mark.parametrize("less,at", [(11, 0), (17, 0), (19, 2740)])
+def test_groups_far_below_their_rows_largest(dtype, new, d, factors, less, at):
+    """Values whose group has a factor of 2^-factors[g], and eight keys without a value, 32 apart, that outweigh each other one by
+    2^less: what is left of a group is its own, and as exact as the others. Enough sequences (on the same pages) that each has blocks
+    of its own, whose warps see such a key each. All values are positive, so that a sum of weights times values is the output:
+    a weight, 2^7 times 2^-less times the row's scale over a power of two, is a normal fp16 number and rounds by 2^-11 of itself;
+    the output by its type's half step (and half of fp16's smallest number, 2^-25); scores are sums of 15 numbers times 1 at most, off by 2^-20 of 15
+    steps (0.25 here, times q of 4 log 2: less than 2^-16 a score, twice that of a weight), the tensor core's 3000 / 16 additions by 2^-22 each, all else in 32 bits: 2e-4 together."""
+    L, heads, hq, page = 3000, 2, 4, 32
+    g = gen(d + less)
+    pages = -(-L // page)
+    shape = (pages, heads, page)
+    table = torch.arange(pages, dtype=torch.int32, device=DEV)[None]
+    k, v = torch.zeros(*shape, d, dtype=torch.int8, device=DEV), torch.randint(1, 8, (*shape, d), generator=g, device=DEV, dtype=torch.int8)
+    k[..., 1:] = torch.randint(-7, 8, (*shape, d - 1), generator=g, device=DEV, dtype=torch.int8)
+    heavy = (at // page + torch.arange(8, device=DEV), slice(None), at % page)   # a row of eight pages
+    k[*heavy, 0] = 4      # times 0.25 and q: a score of less * log 2
+    v_scale = torch.tensor([16 * 1.3, 16 * 1.9], device=DEV)[None, :, None].repeat(pages, 1, page)   # roundings that do not average out
+    v_scale[heavy] = 0
+    f = torch.tensor([2.0 ** -e for e in factors], device=DEV).expand(*shape, -1)
+    kp, ks = pools_of(k, torch.full(shape, 0.25, device=DEV), torch.ones(*shape, len(factors), device=DEV))
+    vp, vs = pools_of(v, v_scale, f)
+    seqs = 2 if new == 100 else 225
+    q = torch.zeros(seqs * new, hq, d, dtype=dtype, device=DEV)
+    q[..., 0] = less
+    lens, starts = torch.full((seqs,), L, dtype=torch.int32, device=DEV), torch.arange(0, seqs * new + 1, new, dtype=torch.int32, device=DEV)
+    got = A.paged_attention(q, kp, vp, table.expand(seqs, -1), lens, starts, k_scale=ks, v_scale=vs, scale=math.log(2.0), causal=False, max_new=new)
+    v64 = v.double() * v_scale.double()[..., None] * f.double().repeat_interleave(64, -1)[..., :d]
+    w = torch.full((pages, page), 2.0 ** -less, dtype=torch.float64, device=DEV)
+    w.view(-1)[L:] = 0
+    w[heavy[0], heavy[2]] = 1
+    want = torch.einsum("np,nhpd->hd", w, v64) / w.sum()
+    want = want.repeat_interleave(hq // heads, 0)
+    eps = 2.0 ** -11 if dtype == torch.float16 else 2.0 ** -8
+    tol = (eps + 2.0 ** -11 + 2e-4) * want + 2.0 ** -25
+    assert ((got.double() - want).abs() <= tol).all(), (((got.double() - want).abs() / want).amax((0, 1)), less)
