@@ -40,7 +40,8 @@ __device__ __forceinline__ float quantiser4(float group, float row, uint32_t& by
   if (bad || row < 1e-30f) return 0.f;
   float u;
   byte = factor_of(group, reciprocal(row), u);
-  scale = row * 0.14285714924335479736f;   // 1 / 7: off by 2^-23 at most
+  scale = row * (1.f / 7.f);
+  scale = fmaf(fmaf(-7.f, scale, row), 1.f / 7.f, scale);   // a Newton step from the exact remainder: row / 7 rounded once
   return u == 0.f ? 0.f : reciprocal(row * u) * (7.f + 7.f / 1048576.f);
 }
 

@@ -1,4 +1,5 @@
-"""Attention over a 4-bit cache where it adds up many keys, or weights and values of very different sizes, against 64 bits."""
+"""A 4-bit cache's numbers to the last bit where the definition gives them, and attention over it where it adds up many keys, or
+weights and values of very different sizes, against 64 bits."""
 import math
 
 import pytest
@@ -94,3 +95,28 @@ def test_groups_far_below_their_rows_largest(dtype, new, d, factors, less, at):
     eps = 2.0 ** -11 if dtype == torch.float16 else 2.0 ** -8
     tol = (eps + 2.0 ** -11 + 2e-4) * want + 2.0 ** -25
     assert ((got.double() - want).abs() <= tol).all(), (((got.double() - want).abs() / want).amax((0, 1)), less)
+
+
+def write_rows(x, page, **kw):
+    """Rows x [T, 1, D] written as K and V of one sequence: the pools with their scales, and what cache_read needs."""
+    T, _, d = x.shape
+    n = -(-T // page)
+    pools = [A.empty_pool(n, 1, page, d, torch.int4) for _ in range(2)]
+    table = torch.arange(n, dtype=torch.int32, device=DEV)[None]
+    lens, starts = torch.tensor([T], dtype=torch.int32, device=DEV), torch.tensor([0, T], dtype=torch.int32, device=DEV)
+    A.cache_write(x, x, pools[0][0], pools[1][0], table, lens, starts, k_scale=pools[0][1], v_scale=pools[1][1], **kw)
+    return pools, table, starts
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("turned,every", [(False, 1), (True, 1), (True, 300)])
+def test_scales_are_a_seventh_rounded_once(dtype, turned, every):
+    """Of every 16-bit number from 1e-30 on, by each kernel that writes (few tokens and many are turned by two). V's rows are never turned."""
+    top = torch.arange(0x7f80 if dtype == torch.bfloat16 else 0x7c00, device=DEV).to(torch.int16).view(dtype)
+    top = top[top.float() >= 1e-30][::every]
+    x = torch.zeros(top.numel(), 1, 32, dtype=dtype, device=DEV)
+    x[torch.arange(top.numel(), device=DEV), 0, torch.arange(top.numel(), device=DEV) % 32] = -top
+    pools, _, _ = write_rows(x, 64, **(dict(inv_freq=A.rope_frequencies(32)[0].to(DEV)) if turned else {}))
+    for _, scales in pools[turned:]:
+        got = scales[..., :4, :].flatten(-2).contiguous().view(torch.float32).flatten()[: top.numel()]
+        assert torch.equal(got, (top.double() / 7).float())   # no quotient by 7 is near enough to a tie of 32 bits for the rounding to 64 to matter
