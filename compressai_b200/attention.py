@@ -259,29 +259,40 @@ class PagedKVCache:
 
     def resize(self, pages):
         """Pools of ``pages`` pages, the ones in use compacted into them; memory is taken and given back a pool at a time.
-        Where it runs out on the way, more pages than before are not had, fewer are."""
+        Where it runs out on the way, more pages than before are not had, fewer are; the pools are of one size then too (and
+        where there is not even memory to move them into that size, views of larger ones)."""
         n = sum(1 for u in self.users if u)
         if pages < max(n, 1):
             raise ValueError(f"{n} pages are in use: {pages} do not hold them")
         self.compact()
         size = min(pages, len(self.users))
 
-        def moved(x):
-            y = x.new_empty(pages, *x.shape[1:])
+        def moved(x, rows):
+            y = x.new_empty(rows, *x.shape[1:])
             y[:n].copy_(x[:n])
             return y
-        try:
+
+        def resized(rows, move):   # by index: a loop over the pairs would hold the old pools until its next turn
             for kept in (self.pools, self.scales):
-                for i, (k, v) in enumerate(kept):
-                    if k is not None:
-                        kept[i] = (moved(k), v)
-                        del k
-                        kept[i] = (kept[i][0], moved(v))
-                    del v
+                for i in range(len(kept)):
+                    if kept[i][0] is not None:
+                        kept[i] = (move(kept[i][0], rows), kept[i][1])
+                        kept[i] = (kept[i][0], move(kept[i][1], rows))
+
+        def left(x, rows):
+            if x.shape[0] == rows:
+                return x
+            try:
+                return moved(x, rows)
+            except RuntimeError:
+                return x[:rows]
+        try:
+            resized(pages, moved)
             size = pages
+        except BaseException:
+            resized(size, left)
+            raise
         finally:
-            for kept in (self.pools, self.scales):   # all of one size, also where memory ran out on the way
-                kept[:] = [tuple(x if x is None else x[:size] for x in pair) for pair in kept]
             self.users = self.users[:n] + [0] * (size - n)
             self.free = list(range(size - 1, n - 1, -1))
 

@@ -1,5 +1,6 @@
 """PagedKVCache's bookkeeping of shared pages on the host, and the refusals of 4-bit pools and page copies (no device needed)."""
 import ctypes
+import weakref
 
 import pytest
 import torch
@@ -255,3 +256,49 @@ def test_cpu_tensors_are_refused():
     for src, dst in (([0], [4]), ([-1], [0]), ([0, 1], [2, 2]), ([0, 1], [1, 2]), ([0, 1], [2])):
         with pytest.raises(ValueError):
             A.copy_pages([pool], src, dst)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.int4])
+@pytest.mark.parametrize("to", [4, 20])
+def test_resize_gives_a_pool_back_before_it_takes_the_next(dtype, to, monkeypatch):
+    c = cache(dtype=dtype)
+    a = c.add()
+    c.begin([a], [40])
+    old = [weakref.ref(x) for both in (c.pools, c.scales) for pair in both for x in pair if x is not None]
+    real, alive = torch.Tensor.new_empty, []
+
+    def new_empty(self, *shape):
+        alive.append([r() is not None for r in old])
+        return real(self, *shape)
+    monkeypatch.setattr(torch.Tensor, "new_empty", new_empty)
+    c.resize(to)
+    assert alive == [[j >= i for j in range(len(old))] for i in range(len(old))]
+    assert all(x.untyped_storage().nbytes() == x.nbytes for both in (c.pools, c.scales) for pair in both for x in pair if x is not None)
+
+
+@pytest.mark.parametrize("to", [4, 20])
+@pytest.mark.parametrize("again", [False, True])
+def test_resize_that_runs_out_of_memory_keeps_no_more_than_it_says(to, again, monkeypatch):
+    """The pools that were moved already go back to the size that is left, or, where there is no memory for that either, are cut."""
+    c = cache(dtype=torch.int8)
+    a = c.add()
+    c.begin([a], [40])
+    for i, pair in enumerate(c.pools + c.scales):
+        for j, x in enumerate(pair):
+            x[:3] = 10 * i + j
+    real, calls = torch.Tensor.new_empty, []
+
+    def new_empty(self, *shape):
+        calls.append(shape)
+        if len(calls) == 4 or again and len(calls) > 4:
+            raise torch.OutOfMemoryError("full")
+        return real(self, *shape)
+    monkeypatch.setattr(torch.Tensor, "new_empty", new_empty)
+    with pytest.raises(torch.OutOfMemoryError):
+        c.resize(to)
+    size = min(to, 8)
+    assert len(c.users) == size and sorted(c.free) == list(range(3, size))
+    for i, pair in enumerate(c.pools + c.scales):
+        for j, x in enumerate(pair):
+            assert x.shape[0] == size and x.is_contiguous() and (x[:3] == 10 * i + j).all()
+            assert again or x.untyped_storage().nbytes() == x.nbytes
