@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, 5) load4_kernel(const __grid_constan
     for (int n = 0; n < U; ++n)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        x[n][c] = make_uint2(0, 0);
+        x[n][c] = make_uint2(0x88888888u, 0x88888888u);   // codes of 0: rows that are not there are +0, as in other caches
         step[n][c] = 0.f;
         byte[n][c] = 0;
         if (row < 0 || h0 + done + n >= h_end) continue;

@@ -120,3 +120,26 @@ def test_scales_are_a_seventh_rounded_once(dtype, turned, every):
     for _, scales in pools[turned:]:
         got = scales[..., :4, :].flatten(-2).contiguous().view(torch.float32).flatten()[: top.numel()]
         assert torch.equal(got, (top.double() / 7).float())   # no quotient by 7 is near enough to a tie of 32 bits for the rounding to 64 to matter
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads,d", [(1, 32), (3, 96), (2, 256)])
+def test_read_back_rows_and_missing_ones(dtype, heads, d):
+    """Rows that the table names are theirs; a page that does not exist and tokens of no sequence give zeros without a sign."""
+    g, page = gen(d), 16
+    codes = [torch.randint(-7, 8, (4, heads, page, d), generator=g, device=DEV, dtype=torch.int8) for _ in range(2)]
+    scale = [torch.rand(4, heads, page, generator=g, device=DEV) for _ in range(2)]
+    factor = [2.0 ** -torch.randint(0, 9, (4, heads, page, -(-d // 64)), generator=g, device=DEV).float() for _ in range(2)]
+    (kp, ks), (vp, vs) = (pools_of(c, s, f) for c, s, f in zip(codes, scale, factor))
+    table = torch.tensor([[3, -1, 0], [4, 2, 1]], dtype=torch.int32, device=DEV)
+    starts = torch.tensor([0, 37, 37 + 25], dtype=torch.int32, device=DEV)
+    back = A.cache_read(kp, vp, table, starts, 70, k_scale=ks, v_scale=vs, dtype=dtype)
+    eps = 2.0 ** -11 if dtype == torch.float16 else 2.0 ** -8
+    for got, c, s, f in zip(back, codes, scale, factor):
+        x = (c.double() * s.double()[..., None] * f.double().repeat_interleave(64, -1)[..., :d]).transpose(1, 2)   # [page, row, head, D]
+        want = torch.zeros(70, heads, d, dtype=torch.float64, device=DEV)
+        want[:16], want[32:37], want[53:62] = x[3], x[0, :5], x[2, :9]
+        assert ((got.double() - want).abs() <= eps * (1 + 2.0 ** -10) * want.abs() + 2.0 ** -25).all()
+        there = torch.zeros(70, dtype=torch.bool, device=DEV)
+        there[:16] = there[32:37] = there[53:62] = True
+        assert (got[~there].view(torch.int16) == 0).all()
