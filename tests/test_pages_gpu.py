@@ -225,3 +225,14 @@ def test_a_step_on_forks_is_taken_back():
     t.check()
     t.step([a, b], [2, 1])
     t.check()
+
+
+@pytest.mark.parametrize("kind", [list, tuple])
+def test_pages_named_in_lists(kind):
+    pools = [torch.randn(9, 4, 16, generator=gen(i), device=DEV) for i in range(3)]
+    want = [p.clone() for p in pools]
+    for w in want:
+        w[4], w[0] = w[7], w[2]
+    A.copy_pages(kind(pools), kind([7, 2]), kind([4, 0]))
+    for p, w in zip(pools, want):
+        assert torch.equal(p, w)
