@@ -236,3 +236,19 @@ def test_pages_named_in_lists(kind):
     A.copy_pages(kind(pools), kind([7, 2]), kind([4, 0]))
     for p, w in zip(pools, want):
         assert torch.equal(p, w)
+
+
+def test_a_replayed_copy_by_lists_keeps_its_ids():
+    pool = torch.randn(8, 64, generator=gen(0), device=DEV)
+    want = pool.clone()
+    A.copy_pages([pool], [0], [1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        A.copy_pages([pool], [3], [4])
+    others = [torch.tensor([5, 6], dtype=torch.int32).pin_memory() for _ in range(100)]
+    for i in (3, 2):
+        pool[3], want[3] = want[i], want[i].clone()
+        graph.replay()
+        want[1], want[4] = want[0], want[3]
+        assert torch.equal(pool, want)
+    del others
