@@ -151,7 +151,7 @@ def paged_attention(q, k_pages, v_pages, table, lens, starts=None, *, k_scale=No
 
 def copy_pages(pools, src, dst):
     """In every one of ``pools`` (contiguous tensors [pages, ..], of any type, a page a multiple of 16 bytes: K and V of
-    all layers with their scales, say) page ``dst[i]`` becomes what page ``src[i]`` is, in one launch. ``src`` and ``dst``:
+    all layers with their scales, say) page ``dst[i]`` becomes what page ``src[i]`` is, in a launch for 128 pools. ``src`` and ``dst``:
     int32 on the pools' device, read when the kernel runs (ids outside the pools copy nothing), or lists, which are
     checked: pages in ``dst`` are different ones and none is in ``src``. Where a tensor breaks that, such a page
     holds bytes of any of its sources."""
@@ -243,7 +243,7 @@ class PagedKVCache:
         self.lengths[seq] = length
 
     def compact(self):
-        """Move the pages in use to ids 0 .. n - 1, as few of them as that takes, in one launch; returns n."""
+        """Move the pages in use to ids 0 .. n - 1, as few of them as that takes, in one ``copy_pages``; returns n."""
         n = sum(1 for u in self.users if u)
         to = iter([p for p in range(n) if not self.users[p]])
         moves = {p: next(to) for p in range(n, len(self.users)) if self.users[p]}

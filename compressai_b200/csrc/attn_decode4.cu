@@ -7,11 +7,11 @@
 //
 // with mma.m16n8k16 and its own running maximum m and sum; warps, and blocks that split a long sequence, are joined at
 // the end. HBM bounds it (half of int8's bytes) as long as the codes become operands in few instructions, and they still
-// set the pace: 280 a warp for 16 keys of 128 values, K and V.
+// set the pace: 300 a warp for 16 keys of 128 values, K and V.
 //
 //   * A code's bits c in the low end of a 16-bit float are the number c 2^-24 (and one place of four further up,
 //     16 c 2^-24), exactly: a mask takes two codes out of a word and they are an operand register. The 8 codes of a word take
-//     five integer instructions (which run at half rate) and, for K, a subtraction; no conversion.
+//     five integer instructions (which run at half rate) and a subtraction; no conversion.
 //   * What the 16 stands for is put right where it is free: in K in the queries' operand (half of it is divided by 16),
 //     in V in what such codes are multiplied by.
 //   * The 8 in every code: K's sums, of 64 products each, start at -8 sum q. V's sums run over all keys of a warp, and an MMA's
@@ -36,8 +36,9 @@
 // relative to a power of two above the row scales of V that the row sees. Maxima, sums and O are 32 bits. Rescaling is lazy, see
 // attn_decode.cu.
 //
-// Measured (B200, one graph): 64 sequences of 800 to 8000, 16/2 heads of 256 (154 MB) 47.5 us, 4 sequences to 100,003, 32/8 heads
-// of 128 in pages of 32 (372 MB) 81.3; pages of 16 87.4, of 64 and more 79.7. What it took: a warp a row, 32 bits, 1667 and
+// Measured (B200, calls side by side in one graph): 64 sequences of 800 to 8000, 16/2 heads of 256 (154 MB) 48.9 us, 4 sequences
+// to 100,003, 32/8 heads of 128 in pages of 32 (372 MB) 86.3; pages of 16 91.2, of 64 and more 84.0. What earlier builds took, with V's
+// factors on the weights and its codes not signed (81.3 the last of them): a warp a row, 32 bits, 1667 and
 // 3483; the MMAs, splits of 768 keys, K and V fetched by halves 65.8 and 134; whole steps, masks in a branch 60 and 115; splits of
 // 1536 keys 54 and 109, of 4800 117 and 116; equal shares 71 and 93, with the queries loaded ahead of the copies and by all warps
 // (6 us a segment before) 57 and 92, with a pair's start counted as two units 48.7 and 85.7 (these with the copies for a block's four
