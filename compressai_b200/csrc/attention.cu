@@ -17,7 +17,7 @@ int64_t plan(AttnArgs& a, int bits, int64_t max_new, int64_t max_len, bool& chun
   // here, 20 to 40 rows 63 us there; 32 rows here took 100). Over an 8-bit cache, which it has to widen
   // first, from 49 rows on (the same, 32 rows: 96 us here, 156 there; 16/2 heads of 256: 63 and 88); over a 4-bit
   // one, half as many bytes to read again, from 97 on (64 rows: 100 us here, 133 there; 16/2 heads of 256 55 and 77; 96 rows 143
-  // and 134, 71 and 76; 128 rows, of an earlier build here, 180 and 135, 93 and 77). Its
+  // and 134, 71 and 76; 128 rows, of an earlier version here, 180 and 135, 93 and 77). Its
   // fp16 copy of such a cache is kept to 4 GB; past that (a batch of very long sequences) the decode
   // kernel reads the 8 bits again after all.
   // A bound of 0 leaves it one tile: a launch of no blocks is an error.

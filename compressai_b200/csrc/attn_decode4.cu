@@ -37,7 +37,7 @@
 // attn_decode.cu.
 //
 // Measured (B200, calls side by side in one graph): 64 sequences of 800 to 8000, 16/2 heads of 256 (154 MB) 48.9 us, 4 sequences
-// to 100,003, 32/8 heads of 128 in pages of 32 (372 MB) 86.3; pages of 16 91.2, of 64 and more 84.0. What earlier builds took, with V's
+// to 100,003, 32/8 heads of 128 in pages of 32 (372 MB) 86.3; pages of 16 91.2, of 64 and more 84.0. What earlier versions took, with V's
 // factors on the weights and its codes not signed (81.3 the last of them): a warp a row, 32 bits, 1667 and
 // 3483; the MMAs, splits of 768 keys, K and V fetched by halves 65.8 and 134; whole steps, masks in a branch 60 and 115; splits of
 // 1536 keys 54 and 109, of 4800 117 and 116; equal shares 71 and 93, with the queries loaded ahead of the copies and by all warps
